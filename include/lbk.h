@@ -45,6 +45,8 @@ typedef struct lbk_plan lbk_plan;     /* a recorded sequence of fused ternary-li
 #define LBK_MAX_GROUP 4   /* matrices sharing one input in a fused call (q/k/v, gate/up)  */
 #define LBK_COMPUTE_BF16 0 /* the precisions a model family is served in */
 #define LBK_COMPUTE_F32 1 /* everything in 32-bit (families that have it; BitNet does not) */
+#define LBK_DTYPE_F32 0    /* types of a buffer that may have either */
+#define LBK_DTYPE_BF16 1
 #define LBK_GEMV_MAX_M 16 /* token rows served by the bandwidth-bound GEMV kernel         */
 
 /* Message of the last failure on this thread ("" if none). Never NULL. */
@@ -531,6 +533,45 @@ int lbk_moe_route(lbk_ctx *ctx, const float *z_dev, size_t z_pitch, size_t n, si
                   const uint16_t *x_dev, size_t x_pitch, uint16_t *sorted_dev, int32_t *ids_out_dev, float *weights_out_dev,
                   int32_t *place_out_dev, int32_t *offs_out_dev, void *stream);
 
+/* ---- drafted tokens: several tokens of a sequence checked in one pass (no counterpart in the reference) ----------------
+ * A sequence has t node places (1..LBK_TREE_NODES), the first counts_dev[seq] of them in use (counts_dev may be null: all).
+ * parents_dev[seq][i] is the node that node i follows, -1 <= parent < i; -1: it follows the committed position pos_dev[seq] - 1. A
+ * node's depth is the number of its ancestors. Caches as everywhere: bf16 [seq][kv_heads][cap][head_dim]; node i's row is pos + i
+ * whatever its depth, and pos + count <= cap. A sequence whose positions or parents break these rules is not computed and
+ * its buffers are left as they were, except that lbk_attn_tree takes a parent that is none for -1; lbk_check_device_error then returns
+ * LBK_ERR_INVALID. Rows of places not in use are left as they were. b sequences, everything read from device memory: a step can be recorded.
+ * lbk_rope_kv_append_tree  lbk_rope_kv_append for the nodes: q_dev [b][t][n_heads][head_dim] turned in place and k_dev
+ *                          [b][t][kv_heads][head_dim] by position pos + depth, k and v appended at row pos + i. The tables have cap rows or more.
+ * lbk_attn_tree            softmax(scale * q . k) v over the rows 0 .. pos - 1 and those of the node itself and its ancestors, head_dim
+ *                          128. q_dev and out_dev rows [b * t] of n_heads * 128 values, q_pitch and out_pitch values apart: f32 with
+ *                          LBK_COMPUTE_F32 (q and the probabilities as two bf16 terms each), bf16 with LBK_COMPUTE_BF16; pitches and buffers are
+ *                          multiples of 16 bytes. scratch_dev: lbk_attn_tree_scratch floats, 16-byte aligned, what is in them
+ *                          does not matter; calls that may overlap need their own.
+ * lbk_tree_accept          the greedy walk: node 0, then as long as there is one the lowest child whose token (tokens_dev) is best_dev of its
+ *                          parent (the argmax of the parent's logits). path_dev [b][t]: the nodes, then -1; count_out_dev how many, next_dev
+ *                          best_dev of the last one (-1 for a sequence without nodes).
+ * lbk_kv_keep_path         rows pos + path[j] move to pos + j, j < count_dev[seq], of keys and values of `layers` layers that lie
+ *                          layer_elems elements apart. path_dev [b][t] ascending, any accepted nodes. Positions are not changed.
+ * lbk_advance_pos_by       pos_dev[seq] += count_dev[seq]. */
+#define LBK_TREE_NODES 128
+int lbk_rope_kv_append_tree(lbk_ctx *ctx, float *q_dev, const float *k_dev, const float *v_dev, const float *cos_dev, const float *sin_dev,
+                            const int32_t *pos_dev, const int32_t *parents_dev, const int32_t *counts_dev, size_t b, size_t t, size_t n_heads,
+                            size_t kv_heads, size_t head_dim, size_t cap, uint16_t *kcache_dev, uint16_t *vcache_dev, void *stream);
+int lbk_tree_accept(lbk_ctx *ctx, const int32_t *tokens_dev, const int32_t *parents_dev, const int32_t *best_dev, const int32_t *counts_dev, size_t b,
+                    size_t t, int32_t *path_dev, int32_t *count_out_dev, int32_t *next_dev, void *stream);
+int lbk_kv_keep_path(lbk_ctx *ctx, uint16_t *kcache_dev, uint16_t *vcache_dev, size_t layers, size_t layer_elems, size_t b, size_t kv_heads,
+                     size_t head_dim, size_t cap, const int32_t *pos_dev, const int32_t *path_dev, const int32_t *count_dev, size_t t, void *stream);
+int lbk_advance_pos_by(lbk_ctx *ctx, int32_t *pos_dev, const int32_t *count_dev, size_t b, void *stream);
+
+/* Rows of logits (LBK_DTYPE_*, `pitch` values apart, 0 < scale): logprobs_dev [rows][given] = log softmax(scale * logits) at
+ * tokens_dev [rows][given] (NaN for a token outside the vocabulary), entropy_dev [rows] (may be null) in nats, and the `top` (at most
+ * LBK_LOGPROBS_TOP) largest logits: ids top_ids_dev [rows][top], the lower one first among equals, NaN in front, and their log
+ * probabilities. Values of -inf have probability 0; a row with a NaN or +inf, or with nothing above -inf, has NaN log probabilities and entropy. */
+#define LBK_LOGPROBS_TOP 32
+int lbk_token_logprobs(lbk_ctx *ctx, int dtype, const void *logits_dev, size_t pitch, size_t rows, size_t vocab, const int32_t *tokens_dev,
+                       size_t given, float scale, size_t top, float *logprobs_dev, float *entropy_dev, int32_t *top_ids_dev,
+                       float *top_logprobs_dev, void *stream);
+
 /* ---- the decoder as a native runtime (crates/lb-model/src/model.rs) ----------------------------
  * Three families: BitNet (below), Pefolix and Dugulorn (`dir/config.json` with "architecture": "Pefolix" or
  * "Dugulorn" and `dir/model.safetensors`, bf16 tensors), which have the same calls. A Dugulorn cache holds latents
@@ -686,8 +727,6 @@ int lbk_plan_destroy(lbk_plan *plan);
  * tensor walks the digest chain, about 0.03 s per million weights of the largest tensor, all tensors
  * side by side: 0.5 s for a 2B4T-shaped model).
  * Synchronises `stream`. */
-#define LBK_DTYPE_F32 0
-#define LBK_DTYPE_BF16 1
 typedef struct lbk_convert_item {
     const void *src_dev;
     size_t rows, cols;

@@ -122,6 +122,11 @@ SYMBOLS = [
     ("lbk_attn_window", _i, [_vp, _i, _vp, _vp, _vp, _vp, _sz, _i, _sz, _sz, _sz, _sz, _sz, _sz, _sz, _f, _sz, _sz, _i, _vp, _vp, _sz, _vp]),
     ("lbk_moe_route_ints", _sz, [_sz, _sz, _sz]),
     ("lbk_moe_route", _i, [_vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp]),
+    ("lbk_rope_kv_append_tree", _i, [_vp] * 9 + [_sz] * 6 + [_vp] * 3),
+    ("lbk_tree_accept", _i, [_vp] * 5 + [_sz, _sz] + [_vp] * 4),
+    ("lbk_kv_keep_path", _i, [_vp, _vp, _vp] + [_sz] * 6 + [_vp] * 3 + [_sz, _vp]),
+    ("lbk_advance_pos_by", _i, [_vp, _vp, _vp, _sz, _vp]),
+    ("lbk_token_logprobs", _i, [_vp, _i, _vp, _sz, _sz, _sz, _vp, _sz, _f, _sz, _vp, _vp, _vp, _vp, _vp]),
     ("lbk_model_load", _i, [_vp, C.c_char_p, _pp]),
     ("lbk_model_load_compute", _i, [_vp, C.c_char_p, _i, _pp]),
     ("lbk_model_architecture", C.c_char_p, [_vp]),

@@ -86,11 +86,15 @@ int ctx_scratch(Ctx *ctx, size_t bytes, void **out) {
 }
 
 // What a non-zero error word means. Code 7 is written by the decoder-step kernels when a position
-// read from device memory lies outside the cache; every other code marks a bounded wait that ran out.
+// read from device memory lies outside the cache, code 8 when a tree read from device memory is none; every other code marks a
+// bounded wait that ran out.
 int device_error_status(int word) {
     if (word == 7)
         return fail(LBK_ERR_INVALID, "a decode position was outside its cache (position < 0 or >= capacity); the kernels of that step "
                                      "refused to run and its results are invalid");
+    if (word == 8)
+        return fail(LBK_ERR_INVALID, "a tree of drafted tokens had a parent that is not in front of its node, or a path that does not ascend inside it; "
+                                     "the kernels of that step refused the sequence and its results are invalid");
     return fail(LBK_ERR_TIMEOUT, "a bounded device-side wait gave up (code %d); results of that launch are invalid", word);
 }
 

@@ -1,0 +1,269 @@
+// Drafted tokens: the kernels around their attention (lbk_attn_tree.cu).
+//
+//   rope_append_tree   queries and keys turned by their node's DEPTH (position pos + number of ancestors), keys and values
+//                      appended as bf16 at the node's PLACE (row pos + i)
+//   tree_accept        the greedy walk: node 0, then the child whose token is the best one of its parent's row
+//   kv_keep_path       the rows of the accepted nodes moved together behind the committed ones, in all layers
+//   advance_by         positions moved by the accepted nodes
+//
+// A decode step of one token is the tree with one node: the same rows of the cache, the same rotation
+// (crates/lb-model/src/model.rs:295-303, 334-347). Everything is read from device memory, so a step can be recorded once.
+#include "lbk_dense_dev.cuh"
+#include "lbk_tree.cuh"
+
+namespace lbk {
+
+namespace {
+
+using dense::bf16_pair;
+
+// x * cos + other * sin with the rounding of the prompt pass (lbk_decoder.cu): the product with sin rounded, the rest in one step
+__device__ __forceinline__ float turned(float x, float c, float other, float s) { return __fmaf_rn(x, c, __fmul_rn(other, s)); }
+
+// One block per node and part of its heads. A thread takes four dimensions of each half of a head, so that loads and stores are
+// 16 bytes; queries, keys and values are asked for before the node's depth is known. Bound by launch and two dependent trips to memory up to
+// some hundred nodes, then by bytes.
+// VEC: head_dim is a multiple of 8 and every buffer lies on 16 bytes.
+template <bool VEC>
+__global__ void __launch_bounds__(256) rope_append_tree_kernel(float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
+                                                               const float *__restrict__ cos_t, const float *__restrict__ sin_t, const int *__restrict__ pos_dev,
+                                                               const int *__restrict__ parents, const int *__restrict__ counts, int t, int nh, int kvh, int hd, int cap,
+                                                               uint16_t *__restrict__ kcache, uint16_t *__restrict__ vcache, int *err_word) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    __shared__ int s_parent[kTreeNodes];
+    const int row = blockIdx.x, seq = row / t, node = row - seq * t, half = hd >> 1, tid = threadIdx.x;
+    const int quarter = half >> 2, it = blockIdx.y * blockDim.x + tid;  // VEC: this thread's four dimensions of both halves
+    const int h = VEC ? it / quarter : 0, i = VEC ? (it - h * quarter) * 4 : 0;
+    const bool mine = VEC && h < nh + kvh, key = h >= nh;
+    float4 a{}, b{}, va{}, vb{};
+    if (mine) {
+        const float *src = key ? k + (static_cast<size_t>(row) * kvh + h - nh) * hd : q + (static_cast<size_t>(row) * nh + h) * hd;
+        a = *reinterpret_cast<const float4 *>(src + i);
+        b = *reinterpret_cast<const float4 *>(src + i + half);
+        if (key) {
+            const float *vv = v + (static_cast<size_t>(row) * kvh + h - nh) * hd;
+            va = *reinterpret_cast<const float4 *>(vv + i);
+            vb = *reinterpret_cast<const float4 *>(vv + i + half);
+        }
+    }
+    const int pos = pos_dev[seq], count = tree_count(counts, seq, t);
+    bool wrong = false;
+    for (int j = tid; j < count; j += blockDim.x) {
+        const int p = parents[static_cast<size_t>(seq) * t + j];
+        s_parent[j] = p;
+        wrong |= p < -1 || p >= j;
+    }
+    if (__syncthreads_or(wrong)) {
+        if (tid == 0) atomicExch(err_word, kErrTree);
+        return;
+    }
+    if (!tree_in_cache(pos, count, cap, err_word) || node >= count) return;
+    int depth = 0;
+    for (int p = s_parent[node]; p >= 0; p = s_parent[p]) ++depth;  // ends: a parent lies in front of its child
+    const float *c = cos_t + static_cast<size_t>(pos + depth) * hd, *s = sin_t + static_cast<size_t>(pos + depth) * hd;
+    if (VEC) {
+        if (!mine) return;
+        auto ld = [](const float *at) { return *reinterpret_cast<const float4 *>(at); };
+        const float4 c1 = ld(c + i), c2 = ld(c + i + half), s1 = ld(s + i), s2 = ld(s + i + half);
+        const float4 lo = make_float4(turned(a.x, c1.x, -b.x, s1.x), turned(a.y, c1.y, -b.y, s1.y), turned(a.z, c1.z, -b.z, s1.z), turned(a.w, c1.w, -b.w, s1.w));
+        const float4 hi = make_float4(turned(b.x, c2.x, a.x, s2.x), turned(b.y, c2.y, a.y, s2.y), turned(b.z, c2.z, a.z, s2.z), turned(b.w, c2.w, a.w, s2.w));
+        if (!key) {
+            float *dst = q + (static_cast<size_t>(row) * nh + h) * hd;
+            *reinterpret_cast<float4 *>(dst + i) = lo;
+            *reinterpret_cast<float4 *>(dst + i + half) = hi;
+            return;
+        }
+        const size_t slot = ((static_cast<size_t>(seq) * kvh + h - nh) * cap + pos + node) * hd;
+        *reinterpret_cast<uint2 *>(kcache + slot + i) = make_uint2(bf16_pair(lo.x, lo.y), bf16_pair(lo.z, lo.w));
+        *reinterpret_cast<uint2 *>(kcache + slot + i + half) = make_uint2(bf16_pair(hi.x, hi.y), bf16_pair(hi.z, hi.w));
+        *reinterpret_cast<uint2 *>(vcache + slot + i) = make_uint2(bf16_pair(va.x, va.y), bf16_pair(va.z, va.w));
+        *reinterpret_cast<uint2 *>(vcache + slot + i + half) = make_uint2(bf16_pair(vb.x, vb.y), bf16_pair(vb.z, vb.w));
+        return;
+    }
+    for (int e = it; e < (nh + kvh) * half; e += blockDim.x * gridDim.y) {
+        const int hh = e / half, d = e - hh * half;
+        if (hh < nh) {
+            float *qh = q + (static_cast<size_t>(row) * nh + hh) * hd;
+            const float x1 = qh[d], x2 = qh[d + half];
+            qh[d] = turned(x1, c[d], -x2, s[d]);
+            qh[d + half] = turned(x2, c[d + half], x1, s[d + half]);
+        } else {
+            const float *kk = k + (static_cast<size_t>(row) * kvh + hh - nh) * hd, *vv = v + (static_cast<size_t>(row) * kvh + hh - nh) * hd;
+            const size_t slot = ((static_cast<size_t>(seq) * kvh + hh - nh) * cap + pos + node) * hd;
+            const float x1 = kk[d], x2 = kk[d + half];
+            kcache[slot + d] = dense::f32_bf16(turned(x1, c[d], -x2, s[d]));
+            kcache[slot + d + half] = dense::f32_bf16(turned(x2, c[d + half], x1, s[d + half]));
+            vcache[slot + d] = dense::f32_bf16(vv[d]);
+            vcache[slot + d + half] = dense::f32_bf16(vv[d + half]);
+        }
+    }
+}
+
+// One warp per sequence; a lane looks at four nodes.
+__global__ void __launch_bounds__(32) tree_accept_kernel(const int *__restrict__ tokens, const int *__restrict__ parents, const int *__restrict__ best,
+                                                         const int *__restrict__ counts, int t, int *__restrict__ path, int *__restrict__ count_out,
+                                                         int *__restrict__ next, int *err_word) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    constexpr int kEach = kTreeNodes / 32;
+    __shared__ int s_best[kTreeNodes];
+    const int seq = blockIdx.x, lane = threadIdx.x, count = tree_count(counts, seq, t);
+    const size_t at = static_cast<size_t>(seq) * t;
+    int tok[kEach], par[kEach];
+    bool wrong = false;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int i = e * 32 + lane;
+        tok[e] = i < count ? tokens[at + i] : 0;
+        par[e] = i < count ? parents[at + i] : -1;
+        if (i < count) s_best[i] = best[at + i];
+        wrong |= par[e] < -1 || (i < count && par[e] >= i);
+    }
+    __syncwarp();
+    wrong = __any_sync(0xffffffffu, wrong);
+    if (wrong && lane == 0) atomicExch(err_word, kErrTree);
+    int n = 0;
+    for (int node = count && !wrong ? 0 : -1; node >= 0;) {  // ends: a child lies behind its parent
+        if (lane == 0) path[at + n] = node;
+        ++n;
+        const int want = s_best[node];
+        int child = -1;
+#pragma unroll
+        for (int e = kEach - 1; e >= 0; --e) {  // the lowest of several children with that token
+            const unsigned hits = __ballot_sync(0xffffffffu, par[e] == node && tok[e] == want && e * 32 + lane < count);
+            if (hits) child = e * 32 + __ffs(hits) - 1;
+        }
+        if (child < 0 && lane == 0) next[seq] = want;
+        node = child;
+    }
+    for (int i = n + lane; i < t; i += 32) path[at + i] = -1;
+    if (lane == 0) {
+        count_out[seq] = n;
+        if (n == 0) next[seq] = -1;
+    }
+}
+
+// One block per (part of the layers' KV heads, sequence), 16 bytes a thread and row. Rows move down only (path[j] >= j, ascending), so portions in
+// ascending order, each read before it is written, never overwrite a row that is still wanted.
+constexpr int kKeepRows = 8;   // rows a portion
+__global__ void __launch_bounds__(128) kv_keep_path_kernel(uint4 *kcache, uint4 *vcache, size_t layer_units, int heads, int units, int cap, const int *__restrict__ pos_dev,
+                                                           const int *__restrict__ path, const int *__restrict__ counts, int t, int *err_word) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    __shared__ int s_path[kTreeNodes];
+    const int seq = blockIdx.y, tid = threadIdx.x, count = tree_count(counts, seq, t), pos = pos_dev[seq];
+    bool wrong = false;
+    for (int j = tid; j < count; j += blockDim.x) {
+        const int from = path[static_cast<size_t>(seq) * t + j];
+        s_path[j] = from;
+        wrong |= from < j || from >= t || (j > 0 && from <= path[static_cast<size_t>(seq) * t + j - 1]);
+    }
+    if (__syncthreads_or(wrong)) {
+        if (tid == 0) atomicExch(err_word, kErrTree);
+        return;
+    }
+    if (!count || !tree_in_cache(pos, s_path[count - 1] + 1, cap, err_word)) return;
+    int first = 0;
+    while (first < count && s_path[first] == first) ++first;  // these lie where they belong
+    const int layer = blockIdx.x / (2 * heads), rest = blockIdx.x - layer * 2 * heads, head = rest >> 1;
+    uint4 *rows = (rest & 1 ? vcache : kcache) + static_cast<size_t>(layer) * layer_units + ((static_cast<size_t>(seq) * heads + head) * cap + pos) * units;
+    const int n = (count - first) * units;
+    for (int base = 0; base < n; base += kKeepRows * 128) {
+        uint4 held[kKeepRows];
+#pragma unroll
+        for (int e = 0; e < kKeepRows; ++e) {
+            const int i = base + e * 128 + tid, j = i / units;
+            if (i < n) held[e] = rows[static_cast<size_t>(s_path[first + j]) * units + i - j * units];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kKeepRows; ++e) {
+            const int i = base + e * 128 + tid;
+            if (i < n) rows[static_cast<size_t>(first) * units + i] = held[e];
+        }
+        __syncthreads();
+    }
+}
+
+__global__ void advance_by_kernel(int *pos, const int *__restrict__ count, int n) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    // a position that was refused stays refused (advance_pos_kernel)
+    if (i < n && count[i] > 0 && pos[i] < (1 << 30)) pos[i] += min(count[i], kTreeNodes);
+}
+
+}  // namespace
+}  // namespace lbk
+
+using namespace lbk;
+
+extern "C" {
+
+int lbk_rope_kv_append_tree(lbk_ctx *c, float *q_dev, const float *k_dev, const float *v_dev, const float *cos_dev, const float *sin_dev, const int32_t *pos_dev,
+                            const int32_t *parents_dev, const int32_t *counts_dev, size_t b, size_t t, size_t n_heads, size_t kv_heads, size_t head_dim, size_t cap,
+                            uint16_t *kcache_dev, uint16_t *vcache_dev, void *stream) {
+    LBK_TREE_PRE("lbk_rope_kv_append_tree");
+    if (b == 0 || t == 0) return LBK_OK;
+    if (!q_dev || !k_dev || !v_dev || !cos_dev || !sin_dev || !pos_dev || !parents_dev || !kcache_dev || !vcache_dev)
+        return fail(LBK_ERR_INVALID, "lbk_rope_kv_append_tree: null buffer");
+    if (t > LBK_TREE_NODES) return fail(LBK_ERR_UNSUPPORTED, "a tree has at most %d nodes (got %zu)", LBK_TREE_NODES, t);
+    if (!n_heads || !kv_heads || !head_dim || head_dim % 2 || n_heads + kv_heads > (1u << 20) || head_dim > 1024)
+        return fail(LBK_ERR_SHAPE, "lbk_rope_kv_append_tree: %zu and %zu heads of %zu (an even number, at most 1024)", n_heads, kv_heads, head_dim);
+    if (cap > INT32_MAX || b * t > INT32_MAX) return fail(LBK_ERR_UNSUPPORTED, "lbk_rope_kv_append_tree: more rows than 2^31");
+    const uintptr_t all = reinterpret_cast<uintptr_t>(q_dev) | reinterpret_cast<uintptr_t>(k_dev) | reinterpret_cast<uintptr_t>(v_dev) | reinterpret_cast<uintptr_t>(cos_dev) |
+                          reinterpret_cast<uintptr_t>(sin_dev) | reinterpret_cast<uintptr_t>(kcache_dev) | reinterpret_cast<uintptr_t>(vcache_dev);
+    const bool vec = head_dim % 8 == 0 && (all & 15) == 0;
+    const size_t items = (n_heads + kv_heads) * head_dim / (vec ? 8 : 2);
+    const unsigned threads = items < 256 ? static_cast<unsigned>((items + 31) / 32 * 32) : 256;
+    const dim3 grid(static_cast<unsigned>(b * t), static_cast<unsigned>(vec ? (items + threads - 1) / threads : 1));
+    if (grid.y > 65535) return fail(LBK_ERR_UNSUPPORTED, "lbk_rope_kv_append_tree: %zu heads of %zu", n_heads + kv_heads, head_dim);
+    LBK_CUDA(launch_chained(vec ? rope_append_tree_kernel<true> : rope_append_tree_kernel<false>, grid, dim3(threads), 0, st, q_dev, k_dev, v_dev, cos_dev, sin_dev, pos_dev, parents_dev,
+                            counts_dev, static_cast<int>(t), static_cast<int>(n_heads), static_cast<int>(kv_heads), static_cast<int>(head_dim), static_cast<int>(cap), kcache_dev,
+                            vcache_dev, ctx->err_word));
+    ctx->launches++;
+    return LBK_OK;
+}
+
+int lbk_tree_accept(lbk_ctx *c, const int32_t *tokens_dev, const int32_t *parents_dev, const int32_t *best_dev, const int32_t *counts_dev, size_t b, size_t t,
+                    int32_t *path_dev, int32_t *count_out_dev, int32_t *next_dev, void *stream) {
+    LBK_TREE_PRE("lbk_tree_accept");
+    if (b == 0) return LBK_OK;
+    if (!tokens_dev || !parents_dev || !best_dev || !path_dev || !count_out_dev || !next_dev) return fail(LBK_ERR_INVALID, "lbk_tree_accept: null buffer");
+    if (t == 0 || t > LBK_TREE_NODES) return fail(LBK_ERR_UNSUPPORTED, "a tree has 1 to %d nodes (got %zu)", LBK_TREE_NODES, t);
+    if (b > INT32_MAX) return fail(LBK_ERR_UNSUPPORTED, "lbk_tree_accept: more sequences than 2^31");
+    LBK_CUDA(launch_chained(tree_accept_kernel, dim3(static_cast<unsigned>(b)), dim3(32), 0, st, tokens_dev, parents_dev, best_dev, counts_dev, static_cast<int>(t), path_dev, count_out_dev,
+                            next_dev, ctx->err_word));
+    ctx->launches++;
+    return LBK_OK;
+}
+
+int lbk_kv_keep_path(lbk_ctx *c, uint16_t *kcache_dev, uint16_t *vcache_dev, size_t layers, size_t layer_elems, size_t b, size_t kv_heads, size_t head_dim, size_t cap,
+                     const int32_t *pos_dev, const int32_t *path_dev, const int32_t *count_dev, size_t t, void *stream) {
+    LBK_TREE_PRE("lbk_kv_keep_path");
+    if (b == 0 || layers == 0) return LBK_OK;
+    if (!kcache_dev || !vcache_dev || !pos_dev || !path_dev || !count_dev) return fail(LBK_ERR_INVALID, "lbk_kv_keep_path: null buffer");
+    if (t == 0 || t > LBK_TREE_NODES) return fail(LBK_ERR_UNSUPPORTED, "a tree has 1 to %d nodes (got %zu)", LBK_TREE_NODES, t);
+    if (!kv_heads || !head_dim || head_dim % 8 || layer_elems % 8 || ((reinterpret_cast<uintptr_t>(kcache_dev) | reinterpret_cast<uintptr_t>(vcache_dev)) & 15))
+        return fail(LBK_ERR_SHAPE, "lbk_kv_keep_path: head_dim and layer_elems are multiples of 8, the caches lie on 16 bytes");
+    if (layers > 1 && layer_elems < b * kv_heads * cap * head_dim) return fail(LBK_ERR_SHAPE, "lbk_kv_keep_path: layers of %zu elements overlap", layer_elems);
+    if (cap > INT32_MAX || b > 65535 || layers * kv_heads * 2 > INT32_MAX || head_dim > 8192) return fail(LBK_ERR_UNSUPPORTED, "lbk_kv_keep_path: at most 65535 sequences and 2^31 rows");
+    LBK_CUDA(launch_chained(kv_keep_path_kernel, dim3(static_cast<unsigned>(layers * kv_heads * 2), static_cast<unsigned>(b)), dim3(128), 0, st, reinterpret_cast<uint4 *>(kcache_dev),
+                            reinterpret_cast<uint4 *>(vcache_dev), layer_elems / 8, static_cast<int>(kv_heads), static_cast<int>(head_dim / 8), static_cast<int>(cap), pos_dev, path_dev,
+                            count_dev, static_cast<int>(t), ctx->err_word));
+    ctx->launches++;
+    return LBK_OK;
+}
+
+int lbk_advance_pos_by(lbk_ctx *c, int32_t *pos_dev, const int32_t *count_dev, size_t b, void *stream) {
+    LBK_TREE_PRE("lbk_advance_pos_by");
+    if (b == 0) return LBK_OK;
+    if (!pos_dev || !count_dev) return fail(LBK_ERR_INVALID, "lbk_advance_pos_by: null buffer");
+    if (b > INT32_MAX) return fail(LBK_ERR_UNSUPPORTED, "lbk_advance_pos_by: more sequences than 2^31");
+    LBK_CUDA(launch_chained(advance_by_kernel, dim3(static_cast<unsigned>((b + 127) / 128)), dim3(128), 0, st, pos_dev, count_dev, static_cast<int>(b)));
+    ctx->launches++;
+    return LBK_OK;
+}
+
+}  // extern "C"

@@ -7,7 +7,7 @@ torch is used for device memory and streams only; all arithmetic is in liblbk.so
 from __future__ import annotations
 
 import ctypes as C
-from typing import List, Optional, Sequence
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -164,6 +164,154 @@ def bf16_linear(x: torch.Tensor, w: torch.Tensor, ctx: Optional[Context] = None)
     _lib.check(ctx._lib.lbk_bf16_linear(ctx.handle, C.c_void_p(x.data_ptr()), m, C.c_void_p(w.data_ptr()), n, k,
                                         C.c_void_p(out.data_ptr()), C.c_void_p(_stream_ptr())))
     return out
+
+
+TREE_NODES = 128     # node places of a sequence (LBK_TREE_NODES)
+LOGPROBS_TOP = 32    # alternatives of a row (LBK_LOGPROBS_TOP)
+
+
+def _on(ctx: Context, **tensors) -> int:
+    """Checks that the tensors (None is none) lie on the context's GPU without gaps; the raw current stream of that GPU."""
+    for name, t in tensors.items():
+        if t is not None:
+            if not t.is_cuda or t.get_device() != ctx.device:
+                raise ValueError(f"{name} must live on cuda:{ctx.device}")
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+    return torch._C._cuda_getCurrentRawStream(ctx.device)
+
+
+def _tree(parents: torch.Tensor, counts: Optional[torch.Tensor], pos: Optional[torch.Tensor] = None) -> Tuple[int, int]:
+    """(sequences, node places) of a batch of trees, or of paths through them."""
+    if parents.dim() != 2:
+        raise ValueError("the trees are [sequences, nodes]")
+    b, t = parents.shape
+    if not 1 <= t <= TREE_NODES:
+        raise ValueError(f"a tree has 1 to {TREE_NODES} nodes (got {t})")
+    if parents.dtype != torch.int32:
+        raise TypeError("the trees are int32")
+    for v in (counts, pos):
+        if v is not None and (v.dtype != torch.int32 or v.shape != (b,)):
+            raise ValueError(f"positions and counts are int32, one for each of the {b} sequences")
+    return b, t
+
+
+def _caches(k: torch.Tensor, v: torch.Tensor, b: int, dims: int) -> torch.Size:
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise TypeError("caches are bf16")
+    if k.dim() != dims or k.shape != v.shape or k.shape[dims - 4] != b:
+        raise ValueError(f"caches are [{'layers, ' if dims == 5 else ''}{b}, kv_heads, capacity, head_dim], keys like values")
+    return k.shape
+
+
+def rope_kv_append_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, parents: torch.Tensor,
+                        kcache: torch.Tensor, vcache: torch.Tensor, counts: Optional[torch.Tensor] = None, ctx: Optional[Context] = None) -> None:
+    """Drafted tokens into the cache (lbk_rope_kv_append_tree): q [b, t, heads * head_dim] f32 is turned in place by pos + depth of its
+    node, k and v [b, t, kv_heads * head_dim] f32 go to row pos + i of kcache and vcache [b, kv_heads, cap, head_dim]. parents int32 [b, t]: the
+    node a node follows, -1 the committed row pos - 1; counts int32 [b]: how many nodes a sequence has (all t)."""
+    b, t = _tree(parents, counts, pos)
+    _, kvh, cap, hd = _caches(kcache, vcache, b, 4)
+    for name, x in (("q", q), ("k", k), ("v", v), ("cos", cos), ("sin", sin)):
+        if x.dtype != torch.float32:
+            raise TypeError(f"{name} is f32")
+    nh = q.numel() // max(1, b * t * hd)
+    if q.numel() != b * t * nh * hd or k.numel() != b * t * kvh * hd or v.numel() != k.numel():
+        raise ValueError(f"q, k and v are rows of heads of {hd} for {b} x {t} nodes")
+    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[0] < cap or cos.shape[1] != hd:
+        raise ValueError("the rotation tables have a row for every place of the cache")
+    ctx = ctx or default_context()
+    st = _on(ctx, q=q, k=k, v=v, cos=cos, sin=sin, pos=pos, parents=parents, counts=counts, kcache=kcache, vcache=vcache)
+    status = ctx._lib.lbk_rope_kv_append_tree(ctx.handle, q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), parents.data_ptr(),
+                                              None if counts is None else counts.data_ptr(), b, t, nh, kvh, hd, cap, kcache.data_ptr(), vcache.data_ptr(), st)
+    if status:
+        _lib.check(status)
+
+
+def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, best: torch.Tensor, counts: Optional[torch.Tensor] = None,
+                ctx: Optional[Context] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The greedy walk through drafted tokens (lbk_tree_accept): tokens, parents, best (the argmax of every node's logits) int32 [b, t].
+    Returns (path [b, t]: the accepted nodes, then -1; how many of them [b]; the token that follows the last one [b])."""
+    b, t = _tree(parents, counts)
+    for name, x in (("tokens", tokens), ("best", best)):
+        if x.dtype != torch.int32:
+            raise TypeError(f"{name} are int32")
+        if x.shape != parents.shape:
+            raise ValueError(f"{name} are [{b}, {t}], as parents")
+    ctx = ctx or default_context()
+    st = _on(ctx, tokens=tokens, parents=parents, best=best, counts=counts)
+    out = parents.new_empty(b * (t + 2))
+    path, count, after = out[:b * t].view(b, t), out[b * t:b * (t + 1)], out[b * (t + 1):]
+    at = out.data_ptr()
+    status = ctx._lib.lbk_tree_accept(ctx.handle, tokens.data_ptr(), parents.data_ptr(), best.data_ptr(), None if counts is None else counts.data_ptr(), b, t, at,
+                                      at + 4 * b * t, at + 4 * b * (t + 1), st)
+    if status:
+        _lib.check(status)
+    return path, count, after
+
+
+def kv_keep_path(k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, path: torch.Tensor, count: torch.Tensor, ctx: Optional[Context] = None) -> None:
+    """Closes the gaps that refused drafts leave (lbk_kv_keep_path): of caches [layers, b, kv_heads, cap, head_dim] the rows pos + path[j] move
+    to pos + j for j < count. path int32 [b, t] ascending. Positions are not changed (advance_pos_by)."""
+    b, t = _tree(path, count, pos)
+    layers, _, kvh, cap, hd = _caches(k, v, b, 5)
+    ctx = ctx or default_context()
+    st = _on(ctx, k=k, v=v, pos=pos, path=path, count=count)
+    status = ctx._lib.lbk_kv_keep_path(ctx.handle, k.data_ptr(), v.data_ptr(), layers, b * kvh * cap * hd, b, kvh, hd, cap, pos.data_ptr(), path.data_ptr(), count.data_ptr(), t, st)
+    if status:
+        _lib.check(status)
+
+
+def advance_pos_by(pos: torch.Tensor, count: torch.Tensor, ctx: Optional[Context] = None) -> None:
+    """pos += count, int32 [b] (lbk_advance_pos_by): the accepted nodes are committed."""
+    if pos.dtype != torch.int32 or count.dtype != torch.int32 or pos.dim() != 1 or pos.shape != count.shape:
+        raise ValueError("pos and count are int32, one number for each sequence")
+    ctx = ctx or default_context()
+    st = _on(ctx, pos=pos, count=count)
+    status = ctx._lib.lbk_advance_pos_by(ctx.handle, pos.data_ptr(), count.data_ptr(), pos.shape[0], st)
+    if status:
+        _lib.check(status)
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor      # f32 [rows, given]
+    entropy: torch.Tensor       # f32 [rows]
+    top_ids: torch.Tensor       # int32 [rows, top]
+    top_logprobs: torch.Tensor  # f32 [rows, top]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0, scale: float = 1.0, ctx: Optional[Context] = None) -> TokenLogprobs:
+    """Log softmax(scale * logits) at the given tokens, entropy and the `top` largest logits with their log probabilities
+    (lbk_token_logprobs). logits f32 or bf16 [rows, vocab], rows any distance apart; tokens int32 [rows] or [rows, given]."""
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("logits are f32 or bf16")
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError("logits are [rows, vocab]")
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < vocab:
+        raise ValueError("the values of a row lie side by side, rows do not overlap")
+    if not 0 <= top <= min(vocab, LOGPROBS_TOP):
+        raise ValueError(f"{top} alternatives of {vocab}: at most {LOGPROBS_TOP}")
+    given = 0
+    if tokens is not None:
+        if tokens.dtype != torch.int32:
+            raise TypeError("tokens are int32")
+        if tokens.dim() not in (1, 2) or tokens.shape[0] != rows:
+            raise ValueError("tokens are [rows] or [rows, given]")
+        given = 1 if tokens.dim() == 1 else tokens.shape[1]
+    ctx = ctx or default_context()
+    st = _on(ctx, tokens=tokens)
+    if not logits.is_cuda or logits.get_device() != ctx.device:
+        raise ValueError(f"logits must live on cuda:{ctx.device}")
+    # one allocation for the floats: [rows, given], [rows], [rows, top]
+    floats = torch.empty(rows * (given + 1 + top), dtype=torch.float32, device=logits.device)
+    ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
+    at = floats.data_ptr()
+    status = ctx._lib.lbk_token_logprobs(ctx.handle, 0 if logits.dtype == torch.float32 else 1, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab,
+                                         tokens.data_ptr() if given else None, given, scale, top, at, at + 4 * rows * given, ids.data_ptr(), at + 4 * rows * (given + 1), st)
+    if status:
+        _lib.check(status)
+    lp, entropy, best = floats.split([rows * given, rows, rows * top])
+    return TokenLogprobs(lp.view(rows, given), entropy, ids, best.view(rows, top))
 
 
 class DecodeStep:

@@ -1,0 +1,65 @@
+"""What the calls around drafted tokens refuse before anything is launched (no GPU needed)."""
+import pytest
+import torch
+
+
+def _i(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def _tree_args(b=2, t=3, kvh=1, cap=8, hd=128, nh=2):
+    c = lambda: torch.zeros(b, kvh, cap, hd, dtype=torch.bfloat16)  # noqa: E731
+    return dict(q=torch.zeros(b, t, nh * hd), k=torch.zeros(b, t, kvh * hd), v=torch.zeros(b, t, kvh * hd), cos=torch.zeros(cap, hd), sin=torch.zeros(cap, hd), pos=_i(b),
+                parents=_i(b, t), kcache=c(), vcache=c(), counts=_i(b))
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(parents=_i(2)), ValueError), (dict(parents=_i(2, 0)), ValueError), (dict(parents=_i(2, 129)), ValueError), (dict(parents=_i(2, 3).long()), TypeError),
+    (dict(pos=_i(1)), ValueError), (dict(pos=_i(2).long()), ValueError), (dict(counts=_i(3)), ValueError), (dict(q=torch.zeros(2, 3, 256).half()), TypeError),
+    (dict(q=torch.zeros(2, 3, 250)), ValueError), (dict(k=torch.zeros(2, 3, 256)), ValueError), (dict(kcache=torch.zeros(2, 1, 8, 128)), TypeError),
+    (dict(kcache=torch.zeros(3, 1, 8, 128, dtype=torch.bfloat16)), ValueError), (dict(cos=torch.zeros(7, 128)), ValueError), (dict(), ValueError)])
+def test_append_refuses(change, error):
+    from lemonade_burn_b200 import ops
+    with pytest.raises(error if change else (ValueError, RuntimeError)):  # without a change: the tensors are not on a GPU
+        ops.rope_kv_append_tree(**{**_tree_args(), **change})
+
+
+@pytest.mark.parametrize("args,error", [((_i(2, 3), _i(2, 4), _i(2, 4)), ValueError), ((_i(2, 4), _i(2, 4), _i(2, 4).float()), TypeError),
+                                        ((_i(2, 4), _i(8), _i(2, 4)), ValueError), ((_i(2, 200), _i(2, 200), _i(2, 200)), ValueError)])
+def test_accept_refuses(args, error):
+    from lemonade_burn_b200 import ops
+    with pytest.raises(error):
+        ops.tree_accept(*args)
+
+
+def test_keep_and_advance_refuse():
+    from lemonade_burn_b200 import ops
+    c = lambda b: torch.zeros(3, b, 1, 8, 128, dtype=torch.bfloat16)  # noqa: E731
+    for args, error in (((c(2), c(3), _i(2), _i(2, 4), _i(2)), ValueError), ((c(2), c(2), _i(2), _i(3, 4), _i(2)), ValueError), ((c(2), c(2).float(), _i(2), _i(2, 4), _i(2)), TypeError),
+                        ((c(2)[0], c(2)[0], _i(2), _i(2, 4), _i(2)), ValueError), ((c(2), c(2), _i(3), _i(2, 4), _i(2)), ValueError)):
+        with pytest.raises(error):
+            ops.kv_keep_path(*args)
+    with pytest.raises(ValueError):
+        ops.advance_pos_by(_i(2), _i(3))
+
+
+@pytest.mark.parametrize("logits,tokens,top", [
+    (torch.zeros(3, 5, dtype=torch.float64), None, 1), (torch.zeros(3), None, 1), (torch.zeros(3, 0), None, 0), (torch.zeros(3, 5), None, 6), (torch.zeros(3, 50), None, 33),
+    (torch.zeros(3, 5), None, -1), (torch.zeros(3, 5), _i(2), 1), (torch.zeros(3, 5), _i(3).long(), 1), (torch.zeros(5, 3).T, None, 1),
+    (torch.zeros(5).expand(3, 5), None, 1)])
+def test_logprobs_refuse(logits, tokens, top):
+    from lemonade_burn_b200 import ops
+    with pytest.raises((TypeError, ValueError)):
+        ops.token_logprobs(logits, tokens, top)
+
+
+def test_calls_without_a_context_return_a_status():
+    from lemonade_burn_b200 import _lib, build
+    build.build()
+    lib = _lib.load()
+    assert lib.lbk_rope_kv_append_tree(*[None] * 9, 1, 1, 1, 1, 128, 8, None, None, None) == 1
+    assert lib.lbk_tree_accept(*[None] * 5, 1, 1, None, None, None, None) == 1
+    assert lib.lbk_kv_keep_path(None, None, None, 1, 1024, 1, 1, 128, 8, None, None, None, 1, None) == 1
+    assert lib.lbk_advance_pos_by(None, None, None, 1, None) == 1
+    assert lib.lbk_token_logprobs(None, 0, None, 5, 1, 5, None, 0, 1.0, 0, None, None, None, None, None) == 1
+    assert b"context" in lib.lbk_last_error()

@@ -557,6 +557,10 @@ int lbk_moe_route(lbk_ctx *ctx, const float *z_dev, size_t z_pitch, size_t n, si
 int lbk_rope_kv_append_tree(lbk_ctx *ctx, float *q_dev, const float *k_dev, const float *v_dev, const float *cos_dev, const float *sin_dev,
                             const int32_t *pos_dev, const int32_t *parents_dev, const int32_t *counts_dev, size_t b, size_t t, size_t n_heads,
                             size_t kv_heads, size_t head_dim, size_t cap, uint16_t *kcache_dev, uint16_t *vcache_dev, void *stream);
+size_t lbk_attn_tree_scratch(const lbk_ctx *ctx, size_t t, size_t n_heads, size_t kv_heads);
+int lbk_attn_tree(lbk_ctx *ctx, int compute, const void *q_dev, size_t q_pitch, const uint16_t *kcache_dev, const uint16_t *vcache_dev,
+                  const int32_t *pos_dev, const int32_t *parents_dev, const int32_t *counts_dev, size_t b, size_t t, size_t n_heads, size_t kv_heads,
+                  size_t head_dim, size_t cap, float scale, float *scratch_dev, void *out_dev, size_t out_pitch, void *stream);
 int lbk_tree_accept(lbk_ctx *ctx, const int32_t *tokens_dev, const int32_t *parents_dev, const int32_t *best_dev, const int32_t *counts_dev, size_t b,
                     size_t t, int32_t *path_dev, int32_t *count_out_dev, int32_t *next_dev, void *stream);
 int lbk_kv_keep_path(lbk_ctx *ctx, uint16_t *kcache_dev, uint16_t *vcache_dev, size_t layers, size_t layer_elems, size_t b, size_t kv_heads,

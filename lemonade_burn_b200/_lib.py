@@ -123,6 +123,8 @@ SYMBOLS = [
     ("lbk_moe_route_ints", _sz, [_sz, _sz, _sz]),
     ("lbk_moe_route", _i, [_vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp]),
     ("lbk_rope_kv_append_tree", _i, [_vp] * 9 + [_sz] * 6 + [_vp] * 3),
+    ("lbk_attn_tree_scratch", _sz, [_vp, _sz, _sz, _sz]),
+    ("lbk_attn_tree", _i, [_vp, _i, _vp, _sz] + [_vp] * 5 + [_sz] * 6 + [_f, _vp, _vp, _sz, _vp]),
     ("lbk_tree_accept", _i, [_vp] * 5 + [_sz, _sz] + [_vp] * 4),
     ("lbk_kv_keep_path", _i, [_vp, _vp, _vp] + [_sz] * 6 + [_vp] * 3 + [_sz, _vp]),
     ("lbk_advance_pos_by", _i, [_vp, _vp, _vp, _sz, _vp]),

@@ -1,0 +1,584 @@
+// Attention of drafted tokens: the nodes of a tree over the committed rows of their sequence and their own ancestors.
+//
+//   o_i = sum_j p_ij V_j,  p_i = softmax_j(scale * q_i . K_j),  j < pos and j = pos + n for n = i and the ancestors of i
+//
+// The query heads that share a KV head and the nodes of a sequence are the rows of one problem (row = node * group + head of the group), so that
+// the cache is read once for all of them. A problem's rows are cut into tiles, its keys into blocks; the (problem, tile, block) units of the whole batch stand in one
+// line that is cut evenly among the CTAs, whatever the sequences' lengths (cut_line): a CTA takes neighbouring blocks of a tile, then of the
+// next. A tile whose blocks went to one CTA is written out by it; of the others each CTA leaves the unnormalised sum, the maximum
+// and the weight of its part in the scratch, and attn_tree_merge_kernel joins them.
+//
+// f32 queries and probabilities are two bf16 terms each, hi + lo (|error| <= 2^-17 |x|): with f32 sums that leaves the bf16 of the cache
+// as the only rounding that shows, as in the decode and prompt kernels. bf16 queries are exact in one term; their results are
+// rounded to bf16, 2^-8 of themselves at most, and so is a probability, whose roundings are of either sign and average out over the keys.
+//
+// Rows of V that nobody has written may hold anything, and 0 * NaN is NaN: values past the sequence's last node are taken as zeros. Values of OTHER
+// branches may be infinite or NaN too; a row that does not see them must not notice. So in the blocks of the nodes values that are no numbers are
+// taken as zeros as well, and added at the end to the rows that see them (a weight is never zero in exact arithmetic).
+#include "lbk_dense_dev.cuh"
+#include "lbk_tree.cuh"
+
+namespace lbk {
+
+namespace {
+
+using dense::bf16_pair;
+
+constexpr int kHd = 128;
+constexpr int kMaxSeqs = 256;
+constexpr uint32_t kWaitLimit = 1u << 22;
+constexpr float kNoMax = -3.0e38f;  // a row that has seen nothing: finite, so that -inf scores less it are no NaN
+
+struct TreeParams {
+    CUtensorMap k, v;   // bytes [cache rows][256], box [128 bytes][64 rows], SWIZZLE_128B
+    const void *q;
+    void *out;
+    long q_pitch, out_pitch;
+    const uint16_t *vcache;
+    const int *pos, *parents, *counts;
+    int b, t, nh, kvh, cap;
+    float scale;        // log2(e) * scale: scores in units of log 2
+    float *part;        // [CTA][2][tile rows][128]
+    float2 *part_ml;    // [CTA][2][tile rows]: maximum, weight
+    int workers;        // CTAs of the attention kernel
+    int *err_word;
+};
+
+__device__ __forceinline__ float ex2(float x) {  // 2^x, the hardware's approximation
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// x = hi + lo with hi = bf16(x), lo = bf16(x - hi), for two values at once
+__device__ __forceinline__ void split_pair(float x0, float x1, uint32_t &hi, uint32_t &lo) {
+    hi = bf16_pair(x0, x1);
+    lo = bf16_pair(x0 - __uint_as_float(hi << 16), x1 - __uint_as_float(hi & 0xffff0000u));
+}
+
+// ---- the line of units ----------------------------------------------------------------------------
+struct Line {
+    int first[kMaxSeqs + 1];   // units in front of a sequence; [b] is all of them
+    int pos[kMaxSeqs], count[kMaxSeqs];
+};
+// A sequence: kv_heads * tiles problems of `blocks` units each.
+__device__ __forceinline__ int line_blocks(const Line &l, int seq, int block_keys) { return (l.pos[seq] + l.count[seq] + block_keys - 1) / block_keys; }
+__device__ __forceinline__ int line_tiles(const Line &l, int seq, int group, int rows) { return (l.count[seq] * group + rows - 1) / rows; }
+
+// Fills the line; a sequence outside its cache has no units. All threads of the block.
+template <int ROWS, int KEYS>
+__device__ void cut_line(const TreeParams &p, Line &l) {
+    const int group = p.nh / p.kvh;
+    for (int i = threadIdx.x; i < p.b; i += blockDim.x) {
+        const int pos = p.pos[i], count = tree_count(p.counts, i, p.t);
+        const bool fits = pos >= 0 && pos <= p.cap - count;
+        if (!fits && blockIdx.x == 0) atomicExch(p.err_word, kErrPos);
+        l.pos[i] = pos;
+        l.count[i] = fits ? count : 0;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        int before = 0;
+        for (int i0 = 0; i0 < p.b; i0 += 32) {
+            const int i = i0 + threadIdx.x;
+            const int mine = i < p.b && l.count[i] ? line_blocks(l, i, KEYS) * line_tiles(l, i, group, ROWS) * p.kvh : 0;
+            int sum = mine;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, sum, o);
+                if (static_cast<int>(threadIdx.x) >= o) sum += up;
+            }
+            if (i < p.b) l.first[i] = before + sum - mine;
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (threadIdx.x == 0) l.first[p.b] = before;
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ int share_begin(int units, int worker, int workers) { return static_cast<int>(static_cast<long long>(units) * worker / workers); }
+
+struct Segment {
+    int seq, kh, tile;     // the problem
+    int begin, end;        // its blocks
+    int blocks;            // of all there are
+};
+__device__ __forceinline__ Segment segment_at(const TreeParams &p, const Line &l, int unit, int last, int rows, int keys) {
+    Segment s;
+    int lo = 0, hi = p.b - 1;   // the last sequence whose units begin at or before this one and that has any
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (l.first[mid] <= unit) lo = mid;
+        else hi = mid - 1;
+    }
+    s.seq = lo;
+    s.blocks = line_blocks(l, lo, keys);
+    const int tiles = line_tiles(l, lo, p.nh / p.kvh, rows), at = unit - l.first[lo], problem = at / s.blocks;
+    s.begin = at - problem * s.blocks;
+    s.end = min(s.blocks, s.begin + last - unit);
+    s.kh = problem / tiles;
+    s.tile = problem - s.kh * tiles;
+    return s;
+}
+
+// Who sees whom: bit n of mask[i]. A parent that is none counts as -1.
+__device__ __forceinline__ void tree_masks(const int *parent, ulonglong2 *mask, int i) {
+    unsigned long long lo = 0, hi = 0;
+    for (int n = i; n >= 0; n = parent[n]) {
+        if (n < 64) lo |= 1ull << n;
+        else hi |= 1ull << (n - 64);
+    }
+    mask[i] = make_ulonglong2(lo, hi);
+}
+__device__ __forceinline__ bool sees(const ulonglong2 &m, int n) { return ((n < 64 ? m.x : m.y) >> (n & 63)) & 1; }
+
+// ---- few rows: mma.sync, 16 rows a warp ---------------------------------------------------------------
+// Tiles of ROWS = 16 or 32 rows (up to 16 or 32 products of nodes and heads of a group). Every key is 512 bytes from HBM, 22 cycles of an SM at the
+// full rate, and 4 to 8 cycles of mma.sync work for 16 rows in two terms: the stream is the bound, and the 128 rows
+// of a tcgen05 tile would be padding. Four warps take 16 keys each of a block of 64 for 16 rows; a fifth (ninth) fetches blocks by TMA, kStages deep.
+template <int RG>
+struct Few {
+    static constexpr int kRows = 16 * RG, kWarps = 4 * RG, kThreads = (kWarps + 1) * 32, kKeys = 64;
+    static constexpr int kHalf = kKeys * 128, kStage = 4 * kHalf, kStages = RG == 1 ? 6 : 5;
+    static constexpr int kQPitch = 272;                               // bytes: eight rows start in eight different bank groups
+    static constexpr int kQ0 = kStages * kStage, kQBytes = 2 * kRows * kQPitch;
+    static constexpr int kMergePitch = 132;                           // floats
+    static constexpr int kMerge0 = kQ0 + kQBytes, kMergeBytes = 2 * kRows * kMergePitch * 4;
+    static constexpr int kBars = kMerge0 + kMergeBytes, kSmem = kBars + 2 * kStages * 8 + 1024;
+};
+struct FewShared {
+    Line line;
+    int parent[kTreeNodes];
+    ulonglong2 mask[kTreeNodes];
+    int abort, odd;
+};
+
+template <int TERMS, int RG>
+__global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(const __grid_constant__ TreeParams p) {
+    using F = Few<RG>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ FewShared sh;
+    const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t *sm = smem_raw + (base - raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto full = [&](int s) { return base + F::kBars + s * 8; };
+    auto empty = [&](int s) { return base + F::kBars + (F::kStages + s) * 8; };
+    volatile int *abort = &sh.abort;
+    if (tid == 0) {
+        for (int s = 0; s < F::kStages; ++s) {
+            ptx::mbar_init(full(s), 1);
+            ptx::mbar_init(empty(s), F::kWarps);
+        }
+        sh.abort = sh.odd = 0;
+        ptx::fence_barrier_init();
+    }
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    cut_line<F::kRows, F::kKeys>(p, sh.line);
+    const int units = sh.line.first[p.b], u0 = share_begin(units, blockIdx.x, p.workers), u1 = share_begin(units, blockIdx.x + 1, p.workers);
+    if (u0 == u1) return;
+    const int group = p.nh / p.kvh;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        for (uint32_t i = 0; i < kWaitLimit; ++i) {
+            if (ptx::mbar_try_wait(bar, parity)) return true;
+            if (*abort) return false;
+        }
+        *abort = 1;
+        return false;
+    };
+
+    if (warp == F::kWarps) {
+        // ================= TMA producer =================
+        if (lane != 0) return;
+        int stage = 0, round = 0, sent = 0;
+        bool ok = true;
+        for (int u = u0; u < u1 && ok;) {
+            const Segment s = segment_at(p, sh.line, u, u1, F::kRows, F::kKeys);
+            const int row0 = (s.seq * p.kvh + s.kh) * p.cap;
+            for (int j = s.begin; j < s.end; ++j, ++sent) {
+                if (round > 0 && !wait(empty(stage), (round - 1) & 1)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t at = base + stage * F::kStage;
+                ptx::mbar_arrive_expect_tx(full(stage), F::kStage);
+                ptx::tma_load_2d(at, &p.k, full(stage), 0, row0 + j * F::kKeys);
+                ptx::tma_load_2d(at + F::kHalf, &p.k, full(stage), 128, row0 + j * F::kKeys);
+                ptx::tma_load_2d(at + 2 * F::kHalf, &p.v, full(stage), 0, row0 + j * F::kKeys);
+                ptx::tma_load_2d(at + 3 * F::kHalf, &p.v, full(stage), 128, row0 + j * F::kKeys);
+                if (++stage == F::kStages) {
+                    stage = 0;
+                    ++round;
+                }
+            }
+            u += s.end - s.begin;
+        }
+        if (!ok) atomicExch(p.err_word, 5);
+        // the copies in flight land before the block may go, whoever has given up
+        for (int n = max(0, sent - F::kStages); n < sent; ++n) ptx::mbar_wait(full(n % F::kStages), (n / F::kStages) & 1, kWaitLimit);
+        return;
+    }
+
+    // ================= the other warps: 16 rows, 16 keys of every block each =================
+    const int kg = warp & 3, rg = warp >> 2, g = lane >> 2, tq = lane & 3;
+    auto meet = [&]() { ptx::named_barrier(1, F::kWarps * 32); };
+    int stage = 0, phase = 0;
+    bool ok = true;
+    for (int u = u0; u < u1;) {
+        const Segment s = segment_at(p, sh.line, u, u1, F::kRows, F::kKeys);
+        const int pos = sh.line.pos[s.seq], count = sh.line.count[s.seq], written = pos + count;
+        const int rows_all = count * group, row0 = s.tile * F::kRows;
+        const bool nodes = s.end * F::kKeys > pos;  // some of these blocks hold nodes
+        if (nodes)
+            for (int i = tid; i < count; i += F::kWarps * 32) {
+                const int up = p.parents[static_cast<size_t>(s.seq) * p.t + i];
+                const bool good = up >= -1 && up < i;
+                if (!good) atomicExch(p.err_word, kErrTree);
+                sh.parent[i] = good ? up : -1;
+            }
+        // the tile's queries, a row as one load of a warp
+        for (int r = warp; r < F::kRows; r += F::kWarps) {
+            const int row = row0 + r, node = row / group;
+            uint8_t *dst = sm + F::kQ0 + r * F::kQPitch + lane * 8;
+            uint2 hi = make_uint2(0u, 0u), lo = hi;
+            if (row < rows_all) {
+                const size_t at = (static_cast<size_t>(s.seq) * p.t + node) * p.q_pitch + static_cast<size_t>(s.kh * group + row - node * group) * kHd + lane * 4;
+                if (TERMS == 2) {
+                    const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + at);
+                    split_pair(a.x, a.y, hi.x, lo.x);
+                    split_pair(a.z, a.w, hi.y, lo.y);
+                } else {
+                    hi = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p.q) + at);
+                }
+            }
+            *reinterpret_cast<uint2 *>(dst) = hi;
+            if (TERMS == 2) *reinterpret_cast<uint2 *>(dst + F::kRows * F::kQPitch) = lo;
+        }
+        meet();
+        if (nodes)
+            for (int i = tid; i < count; i += F::kWarps * 32) tree_masks(sh.parent, sh.mask, i);
+        uint32_t qf[TERMS][8][4];  // 16 rows x 16 dimensions each
+        {
+            const uint32_t at = base + F::kQ0 + (rg * 16 + (lane & 15)) * F::kQPitch + (lane >> 4) * 16;
+#pragma unroll
+            for (int x = 0; x < TERMS; ++x)
+#pragma unroll
+                for (int d = 0; d < 8; ++d) ptx::ldmatrix_x4(qf[x][d], at + x * F::kRows * F::kQPitch + d * 32);
+        }
+        if (nodes) meet();
+        float o[16][4], m[2] = {kNoMax, kNoMax}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int d = 0; d < 16; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
+        bool odd = false;  // a value of some node is no number
+        for (int j = s.begin; j < s.end; ++j) {
+            if (ok) ok = __all_sync(0xffffffffu, wait(full(stage), phase));
+            if (ok) {
+                const uint32_t ks = base + stage * F::kStage, vs = ks + 2 * F::kHalf;
+                const int key0 = j * F::kKeys + kg * 16;
+                const bool edge = key0 + 16 > pos;
+                // scores: keys 0..7 and 8..15 of the warp's, each term in a sum of its own
+                float sc[2][TERMS][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int x = 0; x < TERMS; ++x) sc[h][x][0] = sc[h][x][1] = sc[h][x][2] = sc[h][x][3] = 0.0f;
+#pragma unroll
+                for (int d2 = 0; d2 < 4; ++d2)  // 32 dimensions at a time
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int key = kg * 16 + h * 8 + (lane & 7), unit = (d2 & 1) * 4 + (lane >> 3);
+                        uint32_t kb[4];
+                        ptx::ldmatrix_x4(kb, ks + (d2 >> 1) * F::kHalf + key * 128 + ((unit ^ (key & 7)) << 4));
+#pragma unroll
+                        for (int x = 0; x < TERMS; ++x) {
+                            ptx::mma_bf16(sc[h][x], qf[x][2 * d2], kb[0], kb[1]);
+                            ptx::mma_bf16(sc[h][x], qf[x][2 * d2 + 1], kb[2], kb[3]);
+                        }
+                    }
+                float sv[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sv[h][e] = (TERMS == 2 ? sc[h][0][e] + sc[h][TERMS - 1][e] : sc[h][0][e]) * p.scale;
+                if (edge) {
+                    const int ra = row0 + rg * 16 + g, rb = ra + 8;
+                    const ulonglong2 none = make_ulonglong2(0ull, 0ull), ma = ra < rows_all ? sh.mask[ra / group] : none, mb = rb < rows_all ? sh.mask[rb / group] : none;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = key0 + h * 8 + tq * 2 + (e & 1), n = key - pos;
+                            if (n >= 0 && (n >= count || !sees(e < 2 ? ma : mb, n))) sv[h][e] = -INFINITY;
+                        }
+                }
+                uint32_t ph[4], pl[4];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {  // rows g and g + 8
+                    const int e = half * 2;
+                    float mx = fmaxf(fmaxf(sv[0][e], sv[0][e + 1]), fmaxf(sv[1][e], sv[1][e + 1]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    const float nm = fmaxf(m[half], mx), corr = ex2(m[half] - nm);
+                    m[half] = nm;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float e0 = ex2(sv[h][e] - nm), e1 = ex2(sv[h][e + 1] - nm);
+                        sum += e0 + e1;
+                        if (TERMS == 2) split_pair(e0, e1, ph[2 * h + half], pl[2 * h + half]);
+                        else ph[2 * h + half] = bf16_pair(e0, e1);
+                    }
+                    l[half] = l[half] * corr + sum;
+#pragma unroll
+                    for (int d = 0; d < 16; ++d) {
+                        o[d][e] *= corr;
+                        o[d][e + 1] *= corr;
+                    }
+                }
+                const int key = kg * 16 + (lane & 15);
+#pragma unroll
+                for (int d2 = 0; d2 < 8; ++d2) {  // 16 dimensions at a time
+                    const int unit = (d2 & 3) * 2 + (lane >> 4);
+                    uint32_t vb[4];
+                    ptx::ldmatrix_x4_trans(vb, vs + (d2 >> 2) * F::kHalf + key * 128 + ((unit ^ (key & 7)) << 4));
+                    if (edge) {  // a register: two keys of one dimension
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int n = key0 + (r & 1) * 8 + tq * 2 + e - pos;
+                                const bool strange = n >= 0 && ((vb[r] >> (16 * e)) & 0x7f80u) == 0x7f80u;
+                                if (strange && n < count) odd = true;
+                                if (strange || n >= count) vb[r] &= e ? 0x0000ffffu : 0xffff0000u;
+                            }
+                    }
+                    ptx::mma_bf16(o[2 * d2], ph, vb[0], vb[1]);
+                    ptx::mma_bf16(o[2 * d2 + 1], ph, vb[2], vb[3]);
+                    if (TERMS == 2) {
+                        ptx::mma_bf16(o[2 * d2], pl, vb[0], vb[1]);
+                        ptx::mma_bf16(o[2 * d2 + 1], pl, vb[2], vb[3]);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(empty(stage));
+            }
+            if (++stage == F::kStages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+        if (odd) sh.odd = u + 1;  // read behind the meetings below, written again behind the next segment's first
+        // the four warps of a row meet: 2 and 3 hand over to 0 and 1, then 1 to 0
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+        }
+        float *const place = reinterpret_cast<float *>(sm + F::kMerge0);
+#pragma unroll 1
+        for (int from = 2; from >= 1; --from) {
+            const int slot = from == 2 ? kg & 1 : 0;
+            const bool gives = from == 2 ? kg >= 2 : kg == 1, takes = from == 2 ? kg < 2 : kg == 0;
+            float *ra = place + (slot * F::kRows + rg * 16 + g) * F::kMergePitch, *rb = ra + 8 * F::kMergePitch;
+            if (gives) {
+#pragma unroll
+                for (int d = 0; d < 16; ++d) {
+                    *reinterpret_cast<float2 *>(ra + d * 8 + tq * 2) = make_float2(o[d][0], o[d][1]);
+                    *reinterpret_cast<float2 *>(rb + d * 8 + tq * 2) = make_float2(o[d][2], o[d][3]);
+                }
+                if (tq == 0) {
+                    *reinterpret_cast<float2 *>(ra + kHd) = make_float2(m[0], l[0]);
+                    *reinterpret_cast<float2 *>(rb + kHd) = make_float2(m[1], l[1]);
+                }
+            }
+            meet();
+            if (takes) {
+                const float2 xa = *reinterpret_cast<const float2 *>(ra + kHd), xb = *reinterpret_cast<const float2 *>(rb + kHd);
+                const float na = fmaxf(m[0], xa.x), nb = fmaxf(m[1], xb.x);
+                const float wa = ex2(m[0] - na), wb = ex2(m[1] - nb), va = ex2(xa.x - na), vb = ex2(xb.x - nb);
+                m[0] = na;
+                m[1] = nb;
+                l[0] = l[0] * wa + xa.y * va;
+                l[1] = l[1] * wb + xb.y * vb;
+#pragma unroll
+                for (int d = 0; d < 16; ++d) {
+                    const float2 ya = *reinterpret_cast<const float2 *>(ra + d * 8 + tq * 2), yb = *reinterpret_cast<const float2 *>(rb + d * 8 + tq * 2);
+                    o[d][0] = o[d][0] * wa + ya.x * va;
+                    o[d][1] = o[d][1] * wa + ya.y * va;
+                    o[d][2] = o[d][2] * wb + yb.x * vb;
+                    o[d][3] = o[d][3] * wb + yb.y * vb;
+                }
+            }
+            meet();
+        }
+        if (kg == 0) {
+            const bool fix = nodes && sh.odd == u + 1, whole = s.begin == 0 && s.end == s.blocks;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = rg * 16 + half * 8 + g, row = row0 + r, node = row / group;
+                if (row >= rows_all) continue;
+                if (fix) {  // what this row sees that is no number
+                    const ulonglong2 mine = sh.mask[node];
+                    for (int n = max(0, s.begin * F::kKeys - pos); n < min(count, s.end * F::kKeys - pos); ++n) {
+                        if (!sees(mine, n)) continue;
+                        const uint16_t *v = p.vcache + (static_cast<size_t>(s.seq * p.kvh + s.kh) * p.cap + pos + n) * kHd + tq * 2;
+#pragma unroll
+                        for (int d = 0; d < 16; ++d)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                if ((v[d * 8 + e] & 0x7f80u) == 0x7f80u) o[d][half * 2 + e] += dense::bf16_f32(v[d * 8 + e]);
+                    }
+                }
+                if (whole) {
+                    const float inv = 1.0f / l[half];
+                    const size_t at = (static_cast<size_t>(s.seq) * p.t + node) * p.out_pitch + static_cast<size_t>(s.kh * group + row - node * group) * kHd + tq * 2;
+#pragma unroll
+                    for (int d = 0; d < 16; ++d) {
+                        const float x = o[d][half * 2] * inv, y = o[d][half * 2 + 1] * inv;
+                        if (TERMS == 2) *reinterpret_cast<float2 *>(static_cast<float *>(p.out) + at + d * 8) = make_float2(x, y);
+                        else *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + at + d * 8) = bf16_pair(x, y);
+                    }
+                } else {
+                    const size_t at = (static_cast<size_t>(blockIdx.x) * 2 + (u == u0 ? 0 : 1)) * F::kRows + r;
+#pragma unroll
+                    for (int d = 0; d < 16; ++d) *reinterpret_cast<float2 *>(p.part + at * kHd + d * 8 + tq * 2) = make_float2(o[d][half * 2], o[d][half * 2 + 1]);
+                    if (tq == 0) p.part_ml[at] = make_float2(m[half], l[half]);
+                }
+            }
+        }
+        u += s.end - s.begin;
+    }
+    if (!ok && lane == 0) atomicExch(p.err_word, 5);
+}
+
+// Joins the parts of the tiles that were cut: a warp a row, four dimensions a lane.
+template <int TERMS, int ROWS, int KEYS>
+__global__ void __launch_bounds__(256) attn_tree_merge_kernel(const __grid_constant__ TreeParams p) {
+    __shared__ Line line;
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    cut_line<ROWS, KEYS>(p, line);
+    const int group = p.nh / p.kvh, tiles_most = (p.t * group + ROWS - 1) / ROWS, lane = threadIdx.x & 31;
+    const int seq = blockIdx.x / (p.kvh * tiles_most), rest = blockIdx.x - seq * p.kvh * tiles_most, kh = rest / tiles_most, tile = rest - kh * tiles_most;
+    const int r = blockIdx.y * 8 + (threadIdx.x >> 5), row = tile * ROWS + r, node = row / group;
+    if (row >= line.count[seq] * group) return;
+    const int units = line.first[p.b], blocks = line_blocks(line, seq, KEYS);
+    const int begin = line.first[seq] + (kh * line_tiles(line, seq, group, ROWS) + tile) * blocks;
+    auto owner = [&](int u) { return static_cast<int>((static_cast<long long>(u + 1) * p.workers - 1) / units); };
+    const int c0 = owner(begin), c1 = owner(begin + blocks - 1);
+    if (c0 == c1) return;  // written by its worker
+    auto place = [&](int c) { return (static_cast<size_t>(c) * 2 + (c == c0 && share_begin(units, c, p.workers) < begin ? 1 : 0)) * ROWS + r; };
+    auto part_of = [&](int c) {  // maximum and weight; a worker without a share left nothing
+        const bool any = c <= c1 && share_begin(units, c, p.workers) < share_begin(units, c + 1, p.workers);
+        return any ? p.part_ml[place(c)] : make_float2(kNoMax, 0.0f);
+    };
+    float m = kNoMax;
+    for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, part_of(c).x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.0f;
+    for (int base = c0; base <= c1; base += 32) {
+        const float2 ml = part_of(base + lane);
+        const float w = ex2(ml.x - m);
+        const bool any = base + lane <= c1 && share_begin(units, base + lane, p.workers) < share_begin(units, base + lane + 1, p.workers);
+        const unsigned some = __ballot_sync(0xffffffffu, any);
+        l += any ? ml.y * w : 0.0f;
+#pragma unroll 4
+        for (int i = 0; i < min(32, c1 - base + 1); ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            if (!(some >> i & 1)) continue;
+            const float4 x = *reinterpret_cast<const float4 *>(p.part + place(base + i) * kHd + lane * 4);
+            sum.x += x.x * wi;
+            sum.y += x.y * wi;
+            sum.z += x.z * wi;
+            sum.w += x.w * wi;
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    const float inv = 1.0f / l;
+    const size_t at = (static_cast<size_t>(seq) * p.t + node) * p.out_pitch + static_cast<size_t>(kh * group + row - node * group) * kHd + lane * 4;
+    if (TERMS == 2) dense::put4(static_cast<float *>(p.out) + at, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+    else dense::put4(static_cast<uint16_t *>(p.out) + at, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+}
+
+int attn_tree_init(Ctx *ctx) {
+    struct { void (*k)(TreeParams); int smem; } few[] = {{attn_tree_few_kernel<1, 1>, Few<1>::kSmem}, {attn_tree_few_kernel<2, 1>, Few<1>::kSmem},
+                                                         {attn_tree_few_kernel<1, 2>, Few<2>::kSmem}, {attn_tree_few_kernel<2, 2>, Few<2>::kSmem}};
+    for (auto &f : few) {
+        LBK_CUDA(cudaFuncSetAttribute(f.k, cudaFuncAttributeMaxDynamicSharedMemorySize, f.smem));
+    }
+    return LBK_OK;
+}
+const InitHook kInitAttnTree(attn_tree_init);
+
+// Rows of a tile for t nodes of `group` heads.
+int tile_rows(size_t t, size_t group) { return t * group <= 16 ? 16 : 32; }
+
+template <int ROWS, int KEYS>
+int launch_tree(Ctx *ctx, int terms, TreeParams &p, void (*one)(TreeParams), void (*two)(TreeParams), int threads, int smem, cudaStream_t st) {
+    const int group = p.nh / p.kvh, tiles = (p.t * group + ROWS - 1) / ROWS;
+    LBK_CUDA(launch_chained(terms == 2 ? two : one, dim3(static_cast<unsigned>(p.workers)), dim3(threads), static_cast<size_t>(smem), st, p));
+    ctx->launches++;
+    LBK_CUDA(launch_chained(terms == 2 ? attn_tree_merge_kernel<2, ROWS, KEYS> : attn_tree_merge_kernel<1, ROWS, KEYS>, dim3(static_cast<unsigned>(p.b * p.kvh * tiles), ROWS / 8), dim3(256), 0, st,
+                            p));
+    ctx->launches++;
+    return LBK_OK;
+}
+
+}  // namespace
+}  // namespace lbk
+
+using namespace lbk;
+
+extern "C" {
+
+size_t lbk_attn_tree_scratch(const lbk_ctx *c, size_t t, size_t n_heads, size_t kv_heads) {
+    if (!c || !kv_heads) return 0;
+    return static_cast<size_t>(reinterpret_cast<const Ctx *>(c)->sm_count) * 2 * tile_rows(t, n_heads / kv_heads) * (kHd + 2);
+}
+
+int lbk_attn_tree(lbk_ctx *c, int compute, const void *q_dev, size_t q_pitch, const uint16_t *kcache_dev, const uint16_t *vcache_dev, const int32_t *pos_dev,
+                  const int32_t *parents_dev, const int32_t *counts_dev, size_t b, size_t t, size_t n_heads, size_t kv_heads, size_t head_dim, size_t cap, float scale,
+                  float *scratch_dev, void *out_dev, size_t out_pitch, void *stream) {
+    LBK_TREE_PRE("lbk_attn_tree");
+    if (b == 0 || t == 0) return LBK_OK;
+    if (!q_dev || !kcache_dev || !vcache_dev || !pos_dev || !parents_dev || !scratch_dev || !out_dev) return fail(LBK_ERR_INVALID, "lbk_attn_tree: null buffer");
+    if (compute != LBK_COMPUTE_BF16 && compute != LBK_COMPUTE_F32) return fail(LBK_ERR_INVALID, "lbk_attn_tree: unknown compute type %d", compute);
+    if (t > LBK_TREE_NODES || b > kMaxSeqs) return fail(LBK_ERR_UNSUPPORTED, "lbk_attn_tree: at most %d nodes of %d sequences (got %zu of %zu)", LBK_TREE_NODES, kMaxSeqs, t, b);
+    if (head_dim != kHd || !kv_heads || !n_heads || n_heads % kv_heads) return fail(LBK_ERR_SHAPE, "lbk_attn_tree: heads of %d, a multiple of the KV heads", kHd);
+    if (!(scale > 0.0f) || scale > 1e30f) return fail(LBK_ERR_INVALID, "lbk_attn_tree: the scale is a positive number");
+    const size_t unit = compute == LBK_COMPUTE_F32 ? 4 : 8, width = n_heads * kHd;
+    if (q_pitch < width || out_pitch < width || q_pitch % unit || out_pitch % unit) return fail(LBK_ERR_SHAPE, "lbk_attn_tree: rows of %zu values, pitches of %zu and %zu", width, q_pitch, out_pitch);
+    if ((reinterpret_cast<uintptr_t>(q_dev) | reinterpret_cast<uintptr_t>(kcache_dev) | reinterpret_cast<uintptr_t>(vcache_dev) | reinterpret_cast<uintptr_t>(scratch_dev) |
+         reinterpret_cast<uintptr_t>(out_dev)) & 15)
+        return fail(LBK_ERR_SHAPE, "lbk_attn_tree: buffers lie on 16 bytes");
+    if (n_heads > 65536 || cap > (1u << 30)) return fail(LBK_ERR_UNSUPPORTED, "lbk_attn_tree: %zu heads, %zu positions", n_heads, cap);
+    const size_t rows = b * kv_heads * cap, group = n_heads / kv_heads;
+    if (rows > INT32_MAX || b * kv_heads * ((t * group + 15) / 16) * (cap / 64 + 1) > INT32_MAX)
+        return fail(LBK_ERR_UNSUPPORTED, "lbk_attn_tree: a cache of %zu rows", rows);
+    TreeParams p{};
+    p.q = q_dev;
+    p.out = out_dev;
+    p.q_pitch = static_cast<long>(q_pitch);
+    p.out_pitch = static_cast<long>(out_pitch);
+    p.vcache = vcache_dev;
+    p.pos = pos_dev;
+    p.parents = parents_dev;
+    p.counts = counts_dev;
+    p.b = static_cast<int>(b);
+    p.t = static_cast<int>(t);
+    p.nh = static_cast<int>(n_heads);
+    p.kvh = static_cast<int>(kv_heads);
+    p.cap = static_cast<int>(cap);
+    p.scale = scale * 1.4426950408889634f;
+    p.workers = ctx->sm_count;
+    p.err_word = ctx->err_word;
+    const int tile = tile_rows(t, group), terms = compute == LBK_COMPUTE_F32 ? 2 : 1;
+    p.part = scratch_dev;
+    p.part_ml = reinterpret_cast<float2 *>(scratch_dev + static_cast<size_t>(p.workers) * 2 * tile * kHd);
+    LBK_TRY(encode_bytes_map(&p.k, kcache_dev, 256, rows, 256, 128, 64));
+    LBK_TRY(encode_bytes_map(&p.v, vcache_dev, 256, rows, 256, 128, 64));
+    if (tile == 16) return launch_tree<16, 64>(ctx, terms, p, attn_tree_few_kernel<1, 1>, attn_tree_few_kernel<2, 1>, Few<1>::kThreads, Few<1>::kSmem, st);
+    return launch_tree<32, 64>(ctx, terms, p, attn_tree_few_kernel<1, 2>, attn_tree_few_kernel<2, 2>, Few<2>::kThreads, Few<2>::kSmem, st);
+}
+
+}  // extern "C"

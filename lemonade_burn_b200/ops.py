@@ -227,6 +227,45 @@ def rope_kv_append_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: 
         _lib.check(status)
 
 
+def attn_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, pos: torch.Tensor, parents: torch.Tensor, counts: Optional[torch.Tensor] = None,
+              scale: Optional[float] = None, out: Optional[torch.Tensor] = None, ctx: Optional[Context] = None) -> torch.Tensor:
+    """Attention of drafted tokens (lbk_attn_tree): q [b, t, heads, 128] f32 or bf16 (nodes any distance apart) over rows 0 .. pos - 1 of kcache
+    and vcache [b, kv_heads, cap, 128] and over the node itself and its ancestors, whose rows are pos + node. scale: 128 ** -0.5. Returns
+    `out` (made like q without one: rows of places not in use are then whatever was there)."""
+    b, t = _tree(parents, counts, pos)
+    _, kvh, cap, hd = _caches(kcache, vcache, b, 4)
+    if q.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("queries are f32 or bf16")
+    if q.dim() != 4 or q.shape[:2] != (b, t) or q.shape[3] != hd:
+        raise ValueError(f"queries are [{b}, {t}, heads, {hd}]")
+    nh = q.shape[2]
+    if hd != 128 or not nh or not kvh or nh % kvh:
+        raise ValueError(f"heads of 128, a multiple of the KV heads (got {nh} and {kvh} heads of {hd})")
+    if out is None:
+        out = q.new_empty((b, t, nh, hd))
+    elif out.dtype != q.dtype or out.shape != q.shape:
+        raise ValueError("out is like q")
+    pitches = []
+    for x in (q, out):
+        row, seq = (x.stride(1) if t > 1 else nh * hd), x.stride(0)
+        if x.stride(3) != 1 or (nh > 1 and x.stride(2) != hd) or (b > 1 and t > 1 and seq != t * row) or row < nh * hd:
+            raise ValueError("the heads of a node lie side by side, nodes and sequences at one distance")
+        pitches.append(seq if b > 1 and t == 1 else row)
+    ctx = ctx or default_context()
+    st = _on(ctx, kcache=kcache, vcache=vcache, pos=pos, parents=parents, counts=counts)
+    for x in (q, out):
+        if not x.is_cuda or x.get_device() != ctx.device:
+            raise ValueError(f"queries and out must live on cuda:{ctx.device}")
+    lib = ctx._lib
+    scratch = torch.empty(lib.lbk_attn_tree_scratch(ctx.handle, t, nh, kvh), dtype=torch.float32, device=q.device)
+    status = lib.lbk_attn_tree(ctx.handle, 1 if q.dtype == torch.float32 else 0, q.data_ptr(), pitches[0], kcache.data_ptr(), vcache.data_ptr(), pos.data_ptr(), parents.data_ptr(),
+                               None if counts is None else counts.data_ptr(), b, t, nh, kvh, hd, cap, hd ** -0.5 if scale is None else scale, scratch.data_ptr(), out.data_ptr(),
+                               pitches[1], st)
+    if status:
+        _lib.check(status)
+    return out
+
+
 def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, best: torch.Tensor, counts: Optional[torch.Tensor] = None,
                 ctx: Optional[Context] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The greedy walk through drafted tokens (lbk_tree_accept): tokens, parents, best (the argmax of every node's logits) int32 [b, t].

@@ -8,9 +8,11 @@
 // next. A tile whose blocks went to one CTA is written out by it; of the others each CTA leaves the unnormalised sum, the maximum
 // and the weight of its part in the scratch, and attn_tree_merge_kernel joins them.
 //
-// f32 queries and probabilities are two bf16 terms each, hi + lo (|error| <= 2^-17 |x|): with f32 sums that leaves the bf16 of the cache
-// as the only rounding that shows, as in the decode and prompt kernels. bf16 queries are exact in one term; their results are
-// rounded to bf16, 2^-8 of themselves at most, and so is a probability, whose roundings are of either sign and average out over the keys.
+// f32 queries and probabilities are three bf16 terms each (8 bits a term: an f32 has 24), keys and values are bf16 as they are: every product is exact, and
+// what is left are f32 sums. Two terms, as in the decode and prompt kernels, are off by 2^-17 of a query or probability, which was 3 to 6 times
+// the error of plain f32 arithmetic. A tensor core cuts its sums off instead of rounding them (2e-8 of a sum for 16 keys), so the products of a block of keys start from
+// zero and are added to the row in registers, one rounded addition a block. bf16 queries are exact in one term; their results are rounded to bf16,
+// 2^-8 of themselves at most, and so is a probability, whose roundings are of either sign and average out over the keys.
 //
 // Rows of V that nobody has written may hold anything, and 0 * NaN is NaN: values past the sequence's last node are taken as zeros. Values of OTHER
 // branches may be infinite or NaN too; a row that does not see them must not notice. So in the blocks of the nodes values that are no numbers are
@@ -49,10 +51,17 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, the hardware's approxim
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// x = hi + lo with hi = bf16(x), lo = bf16(x - hi), for two values at once
-__device__ __forceinline__ void split_pair(float x0, float x1, uint32_t &hi, uint32_t &lo) {
-    hi = bf16_pair(x0, x1);
-    lo = bf16_pair(x0 - __uint_as_float(hi << 16), x1 - __uint_as_float(hi & 0xffff0000u));
+// Two values at once as bf16 terms: term[i] = bf16(x - the terms in front of it), and with three of them their sum is x
+template <int TERMS>
+__device__ __forceinline__ void split_pair(float x0, float x1, uint32_t (&term)[TERMS]) {
+#pragma unroll
+    for (int i = 0; i < TERMS; ++i) {
+        term[i] = bf16_pair(x0, x1);
+        if (i + 1 < TERMS) {
+            x0 -= __uint_as_float(term[i] << 16);
+            x1 -= __uint_as_float(term[i] & 0xffff0000u);
+        }
+    }
 }
 
 // ---- the line of units ----------------------------------------------------------------------------
@@ -131,14 +140,14 @@ __device__ __forceinline__ bool sees(const ulonglong2 &m, int n) { return ((n < 
 
 // ---- few rows: mma.sync, 16 rows a warp ---------------------------------------------------------------
 // Tiles of ROWS = 16 or 32 rows (up to 16 or 32 products of nodes and heads of a group). Every key is 512 bytes from HBM, 22 cycles of an SM at the
-// full rate, and 4 to 8 cycles of mma.sync work for 16 rows in two terms: the stream is the bound, and the 128 rows
+// full rate, and some 6 cycles of mma.sync work for 16 rows in three terms: the stream is the bound, and the 128 rows
 // of a tcgen05 tile would be padding. Four warps take 16 keys each of a block of 64 for 16 rows; a fifth (ninth) fetches blocks by TMA, kStages deep.
 template <int RG>
 struct Few {
     static constexpr int kRows = 16 * RG, kWarps = 4 * RG, kThreads = (kWarps + 1) * 32, kKeys = 64;
-    static constexpr int kHalf = kKeys * 128, kStage = 4 * kHalf, kStages = RG == 1 ? 6 : 5;
+    static constexpr int kHalf = kKeys * 128, kStage = 4 * kHalf, kStages = 5;
     static constexpr int kQPitch = 272;                               // bytes: eight rows start in eight different bank groups
-    static constexpr int kQ0 = kStages * kStage, kQBytes = 2 * kRows * kQPitch;
+    static constexpr int kQ0 = kStages * kStage, kQBytes = 3 * kRows * kQPitch;
     static constexpr int kMergePitch = 132;                           // floats
     static constexpr int kMerge0 = kQ0 + kQBytes, kMergeBytes = 2 * kRows * kMergePitch * 4;
     static constexpr int kBars = kMerge0 + kMergeBytes, kSmem = kBars + 2 * kStages * 8 + 1024;
@@ -223,7 +232,7 @@ __global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(con
     bool ok = true;
     for (int u = u0; u < u1;) {
         const Segment s = segment_at(p, sh.line, u, u1, F::kRows, F::kKeys);
-        const int pos = sh.line.pos[s.seq], count = sh.line.count[s.seq], written = pos + count;
+        const int pos = sh.line.pos[s.seq], count = sh.line.count[s.seq];
         const int rows_all = count * group, row0 = s.tile * F::kRows;
         const bool nodes = s.end * F::kKeys > pos;  // some of these blocks hold nodes
         if (nodes)
@@ -237,31 +246,26 @@ __global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(con
         for (int r = warp; r < F::kRows; r += F::kWarps) {
             const int row = row0 + r, node = row / group;
             uint8_t *dst = sm + F::kQ0 + r * F::kQPitch + lane * 8;
-            uint2 hi = make_uint2(0u, 0u), lo = hi;
+            uint32_t x01[TERMS] = {}, x23[TERMS] = {};
             if (row < rows_all) {
                 const size_t at = (static_cast<size_t>(s.seq) * p.t + node) * p.q_pitch + static_cast<size_t>(s.kh * group + row - node * group) * kHd + lane * 4;
-                if (TERMS == 2) {
+                if (TERMS > 1) {
                     const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + at);
-                    split_pair(a.x, a.y, hi.x, lo.x);
-                    split_pair(a.z, a.w, hi.y, lo.y);
+                    split_pair<TERMS>(a.x, a.y, x01);
+                    split_pair<TERMS>(a.z, a.w, x23);
                 } else {
-                    hi = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p.q) + at);
+                    const uint2 a = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p.q) + at);
+                    x01[0] = a.x;
+                    x23[0] = a.y;
                 }
             }
-            *reinterpret_cast<uint2 *>(dst) = hi;
-            if (TERMS == 2) *reinterpret_cast<uint2 *>(dst + F::kRows * F::kQPitch) = lo;
+#pragma unroll
+            for (int x = 0; x < TERMS; ++x) *reinterpret_cast<uint2 *>(dst + x * F::kRows * F::kQPitch) = make_uint2(x01[x], x23[x]);
         }
         meet();
         if (nodes)
             for (int i = tid; i < count; i += F::kWarps * 32) tree_masks(sh.parent, sh.mask, i);
-        uint32_t qf[TERMS][8][4];  // 16 rows x 16 dimensions each
-        {
-            const uint32_t at = base + F::kQ0 + (rg * 16 + (lane & 15)) * F::kQPitch + (lane >> 4) * 16;
-#pragma unroll
-            for (int x = 0; x < TERMS; ++x)
-#pragma unroll
-                for (int d = 0; d < 8; ++d) ptx::ldmatrix_x4(qf[x][d], at + x * F::kRows * F::kQPitch + d * 32);
-        }
+        const uint32_t q_at = base + F::kQ0 + (rg * 16 + (lane & 15)) * F::kQPitch + (lane >> 4) * 16;
         if (nodes) meet();
         float o[16][4], m[2] = {kNoMax, kNoMax}, l[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -280,23 +284,28 @@ __global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(con
 #pragma unroll
                     for (int x = 0; x < TERMS; ++x) sc[h][x][0] = sc[h][x][1] = sc[h][x][2] = sc[h][x][3] = 0.0f;
 #pragma unroll
-                for (int d2 = 0; d2 < 4; ++d2)  // 32 dimensions at a time
+                for (int d2 = 0; d2 < 4; ++d2) {  // 32 dimensions at a time
+                    uint32_t kb[2][4];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int key = kg * 16 + h * 8 + (lane & 7), unit = (d2 & 1) * 4 + (lane >> 3);
-                        uint32_t kb[4];
-                        ptx::ldmatrix_x4(kb, ks + (d2 >> 1) * F::kHalf + key * 128 + ((unit ^ (key & 7)) << 4));
-#pragma unroll
-                        for (int x = 0; x < TERMS; ++x) {
-                            ptx::mma_bf16(sc[h][x], qf[x][2 * d2], kb[0], kb[1]);
-                            ptx::mma_bf16(sc[h][x], qf[x][2 * d2 + 1], kb[2], kb[3]);
-                        }
+                        ptx::ldmatrix_x4(kb[h], ks + (d2 >> 1) * F::kHalf + key * 128 + ((unit ^ (key & 7)) << 4));
                     }
+#pragma unroll
+                    for (int x = 0; x < TERMS; ++x)
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            uint32_t qf[4];
+                            ptx::ldmatrix_x4(qf, q_at + x * F::kRows * F::kQPitch + (2 * d2 + d) * 32);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) ptx::mma_bf16(sc[h][x], qf, kb[h][2 * d], kb[h][2 * d + 1]);
+                        }
+                }
                 float sv[2][4];
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sv[h][e] = (TERMS == 2 ? sc[h][0][e] + sc[h][TERMS - 1][e] : sc[h][0][e]) * p.scale;
+                    for (int e = 0; e < 4; ++e) sv[h][e] = (TERMS > 1 ? sc[h][0][e] + (sc[h][1 % TERMS][e] + sc[h][2 % TERMS][e]) : sc[h][0][e]) * p.scale;
                 if (edge) {
                     const int ra = row0 + rg * 16 + g, rb = ra + 8;
                     const ulonglong2 none = make_ulonglong2(0ull, 0ull), ma = ra < rows_all ? sh.mask[ra / group] : none, mb = rb < rows_all ? sh.mask[rb / group] : none;
@@ -308,29 +317,25 @@ __global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(con
                             if (n >= 0 && (n >= count || !sees(e < 2 ? ma : mb, n))) sv[h][e] = -INFINITY;
                         }
                 }
-                uint32_t ph[4], pl[4];
+                uint32_t pr[4][TERMS];
+                float corr[2];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {  // rows g and g + 8
                     const int e = half * 2;
                     float mx = fmaxf(fmaxf(sv[0][e], sv[0][e + 1]), fmaxf(sv[1][e], sv[1][e + 1]));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    const float nm = fmaxf(m[half], mx), corr = ex2(m[half] - nm);
+                    const float nm = fmaxf(m[half], mx);
+                    corr[half] = ex2(m[half] - nm);
                     m[half] = nm;
                     float sum = 0.0f;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float e0 = ex2(sv[h][e] - nm), e1 = ex2(sv[h][e + 1] - nm);
                         sum += e0 + e1;
-                        if (TERMS == 2) split_pair(e0, e1, ph[2 * h + half], pl[2 * h + half]);
-                        else ph[2 * h + half] = bf16_pair(e0, e1);
+                        split_pair<TERMS>(e0, e1, pr[2 * h + half]);
                     }
-                    l[half] = l[half] * corr + sum;
-#pragma unroll
-                    for (int d = 0; d < 16; ++d) {
-                        o[d][e] *= corr;
-                        o[d][e + 1] *= corr;
-                    }
+                    l[half] = l[half] * corr[half] + sum;
                 }
                 const int key = kg * 16 + (lane & 15);
 #pragma unroll
@@ -349,12 +354,17 @@ __global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(con
                                 if (strange || n >= count) vb[r] &= e ? 0x0000ffffu : 0xffff0000u;
                             }
                     }
-                    ptx::mma_bf16(o[2 * d2], ph, vb[0], vb[1]);
-                    ptx::mma_bf16(o[2 * d2 + 1], ph, vb[2], vb[3]);
-                    if (TERMS == 2) {
-                        ptx::mma_bf16(o[2 * d2], pl, vb[0], vb[1]);
-                        ptx::mma_bf16(o[2 * d2 + 1], pl, vb[2], vb[3]);
+                    float add[2][4] = {};
+#pragma unroll
+                    for (int x = TERMS - 1; x >= 0; --x) {  // the small ones first
+                        const uint32_t a[4] = {pr[0][x], pr[1][x], pr[2][x], pr[3][x]};
+                        ptx::mma_bf16(add[0], a, vb[0], vb[1]);
+                        ptx::mma_bf16(add[1], a, vb[2], vb[3]);
                     }
+#pragma unroll
+                    for (int d = 0; d < 2; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[2 * d2 + d][e] = o[2 * d2 + d][e] * corr[e >> 1] + add[d][e];
                 }
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(empty(stage));
@@ -432,7 +442,7 @@ __global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(con
 #pragma unroll
                     for (int d = 0; d < 16; ++d) {
                         const float x = o[d][half * 2] * inv, y = o[d][half * 2 + 1] * inv;
-                        if (TERMS == 2) *reinterpret_cast<float2 *>(static_cast<float *>(p.out) + at + d * 8) = make_float2(x, y);
+                        if (TERMS > 1) *reinterpret_cast<float2 *>(static_cast<float *>(p.out) + at + d * 8) = make_float2(x, y);
                         else *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + at + d * 8) = bf16_pair(x, y);
                     }
                 } else {
@@ -496,16 +506,14 @@ __global__ void __launch_bounds__(256) attn_tree_merge_kernel(const __grid_const
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     const float inv = 1.0f / l;
     const size_t at = (static_cast<size_t>(seq) * p.t + node) * p.out_pitch + static_cast<size_t>(kh * group + row - node * group) * kHd + lane * 4;
-    if (TERMS == 2) dense::put4(static_cast<float *>(p.out) + at, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+    if (TERMS > 1) dense::put4(static_cast<float *>(p.out) + at, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
     else dense::put4(static_cast<uint16_t *>(p.out) + at, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
 }
 
 int attn_tree_init(Ctx *ctx) {
-    struct { void (*k)(TreeParams); int smem; } few[] = {{attn_tree_few_kernel<1, 1>, Few<1>::kSmem}, {attn_tree_few_kernel<2, 1>, Few<1>::kSmem},
-                                                         {attn_tree_few_kernel<1, 2>, Few<2>::kSmem}, {attn_tree_few_kernel<2, 2>, Few<2>::kSmem}};
-    for (auto &f : few) {
-        LBK_CUDA(cudaFuncSetAttribute(f.k, cudaFuncAttributeMaxDynamicSharedMemorySize, f.smem));
-    }
+    struct { void (*k)(TreeParams); int smem; } kernels[] = {{attn_tree_few_kernel<1, 1>, Few<1>::kSmem}, {attn_tree_few_kernel<3, 1>, Few<1>::kSmem},
+                                                         {attn_tree_few_kernel<1, 2>, Few<2>::kSmem}, {attn_tree_few_kernel<3, 2>, Few<2>::kSmem}};
+    for (auto &f : kernels) LBK_CUDA(cudaFuncSetAttribute(f.k, cudaFuncAttributeMaxDynamicSharedMemorySize, f.smem));
     return LBK_OK;
 }
 const InitHook kInitAttnTree(attn_tree_init);
@@ -514,11 +522,11 @@ const InitHook kInitAttnTree(attn_tree_init);
 int tile_rows(size_t t, size_t group) { return t * group <= 16 ? 16 : 32; }
 
 template <int ROWS, int KEYS>
-int launch_tree(Ctx *ctx, int terms, TreeParams &p, void (*one)(TreeParams), void (*two)(TreeParams), int threads, int smem, cudaStream_t st) {
+int launch_tree(Ctx *ctx, int terms, TreeParams &p, void (*one)(TreeParams), void (*three)(TreeParams), int threads, int smem, cudaStream_t st) {
     const int group = p.nh / p.kvh, tiles = (p.t * group + ROWS - 1) / ROWS;
-    LBK_CUDA(launch_chained(terms == 2 ? two : one, dim3(static_cast<unsigned>(p.workers)), dim3(threads), static_cast<size_t>(smem), st, p));
+    LBK_CUDA(launch_chained(terms == 3 ? three : one, dim3(static_cast<unsigned>(p.workers)), dim3(threads), static_cast<size_t>(smem), st, p));
     ctx->launches++;
-    LBK_CUDA(launch_chained(terms == 2 ? attn_tree_merge_kernel<2, ROWS, KEYS> : attn_tree_merge_kernel<1, ROWS, KEYS>, dim3(static_cast<unsigned>(p.b * p.kvh * tiles), ROWS / 8), dim3(256), 0, st,
+    LBK_CUDA(launch_chained(terms == 3 ? attn_tree_merge_kernel<3, ROWS, KEYS> : attn_tree_merge_kernel<1, ROWS, KEYS>, dim3(static_cast<unsigned>(p.b * p.kvh * tiles), ROWS / 8), dim3(256), 0, st,
                             p));
     ctx->launches++;
     return LBK_OK;
@@ -572,13 +580,13 @@ int lbk_attn_tree(lbk_ctx *c, int compute, const void *q_dev, size_t q_pitch, co
     p.scale = scale * 1.4426950408889634f;
     p.workers = ctx->sm_count;
     p.err_word = ctx->err_word;
-    const int tile = tile_rows(t, group), terms = compute == LBK_COMPUTE_F32 ? 2 : 1;
+    const int tile = tile_rows(t, group), terms = compute == LBK_COMPUTE_F32 ? 3 : 1;
     p.part = scratch_dev;
     p.part_ml = reinterpret_cast<float2 *>(scratch_dev + static_cast<size_t>(p.workers) * 2 * tile * kHd);
     LBK_TRY(encode_bytes_map(&p.k, kcache_dev, 256, rows, 256, 128, 64));
     LBK_TRY(encode_bytes_map(&p.v, vcache_dev, 256, rows, 256, 128, 64));
-    if (tile == 16) return launch_tree<16, 64>(ctx, terms, p, attn_tree_few_kernel<1, 1>, attn_tree_few_kernel<2, 1>, Few<1>::kThreads, Few<1>::kSmem, st);
-    return launch_tree<32, 64>(ctx, terms, p, attn_tree_few_kernel<1, 2>, attn_tree_few_kernel<2, 2>, Few<2>::kThreads, Few<2>::kSmem, st);
+    if (tile == 16) return launch_tree<16, 64>(ctx, terms, p, attn_tree_few_kernel<1, 1>, attn_tree_few_kernel<3, 1>, Few<1>::kThreads, Few<1>::kSmem, st);
+    return launch_tree<32, 64>(ctx, terms, p, attn_tree_few_kernel<1, 2>, attn_tree_few_kernel<3, 2>, Few<2>::kThreads, Few<2>::kSmem, st);
 }
 
 }  // extern "C"

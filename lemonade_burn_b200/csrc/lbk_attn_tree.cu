@@ -18,6 +18,7 @@
 // branches may be infinite or NaN too; a row that does not see them must not notice. So in the blocks of the nodes values that are no numbers are
 // taken as zeros as well, and added at the end to the rows that see them (a weight is never zero in exact arithmetic).
 #include "lbk_dense_dev.cuh"
+#include "lbk_tcgen05.cuh"
 #include "lbk_tree.cuh"
 
 namespace lbk {
@@ -32,7 +33,7 @@ constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr float kNoMax = -3.0e38f;  // a row that has seen nothing: finite, so that -inf scores less it are no NaN
 
 struct TreeParams {
-    CUtensorMap k, v;   // bytes [cache rows][256], box [128 bytes][64 rows], SWIZZLE_128B
+    CUtensorMap k, v;   // bytes [cache rows][256], boxes of 128 bytes and 64 rows (K of many rows: 128), SWIZZLE_128B
     const void *q;
     void *out;
     long q_pitch, out_pitch;
@@ -458,6 +459,407 @@ __global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(con
     if (!ok && lane == 0) atomicExch(p.err_word, 5);
 }
 
+// ---- many rows: tcgen05, tiles of 128 rows ---------------------------------------------------------------
+// Blocks of 128 keys. S = Q K^T: the queries' terms and the K block from shared memory, scores in tensor memory. P V: the probabilities' terms from tensor
+// memory, the V block as it lies in the cache (its contraction index, the key, is the strided one: the MN-major operand form), every
+// block into zeroed sums, which the softmax warps add to the rows in their registers.
+//
+//   8 softmax warps  two to a quadrant of 32 lanes = rows: warp w and w + 4 share rows and take 64 of a block's keys, and of the dimensions, each
+//   K, V producers   a warp each: K blocks of 128 keys are free again after the scores, V in pieces of 64 keys after their product, and one order for
+//                    both would have the next K block wait for a piece of V
+//   MMA warp         P V of block j - 1, then Q K^T of block j + 1, while the softmax warps work on block j
+//
+// 512 bytes a key from HBM are 22 cycles of an SM, its products for 128 rows 24 in three terms and 8 in one: f32 is bound by the tensor core, bf16 by
+// the stream and by the softmax warps (64 exponentials a thread and block). Padding rows cost nothing but the products: their warps only keep step.
+template <int TERMS>
+struct Many {
+    static constexpr int kRows = 128, kKeys = 128, kHalf = kKeys * 128, kKBytes = 2 * kHalf;
+    static constexpr int kPiece = 64, kPieceHalf = kPiece * 128, kPieceBytes = 2 * kPieceHalf;   // V: 64 keys, two halves of 64 dimensions
+    static constexpr int kKStages = TERMS == 3 ? 2 : 3, kVStages = TERMS == 3 ? 3 : 5;
+    static constexpr int kK0 = TERMS * 2 * kHalf, kV0 = kK0 + kKStages * kKBytes, kBars = kV0 + kVStages * kPieceBytes;
+    static constexpr int kPair = kBars + 256, kSmem = kPair + 2 * 2 * kRows * 4 + 1024;
+    static constexpr int kSoftWarps = 8, kKWarp = 8, kVWarp = 9, kMmaWarp = 10, kThreads = 12 * 32;
+    static constexpr uint32_t kColS = 0, kColO = 128, kColP = 256;                                // term x of P at kColP + 64 x
+};
+struct ManyShared {
+    Line line;
+    int parent[kTreeNodes];
+    ulonglong2 mask[kTreeNodes];
+    int abort, odd;
+    uint32_t tmem;
+};
+// MN-major SWIZZLE_128B operand: groups of 8 keys 1024 bytes apart (stride byte offset), the halves of 64 dimensions `apart` bytes (leading byte offset)
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t apart) {
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | static_cast<uint64_t>(apart >> 4) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 |
+           static_cast<uint64_t>(2) << 61;
+}
+
+template <int TERMS>
+__global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kernel(const __grid_constant__ TreeParams p) {
+    using M = Many<TERMS>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ ManyShared sh;
+    const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t *sm = smem_raw + (base - raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int kKFull = 0, kKEmpty = 3, kVFull = 6, kVEmpty = 11, kQFull = 16, kSFull = 17, kSFree = 18, kPReady = 19, kOFull = 20;
+    auto bar = [&](int i) { return base + M::kBars + i * 8; };
+    volatile int *abort = &sh.abort;
+    if (tid == 0) {
+        for (int s = 0; s < M::kKStages; ++s) {
+            ptx::mbar_init(bar(kKFull + s), 1);
+            ptx::mbar_init(bar(kKEmpty + s), 1);
+        }
+        for (int s = 0; s < M::kVStages; ++s) {
+            ptx::mbar_init(bar(kVFull + s), 1);
+            ptx::mbar_init(bar(kVEmpty + s), 1);
+        }
+        for (int i : {kQFull, kSFree, kPReady}) ptx::mbar_init(bar(i), M::kSoftWarps);
+        for (int i : {kSFull, kOFull}) ptx::mbar_init(bar(i), 1);
+        sh.abort = sh.odd = 0;
+        ptx::fence_barrier_init();
+    }
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    cut_line<M::kRows, M::kKeys>(p, sh.line);
+    const int units = sh.line.first[p.b], u0 = share_begin(units, blockIdx.x, p.workers), u1 = share_begin(units, blockIdx.x + 1, p.workers);
+    if (u0 == u1) return;
+    if (warp == M::kMmaWarp) {
+        tc::tmem_alloc(ptx::smem_u32(&sh.tmem), 512);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = *static_cast<volatile uint32_t *>(&sh.tmem);
+    const int group = p.nh / p.kvh;
+    bool ok = true;
+
+    // The launch has 12 warps x 168 registers; 4 x 72 + 8 x 216 are as many.
+    if (warp >= M::kSoftWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == M::kKWarp || warp == M::kVWarp) {
+            // ================= TMA producers =================
+            const bool is_k = warp == M::kKWarp;
+            const int stages = is_k ? M::kKStages : M::kVStages, full = is_k ? kKFull : kVFull, empty = is_k ? kKEmpty : kVEmpty;
+            if (lane == 0) {
+                int stage = 0, round = 0, sent = 0;
+                for (int u = u0; u < u1 && ok;) {
+                    const Segment s = segment_at(p, sh.line, u, u1, M::kRows, M::kKeys);
+                    const int row0 = (s.seq * p.kvh + s.kh) * p.cap;
+                    for (int i = is_k ? s.begin : 2 * s.begin; i < (is_k ? s.end : 2 * s.end); ++i, ++sent) {
+                        if (round > 0 && !tc::wait_bar(bar(empty + stage), (round - 1) & 1, abort)) {
+                            ok = false;
+                            break;
+                        }
+                        if (is_k) {
+                            const uint32_t at = base + M::kK0 + stage * M::kKBytes;
+                            ptx::mbar_arrive_expect_tx(bar(full + stage), M::kKBytes);
+                            ptx::tma_load_2d(at, &p.k, bar(full + stage), 0, row0 + i * M::kKeys);
+                            ptx::tma_load_2d(at + M::kHalf, &p.k, bar(full + stage), 128, row0 + i * M::kKeys);
+                        } else {
+                            const uint32_t at = base + M::kV0 + stage * M::kPieceBytes;
+                            ptx::mbar_arrive_expect_tx(bar(full + stage), M::kPieceBytes);
+                            ptx::tma_load_2d(at, &p.v, bar(full + stage), 0, row0 + i * M::kPiece);
+                            ptx::tma_load_2d(at + M::kPieceHalf, &p.v, bar(full + stage), 128, row0 + i * M::kPiece);
+                        }
+                        if (++stage == stages) {
+                            stage = 0;
+                            ++round;
+                        }
+                    }
+                    u += s.end - s.begin;
+                }
+                // the copies in flight land before the block may go, whoever has given up
+                for (int n = max(0, sent - stages); n < sent; ++n) ptx::mbar_wait(bar(full + n % stages), (n / stages) & 1, tc::kTcWaitLimit);
+            }
+        } else if (warp == M::kMmaWarp) {
+            // ================= MMA issue: the warp walks, one lane issues =================
+            // D f32, A and B bf16, M = 128, N = 128; for P V the B operand is MN-major (bit 16)
+            constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24), idesc_o = idesc_s | (1u << 16);
+            const uint64_t q_desc = tc::smem_desc_sw128(base);
+            int ks = 0, kphase = 0, vs = 0, vphase = 0, n = 0, seg = 0;  // n: blocks whose scores have been asked for
+            auto wait = [&](int i, int parity) {
+                if (ok) ok = tc::warp_wait(bar(i), parity, abort);
+                return ok;
+            };
+            auto scores = [&]() {
+                if (!wait(kKFull + ks, kphase)) return;
+                tc::tc_fence_after();
+                if (tc::elect_one()) {
+                    const uint64_t k_desc = tc::smem_desc_sw128(base + M::kK0 + ks * M::kKBytes);
+#pragma unroll 1
+                    for (int x = TERMS - 1; x >= 0; --x)  // the small ones first
+#pragma unroll
+                        for (int st = 0; st < 8; ++st) {
+                            const uint64_t off = static_cast<uint64_t>((st >> 2) * (M::kHalf >> 4) + (st & 3) * 2);
+                            tc::umma_f16_ss(tmem + M::kColS, q_desc + static_cast<uint64_t>(x * 2 * (M::kHalf >> 4)) + off, k_desc + off, idesc_s, x < TERMS - 1 || st ? 1u : 0u);
+                        }
+                    tc::umma_commit(bar(kSFull));
+                    tc::umma_commit(bar(kKEmpty + ks));
+                }
+                __syncwarp();
+                ++n;
+                if (++ks == M::kKStages) {
+                    ks = 0;
+                    kphase ^= 1;
+                }
+            };
+            for (int u = u0; u < u1 && ok; ++seg) {
+                const Segment s = segment_at(p, sh.line, u, u1, M::kRows, M::kKeys);
+                const int blocks = s.end - s.begin;
+                if (wait(kQFull, seg & 1)) scores();
+                for (int j = 1; j <= blocks && ok; ++j) {  // P V of block j - 1, scores of block j + 1
+                    if (j == 1 && blocks > 1 && wait(kSFree, (n - 1) & 1)) scores();
+                    const int done = n - (j < blocks ? 2 : 1);  // the number, in the whole walk, of the block whose P V this is
+                    if (!wait(kPReady, done & 1)) break;
+#pragma unroll 1
+                    for (int piece = 0; piece < 2; ++piece) {
+                        if (!wait(kVFull + vs, vphase)) break;
+                        tc::tc_fence_after();
+                        if (tc::elect_one()) {
+                            const uint64_t v_desc = desc_mn_sw128(base + M::kV0 + vs * M::kPieceBytes, M::kPieceHalf);
+#pragma unroll
+                            for (int st = 0; st < 4; ++st)  // 16 keys: 8 columns of P, two groups of V
+#pragma unroll
+                                for (int x = TERMS - 1; x >= 0; --x)
+                                    tc::umma_f16_ts(tmem + M::kColO, tmem + M::kColP + x * 64 + (piece * 4 + st) * 8, v_desc + static_cast<uint64_t>(st * (2048 >> 4)), idesc_o,
+                                                    piece || st || x < TERMS - 1 ? 1u : 0u);
+                            tc::umma_commit(bar(kVEmpty + vs));
+                            if (piece) tc::umma_commit(bar(kOFull));
+                        }
+                        __syncwarp();
+                        if (++vs == M::kVStages) {
+                            vs = 0;
+                            vphase ^= 1;
+                        }
+                    }
+                    // block j is in the softmax warps' registers: its scores' place is free
+                    if (j + 1 < blocks && wait(kSFree, (n - 1) & 1)) scores();
+                }
+                u += blocks;
+            }
+        }
+    } else {
+        // ================= softmax =================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int quad = warp & 3, kh2 = warp >> 2, r = quad * 32 + lane;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+        float *const s_pair = reinterpret_cast<float *>(sm + M::kPair);
+        auto wait = [&](int i, int parity) {
+            if (ok) ok = tc::warp_wait(bar(i), parity, abort);
+            return ok;
+        };
+        auto arrive = [&](int i) {
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar(i));
+        };
+        auto meet = [&]() { ptx::named_barrier(1, M::kSoftWarps * 32); };
+        auto pair_sync = [&]() { ptx::named_barrier(2 + quad, 64); };  // the two warps of a quadrant
+        int n = 0;  // blocks so far, over all segments
+        for (int u = u0; u < u1;) {
+            const Segment s = segment_at(p, sh.line, u, u1, M::kRows, M::kKeys);
+            const int pos = sh.line.pos[s.seq], count = sh.line.count[s.seq];
+            const int rows_all = count * group, row0 = s.tile * M::kRows, row = row0 + r, node = row / group;
+            const bool nodes = s.end * M::kKeys > pos, live = row0 + quad * 32 < rows_all;  // some blocks hold nodes; some row of the warp exists
+            meet();  // nobody reads what the last segment left in the queries' place and in the tree's any more
+            if (nodes)
+                for (int i = tid; i < count; i += M::kSoftWarps * 32) {
+                    const int up = p.parents[static_cast<size_t>(s.seq) * p.t + i];
+                    const bool good = up >= -1 && up < i;
+                    if (!good) atomicExch(p.err_word, kErrTree);
+                    sh.parent[i] = good ? up : -1;
+                }
+            // the tile's queries, a row as one load of a warp; in the K-major SWIZZLE_128B layout (row r of a half at r * 128, its 16-byte units XOR-ed with r & 7)
+#pragma unroll 8
+            for (int i = 0; i < 16; ++i) {
+                const int qr = warp * 16 + i, at_row = row0 + qr, at_node = at_row / group;
+                uint32_t x01[TERMS] = {}, x23[TERMS] = {};
+                if (at_row < rows_all) {
+                    const size_t at = (static_cast<size_t>(s.seq) * p.t + at_node) * p.q_pitch + static_cast<size_t>(s.kh * group + at_row - at_node * group) * kHd + lane * 4;
+                    if (TERMS > 1) {
+                        const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + at);
+                        split_pair<TERMS>(a.x, a.y, x01);
+                        split_pair<TERMS>(a.z, a.w, x23);
+                    } else {
+                        const uint2 a = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p.q) + at);
+                        x01[0] = a.x;
+                        x23[0] = a.y;
+                    }
+                }
+                uint8_t *dst = sm + (lane >> 4) * M::kHalf + qr * 128 + ((((lane & 15) >> 1) ^ (qr & 7)) << 4) + (lane & 1) * 8;
+#pragma unroll
+                for (int x = 0; x < TERMS; ++x) *reinterpret_cast<uint2 *>(dst + x * 2 * M::kHalf) = make_uint2(x01[x], x23[x]);
+            }
+            ptx::fence_proxy_async();  // the tensor core reads them through the asynchronous proxy
+            arrive(kQFull);
+            if (nodes) {
+                meet();
+                for (int i = tid; i < count; i += M::kSoftWarps * 32) tree_masks(sh.parent, sh.mask, i);
+                meet();
+            }
+            float acc[64], m = kNoMax, l = 0.0f, corr = 0.0f;  // 64 dimensions of the row; corr: what brings acc to the present maximum
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
+            // acc = acc * corr + the products of block n - 1
+            auto add_products = [&]() {
+                tc::tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t v[16];
+                    tc::tmem_ld16(lanes + M::kColO + kh2 * 64 + c * 16, v);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[c * 16 + i] = acc[c * 16 + i] * corr + __uint_as_float(v[i]);
+                }
+            };
+            for (int j = s.begin; j < s.end; ++j, ++n) {
+                uint32_t sv[64];
+                const int key0 = j * M::kKeys + kh2 * 64;
+                float step = 0.0f;
+                wait(kSFull, n & 1);
+                if (live) {
+                    tc::tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) tc::tmem_ld32(lanes + M::kColS + kh2 * 64 + c * 32, reinterpret_cast<uint32_t(&)[32]>(sv[c * 32]));
+                    tc::tmem_ld_wait();
+                    tc::tc_fence_before();
+                }
+                arrive(kSFree);
+                if (live) {
+                    if (key0 + 64 > pos) {  // some of these keys are nodes, or nothing: bit i of `seen` is key0 + i
+                        const ulonglong2 mine = row < rows_all ? sh.mask[node] : make_ulonglong2(0ull, 0ull);
+                        const int n0 = key0 - pos;
+                        const unsigned long long seen = n0 < 0 ? mine.x << -n0 | ((1ull << -n0) - 1) : n0 == 0 ? mine.x : n0 < 64 ? mine.x >> n0 | mine.y << (64 - n0) : n0 < 128 ? mine.y >> (n0 - 64) : 0ull;
+#pragma unroll
+                        for (int i = 0; i < 64; ++i)
+                            if (!(seen >> i & 1)) sv[i] = 0xff800000u;  // -inf
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(sv[i]));
+                    float *pair = s_pair + (n & 1) * 2 * M::kRows;
+                    const float own = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    pair[kh2 * M::kRows + r] = own;
+                    pair_sync();  // the next block but one writes here again, behind the next block's meeting
+                    const float nm = fmaxf(m, fmaxf(own, pair[(kh2 ^ 1) * M::kRows + r]) * p.scale);
+                    step = ex2(m - nm);
+                    m = nm;
+                    float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) {
+                        const float e0 = ex2(__fmaf_rn(__uint_as_float(sv[i]), p.scale, -nm)), e1 = ex2(__fmaf_rn(__uint_as_float(sv[i + 1]), p.scale, -nm));
+                        sum0 += e0;
+                        sum1 += e1;
+                        sv[i] = __float_as_uint(e0);
+                        sv[i + 1] = __float_as_uint(e1);
+                    }
+                    l = l * step + (sum0 + sum1);
+                }
+                // the products of the block in front are complete: they are added, and the probabilities' place is free
+                if (j > s.begin) {
+                    wait(kOFull, (n - 1) & 1);
+                    if (live) add_products();
+                }
+                corr = step;
+                if (live) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t w[TERMS][16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            uint32_t term[TERMS];
+                            split_pair<TERMS>(__uint_as_float(sv[c * 32 + 2 * i]), __uint_as_float(sv[c * 32 + 2 * i + 1]), term);
+#pragma unroll
+                            for (int x = 0; x < TERMS; ++x) w[x][i] = term[x];
+                        }
+#pragma unroll
+                        for (int x = 0; x < TERMS; ++x) tc::tmem_st16(lanes + M::kColP + x * 64 + kh2 * 32 + c * 16, w[x]);
+                    }
+                }
+                if (j * M::kKeys + M::kKeys > pos) {  // values past the last node, and values of nodes that are no numbers: a thread half a row of this warp's piece
+                    const int piece = 2 * n + kh2, vs = piece % M::kVStages, key = r & 63, at = key0 + key - pos;
+                    if (wait(kVFull + vs, (piece / M::kVStages) & 1) && at >= 0) {
+                        uint4 *v = reinterpret_cast<uint4 *>(sm + M::kV0 + vs * M::kPieceBytes + (r >> 6) * M::kPieceHalf + key * 128);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            uint4 x = v[i];
+                            bool strange = false;
+                            for (uint32_t *w = &x.x; w <= &x.w; ++w)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+                                    if (at >= count || ((*w >> (16 * e)) & 0x7f80u) == 0x7f80u) {
+                                        *w &= e ? 0x0000ffffu : 0xffff0000u;
+                                        strange = true;
+                                    }
+                            if (strange) v[i] = x;
+                            if (strange && at < count) sh.odd = u + 1;  // read behind a meeting below, written again behind the next segment's first
+                        }
+                    }
+                    ptx::fence_proxy_async();
+                }
+                if (live) tc::tmem_st_wait();
+                tc::tc_fence_before();
+                arrive(kPReady);
+            }
+            wait(kOFull, (n - 1) & 1);
+            if (live) add_products();
+            // the row's weight: the two halves of the keys meet
+            float *pair = s_pair + (n & 1) * 2 * M::kRows;
+            pair[kh2 * M::kRows + r] = l;
+            meet();
+            l += pair[(kh2 ^ 1) * M::kRows + r];
+            if (nodes && sh.odd == u + 1 && row < rows_all) {  // what this row sees that is no number
+                const ulonglong2 mine = sh.mask[node];
+                for (int i = max(0, s.begin * M::kKeys - pos); i < min(count, s.end * M::kKeys - pos); ++i) {
+                    if (!sees(mine, i)) continue;
+                    const uint16_t *v = p.vcache + (static_cast<size_t>(s.seq * p.kvh + s.kh) * p.cap + pos + i) * kHd + kh2 * 64;
+#pragma unroll
+                    for (int d = 0; d < 64; ++d)
+                        if ((v[d] & 0x7f80u) == 0x7f80u) acc[d] += dense::bf16_f32(v[d]);
+                }
+            }
+            // Rows leave through the queries' place, whose products are done, so that a store writes whole lines: a warp's 32 rows of 32 dimensions at a
+            // time, 16-byte units XOR-ed with the row.
+            const bool whole = s.begin == 0 && s.end == s.blocks;
+            if (live && ok) {
+                const float inv = whole ? 1.0f / l : 1.0f;
+                const size_t part0 = (static_cast<size_t>(blockIdx.x) * 2 + (u == u0 ? 0 : 1)) * M::kRows;
+                if (!whole && kh2 == 0 && row < rows_all) p.part_ml[part0 + r] = make_float2(m, l);
+                float *own = reinterpret_cast<float *>(sm + warp * 4096);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<float4 *>(own + lane * 32 + ((i ^ (lane & 7)) << 2)) =
+                            make_float4(acc[c * 32 + 4 * i] * inv, acc[c * 32 + 4 * i + 1] * inv, acc[c * 32 + 4 * i + 2] * inv, acc[c * 32 + 4 * i + 3] * inv);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int rr = i * 4 + (lane >> 3), at_row = row0 + quad * 32 + rr, at_node = at_row / group, d = kh2 * 64 + c * 32 + (lane & 7) * 4;
+                        if (at_row < rows_all) {
+                            const float4 x = *reinterpret_cast<const float4 *>(own + rr * 32 + (((lane & 7) ^ (rr & 7)) << 2));
+                            const size_t at = (static_cast<size_t>(s.seq) * p.t + at_node) * p.out_pitch + static_cast<size_t>(s.kh * group + at_row - at_node * group) * kHd + d;
+                            if (!whole) *reinterpret_cast<float4 *>(p.part + (part0 + quad * 32 + rr) * kHd + d) = x;
+                            else if (TERMS > 1) dense::put4(static_cast<float *>(p.out) + at, x);
+                            else dense::put4(static_cast<uint16_t *>(p.out) + at, x);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            u += s.end - s.begin;
+        }
+    }
+    if (!ok && lane == 0) atomicExch(p.err_word, 5);
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == M::kMmaWarp) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, 512);
+    }
+}
+
 // Joins the parts of the tiles that were cut: a warp a row, four dimensions a lane.
 template <int TERMS, int ROWS, int KEYS>
 __global__ void __launch_bounds__(256) attn_tree_merge_kernel(const __grid_constant__ TreeParams p) {
@@ -512,14 +914,14 @@ __global__ void __launch_bounds__(256) attn_tree_merge_kernel(const __grid_const
 
 int attn_tree_init(Ctx *ctx) {
     struct { void (*k)(TreeParams); int smem; } kernels[] = {{attn_tree_few_kernel<1, 1>, Few<1>::kSmem}, {attn_tree_few_kernel<3, 1>, Few<1>::kSmem},
-                                                         {attn_tree_few_kernel<1, 2>, Few<2>::kSmem}, {attn_tree_few_kernel<3, 2>, Few<2>::kSmem}};
+                                                         {attn_tree_few_kernel<1, 2>, Few<2>::kSmem}, {attn_tree_few_kernel<3, 2>, Few<2>::kSmem}, {attn_tree_many_kernel<1>, Many<1>::kSmem}, {attn_tree_many_kernel<3>, Many<3>::kSmem}};
     for (auto &f : kernels) LBK_CUDA(cudaFuncSetAttribute(f.k, cudaFuncAttributeMaxDynamicSharedMemorySize, f.smem));
     return LBK_OK;
 }
 const InitHook kInitAttnTree(attn_tree_init);
 
 // Rows of a tile for t nodes of `group` heads.
-int tile_rows(size_t t, size_t group) { return t * group <= 16 ? 16 : 32; }
+int tile_rows(size_t t, size_t group) { return t * group <= 16 ? 16 : t * group <= 32 ? 32 : 128; }
 
 template <int ROWS, int KEYS>
 int launch_tree(Ctx *ctx, int terms, TreeParams &p, void (*one)(TreeParams), void (*three)(TreeParams), int threads, int smem, cudaStream_t st) {
@@ -583,9 +985,10 @@ int lbk_attn_tree(lbk_ctx *c, int compute, const void *q_dev, size_t q_pitch, co
     const int tile = tile_rows(t, group), terms = compute == LBK_COMPUTE_F32 ? 3 : 1;
     p.part = scratch_dev;
     p.part_ml = reinterpret_cast<float2 *>(scratch_dev + static_cast<size_t>(p.workers) * 2 * tile * kHd);
-    LBK_TRY(encode_bytes_map(&p.k, kcache_dev, 256, rows, 256, 128, 64));
+    LBK_TRY(encode_bytes_map(&p.k, kcache_dev, 256, rows, 256, 128, tile == 128 ? 128 : 64));
     LBK_TRY(encode_bytes_map(&p.v, vcache_dev, 256, rows, 256, 128, 64));
     if (tile == 16) return launch_tree<16, 64>(ctx, terms, p, attn_tree_few_kernel<1, 1>, attn_tree_few_kernel<3, 1>, Few<1>::kThreads, Few<1>::kSmem, st);
+    if (tile == 128) return launch_tree<128, 128>(ctx, terms, p, attn_tree_many_kernel<1>, attn_tree_many_kernel<3>, Many<1>::kThreads, Many<1>::kSmem, st);
     return launch_tree<32, 64>(ctx, terms, p, attn_tree_few_kernel<1, 2>, attn_tree_few_kernel<3, 2>, Few<2>::kThreads, Few<2>::kSmem, st);
 }
 

@@ -17,6 +17,8 @@
 // Rows of V that nobody has written may hold anything, and 0 * NaN is NaN: values past the sequence's last node are taken as zeros. Values of OTHER
 // branches may be infinite or NaN too; a row that does not see them must not notice. So in the blocks of the nodes values that are no numbers are
 // taken as zeros as well, and added at the end to the rows that see them (a weight is never zero in exact arithmetic).
+#include <algorithm>
+
 #include "lbk_dense_dev.cuh"
 #include "lbk_tcgen05.cuh"
 #include "lbk_tree.cuh"
@@ -44,7 +46,9 @@ struct TreeParams {
     float *part;        // [CTA][2][tile rows][128]
     float2 *part_ml;    // [CTA][2][tile rows]: maximum, weight
     int workers;        // CTAs of the attention kernel
+    unsigned per_group; // 2^32 / heads of a group, rounded up; 0 for one head
     int *err_word;
+    __device__ __forceinline__ int node_of(int row) const { return per_group ? static_cast<int>(__umulhi(static_cast<unsigned>(row), per_group)) : row; }
 };
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x, the hardware's approximation
@@ -65,6 +69,13 @@ __device__ __forceinline__ void split_pair(float x0, float x1, uint32_t (&term)[
     }
 }
 
+// two bf16 with zeros in the place of what is no number
+__device__ __forceinline__ uint32_t only_numbers(uint32_t x) {
+    if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
+    if ((x & 0x7f800000u) == 0x7f800000u) x &= 0x0000ffffu;
+    return x;
+}
+
 // ---- the line of units ----------------------------------------------------------------------------
 struct Line {
     int first[kMaxSeqs + 1];   // units in front of a sequence; [b] is all of them
@@ -74,12 +85,12 @@ struct Line {
 __device__ __forceinline__ int line_blocks(const Line &l, int seq, int block_keys) { return (l.pos[seq] + l.count[seq] + block_keys - 1) / block_keys; }
 __device__ __forceinline__ int line_tiles(const Line &l, int seq, int group, int rows) { return (l.count[seq] * group + rows - 1) / rows; }
 
-// Fills the line; a sequence outside its cache has no units. All threads of the block.
+// Fills the line; a sequence outside its cache has no units. All threads of the block. (Loads from L2: the merging kernel comes here in front of its wait.)
 template <int ROWS, int KEYS>
 __device__ void cut_line(const TreeParams &p, Line &l) {
     const int group = p.nh / p.kvh;
     for (int i = threadIdx.x; i < p.b; i += blockDim.x) {
-        const int pos = p.pos[i], count = tree_count(p.counts, i, p.t);
+        const int pos = __ldcg(p.pos + i), count = p.counts ? min(max(__ldcg(p.counts + i), 0), p.t) : p.t;
         const bool fits = pos >= 0 && pos <= p.cap - count;
         if (!fits && blockIdx.x == 0) atomicExch(p.err_word, kErrPos);
         l.pos[i] = pos;
@@ -103,7 +114,13 @@ __device__ void cut_line(const TreeParams &p, Line &l) {
     }
     __syncthreads();
 }
-__device__ __forceinline__ int share_begin(int units, int worker, int workers) { return static_cast<int>(static_cast<long long>(units) * worker / workers); }
+// Worker w takes the units share_begin(w) .. share_begin(w + 1) - 1: `each` of them, one more the first `more` workers.
+struct Shares {
+    int each, more;
+    __device__ __forceinline__ Shares(int units, int workers) : each(units / workers), more(units - units / workers * workers) {}
+    __device__ __forceinline__ int begin(int w) const { return w * each + min(w, more); }
+    __device__ __forceinline__ int owner(int u) const { return u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each; }
+};
 
 struct Segment {
     int seq, kh, tile;     // the problem
@@ -136,6 +153,37 @@ __device__ __forceinline__ void tree_masks(const int *parent, ulonglong2 *mask, 
         else hi |= 1ull << (n - 64);
     }
     mask[i] = make_ulonglong2(lo, hi);
+}
+// Parents into shared memory, those that are none as -1, by the first `threads` threads of the block.
+__device__ __forceinline__ void load_parents(const TreeParams &p, int *parent, int seq, int count, int threads) {
+    for (int i = threadIdx.x; i < count; i += threads) {
+        const int up = p.parents[static_cast<size_t>(seq) * p.t + i];
+        const bool good = up >= -1 && up < i;
+        if (!good) atomicExch(p.err_word, kErrTree);
+        parent[i] = good ? up : -1;
+    }
+}
+// Four dimensions of a problem's query row (zeros past the last): f32, or the bits of four bf16 in x and y
+template <int TERMS>
+__device__ __forceinline__ float4 query(const TreeParams &p, int seq, int kh, int group, int row, int rows_all, int lane) {
+    if (row >= rows_all) return make_float4(0.f, 0.f, 0.f, 0.f);
+    const int node = p.node_of(row);
+    const size_t at = (static_cast<size_t>(seq) * p.t + node) * p.q_pitch + (kh * group + row - node * group) * kHd + lane * 4;
+    if (TERMS > 1) return *reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + at);
+    const float2 a = *reinterpret_cast<const float2 *>(static_cast<const uint16_t *>(p.q) + at);
+    return make_float4(a.x, a.y, 0.f, 0.f);
+}
+template <int TERMS>
+__device__ __forceinline__ void query_terms(const float4 &a, uint2 (&term)[TERMS]) {
+    if (TERMS == 1) {
+        term[0] = make_uint2(__float_as_uint(a.x), __float_as_uint(a.y));
+        return;
+    }
+    uint32_t x01[TERMS], x23[TERMS];
+    split_pair<TERMS>(a.x, a.y, x01);
+    split_pair<TERMS>(a.z, a.w, x23);
+#pragma unroll
+    for (int x = 0; x < TERMS; ++x) term[x] = make_uint2(x01[x], x23[x]);
 }
 __device__ __forceinline__ bool sees(const ulonglong2 &m, int n) { return ((n < 64 ? m.x : m.y) >> (n & 63)) & 1; }
 
@@ -179,10 +227,11 @@ __global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(con
         sh.abort = sh.odd = 0;
         ptx::fence_barrier_init();
     }
-    ptx::pdl_trigger();
     ptx::pdl_wait();
+    ptx::pdl_trigger();  // behind the wait: what the merging kernel reads in front of its own is settled then
     cut_line<F::kRows, F::kKeys>(p, sh.line);
-    const int units = sh.line.first[p.b], u0 = share_begin(units, blockIdx.x, p.workers), u1 = share_begin(units, blockIdx.x + 1, p.workers);
+    const Shares shares(sh.line.first[p.b], p.workers);
+    const int u0 = shares.begin(blockIdx.x), u1 = shares.begin(blockIdx.x + 1);
     if (u0 == u1) return;
     const int group = p.nh / p.kvh;
     auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -236,32 +285,17 @@ __global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(con
         const int pos = sh.line.pos[s.seq], count = sh.line.count[s.seq];
         const int rows_all = count * group, row0 = s.tile * F::kRows;
         const bool nodes = s.end * F::kKeys > pos;  // some of these blocks hold nodes
-        if (nodes)
-            for (int i = tid; i < count; i += F::kWarps * 32) {
-                const int up = p.parents[static_cast<size_t>(s.seq) * p.t + i];
-                const bool good = up >= -1 && up < i;
-                if (!good) atomicExch(p.err_word, kErrTree);
-                sh.parent[i] = good ? up : -1;
-            }
-        // the tile's queries, a row as one load of a warp
-        for (int r = warp; r < F::kRows; r += F::kWarps) {
-            const int row = row0 + r, node = row / group;
-            uint8_t *dst = sm + F::kQ0 + r * F::kQPitch + lane * 8;
-            uint32_t x01[TERMS] = {}, x23[TERMS] = {};
-            if (row < rows_all) {
-                const size_t at = (static_cast<size_t>(s.seq) * p.t + node) * p.q_pitch + static_cast<size_t>(s.kh * group + row - node * group) * kHd + lane * 4;
-                if (TERMS > 1) {
-                    const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + at);
-                    split_pair<TERMS>(a.x, a.y, x01);
-                    split_pair<TERMS>(a.z, a.w, x23);
-                } else {
-                    const uint2 a = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p.q) + at);
-                    x01[0] = a.x;
-                    x23[0] = a.y;
-                }
-            }
+        // the tile's queries, a row as one load of a warp, all of them asked for before the first is looked at
+        float4 qv[F::kRows / F::kWarps];
 #pragma unroll
-            for (int x = 0; x < TERMS; ++x) *reinterpret_cast<uint2 *>(dst + x * F::kRows * F::kQPitch) = make_uint2(x01[x], x23[x]);
+        for (int i = 0; i < F::kRows / F::kWarps; ++i) qv[i] = query<TERMS>(p, s.seq, s.kh, group, row0 + i * F::kWarps + warp, rows_all, lane);
+        if (nodes) load_parents(p, sh.parent, s.seq, count, F::kWarps * 32);
+#pragma unroll
+        for (int i = 0; i < F::kRows / F::kWarps; ++i) {
+            uint2 term[TERMS];
+            query_terms<TERMS>(qv[i], term);
+#pragma unroll
+            for (int x = 0; x < TERMS; ++x) *reinterpret_cast<uint2 *>(sm + F::kQ0 + (x * F::kRows + i * F::kWarps + warp) * F::kQPitch + lane * 8) = term[x];
         }
         meet();
         if (nodes)
@@ -309,7 +343,7 @@ __global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(con
                     for (int e = 0; e < 4; ++e) sv[h][e] = (TERMS > 1 ? sc[h][0][e] + (sc[h][1 % TERMS][e] + sc[h][2 % TERMS][e]) : sc[h][0][e]) * p.scale;
                 if (edge) {
                     const int ra = row0 + rg * 16 + g, rb = ra + 8;
-                    const ulonglong2 none = make_ulonglong2(0ull, 0ull), ma = ra < rows_all ? sh.mask[ra / group] : none, mb = rb < rows_all ? sh.mask[rb / group] : none;
+                    const ulonglong2 none = make_ulonglong2(0ull, 0ull), ma = ra < rows_all ? sh.mask[p.node_of(ra)] : none, mb = rb < rows_all ? sh.mask[p.node_of(rb)] : none;
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -423,7 +457,7 @@ __global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(con
             const bool fix = nodes && sh.odd == u + 1, whole = s.begin == 0 && s.end == s.blocks;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int r = rg * 16 + half * 8 + g, row = row0 + r, node = row / group;
+                const int r = rg * 16 + half * 8 + g, row = row0 + r, node = p.node_of(row);
                 if (row >= rows_all) continue;
                 if (fix) {  // what this row sees that is no number
                     const ulonglong2 mine = sh.mask[node];
@@ -464,22 +498,24 @@ __global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(con
 // memory, the V block as it lies in the cache (its contraction index, the key, is the strided one: the MN-major operand form), every
 // block into zeroed sums, which the softmax warps add to the rows in their registers.
 //
-//   8 softmax warps  two to a quadrant of 32 lanes = rows: warp w and w + 4 share rows and take 64 of a block's keys, and of the dimensions, each
+//   16 softmax warps four to a quadrant of 32 lanes = rows: warps w, w + 4, .. share rows and take 32 of a block's keys, and of the dimensions, each (eight
+//                    warps with 64 took 5900 cycles a block in three terms where the products take 3072: two warps a scheduler do not hide their latencies)
 //   K, V producers   a warp each: K blocks of 128 keys are free again after the scores, V in pieces of 64 keys after their product, and one order for
 //                    both would have the next K block wait for a piece of V
 //   MMA warp         P V of block j - 1, then Q K^T of block j + 1, while the softmax warps work on block j
 //
 // 512 bytes a key from HBM are 22 cycles of an SM, its products for 128 rows 24 in three terms and 8 in one: f32 is bound by the tensor core, bf16 by
-// the stream and by the softmax warps (64 exponentials a thread and block). Padding rows cost nothing but the products: their warps only keep step.
+// the stream and by the softmax warps (an exponential per row and key). Padding rows cost nothing but the products: their warps only keep step.
 template <int TERMS>
 struct Many {
     static constexpr int kRows = 128, kKeys = 128, kHalf = kKeys * 128, kKBytes = 2 * kHalf;
     static constexpr int kPiece = 64, kPieceHalf = kPiece * 128, kPieceBytes = 2 * kPieceHalf;   // V: 64 keys, two halves of 64 dimensions
     static constexpr int kKStages = TERMS == 3 ? 2 : 3, kVStages = TERMS == 3 ? 3 : 5;
     static constexpr int kK0 = TERMS * 2 * kHalf, kV0 = kK0 + kKStages * kKBytes, kBars = kV0 + kVStages * kPieceBytes;
-    static constexpr int kPair = kBars + 256, kSmem = kPair + 2 * 2 * kRows * 4 + 1024;
-    static constexpr int kSoftWarps = 8, kKWarp = 8, kVWarp = 9, kMmaWarp = 10, kThreads = 12 * 32;
-    static constexpr uint32_t kColS = 0, kColO = 128, kColP = 256;                                // term x of P at kColP + 64 x
+    static constexpr int kPair = kBars + 256, kSmem = kPair + 2 * 4 * kRows * 4 + 1024;
+    static constexpr int kSoftWarps = 16, kKWarp = 16, kVWarp = 17, kMmaWarp = 18, kThreads = 20 * 32;
+    // Scores (128 columns) and, when all have been read, the probabilities (64 a term) of even blocks in one place, of odd ones in another
+    static constexpr uint32_t kPlace = 192, kColO = 384;
 };
 struct ManyShared {
     Line line;
@@ -502,7 +538,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
     const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t *sm = smem_raw + (base - raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int kKFull = 0, kKEmpty = 3, kVFull = 6, kVEmpty = 11, kQFull = 16, kSFull = 17, kSFree = 18, kPReady = 19, kOFull = 20;
+    constexpr int kKFull = 0, kKEmpty = 3, kVFull = 6, kVEmpty = 11, kQFull = 16, kPReady = 17, kOFull = 18, kSFull = 19;  // scores: one for even, one for odd blocks
     auto bar = [&](int i) { return base + M::kBars + i * 8; };
     volatile int *abort = &sh.abort;
     if (tid == 0) {
@@ -514,30 +550,33 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
             ptx::mbar_init(bar(kVFull + s), 1);
             ptx::mbar_init(bar(kVEmpty + s), 1);
         }
-        for (int i : {kQFull, kSFree, kPReady}) ptx::mbar_init(bar(i), M::kSoftWarps);
-        for (int i : {kSFull, kOFull}) ptx::mbar_init(bar(i), 1);
+        for (int i : {kQFull, kPReady}) ptx::mbar_init(bar(i), M::kSoftWarps);
+        for (int i : {kSFull, kSFull + 1, kOFull}) ptx::mbar_init(bar(i), 1);
         sh.abort = sh.odd = 0;
         ptx::fence_barrier_init();
     }
-    ptx::pdl_trigger();
-    ptx::pdl_wait();
-    cut_line<M::kRows, M::kKeys>(p, sh.line);
-    const int units = sh.line.first[p.b], u0 = share_begin(units, blockIdx.x, p.workers), u1 = share_begin(units, blockIdx.x + 1, p.workers);
-    if (u0 == u1) return;
     if (warp == M::kMmaWarp) {
         tc::tmem_alloc(ptx::smem_u32(&sh.tmem), 512);
         tc::tmem_relinquish();
     }
     tc::tc_fence_before();
-    __syncthreads();
+    ptx::pdl_wait();
+    ptx::pdl_trigger();  // behind the wait: what the merging kernel reads in front of its own is settled then
+    cut_line<M::kRows, M::kKeys>(p, sh.line);
     tc::tc_fence_after();
     const uint32_t tmem = *static_cast<volatile uint32_t *>(&sh.tmem);
+    const Shares shares(sh.line.first[p.b], p.workers);
+    const int u0 = shares.begin(blockIdx.x), u1 = shares.begin(blockIdx.x + 1);
+    if (u0 == u1) {
+        if (warp == M::kMmaWarp) tc::tmem_dealloc(tmem, 512);
+        return;
+    }
     const int group = p.nh / p.kvh;
     bool ok = true;
 
-    // The launch has 12 warps x 168 registers; 4 x 72 + 8 x 216 are as many.
+    // The launch has 20 warps x 96 registers; 4 x 64 + 16 x 104 are as many.
     if (warp >= M::kSoftWarps) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == M::kKWarp || warp == M::kVWarp) {
             // ================= TMA producers =================
             const bool is_k = warp == M::kKWarp;
@@ -593,9 +632,9 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
 #pragma unroll
                         for (int st = 0; st < 8; ++st) {
                             const uint64_t off = static_cast<uint64_t>((st >> 2) * (M::kHalf >> 4) + (st & 3) * 2);
-                            tc::umma_f16_ss(tmem + M::kColS, q_desc + static_cast<uint64_t>(x * 2 * (M::kHalf >> 4)) + off, k_desc + off, idesc_s, x < TERMS - 1 || st ? 1u : 0u);
+                            tc::umma_f16_ss(tmem + (n & 1) * M::kPlace, q_desc + static_cast<uint64_t>(x * 2 * (M::kHalf >> 4)) + off, k_desc + off, idesc_s, x < TERMS - 1 || st ? 1u : 0u);
                         }
-                    tc::umma_commit(bar(kSFull));
+                    tc::umma_commit(bar(kSFull + (n & 1)));
                     tc::umma_commit(bar(kKEmpty + ks));
                 }
                 __syncwarp();
@@ -609,9 +648,10 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                 const Segment s = segment_at(p, sh.line, u, u1, M::kRows, M::kKeys);
                 const int blocks = s.end - s.begin;
                 if (wait(kQFull, seg & 1)) scores();
-                for (int j = 1; j <= blocks && ok; ++j) {  // P V of block j - 1, scores of block j + 1
-                    if (j == 1 && blocks > 1 && wait(kSFree, (n - 1) & 1)) scores();
-                    const int done = n - (j < blocks ? 2 : 1);  // the number, in the whole walk, of the block whose P V this is
+                // Products are carried out in the order they are asked for: the scores of block j + 1 go where the probabilities of block j - 1 were read from
+                if (ok && blocks > 1) scores();
+                for (int j = 0; j < blocks && ok; ++j) {
+                    const int done = n - (j + 1 < blocks ? 2 : 1);  // the number, in the whole walk, of block j
                     if (!wait(kPReady, done & 1)) break;
 #pragma unroll 1
                     for (int piece = 0; piece < 2; ++piece) {
@@ -623,7 +663,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                             for (int st = 0; st < 4; ++st)  // 16 keys: 8 columns of P, two groups of V
 #pragma unroll
                                 for (int x = TERMS - 1; x >= 0; --x)
-                                    tc::umma_f16_ts(tmem + M::kColO, tmem + M::kColP + x * 64 + (piece * 4 + st) * 8, v_desc + static_cast<uint64_t>(st * (2048 >> 4)), idesc_o,
+                                    tc::umma_f16_ts(tmem + M::kColO, tmem + (done & 1) * M::kPlace + x * 64 + (piece * 4 + st) * 8, v_desc + static_cast<uint64_t>(st * (2048 >> 4)), idesc_o,
                                                     piece || st || x < TERMS - 1 ? 1u : 0u);
                             tc::umma_commit(bar(kVEmpty + vs));
                             if (piece) tc::umma_commit(bar(kOFull));
@@ -634,18 +674,17 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                             vphase ^= 1;
                         }
                     }
-                    // block j is in the softmax warps' registers: its scores' place is free
-                    if (j + 1 < blocks && wait(kSFree, (n - 1) & 1)) scores();
+                    if (ok && j + 2 < blocks) scores();
                 }
                 u += blocks;
             }
         }
     } else {
         // ================= softmax =================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        const int quad = warp & 3, kh2 = warp >> 2, r = quad * 32 + lane;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        const int quad = warp & 3, part = warp >> 2, r = quad * 32 + lane;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-        float *const s_pair = reinterpret_cast<float *>(sm + M::kPair);
+        float *const s_quad = reinterpret_cast<float *>(sm + M::kPair);  // [2][4 parts][128 rows]
         auto wait = [&](int i, int parity) {
             if (ok) ok = tc::warp_wait(bar(i), parity, abort);
             return ok;
@@ -655,41 +694,27 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
             if (lane == 0) ptx::mbar_arrive(bar(i));
         };
         auto meet = [&]() { ptx::named_barrier(1, M::kSoftWarps * 32); };
-        auto pair_sync = [&]() { ptx::named_barrier(2 + quad, 64); };  // the two warps of a quadrant
+        auto quad_sync = [&]() { ptx::named_barrier(2 + quad, 128); };  // the four warps of a quadrant
         int n = 0;  // blocks so far, over all segments
         for (int u = u0; u < u1;) {
             const Segment s = segment_at(p, sh.line, u, u1, M::kRows, M::kKeys);
             const int pos = sh.line.pos[s.seq], count = sh.line.count[s.seq];
-            const int rows_all = count * group, row0 = s.tile * M::kRows, row = row0 + r, node = row / group;
+            const int rows_all = count * group, row0 = s.tile * M::kRows, row = row0 + r, node = p.node_of(row);
             const bool nodes = s.end * M::kKeys > pos, live = row0 + quad * 32 < rows_all;  // some blocks hold nodes; some row of the warp exists
             meet();  // nobody reads what the last segment left in the queries' place and in the tree's any more
-            if (nodes)
-                for (int i = tid; i < count; i += M::kSoftWarps * 32) {
-                    const int up = p.parents[static_cast<size_t>(s.seq) * p.t + i];
-                    const bool good = up >= -1 && up < i;
-                    if (!good) atomicExch(p.err_word, kErrTree);
-                    sh.parent[i] = good ? up : -1;
-                }
-            // the tile's queries, a row as one load of a warp; in the K-major SWIZZLE_128B layout (row r of a half at r * 128, its 16-byte units XOR-ed with r & 7)
-#pragma unroll 8
-            for (int i = 0; i < 16; ++i) {
-                const int qr = warp * 16 + i, at_row = row0 + qr, at_node = at_row / group;
-                uint32_t x01[TERMS] = {}, x23[TERMS] = {};
-                if (at_row < rows_all) {
-                    const size_t at = (static_cast<size_t>(s.seq) * p.t + at_node) * p.q_pitch + static_cast<size_t>(s.kh * group + at_row - at_node * group) * kHd + lane * 4;
-                    if (TERMS > 1) {
-                        const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + at);
-                        split_pair<TERMS>(a.x, a.y, x01);
-                        split_pair<TERMS>(a.z, a.w, x23);
-                    } else {
-                        const uint2 a = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p.q) + at);
-                        x01[0] = a.x;
-                        x23[0] = a.y;
-                    }
-                }
-                uint8_t *dst = sm + (lane >> 4) * M::kHalf + qr * 128 + ((((lane & 15) >> 1) ^ (qr & 7)) << 4) + (lane & 1) * 8;
+            // the tile's queries, a row as one load of a warp, all of them asked for before the first is looked at; in the K-major SWIZZLE_128B layout
+            // (row r of a half at r * 128, its 16-byte units XOR-ed with r & 7)
+            float4 qv[8];
 #pragma unroll
-                for (int x = 0; x < TERMS; ++x) *reinterpret_cast<uint2 *>(dst + x * 2 * M::kHalf) = make_uint2(x01[x], x23[x]);
+            for (int i = 0; i < 8; ++i) qv[i] = query<TERMS>(p, s.seq, s.kh, group, row0 + warp * 8 + i, rows_all, lane);
+            if (nodes) load_parents(p, sh.parent, s.seq, count, M::kSoftWarps * 32);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                uint2 term[TERMS];
+                query_terms<TERMS>(qv[i], term);
+                uint8_t *dst = sm + (lane >> 4) * M::kHalf + (warp * 8 + i) * 128 + ((((lane & 15) >> 1) ^ i) << 4) + (lane & 1) * 8;
+#pragma unroll
+                for (int x = 0; x < TERMS; ++x) *reinterpret_cast<uint2 *>(dst + x * 2 * M::kHalf) = term[x];
             }
             ptx::fence_proxy_async();  // the tensor core reads them through the asynchronous proxy
             arrive(kQFull);
@@ -698,147 +723,135 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                 for (int i = tid; i < count; i += M::kSoftWarps * 32) tree_masks(sh.parent, sh.mask, i);
                 meet();
             }
-            float acc[64], m = kNoMax, l = 0.0f, corr = 0.0f;  // 64 dimensions of the row; corr: what brings acc to the present maximum
+            float acc[32], m = kNoMax, l = 0.0f, corr = 0.0f;  // 32 dimensions of the row; corr: what brings acc to the present maximum
 #pragma unroll
-            for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
+            for (int i = 0; i < 32; ++i) acc[i] = 0.0f;
             // acc = acc * corr + the products of block n - 1
             auto add_products = [&]() {
                 tc::tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < 2; ++c) {
                     uint32_t v[16];
-                    tc::tmem_ld16(lanes + M::kColO + kh2 * 64 + c * 16, v);
+                    tc::tmem_ld16(lanes + M::kColO + part * 32 + c * 16, v);
                     tc::tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 16; ++i) acc[c * 16 + i] = acc[c * 16 + i] * corr + __uint_as_float(v[i]);
                 }
             };
             for (int j = s.begin; j < s.end; ++j, ++n) {
-                uint32_t sv[64];
-                const int key0 = j * M::kKeys + kh2 * 64;
+                uint32_t sv[32];
+                const int key0 = j * M::kKeys + part * 32;
+                const uint32_t place = lanes + (n & 1) * M::kPlace;
                 float step = 0.0f;
-                wait(kSFull, n & 1);
+                wait(kSFull + (n & 1), n >> 1 & 1);
                 if (live) {
                     tc::tc_fence_after();
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) tc::tmem_ld32(lanes + M::kColS + kh2 * 64 + c * 32, reinterpret_cast<uint32_t(&)[32]>(sv[c * 32]));
+                    tc::tmem_ld32(place + part * 32, sv);
                     tc::tmem_ld_wait();
-                    tc::tc_fence_before();
-                }
-                arrive(kSFree);
-                if (live) {
-                    if (key0 + 64 > pos) {  // some of these keys are nodes, or nothing: bit i of `seen` is key0 + i
+                    if (key0 + 32 > pos) {  // some of these keys are nodes, or nothing: bit i of `seen` is key0 + i
                         const ulonglong2 mine = row < rows_all ? sh.mask[node] : make_ulonglong2(0ull, 0ull);
                         const int n0 = key0 - pos;
-                        const unsigned long long seen = n0 < 0 ? mine.x << -n0 | ((1ull << -n0) - 1) : n0 == 0 ? mine.x : n0 < 64 ? mine.x >> n0 | mine.y << (64 - n0) : n0 < 128 ? mine.y >> (n0 - 64) : 0ull;
+                        const uint32_t seen = static_cast<uint32_t>(n0 < 0 ? mine.x << -n0 | ((1ull << -n0) - 1) : n0 == 0 ? mine.x : n0 < 64 ? mine.x >> n0 | mine.y << (64 - n0) : n0 < 128 ? mine.y >> (n0 - 64) : 0ull);
 #pragma unroll
-                        for (int i = 0; i < 64; ++i)
+                        for (int i = 0; i < 32; ++i)
                             if (!(seen >> i & 1)) sv[i] = 0xff800000u;  // -inf
                     }
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(sv[i]));
-                    float *pair = s_pair + (n & 1) * 2 * M::kRows;
-                    const float own = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    pair[kh2 * M::kRows + r] = own;
-                    pair_sync();  // the next block but one writes here again, behind the next block's meeting
-                    const float nm = fmaxf(m, fmaxf(own, pair[(kh2 ^ 1) * M::kRows + r]) * p.scale);
+                    for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(sv[i]));
+                    float *quarter = s_quad + (n & 1) * 4 * M::kRows + r;
+                    quarter[part * M::kRows] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    quad_sync();  // the row's scores have all been read; the next block but one writes here again, behind the next block's meeting
+                    const float all = fmaxf(fmaxf(quarter[0], quarter[M::kRows]), fmaxf(quarter[2 * M::kRows], quarter[3 * M::kRows]));
+                    const float nm = fmaxf(m, all * p.scale);
                     step = ex2(m - nm);
                     m = nm;
                     float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 64; i += 2) {
-                        const float e0 = ex2(__fmaf_rn(__uint_as_float(sv[i]), p.scale, -nm)), e1 = ex2(__fmaf_rn(__uint_as_float(sv[i + 1]), p.scale, -nm));
-                        sum0 += e0;
-                        sum1 += e1;
-                        sv[i] = __float_as_uint(e0);
-                        sv[i + 1] = __float_as_uint(e1);
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t w[TERMS][8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float e0 = ex2(__fmaf_rn(__uint_as_float(sv[c * 16 + 2 * i]), p.scale, -nm)), e1 = ex2(__fmaf_rn(__uint_as_float(sv[c * 16 + 2 * i + 1]), p.scale, -nm));
+                            sum0 += e0;
+                            sum1 += e1;
+                            uint32_t term[TERMS];
+                            split_pair<TERMS>(e0, e1, term);
+#pragma unroll
+                            for (int x = 0; x < TERMS; ++x) w[x][i] = term[x];
+                        }
+#pragma unroll
+                        for (int x = 0; x < TERMS; ++x) tc::tmem_st8(place + x * 64 + part * 16 + c * 8, w[x]);
                     }
                     l = l * step + (sum0 + sum1);
                 }
-                // the products of the block in front are complete: they are added, and the probabilities' place is free
+                if (j * M::kKeys + M::kKeys > pos) {  // values past the last node, and values of nodes that are no numbers: a thread 32 dimensions of a row of this warp's piece
+                    const int piece = 2 * n + (part >> 1), vs = piece % M::kVStages, quarter = (part & 1) * 2 + (r >> 6), key = r & 63, at = j * M::kKeys + (part >> 1) * 64 + key - pos;
+                    if (wait(kVFull + vs, (piece / M::kVStages) & 1) && at >= 0) {
+                        uint4 *v = reinterpret_cast<uint4 *>(sm + M::kV0 + vs * M::kPieceBytes + (quarter >> 1) * M::kPieceHalf + key * 128 + (quarter & 1) * 64);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint4 x = v[i];
+                            if (at >= count) {
+                                v[i] = make_uint4(0u, 0u, 0u, 0u);
+                            } else {
+                                const uint4 y = make_uint4(only_numbers(x.x), only_numbers(x.y), only_numbers(x.z), only_numbers(x.w));
+                                if (((x.x ^ y.x) | (x.y ^ y.y) | (x.z ^ y.z) | (x.w ^ y.w)) != 0u) {
+                                    v[i] = y;
+                                    sh.odd = u + 1;  // read behind a meeting below, written again behind the next segment's first
+                                }
+                            }
+                        }
+                    }
+                    ptx::fence_proxy_async();
+                }
+                // the products of the block in front are added, then their place is free
                 if (j > s.begin) {
                     wait(kOFull, (n - 1) & 1);
                     if (live) add_products();
                 }
                 corr = step;
-                if (live) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t w[TERMS][16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            uint32_t term[TERMS];
-                            split_pair<TERMS>(__uint_as_float(sv[c * 32 + 2 * i]), __uint_as_float(sv[c * 32 + 2 * i + 1]), term);
-#pragma unroll
-                            for (int x = 0; x < TERMS; ++x) w[x][i] = term[x];
-                        }
-#pragma unroll
-                        for (int x = 0; x < TERMS; ++x) tc::tmem_st16(lanes + M::kColP + x * 64 + kh2 * 32 + c * 16, w[x]);
-                    }
-                }
-                if (j * M::kKeys + M::kKeys > pos) {  // values past the last node, and values of nodes that are no numbers: a thread half a row of this warp's piece
-                    const int piece = 2 * n + kh2, vs = piece % M::kVStages, key = r & 63, at = key0 + key - pos;
-                    if (wait(kVFull + vs, (piece / M::kVStages) & 1) && at >= 0) {
-                        uint4 *v = reinterpret_cast<uint4 *>(sm + M::kV0 + vs * M::kPieceBytes + (r >> 6) * M::kPieceHalf + key * 128);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            uint4 x = v[i];
-                            bool strange = false;
-                            for (uint32_t *w = &x.x; w <= &x.w; ++w)
-#pragma unroll
-                                for (int e = 0; e < 2; ++e)
-                                    if (at >= count || ((*w >> (16 * e)) & 0x7f80u) == 0x7f80u) {
-                                        *w &= e ? 0x0000ffffu : 0xffff0000u;
-                                        strange = true;
-                                    }
-                            if (strange) v[i] = x;
-                            if (strange && at < count) sh.odd = u + 1;  // read behind a meeting below, written again behind the next segment's first
-                        }
-                    }
-                    ptx::fence_proxy_async();
-                }
                 if (live) tc::tmem_st_wait();
                 tc::tc_fence_before();
                 arrive(kPReady);
             }
             wait(kOFull, (n - 1) & 1);
             if (live) add_products();
-            // the row's weight: the two halves of the keys meet
-            float *pair = s_pair + (n & 1) * 2 * M::kRows;
-            pair[kh2 * M::kRows + r] = l;
+            // the row's weight: the four parts of the keys meet
+            float *quarter = s_quad + (n & 1) * 4 * M::kRows + r;
+            quarter[part * M::kRows] = l;
             meet();
-            l += pair[(kh2 ^ 1) * M::kRows + r];
+            l = (quarter[0] + quarter[M::kRows]) + (quarter[2 * M::kRows] + quarter[3 * M::kRows]);
             if (nodes && sh.odd == u + 1 && row < rows_all) {  // what this row sees that is no number
                 const ulonglong2 mine = sh.mask[node];
                 for (int i = max(0, s.begin * M::kKeys - pos); i < min(count, s.end * M::kKeys - pos); ++i) {
                     if (!sees(mine, i)) continue;
-                    const uint16_t *v = p.vcache + (static_cast<size_t>(s.seq * p.kvh + s.kh) * p.cap + pos + i) * kHd + kh2 * 64;
+                    const uint16_t *v = p.vcache + (static_cast<size_t>(s.seq * p.kvh + s.kh) * p.cap + pos + i) * kHd + part * 32;
 #pragma unroll
-                    for (int d = 0; d < 64; ++d)
+                    for (int d = 0; d < 32; ++d)
                         if ((v[d] & 0x7f80u) == 0x7f80u) acc[d] += dense::bf16_f32(v[d]);
                 }
             }
-            // Rows leave through the queries' place, whose products are done, so that a store writes whole lines: a warp's 32 rows of 32 dimensions at a
-            // time, 16-byte units XOR-ed with the row.
+            // Rows leave through the queries' place, whose products are done, so that a store instruction writes whole sectors: a warp's 32 rows of 16
+            // dimensions at a time, 16-byte units XOR-ed with the row.
             const bool whole = s.begin == 0 && s.end == s.blocks;
             if (live && ok) {
                 const float inv = whole ? 1.0f / l : 1.0f;
                 const size_t part0 = (static_cast<size_t>(blockIdx.x) * 2 + (u == u0 ? 0 : 1)) * M::kRows;
-                if (!whole && kh2 == 0 && row < rows_all) p.part_ml[part0 + r] = make_float2(m, l);
-                float *own = reinterpret_cast<float *>(sm + warp * 4096);
+                if (!whole && part == 0 && row < rows_all) p.part_ml[part0 + r] = make_float2(m, l);
+                float *own = reinterpret_cast<float *>(sm + warp * 2048);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<float4 *>(own + lane * 32 + ((i ^ (lane & 7)) << 2)) =
-                            make_float4(acc[c * 32 + 4 * i] * inv, acc[c * 32 + 4 * i + 1] * inv, acc[c * 32 + 4 * i + 2] * inv, acc[c * 32 + 4 * i + 3] * inv);
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<float4 *>(own + lane * 16 + ((i ^ (lane >> 1 & 3)) << 2)) =
+                            make_float4(acc[c * 16 + 4 * i] * inv, acc[c * 16 + 4 * i + 1] * inv, acc[c * 16 + 4 * i + 2] * inv, acc[c * 16 + 4 * i + 3] * inv);
                     __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int rr = i * 4 + (lane >> 3), at_row = row0 + quad * 32 + rr, at_node = at_row / group, d = kh2 * 64 + c * 32 + (lane & 7) * 4;
+                    for (int i = 0; i < 4; ++i) {
+                        const int rr = i * 8 + (lane >> 2), at_row = row0 + quad * 32 + rr, at_node = p.node_of(at_row), d = part * 32 + c * 16 + (lane & 3) * 4;
                         if (at_row < rows_all) {
-                            const float4 x = *reinterpret_cast<const float4 *>(own + rr * 32 + (((lane & 7) ^ (rr & 7)) << 2));
+                            const float4 x = *reinterpret_cast<const float4 *>(own + rr * 16 + (((lane & 3) ^ (rr >> 1 & 3)) << 2));
                             const size_t at = (static_cast<size_t>(s.seq) * p.t + at_node) * p.out_pitch + static_cast<size_t>(s.kh * group + at_row - at_node * group) * kHd + d;
                             if (!whole) *reinterpret_cast<float4 *>(p.part + (part0 + quad * 32 + rr) * kHd + d) = x;
                             else if (TERMS > 1) dense::put4(static_cast<float *>(p.out) + at, x);
@@ -860,54 +873,49 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
     }
 }
 
-// Joins the parts of the tiles that were cut: a warp a row, four dimensions a lane.
+// Joins the parts of the tiles that were cut. A block takes some rows of the tile that begins in its worker's share and ends behind it, if there is one: a
+// warp a row, four dimensions a lane. Which that is is known before the attention kernel is done.
+constexpr int kMergeRows = 16;  // rows a block
 template <int TERMS, int ROWS, int KEYS>
-__global__ void __launch_bounds__(256) attn_tree_merge_kernel(const __grid_constant__ TreeParams p) {
+__global__ void __launch_bounds__(kMergeRows * 32) attn_tree_merge_kernel(const __grid_constant__ TreeParams p) {
     __shared__ Line line;
     ptx::pdl_trigger();
-    ptx::pdl_wait();
     cut_line<ROWS, KEYS>(p, line);
-    const int group = p.nh / p.kvh, tiles_most = (p.t * group + ROWS - 1) / ROWS, lane = threadIdx.x & 31;
-    const int seq = blockIdx.x / (p.kvh * tiles_most), rest = blockIdx.x - seq * p.kvh * tiles_most, kh = rest / tiles_most, tile = rest - kh * tiles_most;
-    const int r = blockIdx.y * 8 + (threadIdx.x >> 5), row = tile * ROWS + r, node = row / group;
-    if (row >= line.count[seq] * group) return;
-    const int units = line.first[p.b], blocks = line_blocks(line, seq, KEYS);
-    const int begin = line.first[seq] + (kh * line_tiles(line, seq, group, ROWS) + tile) * blocks;
-    auto owner = [&](int u) { return static_cast<int>((static_cast<long long>(u + 1) * p.workers - 1) / units); };
-    const int c0 = owner(begin), c1 = owner(begin + blocks - 1);
-    if (c0 == c1) return;  // written by its worker
-    auto place = [&](int c) { return (static_cast<size_t>(c) * 2 + (c == c0 && share_begin(units, c, p.workers) < begin ? 1 : 0)) * ROWS + r; };
-    auto part_of = [&](int c) {  // maximum and weight; a worker without a share left nothing
-        const bool any = c <= c1 && share_begin(units, c, p.workers) < share_begin(units, c + 1, p.workers);
-        return any ? p.part_ml[place(c)] : make_float2(kNoMax, 0.0f);
-    };
+    const Shares shares(line.first[p.b], p.workers);
+    const int lane = threadIdx.x & 31, r = blockIdx.y * kMergeRows + (threadIdx.x >> 5), group = p.nh / p.kvh, c0 = blockIdx.x;
+    const int u0 = shares.begin(c0), u1 = shares.begin(c0 + 1);
+    Segment s{};
+    int begin = 0, row = 0, parts = 0;
+    if (u0 < u1) {
+        s = segment_at(p, line, u1 - 1, u1, ROWS, KEYS);  // the last block of the share
+        begin = u1 - 1 - s.begin;
+        row = s.tile * ROWS + r;
+        const int end = begin + s.blocks;
+        if (begin >= u0 && end > u1 && row < line.count[s.seq] * group) parts = shares.owner(end - 1) - c0 + 1;  // neighbours that all have a share: this tile goes on in it
+    }
+    ptx::pdl_wait();  // blocks without a tile too: the next kernel of the stream waits for this one only
+    if (!parts) return;
+    const int node = p.node_of(row);
+    auto place = [&](int i) { return (static_cast<size_t>(c0 + i) * 2 + (i == 0 && u0 < begin ? 1 : 0)) * ROWS + r; };
     float m = kNoMax;
-    for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, part_of(c).x);
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.part_ml[place(i)].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.0f;
-    for (int base = c0; base <= c1; base += 32) {
-        const float2 ml = part_of(base + lane);
-        const float w = ex2(ml.x - m);
-        const bool any = base + lane <= c1 && share_begin(units, base + lane, p.workers) < share_begin(units, base + lane + 1, p.workers);
-        const unsigned some = __ballot_sync(0xffffffffu, any);
-        l += any ? ml.y * w : 0.0f;
 #pragma unroll 4
-        for (int i = 0; i < min(32, c1 - base + 1); ++i) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            if (!(some >> i & 1)) continue;
-            const float4 x = *reinterpret_cast<const float4 *>(p.part + place(base + i) * kHd + lane * 4);
-            sum.x += x.x * wi;
-            sum.y += x.y * wi;
-            sum.z += x.z * wi;
-            sum.w += x.w * wi;
-        }
+    for (int i = 0; i < parts; ++i) {
+        const float2 ml = p.part_ml[place(i)];
+        const float4 x = *reinterpret_cast<const float4 *>(p.part + place(i) * kHd + lane * 4);
+        const float w = ex2(ml.x - m);
+        l += ml.y * w;
+        sum.x += x.x * w;
+        sum.y += x.y * w;
+        sum.z += x.z * w;
+        sum.w += x.w * w;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     const float inv = 1.0f / l;
-    const size_t at = (static_cast<size_t>(seq) * p.t + node) * p.out_pitch + static_cast<size_t>(kh * group + row - node * group) * kHd + lane * 4;
+    const size_t at = (static_cast<size_t>(s.seq) * p.t + node) * p.out_pitch + static_cast<size_t>(s.kh * group + row - node * group) * kHd + lane * 4;
     if (TERMS > 1) dense::put4(static_cast<float *>(p.out) + at, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
     else dense::put4(static_cast<uint16_t *>(p.out) + at, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
 }
@@ -925,11 +933,10 @@ int tile_rows(size_t t, size_t group) { return t * group <= 16 ? 16 : t * group 
 
 template <int ROWS, int KEYS>
 int launch_tree(Ctx *ctx, int terms, TreeParams &p, void (*one)(TreeParams), void (*three)(TreeParams), int threads, int smem, cudaStream_t st) {
-    const int group = p.nh / p.kvh, tiles = (p.t * group + ROWS - 1) / ROWS;
     LBK_CUDA(launch_chained(terms == 3 ? three : one, dim3(static_cast<unsigned>(p.workers)), dim3(threads), static_cast<size_t>(smem), st, p));
     ctx->launches++;
-    LBK_CUDA(launch_chained(terms == 3 ? attn_tree_merge_kernel<3, ROWS, KEYS> : attn_tree_merge_kernel<1, ROWS, KEYS>, dim3(static_cast<unsigned>(p.b * p.kvh * tiles), ROWS / 8), dim3(256), 0, st,
-                            p));
+    const dim3 grid(static_cast<unsigned>(p.workers), (std::min(ROWS, p.t * (p.nh / p.kvh)) + kMergeRows - 1) / kMergeRows);
+    LBK_CUDA(launch_chained(terms == 3 ? attn_tree_merge_kernel<3, ROWS, KEYS> : attn_tree_merge_kernel<1, ROWS, KEYS>, grid, dim3(kMergeRows * 32), 0, st, p));
     ctx->launches++;
     return LBK_OK;
 }
@@ -961,7 +968,7 @@ int lbk_attn_tree(lbk_ctx *c, int compute, const void *q_dev, size_t q_pitch, co
     if ((reinterpret_cast<uintptr_t>(q_dev) | reinterpret_cast<uintptr_t>(kcache_dev) | reinterpret_cast<uintptr_t>(vcache_dev) | reinterpret_cast<uintptr_t>(scratch_dev) |
          reinterpret_cast<uintptr_t>(out_dev)) & 15)
         return fail(LBK_ERR_SHAPE, "lbk_attn_tree: buffers lie on 16 bytes");
-    if (n_heads > 65536 || cap > (1u << 30)) return fail(LBK_ERR_UNSUPPORTED, "lbk_attn_tree: %zu heads, %zu positions", n_heads, cap);
+    if (n_heads > 4096 || cap > (1u << 30)) return fail(LBK_ERR_UNSUPPORTED, "lbk_attn_tree: %zu heads, %zu positions", n_heads, cap);
     const size_t rows = b * kv_heads * cap, group = n_heads / kv_heads;
     if (rows > INT32_MAX || b * kv_heads * ((t * group + 15) / 16) * (cap / 64 + 1) > INT32_MAX)
         return fail(LBK_ERR_UNSUPPORTED, "lbk_attn_tree: a cache of %zu rows", rows);
@@ -981,6 +988,7 @@ int lbk_attn_tree(lbk_ctx *c, int compute, const void *q_dev, size_t q_pitch, co
     p.cap = static_cast<int>(cap);
     p.scale = scale * 1.4426950408889634f;
     p.workers = ctx->sm_count;
+    p.per_group = group > 1 ? static_cast<unsigned>((0x100000000ull + group - 1) / group) : 0u;  // exact: rows * heads of a group < 2^32
     p.err_word = ctx->err_word;
     const int tile = tile_rows(t, group), terms = compute == LBK_COMPUTE_F32 ? 3 : 1;
     p.part = scratch_dev;

@@ -49,17 +49,18 @@ __device__ __forceinline__ int key_id(unsigned long long key) { return static_ca
 
 // One pass over the row. A thread keeps the maximum m of what it has seen, s = sum e^(c (x - m)) and t = sum e^(c (x - m)) (x - m); entropy = log s - c t / s.
 //
-// The alternatives come out of the same pass. A warp's `each`-th largest lane maximum is a bound that `each` of its values reach; the least of the bounds of
-// all warps is reached by `top` values (each = top / warps, rounded up), so what lies below it is none of them. Values that reach it go to a list in shared memory, some hundred of
-// 128256; bounds rise as the row goes by and are read without a barrier (an old one is a bound too). At the end the list is put in order. Rows whose list runs
-// over (most values equal, or ascending), or has too few (most of them -inf), and rows with a NaN or +inf are read again, once an alternative.
+// The alternatives come out of the same pass. Eight threads show their maximum, and at least `top` values reach the `top`-th
+// largest of the 32 maxima that are shown: what lies below it is none of the alternatives. Values that reach it go to a list in shared memory, a hundred or so of 128256; the
+// bound is looked for again after 2, 4, 8, .. trips, without a barrier (what other threads show may be old: a bound all the same). At the end the list is put in
+// order. Rows whose list runs over (most values equal, or ascending), or has too few (most of them -inf), and rows with a NaN or +inf are read again, once an
+// alternative.
 //
 // Bytes bound it: 2000 rows of 128256 f32 are 1.03 GB. A row is cut among the CTAs of a cluster where there are fewer rows than the SMs hold CTAs; they
 // meet through distributed shared memory.
-constexpr int kThreads = 512, kWarps = kThreads / 32, kLoads = 4;  // 16-byte loads of a thread in flight
-constexpr int kList = 4096;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kLoads = 4;  // 16-byte loads of a thread in flight
+constexpr int kList = 2048, kOrder = 512;  // keys on the list; how many of them are put in order by comparing all
 constexpr int kTop = LBK_LOGPROBS_TOP, kClusterMost = 16;
-static_assert(kTop <= 2 * kWarps && kClusterMost * kTop <= kThreads, "two maxima a warp, a key a thread");
+static_assert(kThreads == 8 * kTop && kClusterMost * kTop <= kOrder && kClusterMost <= 32, "a maximum of eight threads for each alternative");
 using Key = unsigned long long;
 
 struct Stats {
@@ -77,17 +78,32 @@ __device__ __forceinline__ void raise(Stats &a, float m, float c) {
     a.s *= r;
     a.m = m;
 }
-__device__ __forceinline__ void join(Stats &a, Stats b, float c) {
-    const float m = fmaxf(a.m, b.m);
-    raise(a, m, c);
-    raise(b, m, c);
-    a.s += b.s;
-    a.t += b.t;
-}
 __device__ __forceinline__ Stats join_warp(Stats a, float c) {
+    raise(a, value_of(__reduce_max_sync(0xffffffffu, order_value(a.m))), c);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) join(a, Stats{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.t, o)}, c);
+    for (int o = 16; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+    }
     return a;
+}
+// Two f32 operations in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(d)) : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(d)) : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long &>(d))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)), "l"(reinterpret_cast<unsigned long long &>(c)));
+    return d;
 }
 
 __device__ __forceinline__ void unpack(const uint4 &v, float (&x)[4]) {
@@ -105,26 +121,35 @@ __device__ __forceinline__ void unpack(const uint4 &v, float (&x)[8]) {
     }
 }
 
-struct RowShared {
+struct alignas(16) RowShared {
     Key list[kList];
-    Key best[kThreads];        // the keys that are put in order: some of the list, or all CTAs' alternatives
+    Key best[kOrder];          // the keys that are put in order
+    Key gathered[kOrder];      // all CTAs' alternatives
     Key top[kTop];             // this CTA's alternatives, in order
     Key warp_key[kWarps];
-    Stats warp_stats[kWarps], stats;
-    float bound[kWarps];
+    alignas(16) unsigned shown[kTop];  // order_value of eight threads' maxima
+    Stats warp_stats[kWarps], stats, cta_stats[kClusterMost];
+    float bound;
     int count, kept;
 };
 
-// The `top` largest of n keys of the shared memory, in order, into `out`, zeros behind them. n > kThreads: a search for each.
+// The `top` largest of n keys of the shared memory, in order, into `out`, zeros behind them. n > kOrder: a search for each.
 __device__ void put_in_order(const Key *keys, int n, int top, Key *out, Key *warp_key) {
     const int tid = threadIdx.x;
     if (tid < top) out[tid] = 0;
     __syncthreads();
-    if (n <= kThreads) {
-        if (tid < n) {
-            const Key mine = keys[tid];
-            int rank = 0;
-            for (int i = 0; i < n; ++i) rank += keys[i] > mine;
+    if (n <= kOrder) {
+        for (int k = tid; k < n; k += kThreads) {
+            const Key mine = keys[k];
+            int rank = 0, i = 0;
+            for (; i + 8 <= n; i += 8) {
+                ulonglong2 four[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) four[e] = *reinterpret_cast<const ulonglong2 *>(keys + i + 2 * e);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) rank += (four[e].x > mine) + (four[e].y > mine);
+            }
+            for (; i < n; ++i) rank += keys[i] > mine;
             if (rank < top && mine) out[rank] = mine;
         }
         __syncthreads();
@@ -150,9 +175,8 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ void cluster_meet() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t of_cta(const void *p, uint32_t rank) {  // the same place in another CTA of the cluster
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(ptx::smem_u32(p)), "r"(rank));
@@ -161,7 +185,7 @@ __device__ __forceinline__ uint32_t of_cta(const void *p, uint32_t rank) {  // t
 
 // ctas: how many share a row, neighbours in the grid and a cluster
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const ScoreParams p, int ctas) {
+__global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const ScoreParams p, int ctas) {
     constexpr int kVec = 16 / sizeof(T);
     __shared__ RowShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -174,71 +198,104 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const ScoreParams
     const int vectors = (p.vocab - lead) / kVec, odd = rank == 0 ? p.vocab - vectors * kVec : 0;
     const int v0 = static_cast<int>(static_cast<long long>(vectors) * rank / ctas), v1 = static_cast<int>(static_cast<long long>(vectors) * (rank + 1) / ctas);
     const uint4 *units = reinterpret_cast<const uint4 *>(x + lead);
-    const int each = (p.top + kWarps - 1) / kWarps;
-    if (tid == 0) sh.count = sh.kept = 0;
+    if (tid == 0) {
+        sh.count = sh.kept = 0;
+        sh.bound = -FLT_MAX;  // what a value has to reach to go on the list; -inf never does
+    }
+    if (ctas > 1) cluster_arrive();
     ptx::pdl_trigger();
     ptx::pdl_wait();
 
     Stats a{-FLT_MAX, 0.0f, 0.0f};
-    float floor = -FLT_MAX;  // what a value has to reach to go on the list; -inf never does
-    auto write_bound = [&]() {
-        unsigned mine = order_value(a.m);
-        unsigned best = __reduce_max_sync(0xffffffffu, mine);
-        if (each > 1) {  // the second largest: without one lane that has the largest
-            if (lane == __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1) mine = 0;
-            best = __reduce_max_sync(0xffffffffu, mine);
-        }
-        if (lane == 0) sh.bound[warp] = value_of(best);
+    auto show = [&]() {
+        float most = a.m;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        if ((tid & 7) == 0) sh.shown[tid >> 3] = order_value(most);
     };
-    auto read_bound = [&]() { floor = fmaxf(floor, value_of(__reduce_min_sync(0xffffffffu, order_value(static_cast<const volatile float *>(sh.bound)[lane % kWarps])))); };
+    auto look_up = [&]() {  // one warp; a lane finds the rank of one of the maxima
+        const unsigned mine = sh.shown[lane];
+        int rank = 0;
+#pragma unroll
+        for (int i = 0; i < kTop; i += 4) {
+            const uint4 other = *reinterpret_cast<const uint4 *>(sh.shown + i);
+            rank += (other.x > mine || (other.x == mine && i < lane)) + (other.y > mine || (other.y == mine && i + 1 < lane)) + (other.z > mine || (other.z == mine && i + 2 < lane)) +
+                    (other.w > mine || (other.w == mine && i + 3 < lane));
+        }
+        if (rank == p.top - 1) sh.bound = fmaxf(sh.bound, value_of(mine));
+    };
+    float floor = -FLT_MAX;
     auto list = [&](float v, int id) {
         if (v >= floor) {
             const int at = atomicAdd(&sh.count, 1);
             if (at < kList) sh.list[at] = order_key(v, id);
         }
     };
-    auto see = [&](float v) {
-        const float d = v - a.m, e = ex2(d * c);
-        a.s += e;
-        a.t += e * fmaxf(d, -1e30f);  // 0 * -inf is nothing here
+    float2 s2 = make_float2(0.0f, 0.0f), t2 = s2;  // the thread's sums, every other value each
+    const float2 c2 = make_float2(c, c);
+    auto see = [&](float2 v, float2 less) {
+        const float2 d = add2(v, less), f = mul2(d, c2), e = make_float2(ex2(f.x), ex2(f.y));
+        s2 = add2(s2, e);
+        t2 = fma2(e, make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), t2);  // 0 * -inf is nothing here
     };
     const float odd_value = tid < odd ? get(x + (tid < lead ? tid : tid + vectors * kVec)) : -INFINITY;
     const int odd_id = tid < lead ? tid : tid + vectors * kVec;
-    int trip = 0;
-    for (int base = v0; base < v1 || trip == 0; base += kThreads * kLoads, ++trip) {
-        uint4 raw[kLoads];
+    // the first tokens' values are asked for now
+    const bool one_given = rank == 0 && tid < p.given;
+    const int token0 = one_given ? p.tokens[row * p.given + tid] : -1;
+    const float given0 = token0 >= 0 && token0 < p.vocab ? get(x + token0) : 0.0f;
+    uint4 raw[kLoads], next[kLoads];
+    auto ask = [&](uint4 (&into)[kLoads], int base) {
 #pragma unroll
         for (int u = 0; u < kLoads; ++u) {
             const int i = base + u * kThreads + tid;
-            raw[u] = i < v1 ? __ldcs(units + i) : Empty<T>::vector();
+            into[u] = i < v1 ? __ldcs(units + i) : Empty<T>::vector();
         }
-        float high = trip == 0 ? odd_value : -INFINITY;
+    };
+    ask(next, v0);
+    int trip = 0;
+    for (int base = v0; base < v1 || trip == 0; base += kThreads * kLoads, ++trip) {
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) raw[u] = next[u];
+        ask(next, base + kThreads * kLoads);  // on their way while these are looked at
+        float high = trip == 0 ? odd_value : -INFINITY, vector_high[kLoads];
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+            float v[kVec];
+            unpack(raw[u], v);
+            vector_high[u] = v[0];
+#pragma unroll
+            for (int e = 1; e < kVec; ++e) vector_high[u] = fmaxf(vector_high[u], v[e]);
+            high = fmaxf(high, vector_high[u]);
+        }
+        if (high > a.m) {
+            const float d = a.m - high, r = ex2(d * c);
+            t2 = r == 0.0f ? make_float2(0.0f, 0.0f) : mul2(make_float2(r, r), fma2(s2, make_float2(d, d), t2));  // s * d may be -inf for the nothing in front
+            s2 = mul2(s2, make_float2(r, r));
+            a.m = high;
+        }
+        const float2 less = make_float2(-a.m, -a.m);
+        if (trip == 0) see(make_float2(odd_value, -INFINITY), less);
 #pragma unroll
         for (int u = 0; u < kLoads; ++u) {
             float v[kVec];
             unpack(raw[u], v);
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) high = fmaxf(high, v[e]);
-        }
-        if (high > a.m) raise(a, high, c);
-        if (trip == 0) see(odd_value);
-#pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-            float v[kVec];
-            unpack(raw[u], v);
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) see(v[e]);
+            for (int e = 0; e < kVec; e += 2) see(make_float2(v[e], v[e + 1]), less);
         }
         if (p.top) {
-            if ((trip & (trip - 1)) == 0) {  // after 1, 2, 4, .. trips' maxima
-                write_bound();
+            if ((trip & (trip + 1)) == 0) {  // after 1, 2, 4, .. trips
+                show();
+                if (trip == 0) __syncthreads();
+                if (warp == 0) look_up();
                 if (trip == 0) __syncthreads();
             }
-            read_bound();
+            floor = *static_cast<const volatile float *>(&sh.bound);
             if (high >= floor) {
                 if (trip == 0) list(odd_value, odd_id);
 #pragma unroll
                 for (int u = 0; u < kLoads; ++u) {
+                    if (vector_high[u] < floor) continue;
                     float v[kVec];
                     unpack(raw[u], v);
 #pragma unroll
@@ -247,29 +304,32 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const ScoreParams
             }
         }
     }
-    if (p.top) write_bound();
+    a.s = s2.x + s2.y;
+    a.t = t2.x + t2.y;
+    if (p.top) show();
     a = join_warp(a, c);
     if (lane == 0) sh.warp_stats[warp] = a;
     __syncthreads();
+    if (p.top && warp == 1) look_up();
     if (warp == 0) {
         a = join_warp(lane < kWarps ? sh.warp_stats[lane] : Stats{-FLT_MAX, 0.0f, 0.0f}, c);
         if (lane == 0) sh.stats = a;
     }
     if (p.top) {
-        read_bound();
+        __syncthreads();
         const int n = sh.count, here = (v1 - v0) * kVec + odd, want = min(p.top, here);
-        __syncthreads();  // sh.stats
         const float s = sh.stats.s;
+        floor = sh.bound;
         if (n <= kList && n >= want && s == s && s <= FLT_MAX) {
             // what reaches the last bounds
             const Key least = order_key(floor, 0x7fffffff);
             for (int i = tid; i < n; i += kThreads)
                 if (sh.list[i] >= least) {
                     const int at = atomicAdd(&sh.kept, 1);
-                    if (at < kThreads) sh.best[at] = sh.list[i];
+                    if (at < kOrder) sh.best[at] = sh.list[i];
                 }
             __syncthreads();
-            if (sh.kept <= kThreads) put_in_order(sh.best, sh.kept, p.top, sh.top, sh.warp_key);
+            if (sh.kept <= kOrder) put_in_order(sh.best, sh.kept, p.top, sh.top, sh.warp_key);
             else put_in_order(sh.list, n, p.top, sh.top, sh.warp_key);
         } else {
             // the largest value behind the last one found, `top` times over
@@ -299,40 +359,30 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const ScoreParams
         }
     }
     if (ctas > 1) {
-        cluster_meet();  // every CTA's sums and alternatives are in its shared memory
-        if (rank == 0) {
-            if (warp == 0) {
-                Stats b{-FLT_MAX, 0.0f, 0.0f};
-                if (lane < ctas) {
-                    const uint32_t at = of_cta(&sh.stats, lane);
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b.m) : "r"(at));
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b.s) : "r"(at + 4));
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b.t) : "r"(at + 8));
-                }
-                b = join_warp(b, c);
-                if (lane == 0) sh.warp_stats[0] = b;
-            }
-            if (p.top && tid < ctas * p.top)
-                asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(sh.best[tid]) : "r"(of_cta(sh.top + tid % p.top, tid / p.top)));
+        // the first CTA gets every CTA's sums and alternatives into its shared memory
+        __syncthreads();
+        cluster_wait();  // it has begun
+        if (tid < 3) {
+            const uint32_t at = of_cta(&sh.cta_stats[rank], 0) + tid * 4;
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(reinterpret_cast<const float *>(&sh.stats)[tid]) : "memory");
         }
-        cluster_meet();  // nobody leaves while its shared memory is read
+        if (tid < p.top) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(of_cta(sh.gathered + rank * p.top + tid, 0)), "l"(sh.top[tid]) : "memory");
+        cluster_arrive();
+        cluster_wait();
         if (rank != 0) return;
+        a = join_warp(lane < ctas ? sh.cta_stats[lane] : Stats{-FLT_MAX, 0.0f, 0.0f}, c);  // every warp the same
         if (p.top) {
             // a CTA whose last alternative is the largest has `top` that reach it: the others' behind that are none
-            Key least = tid < ctas ? sh.best[tid * p.top + p.top - 1] : 0;
+            Key least = lane < ctas ? sh.gathered[lane * p.top + p.top - 1] : 0;
+#pragma unroll
             for (int o = 16; o > 0; o >>= 1) least = max(least, __shfl_xor_sync(0xffffffffu, least, o));
-            if (tid == 0) {
-                sh.warp_key[0] = least;
-                sh.kept = 0;
-            }
+            if (tid == 0) sh.kept = 0;
             __syncthreads();
-            least = sh.warp_key[0];
-            if (tid < ctas * p.top && sh.best[tid] && sh.best[tid] >= least) sh.list[atomicAdd(&sh.kept, 1)] = sh.best[tid];
+            for (int i = tid; i < ctas * p.top; i += kThreads)
+                if (sh.gathered[i] && sh.gathered[i] >= least) sh.best[atomicAdd(&sh.kept, 1)] = sh.gathered[i];
             __syncthreads();
-            put_in_order(sh.list, sh.kept, p.top, sh.top, sh.warp_key);
+            put_in_order(sh.best, sh.kept, p.top, sh.top, sh.warp_key);
         }
-        __syncthreads();
-        a = sh.warp_stats[0];
     } else {
         __syncthreads();
         a = sh.stats;
@@ -340,14 +390,16 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const ScoreParams
     const float log_s = logf(a.s);
     auto logprob = [&](float v) { return (v - a.m) * p.scale - log_s; };
     if (tid == 0 && p.entropy) p.entropy[row] = log_s - a.t / a.s * p.scale;
-    for (int g = tid; g < p.given; g += kThreads) {
+    const float none = __uint_as_float(0x7fc00000u);
+    if (one_given) p.logprobs[row * p.given + tid] = token0 >= 0 && token0 < p.vocab ? logprob(given0) : none;
+    for (int g = tid + kThreads; g < p.given; g += kThreads) {
         const int token = p.tokens[row * p.given + g];
-        p.logprobs[row * p.given + g] = token >= 0 && token < p.vocab ? logprob(get(x + token)) : __uint_as_float(0x7fc00000u);
+        p.logprobs[row * p.given + g] = token >= 0 && token < p.vocab ? logprob(get(x + token)) : none;
     }
     if (tid < p.top) {
-        const int id = key_id(sh.top[tid]);
-        p.top_ids[row * p.top + tid] = id;
-        p.top_logprobs[row * p.top + tid] = logprob(get(x + id));
+        const Key key = sh.top[tid];
+        p.top_ids[row * p.top + tid] = key_id(key);
+        p.top_logprobs[row * p.top + tid] = logprob(value_of(static_cast<unsigned>(key >> 32)));
     }
 }
 
@@ -377,10 +429,11 @@ int lbk_token_logprobs(lbk_ctx *c, int dtype, const void *logits_dev, size_t pit
         return fail(LBK_ERR_UNSUPPORTED, "lbk_token_logprobs: at most %d alternatives, 2^30 values and 2^20 tokens a row, 2^26 rows", LBK_LOGPROBS_TOP);
     const ScoreParams p{logits_dev, pitch, static_cast<int>(vocab), tokens_dev, static_cast<int>(given), scale, static_cast<int>(top), logprobs_dev, entropy_dev, top_ids_dev,
                         top_logprobs_dev};
-    // As many CTAs to a row as the SMs hold beside one another, two each, and half a trip of loads at least for each
-    const size_t per_trip = static_cast<size_t>(kThreads) * kLoads * 16 / (dtype == LBK_DTYPE_F32 ? 4 : 2);
+    // CTAs a row: as many as the SMs hold beside one another, three each, as long as each has 3.5 trips of loads; of up to 64 CTAs half a trip is
+    // enough. us at 128256 f32 with 1 / 2 / 4 / 8 / 16: 1 row 24 / 19 / 14 / 12 / 10, 30 rows 40 / 28 / 21 / 18 / 26, 100 rows 39 / 30 / 23 / 29 / 42, 300 rows 52 / 59 / 63 / 79 / 132.
+    const size_t trip = static_cast<size_t>(kThreads) * kLoads * 16 / (dtype == LBK_DTYPE_F32 ? 4 : 2);
     unsigned ctas = 1;
-    while (ctas < kClusterMost && rows * ctas * 2 <= 2 * static_cast<size_t>(ctx->sm_count) && vocab >= per_trip * ctas) ctas *= 2;
+    while (ctas < kClusterMost && rows * ctas * 2 <= 3 * static_cast<size_t>(ctx->sm_count) && (vocab >= 7 * trip * ctas || (rows * ctas <= 64 && vocab >= trip * ctas))) ctas *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(rows * ctas));
     cfg.blockDim = dim3(kThreads);

@@ -170,38 +170,42 @@ TREE_NODES = 128     # node places of a sequence (LBK_TREE_NODES)
 LOGPROBS_TOP = 32    # alternatives of a row (LBK_LOGPROBS_TOP)
 
 
-def _on(ctx: Context, **tensors) -> int:
-    """Checks that the tensors (None is none) lie on the context's GPU without gaps; the raw current stream of that GPU."""
-    for name, t in tensors.items():
-        if t is not None:
-            if not t.is_cuda or t.get_device() != ctx.device:
-                raise ValueError(f"{name} must live on cuda:{ctx.device}")
-            if not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous")
-    return torch._C._cuda_getCurrentRawStream(ctx.device)
+# The host side of these calls is most of a small one's time (16 us of attn_tree were 11 us of Python): checks are plain comparisons, every result
+# has an allocation of its own (a view of one costs as much as two), pointers go to the library as integers.
+
+def _on(ctx: Context, *tensors: torch.Tensor) -> int:
+    """Checks that the tensors lie on the context's GPU without gaps; the raw current stream of that GPU."""
+    device = ctx.device
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError(f"every tensor must live on cuda:{device}")
+        if not t.is_contiguous():
+            raise ValueError("tensors must be contiguous")
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _tree(parents: torch.Tensor, counts: Optional[torch.Tensor], pos: Optional[torch.Tensor] = None) -> Tuple[int, int]:
     """(sequences, node places) of a batch of trees, or of paths through them."""
-    if parents.dim() != 2:
+    shape = parents.shape
+    if len(shape) != 2:
         raise ValueError("the trees are [sequences, nodes]")
-    b, t = parents.shape
+    b, t = shape
     if not 1 <= t <= TREE_NODES:
         raise ValueError(f"a tree has 1 to {TREE_NODES} nodes (got {t})")
-    if parents.dtype != torch.int32:
+    if parents.dtype is not torch.int32:
         raise TypeError("the trees are int32")
-    for v in (counts, pos):
-        if v is not None and (v.dtype != torch.int32 or v.shape != (b,)):
-            raise ValueError(f"positions and counts are int32, one for each of the {b} sequences")
+    if pos is not None and (pos.dtype is not torch.int32 or pos.shape != (b,)) or counts is not None and (counts.dtype is not torch.int32 or counts.shape != (b,)):
+        raise ValueError(f"positions and counts are int32, one for each of the {b} sequences")
     return b, t
 
 
 def _caches(k: torch.Tensor, v: torch.Tensor, b: int, dims: int) -> torch.Size:
-    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+    if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16:
         raise TypeError("caches are bf16")
-    if k.dim() != dims or k.shape != v.shape or k.shape[dims - 4] != b:
+    shape = k.shape
+    if len(shape) != dims or shape != v.shape or shape[dims - 4] != b:
         raise ValueError(f"caches are [{'layers, ' if dims == 5 else ''}{b}, kv_heads, capacity, head_dim], keys like values")
-    return k.shape
+    return shape
 
 
 def rope_kv_append_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, parents: torch.Tensor,
@@ -211,20 +215,33 @@ def rope_kv_append_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: 
     node a node follows, -1 the committed row pos - 1; counts int32 [b]: how many nodes a sequence has (all t)."""
     b, t = _tree(parents, counts, pos)
     _, kvh, cap, hd = _caches(kcache, vcache, b, 4)
-    for name, x in (("q", q), ("k", k), ("v", v), ("cos", cos), ("sin", sin)):
-        if x.dtype != torch.float32:
-            raise TypeError(f"{name} is f32")
-    nh = q.numel() // max(1, b * t * hd)
-    if q.numel() != b * t * nh * hd or k.numel() != b * t * kvh * hd or v.numel() != k.numel():
+    f32 = torch.float32
+    if q.dtype is not f32 or k.dtype is not f32 or v.dtype is not f32 or cos.dtype is not f32 or sin.dtype is not f32:
+        raise TypeError("queries, keys, values and rotation tables are f32")
+    values, new = q.numel(), k.numel()
+    nh = values // max(1, b * t * hd)
+    if values != b * t * nh * hd or new != b * t * kvh * hd or v.numel() != new:
         raise ValueError(f"q, k and v are rows of heads of {hd} for {b} x {t} nodes")
-    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[0] < cap or cos.shape[1] != hd:
+    table = cos.shape
+    if len(table) != 2 or table[0] < cap or table[1] != hd or sin.shape != table:
         raise ValueError("the rotation tables have a row for every place of the cache")
     ctx = ctx or default_context()
-    st = _on(ctx, q=q, k=k, v=v, cos=cos, sin=sin, pos=pos, parents=parents, counts=counts, kcache=kcache, vcache=vcache)
+    st = _on(ctx, q, k, v, cos, sin, pos, parents, kcache, vcache) if counts is None else _on(ctx, q, k, v, cos, sin, pos, parents, kcache, vcache, counts)
     status = ctx._lib.lbk_rope_kv_append_tree(ctx.handle, q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), parents.data_ptr(),
                                               None if counts is None else counts.data_ptr(), b, t, nh, kvh, hd, cap, kcache.data_ptr(), vcache.data_ptr(), st)
     if status:
         _lib.check(status)
+
+
+def _node_pitch(x: torch.Tensor, b: int, t: int, nh: int, hd: int) -> int:
+    """Values from one node's row to the next in [b, t, heads, head_dim]."""
+    if x.is_contiguous():
+        return nh * hd
+    seq, row, head, one = x.stride()
+    pitch = row if t > 1 else seq if b > 1 else nh * hd
+    if one != 1 or (nh > 1 and head != hd) or (b > 1 and seq != t * pitch) or pitch < nh * hd:
+        raise ValueError("the heads of a node lie side by side, nodes and sequences at one distance")
+    return pitch
 
 
 def attn_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, pos: torch.Tensor, parents: torch.Tensor, counts: Optional[torch.Tensor] = None,
@@ -234,33 +251,28 @@ def attn_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, pos: 
     `out` (made like q without one: rows of places not in use are then whatever was there)."""
     b, t = _tree(parents, counts, pos)
     _, kvh, cap, hd = _caches(kcache, vcache, b, 4)
-    if q.dtype not in (torch.float32, torch.bfloat16):
+    dtype, shape = q.dtype, q.shape
+    if dtype is not torch.float32 and dtype is not torch.bfloat16:
         raise TypeError("queries are f32 or bf16")
-    if q.dim() != 4 or q.shape[:2] != (b, t) or q.shape[3] != hd:
+    if len(shape) != 4 or shape[0] != b or shape[1] != t or shape[3] != hd:
         raise ValueError(f"queries are [{b}, {t}, heads, {hd}]")
-    nh = q.shape[2]
+    nh = shape[2]
     if hd != 128 or not nh or not kvh or nh % kvh:
         raise ValueError(f"heads of 128, a multiple of the KV heads (got {nh} and {kvh} heads of {hd})")
     if out is None:
-        out = q.new_empty((b, t, nh, hd))
-    elif out.dtype != q.dtype or out.shape != q.shape:
+        out = q.new_empty(shape)
+    elif out.dtype is not dtype or out.shape != shape:
         raise ValueError("out is like q")
-    pitches = []
-    for x in (q, out):
-        row, seq = (x.stride(1) if t > 1 else nh * hd), x.stride(0)
-        if x.stride(3) != 1 or (nh > 1 and x.stride(2) != hd) or (b > 1 and t > 1 and seq != t * row) or row < nh * hd:
-            raise ValueError("the heads of a node lie side by side, nodes and sequences at one distance")
-        pitches.append(seq if b > 1 and t == 1 else row)
+    q_pitch, out_pitch = _node_pitch(q, b, t, nh, hd), _node_pitch(out, b, t, nh, hd)
     ctx = ctx or default_context()
-    st = _on(ctx, kcache=kcache, vcache=vcache, pos=pos, parents=parents, counts=counts)
-    for x in (q, out):
-        if not x.is_cuda or x.get_device() != ctx.device:
-            raise ValueError(f"queries and out must live on cuda:{ctx.device}")
-    lib = ctx._lib
-    scratch = torch.empty(lib.lbk_attn_tree_scratch(ctx.handle, t, nh, kvh), dtype=torch.float32, device=q.device)
-    status = lib.lbk_attn_tree(ctx.handle, 1 if q.dtype == torch.float32 else 0, q.data_ptr(), pitches[0], kcache.data_ptr(), vcache.data_ptr(), pos.data_ptr(), parents.data_ptr(),
+    st = _on(ctx, kcache, vcache, pos, parents) if counts is None else _on(ctx, kcache, vcache, pos, parents, counts)
+    if q.get_device() != ctx.device or out.get_device() != ctx.device:
+        raise ValueError(f"queries and out must live on cuda:{ctx.device}")
+    lib, f32 = ctx._lib, dtype is torch.float32
+    scratch = q.new_empty(lib.lbk_attn_tree_scratch(ctx.handle, t, nh, kvh) * (1 if f32 else 2))
+    status = lib.lbk_attn_tree(ctx.handle, 1 if f32 else 0, q.data_ptr(), q_pitch, kcache.data_ptr(), vcache.data_ptr(), pos.data_ptr(), parents.data_ptr(),
                                None if counts is None else counts.data_ptr(), b, t, nh, kvh, hd, cap, hd ** -0.5 if scale is None else scale, scratch.data_ptr(), out.data_ptr(),
-                               pitches[1], st)
+                               out_pitch, st)
     if status:
         _lib.check(status)
     return out
@@ -271,18 +283,15 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, best: torch.Tensor,
     """The greedy walk through drafted tokens (lbk_tree_accept): tokens, parents, best (the argmax of every node's logits) int32 [b, t].
     Returns (path [b, t]: the accepted nodes, then -1; how many of them [b]; the token that follows the last one [b])."""
     b, t = _tree(parents, counts)
-    for name, x in (("tokens", tokens), ("best", best)):
-        if x.dtype != torch.int32:
-            raise TypeError(f"{name} are int32")
-        if x.shape != parents.shape:
-            raise ValueError(f"{name} are [{b}, {t}], as parents")
+    if tokens.dtype is not torch.int32 or best.dtype is not torch.int32:
+        raise TypeError("tokens and best are int32")
+    if tokens.shape != parents.shape or best.shape != parents.shape:
+        raise ValueError(f"tokens and best are [{b}, {t}], as parents")
     ctx = ctx or default_context()
-    st = _on(ctx, tokens=tokens, parents=parents, best=best, counts=counts)
-    out = parents.new_empty(b * (t + 2))
-    path, count, after = out[:b * t].view(b, t), out[b * t:b * (t + 1)], out[b * (t + 1):]
-    at = out.data_ptr()
-    status = ctx._lib.lbk_tree_accept(ctx.handle, tokens.data_ptr(), parents.data_ptr(), best.data_ptr(), None if counts is None else counts.data_ptr(), b, t, at,
-                                      at + 4 * b * t, at + 4 * b * (t + 1), st)
+    st = _on(ctx, tokens, parents, best) if counts is None else _on(ctx, tokens, parents, best, counts)
+    path, count, after = parents.new_empty((b, t)), parents.new_empty(b), parents.new_empty(b)
+    status = ctx._lib.lbk_tree_accept(ctx.handle, tokens.data_ptr(), parents.data_ptr(), best.data_ptr(), None if counts is None else counts.data_ptr(), b, t, path.data_ptr(),
+                                      count.data_ptr(), after.data_ptr(), st)
     if status:
         _lib.check(status)
     return path, count, after
@@ -294,7 +303,7 @@ def kv_keep_path(k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, path: torc
     b, t = _tree(path, count, pos)
     layers, _, kvh, cap, hd = _caches(k, v, b, 5)
     ctx = ctx or default_context()
-    st = _on(ctx, k=k, v=v, pos=pos, path=path, count=count)
+    st = _on(ctx, k, v, pos, path, count)
     status = ctx._lib.lbk_kv_keep_path(ctx.handle, k.data_ptr(), v.data_ptr(), layers, b * kvh * cap * hd, b, kvh, hd, cap, pos.data_ptr(), path.data_ptr(), count.data_ptr(), t, st)
     if status:
         _lib.check(status)
@@ -302,10 +311,10 @@ def kv_keep_path(k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, path: torc
 
 def advance_pos_by(pos: torch.Tensor, count: torch.Tensor, ctx: Optional[Context] = None) -> None:
     """pos += count, int32 [b] (lbk_advance_pos_by): the accepted nodes are committed."""
-    if pos.dtype != torch.int32 or count.dtype != torch.int32 or pos.dim() != 1 or pos.shape != count.shape:
+    if pos.dtype is not torch.int32 or count.dtype is not torch.int32 or pos.dim() != 1 or pos.shape != count.shape:
         raise ValueError("pos and count are int32, one number for each sequence")
     ctx = ctx or default_context()
-    st = _on(ctx, pos=pos, count=count)
+    st = _on(ctx, pos, count)
     status = ctx._lib.lbk_advance_pos_by(ctx.handle, pos.data_ptr(), count.data_ptr(), pos.shape[0], st)
     if status:
         _lib.check(status)
@@ -321,36 +330,37 @@ class TokenLogprobs(NamedTuple):
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0, scale: float = 1.0, ctx: Optional[Context] = None) -> TokenLogprobs:
     """Log softmax(scale * logits) at the given tokens, entropy and the `top` largest logits with their log probabilities
     (lbk_token_logprobs). logits f32 or bf16 [rows, vocab], rows any distance apart; tokens int32 [rows] or [rows, given]."""
-    if logits.dtype not in (torch.float32, torch.bfloat16):
+    dtype, shape = logits.dtype, logits.shape
+    if dtype is not torch.float32 and dtype is not torch.bfloat16:
         raise TypeError("logits are f32 or bf16")
-    if logits.dim() != 2 or logits.shape[1] < 1:
+    if len(shape) != 2 or shape[1] < 1:
         raise ValueError("logits are [rows, vocab]")
-    rows, vocab = logits.shape
-    if vocab > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < vocab:
+    rows, vocab = shape
+    pitch, one = logits.stride()
+    if vocab > 1 and one != 1 or rows > 1 and pitch < vocab:
         raise ValueError("the values of a row lie side by side, rows do not overlap")
     if not 0 <= top <= min(vocab, LOGPROBS_TOP):
         raise ValueError(f"{top} alternatives of {vocab}: at most {LOGPROBS_TOP}")
     given = 0
     if tokens is not None:
-        if tokens.dtype != torch.int32:
+        if tokens.dtype is not torch.int32:
             raise TypeError("tokens are int32")
         if tokens.dim() not in (1, 2) or tokens.shape[0] != rows:
             raise ValueError("tokens are [rows] or [rows, given]")
         given = 1 if tokens.dim() == 1 else tokens.shape[1]
     ctx = ctx or default_context()
-    st = _on(ctx, tokens=tokens)
-    if not logits.is_cuda or logits.get_device() != ctx.device:
+    st = _on(ctx) if tokens is None else _on(ctx, tokens)
+    device = logits.device
+    if logits.get_device() != ctx.device:
         raise ValueError(f"logits must live on cuda:{ctx.device}")
-    # one allocation for the floats: [rows, given], [rows], [rows, top]
-    floats = torch.empty(rows * (given + 1 + top), dtype=torch.float32, device=logits.device)
-    ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-    at = floats.data_ptr()
-    status = ctx._lib.lbk_token_logprobs(ctx.handle, 0 if logits.dtype == torch.float32 else 1, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab,
-                                         tokens.data_ptr() if given else None, given, scale, top, at, at + 4 * rows * given, ids.data_ptr(), at + 4 * rows * (given + 1), st)
+    logprobs, entropy, top_logprobs = (torch.empty((rows, given), dtype=torch.float32, device=device), torch.empty(rows, dtype=torch.float32, device=device),
+                                       torch.empty((rows, top), dtype=torch.float32, device=device))
+    ids = torch.empty((rows, top), dtype=torch.int32, device=device)
+    status = ctx._lib.lbk_token_logprobs(ctx.handle, 0 if dtype is torch.float32 else 1, logits.data_ptr(), pitch if rows > 1 else vocab, rows, vocab,
+                                         tokens.data_ptr() if given else None, given, scale, top, logprobs.data_ptr(), entropy.data_ptr(), ids.data_ptr(), top_logprobs.data_ptr(), st)
     if status:
         _lib.check(status)
-    lp, entropy, best = floats.split([rows * given, rows, rows * top])
-    return TokenLogprobs(lp.view(rows, given), entropy, ids, best.view(rows, top))
+    return TokenLogprobs(logprobs, entropy, ids, top_logprobs)
 
 
 class DecodeStep:

@@ -18,6 +18,7 @@
 // branches may be infinite or NaN too; a row that does not see them must not notice. So in the blocks of the nodes values that are no numbers are
 // taken as zeros as well, and added at the end to the rows that see them (a weight is never zero in exact arithmetic).
 #include <algorithm>
+#include <type_traits>
 
 #include "lbk_dense_dev.cuh"
 #include "lbk_tcgen05.cuh"
@@ -31,17 +32,16 @@ using dense::bf16_pair;
 
 constexpr int kHd = 128;
 constexpr int kMaxSeqs = 256;
-constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr float kNoMax = -3.0e38f;  // a row that has seen nothing: finite, so that -inf scores less it are no NaN
 
 struct TreeParams {
-    CUtensorMap k, v;   // bytes [cache rows][256], boxes of 128 bytes and 64 rows (K of many rows: 128), SWIZZLE_128B
+    CUtensorMap k, v;   // bytes [cache rows][256], boxes of 128 bytes and 128 rows of K, 64 of V, SWIZZLE_128B
     const void *q;
     void *out;
     long q_pitch, out_pitch;
     const uint16_t *vcache;
     const int *pos, *parents, *counts;
-    int b, t, nh, kvh, cap;
+    int b, t, kvh, group, cap;  // group: query heads of a KV head
     float scale;        // log2(e) * scale: scores in units of log 2
     float *part;        // [CTA][2][tile rows][128]
     float2 *part_ml;    // [CTA][2][tile rows]: maximum, weight
@@ -85,32 +85,39 @@ struct Line {
 __device__ __forceinline__ int line_blocks(const Line &l, int seq, int block_keys) { return (l.pos[seq] + l.count[seq] + block_keys - 1) / block_keys; }
 __device__ __forceinline__ int line_tiles(const Line &l, int seq, int group, int rows) { return (l.count[seq] * group + rows - 1) / rows; }
 
-// Fills the line; a sequence outside its cache has no units. All threads of the block. (Loads from L2: the merging kernel comes here in front of its wait.)
+// Fills the line; a sequence outside its cache has no units. All threads of the block; a warp does it. (Loads from L2: the merging kernel comes here in front of
+// its wait.)
 template <int ROWS, int KEYS>
-__device__ void cut_line(const TreeParams &p, Line &l) {
-    const int group = p.nh / p.kvh;
-    for (int i = threadIdx.x; i < p.b; i += blockDim.x) {
-        const int pos = __ldcg(p.pos + i), count = p.counts ? min(max(__ldcg(p.counts + i), 0), p.t) : p.t;
-        const bool fits = pos >= 0 && pos <= p.cap - count;
-        if (!fits && blockIdx.x == 0) atomicExch(p.err_word, kErrPos);
-        l.pos[i] = pos;
-        l.count[i] = fits ? count : 0;
-    }
-    __syncthreads();
+__device__ __forceinline__ void cut_line(const TreeParams &p, Line &l) {
     if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
         int before = 0;
         for (int i0 = 0; i0 < p.b; i0 += 32) {
-            const int i = i0 + threadIdx.x;
-            const int mine = i < p.b && l.count[i] ? line_blocks(l, i, KEYS) * line_tiles(l, i, group, ROWS) * p.kvh : 0;
+            const int i = i0 + lane;
+            int pos = 0, count = 0;
+            if (i < p.b) {
+                pos = __ldcg(p.pos + i);
+                count = p.counts ? min(max(__ldcg(p.counts + i), 0), p.t) : p.t;
+            }
+            if (pos < 0 || pos > p.cap - count) {
+                if (blockIdx.x == 0) atomicExch(p.err_word, kErrPos);
+                count = 0;
+            }
+            const int mine = count ? (pos + count + KEYS - 1) / KEYS * ((count * p.group + ROWS - 1) / ROWS) * p.kvh : 0;
             int sum = mine;
+#pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int up = __shfl_up_sync(0xffffffffu, sum, o);
-                if (static_cast<int>(threadIdx.x) >= o) sum += up;
+                if (lane >= o) sum += up;
             }
-            if (i < p.b) l.first[i] = before + sum - mine;
+            if (i < p.b) {
+                l.pos[i] = pos;
+                l.count[i] = count;
+                l.first[i] = before + sum - mine;
+            }
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
-        if (threadIdx.x == 0) l.first[p.b] = before;
+        if (lane == 0) l.first[p.b] = before;
     }
     __syncthreads();
 }
@@ -137,7 +144,7 @@ __device__ __forceinline__ Segment segment_at(const TreeParams &p, const Line &l
     }
     s.seq = lo;
     s.blocks = line_blocks(l, lo, keys);
-    const int tiles = line_tiles(l, lo, p.nh / p.kvh, rows), at = unit - l.first[lo], problem = at / s.blocks;
+    const int tiles = line_tiles(l, lo, p.group, rows), at = unit - l.first[lo], problem = at / s.blocks;
     s.begin = at - problem * s.blocks;
     s.end = min(s.blocks, s.begin + last - unit);
     s.kh = problem / tiles;
@@ -187,310 +194,410 @@ __device__ __forceinline__ void query_terms(const float4 &a, uint2 (&term)[TERMS
 }
 __device__ __forceinline__ bool sees(const ulonglong2 &m, int n) { return ((n < 64 ? m.x : m.y) >> (n & 63)) & 1; }
 
-// ---- few rows: mma.sync, 16 rows a warp ---------------------------------------------------------------
-// Tiles of ROWS = 16 or 32 rows (up to 16 or 32 products of nodes and heads of a group). Every key is 512 bytes from HBM, 22 cycles of an SM at the
-// full rate, and some 6 cycles of mma.sync work for 16 rows in three terms: the stream is the bound, and the 128 rows
-// of a tcgen05 tile would be padding. Four warps take 16 keys each of a block of 64 for 16 rows; a fifth (ninth) fetches blocks by TMA, kStages deep.
-template <int RG>
-struct Few {
-    static constexpr int kRows = 16 * RG, kWarps = 4 * RG, kThreads = (kWarps + 1) * 32, kKeys = 64;
-    static constexpr int kHalf = kKeys * 128, kStage = 4 * kHalf, kStages = 5;
-    static constexpr int kQPitch = 272;                               // bytes: eight rows start in eight different bank groups
-    static constexpr int kQ0 = kStages * kStage, kQBytes = 3 * kRows * kQPitch;
-    static constexpr int kMergePitch = 132;                           // floats
-    static constexpr int kMerge0 = kQ0 + kQBytes, kMergeBytes = 2 * kRows * kMergePitch * 4;
-    static constexpr int kBars = kMerge0 + kMergeBytes, kSmem = kBars + 2 * kStages * 8 + 1024;
-};
-struct FewShared {
+struct CtaShared {
     Line line;
     int parent[kTreeNodes];
     ulonglong2 mask[kTreeNodes];
     int abort, odd;
+    uint32_t tmem;
 };
+// MN-major SWIZZLE_128B operand: groups of 8 keys 1024 bytes apart (stride byte offset), the halves of 64 dimensions `apart` bytes (leading byte offset)
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t apart) {
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | static_cast<uint64_t>(apart >> 4) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 |
+           static_cast<uint64_t>(2) << 61;
+}
 
-template <int TERMS, int RG>
-__global__ void __launch_bounds__(Few<RG>::kThreads, 1) attn_tree_few_kernel(const __grid_constant__ TreeParams p) {
-    using F = Few<RG>;
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ FewShared sh;
-    const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-    uint8_t *sm = smem_raw + (base - raw);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    auto full = [&](int s) { return base + F::kBars + s * 8; };
-    auto empty = [&](int s) { return base + F::kBars + (F::kStages + s) * 8; };
-    volatile int *abort = &sh.abort;
-    if (tid == 0) {
-        for (int s = 0; s < F::kStages; ++s) {
-            ptx::mbar_init(full(s), 1);
-            ptx::mbar_init(empty(s), F::kWarps);
+// Zeros for values that are no numbers, or for all of `units` 16-byte units; whether there was one that is no number.
+__device__ __forceinline__ bool clean_values(uint4 *v, int units, bool all) {
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < units; ++i) {
+        if (all) {
+            v[i] = make_uint4(0u, 0u, 0u, 0u);
+            continue;
         }
-        sh.abort = sh.odd = 0;
-        ptx::fence_barrier_init();
+        const uint4 x = v[i], y = make_uint4(only_numbers(x.x), only_numbers(x.y), only_numbers(x.z), only_numbers(x.w));
+        if (((x.x ^ y.x) | (x.y ^ y.y) | (x.z ^ y.z) | (x.w ^ y.w)) == 0u) continue;
+        v[i] = y;
+        odd = true;
     }
-    ptx::pdl_wait();
-    ptx::pdl_trigger();  // behind the wait: what the merging kernel reads in front of its own is settled then
-    cut_line<F::kRows, F::kKeys>(p, sh.line);
-    const Shares shares(sh.line.first[p.b], p.workers);
-    const int u0 = shares.begin(blockIdx.x), u1 = shares.begin(blockIdx.x + 1);
-    if (u0 == u1) return;
-    const int group = p.nh / p.kvh;
-    auto wait = [&](uint32_t bar, uint32_t parity) {
-        for (uint32_t i = 0; i < kWaitLimit; ++i) {
-            if (ptx::mbar_try_wait(bar, parity)) return true;
-            if (*abort) return false;
-        }
-        *abort = 1;
-        return false;
-    };
-
-    if (warp == F::kWarps) {
-        // ================= TMA producer =================
-        if (lane != 0) return;
-        int stage = 0, round = 0, sent = 0;
-        bool ok = true;
-        for (int u = u0; u < u1 && ok;) {
-            const Segment s = segment_at(p, sh.line, u, u1, F::kRows, F::kKeys);
-            const int row0 = (s.seq * p.kvh + s.kh) * p.cap;
-            for (int j = s.begin; j < s.end; ++j, ++sent) {
-                if (round > 0 && !wait(empty(stage), (round - 1) & 1)) {
-                    ok = false;
-                    break;
-                }
-                const uint32_t at = base + stage * F::kStage;
-                ptx::mbar_arrive_expect_tx(full(stage), F::kStage);
-                ptx::tma_load_2d(at, &p.k, full(stage), 0, row0 + j * F::kKeys);
-                ptx::tma_load_2d(at + F::kHalf, &p.k, full(stage), 128, row0 + j * F::kKeys);
-                ptx::tma_load_2d(at + 2 * F::kHalf, &p.v, full(stage), 0, row0 + j * F::kKeys);
-                ptx::tma_load_2d(at + 3 * F::kHalf, &p.v, full(stage), 128, row0 + j * F::kKeys);
-                if (++stage == F::kStages) {
-                    stage = 0;
-                    ++round;
-                }
+    return odd;
+}
+// A producer warp of a kernel with layout M: the K blocks, or the V pieces, of a share. full, empty: the first of the stages' barriers.
+template <class M>
+__device__ __forceinline__ void produce(const TreeParams &p, const Line &line, int u0, int u1, int rows, bool is_k, uint32_t base, uint32_t full, uint32_t empty, volatile int *abort, bool &ok) {
+    if ((threadIdx.x & 31) != 0) return;
+    const int stages = is_k ? M::kKStages : M::kVStages;
+    int stage = 0, round = 0, sent = 0;
+    for (int u = u0; u < u1 && ok;) {
+        const Segment s = segment_at(p, line, u, u1, rows, M::kKeys);
+        const int row0 = (s.seq * p.kvh + s.kh) * p.cap;
+        for (int i = is_k ? s.begin : 2 * s.begin; i < (is_k ? s.end : 2 * s.end); ++i, ++sent) {
+            if (round > 0 && !tc::wait_bar(empty + stage * 8, (round - 1) & 1, abort)) {
+                ok = false;
+                break;
             }
-            u += s.end - s.begin;
-        }
-        if (!ok) atomicExch(p.err_word, 5);
-        // the copies in flight land before the block may go, whoever has given up
-        for (int n = max(0, sent - F::kStages); n < sent; ++n) ptx::mbar_wait(full(n % F::kStages), (n / F::kStages) & 1, kWaitLimit);
-        return;
-    }
-
-    // ================= the other warps: 16 rows, 16 keys of every block each =================
-    const int kg = warp & 3, rg = warp >> 2, g = lane >> 2, tq = lane & 3;
-    auto meet = [&]() { ptx::named_barrier(1, F::kWarps * 32); };
-    int stage = 0, phase = 0;
-    bool ok = true;
-    for (int u = u0; u < u1;) {
-        const Segment s = segment_at(p, sh.line, u, u1, F::kRows, F::kKeys);
-        const int pos = sh.line.pos[s.seq], count = sh.line.count[s.seq];
-        const int rows_all = count * group, row0 = s.tile * F::kRows;
-        const bool nodes = s.end * F::kKeys > pos;  // some of these blocks hold nodes
-        // the tile's queries, a row as one load of a warp, all of them asked for before the first is looked at
-        float4 qv[F::kRows / F::kWarps];
-#pragma unroll
-        for (int i = 0; i < F::kRows / F::kWarps; ++i) qv[i] = query<TERMS>(p, s.seq, s.kh, group, row0 + i * F::kWarps + warp, rows_all, lane);
-        if (nodes) load_parents(p, sh.parent, s.seq, count, F::kWarps * 32);
-#pragma unroll
-        for (int i = 0; i < F::kRows / F::kWarps; ++i) {
-            uint2 term[TERMS];
-            query_terms<TERMS>(qv[i], term);
-#pragma unroll
-            for (int x = 0; x < TERMS; ++x) *reinterpret_cast<uint2 *>(sm + F::kQ0 + (x * F::kRows + i * F::kWarps + warp) * F::kQPitch + lane * 8) = term[x];
-        }
-        meet();
-        if (nodes)
-            for (int i = tid; i < count; i += F::kWarps * 32) tree_masks(sh.parent, sh.mask, i);
-        const uint32_t q_at = base + F::kQ0 + (rg * 16 + (lane & 15)) * F::kQPitch + (lane >> 4) * 16;
-        if (nodes) meet();
-        float o[16][4], m[2] = {kNoMax, kNoMax}, l[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int d = 0; d < 16; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
-        bool odd = false;  // a value of some node is no number
-        for (int j = s.begin; j < s.end; ++j) {
-            if (ok) ok = __all_sync(0xffffffffu, wait(full(stage), phase));
-            if (ok) {
-                const uint32_t ks = base + stage * F::kStage, vs = ks + 2 * F::kHalf;
-                const int key0 = j * F::kKeys + kg * 16;
-                const bool edge = key0 + 16 > pos;
-                // scores: keys 0..7 and 8..15 of the warp's, each term in a sum of its own
-                float sc[2][TERMS][4];
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int x = 0; x < TERMS; ++x) sc[h][x][0] = sc[h][x][1] = sc[h][x][2] = sc[h][x][3] = 0.0f;
-#pragma unroll
-                for (int d2 = 0; d2 < 4; ++d2) {  // 32 dimensions at a time
-                    uint32_t kb[2][4];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int key = kg * 16 + h * 8 + (lane & 7), unit = (d2 & 1) * 4 + (lane >> 3);
-                        ptx::ldmatrix_x4(kb[h], ks + (d2 >> 1) * F::kHalf + key * 128 + ((unit ^ (key & 7)) << 4));
-                    }
-#pragma unroll
-                    for (int x = 0; x < TERMS; ++x)
-#pragma unroll
-                        for (int d = 0; d < 2; ++d) {
-                            uint32_t qf[4];
-                            ptx::ldmatrix_x4(qf, q_at + x * F::kRows * F::kQPitch + (2 * d2 + d) * 32);
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) ptx::mma_bf16(sc[h][x], qf, kb[h][2 * d], kb[h][2 * d + 1]);
-                        }
-                }
-                float sv[2][4];
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sv[h][e] = (TERMS > 1 ? sc[h][0][e] + (sc[h][1 % TERMS][e] + sc[h][2 % TERMS][e]) : sc[h][0][e]) * p.scale;
-                if (edge) {
-                    const int ra = row0 + rg * 16 + g, rb = ra + 8;
-                    const ulonglong2 none = make_ulonglong2(0ull, 0ull), ma = ra < rows_all ? sh.mask[p.node_of(ra)] : none, mb = rb < rows_all ? sh.mask[p.node_of(rb)] : none;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int key = key0 + h * 8 + tq * 2 + (e & 1), n = key - pos;
-                            if (n >= 0 && (n >= count || !sees(e < 2 ? ma : mb, n))) sv[h][e] = -INFINITY;
-                        }
-                }
-                uint32_t pr[4][TERMS];
-                float corr[2];
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {  // rows g and g + 8
-                    const int e = half * 2;
-                    float mx = fmaxf(fmaxf(sv[0][e], sv[0][e + 1]), fmaxf(sv[1][e], sv[1][e + 1]));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    const float nm = fmaxf(m[half], mx);
-                    corr[half] = ex2(m[half] - nm);
-                    m[half] = nm;
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float e0 = ex2(sv[h][e] - nm), e1 = ex2(sv[h][e + 1] - nm);
-                        sum += e0 + e1;
-                        split_pair<TERMS>(e0, e1, pr[2 * h + half]);
-                    }
-                    l[half] = l[half] * corr[half] + sum;
-                }
-                const int key = kg * 16 + (lane & 15);
-#pragma unroll
-                for (int d2 = 0; d2 < 8; ++d2) {  // 16 dimensions at a time
-                    const int unit = (d2 & 3) * 2 + (lane >> 4);
-                    uint32_t vb[4];
-                    ptx::ldmatrix_x4_trans(vb, vs + (d2 >> 2) * F::kHalf + key * 128 + ((unit ^ (key & 7)) << 4));
-                    if (edge) {  // a register: two keys of one dimension
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int n = key0 + (r & 1) * 8 + tq * 2 + e - pos;
-                                const bool strange = n >= 0 && ((vb[r] >> (16 * e)) & 0x7f80u) == 0x7f80u;
-                                if (strange && n < count) odd = true;
-                                if (strange || n >= count) vb[r] &= e ? 0x0000ffffu : 0xffff0000u;
-                            }
-                    }
-                    float add[2][4] = {};
-#pragma unroll
-                    for (int x = TERMS - 1; x >= 0; --x) {  // the small ones first
-                        const uint32_t a[4] = {pr[0][x], pr[1][x], pr[2][x], pr[3][x]};
-                        ptx::mma_bf16(add[0], a, vb[0], vb[1]);
-                        ptx::mma_bf16(add[1], a, vb[2], vb[3]);
-                    }
-#pragma unroll
-                    for (int d = 0; d < 2; ++d)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[2 * d2 + d][e] = o[2 * d2 + d][e] * corr[e >> 1] + add[d][e];
-                }
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(empty(stage));
-            }
-            if (++stage == F::kStages) {
+            const uint32_t at = base + (is_k ? M::kK0 + stage * M::kKBytes : M::kV0 + stage * M::kPieceBytes), done = full + stage * 8;
+            ptx::mbar_arrive_expect_tx(done, is_k ? M::kKBytes : M::kPieceBytes);
+            ptx::tma_load_2d(at, is_k ? &p.k : &p.v, done, 0, row0 + i * (is_k ? M::kKeys : M::kPiece));
+            ptx::tma_load_2d(at + (is_k ? M::kHalf : M::kPieceHalf), is_k ? &p.k : &p.v, done, 128, row0 + i * (is_k ? M::kKeys : M::kPiece));
+            if (++stage == stages) {
                 stage = 0;
-                phase ^= 1;
-            }
-        }
-        if (odd) sh.odd = u + 1;  // read behind the meetings below, written again behind the next segment's first
-        // the four warps of a row meet: 2 and 3 hand over to 0 and 1, then 1 to 0
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-        }
-        float *const place = reinterpret_cast<float *>(sm + F::kMerge0);
-#pragma unroll 1
-        for (int from = 2; from >= 1; --from) {
-            const int slot = from == 2 ? kg & 1 : 0;
-            const bool gives = from == 2 ? kg >= 2 : kg == 1, takes = from == 2 ? kg < 2 : kg == 0;
-            float *ra = place + (slot * F::kRows + rg * 16 + g) * F::kMergePitch, *rb = ra + 8 * F::kMergePitch;
-            if (gives) {
-#pragma unroll
-                for (int d = 0; d < 16; ++d) {
-                    *reinterpret_cast<float2 *>(ra + d * 8 + tq * 2) = make_float2(o[d][0], o[d][1]);
-                    *reinterpret_cast<float2 *>(rb + d * 8 + tq * 2) = make_float2(o[d][2], o[d][3]);
-                }
-                if (tq == 0) {
-                    *reinterpret_cast<float2 *>(ra + kHd) = make_float2(m[0], l[0]);
-                    *reinterpret_cast<float2 *>(rb + kHd) = make_float2(m[1], l[1]);
-                }
-            }
-            meet();
-            if (takes) {
-                const float2 xa = *reinterpret_cast<const float2 *>(ra + kHd), xb = *reinterpret_cast<const float2 *>(rb + kHd);
-                const float na = fmaxf(m[0], xa.x), nb = fmaxf(m[1], xb.x);
-                const float wa = ex2(m[0] - na), wb = ex2(m[1] - nb), va = ex2(xa.x - na), vb = ex2(xb.x - nb);
-                m[0] = na;
-                m[1] = nb;
-                l[0] = l[0] * wa + xa.y * va;
-                l[1] = l[1] * wb + xb.y * vb;
-#pragma unroll
-                for (int d = 0; d < 16; ++d) {
-                    const float2 ya = *reinterpret_cast<const float2 *>(ra + d * 8 + tq * 2), yb = *reinterpret_cast<const float2 *>(rb + d * 8 + tq * 2);
-                    o[d][0] = o[d][0] * wa + ya.x * va;
-                    o[d][1] = o[d][1] * wa + ya.y * va;
-                    o[d][2] = o[d][2] * wb + yb.x * vb;
-                    o[d][3] = o[d][3] * wb + yb.y * vb;
-                }
-            }
-            meet();
-        }
-        if (kg == 0) {
-            const bool fix = nodes && sh.odd == u + 1, whole = s.begin == 0 && s.end == s.blocks;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int r = rg * 16 + half * 8 + g, row = row0 + r, node = p.node_of(row);
-                if (row >= rows_all) continue;
-                if (fix) {  // what this row sees that is no number
-                    const ulonglong2 mine = sh.mask[node];
-                    for (int n = max(0, s.begin * F::kKeys - pos); n < min(count, s.end * F::kKeys - pos); ++n) {
-                        if (!sees(mine, n)) continue;
-                        const uint16_t *v = p.vcache + (static_cast<size_t>(s.seq * p.kvh + s.kh) * p.cap + pos + n) * kHd + tq * 2;
-#pragma unroll
-                        for (int d = 0; d < 16; ++d)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                if ((v[d * 8 + e] & 0x7f80u) == 0x7f80u) o[d][half * 2 + e] += dense::bf16_f32(v[d * 8 + e]);
-                    }
-                }
-                if (whole) {
-                    const float inv = 1.0f / l[half];
-                    const size_t at = (static_cast<size_t>(s.seq) * p.t + node) * p.out_pitch + static_cast<size_t>(s.kh * group + row - node * group) * kHd + tq * 2;
-#pragma unroll
-                    for (int d = 0; d < 16; ++d) {
-                        const float x = o[d][half * 2] * inv, y = o[d][half * 2 + 1] * inv;
-                        if (TERMS > 1) *reinterpret_cast<float2 *>(static_cast<float *>(p.out) + at + d * 8) = make_float2(x, y);
-                        else *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + at + d * 8) = bf16_pair(x, y);
-                    }
-                } else {
-                    const size_t at = (static_cast<size_t>(blockIdx.x) * 2 + (u == u0 ? 0 : 1)) * F::kRows + r;
-#pragma unroll
-                    for (int d = 0; d < 16; ++d) *reinterpret_cast<float2 *>(p.part + at * kHd + d * 8 + tq * 2) = make_float2(o[d][half * 2], o[d][half * 2 + 1]);
-                    if (tq == 0) p.part_ml[at] = make_float2(m[half], l[half]);
-                }
+                ++round;
             }
         }
         u += s.end - s.begin;
     }
+    // the copies in flight land before the block may go, whoever has given up
+    for (int n = max(0, sent - stages); n < sent; ++n) ptx::mbar_wait(full + n % stages * 8, (n / stages) & 1, tc::kTcWaitLimit);
+}
+
+// ---- few rows: tcgen05 with keys and dimensions in the lanes ------------------------------------------------
+// Tiles of 16 and 32 rows. The 128 lanes of an accumulator are a block's keys, S^T = K Q^T, and then the dimensions, O^T = V^T P^T; rows and terms are its columns, so
+// that a product costs what the rows need: 512 and 768 cycles of the tensor core for a block of 128 keys and 16 and 32 rows in three terms, where the block's 64 KB are
+// 2800 cycles of an SM's share of HBM. The stream is the bound. (mma.sync has 16 x 16 x 8 products at a sixteenth of this rate: 16 rows in three terms took 4600 cycles for
+// 128 keys, 32 rows 6400. Tiles of 64 rows, us at 16 sequences of 8100 keys: so 136, bf16 102; tiles of 128 half empty 124 and 81.)
+//
+// All terms of the queries are rows of one operand, and so are those of the probabilities, which go through shared memory. A thread has one key and half of the rows:
+// a row's maximum is not at hand, and not needed: probabilities are 2^(s - m) with any m that keeps them in range. m is the maximum of the tile's first block, and is moved
+// (and the sums with it) when some score is over it by more than kSlack.
+//
+//   8 softmax warps  warp w and w + 4: the quadrant of 32 lanes w % 4, the first and the second half of the rows
+//   K, V producers, MMA warp  as below: Q K^T of block j + 1 as soon as the scores of block j have been read, then P V of block j
+constexpr float kSlack = 8.0f;  // in units of log 2: probabilities stay below 2^8
+template <int TERMS, int ROWS>
+struct Turned {
+    static constexpr int kKeys = 128, kHalf = kKeys * 128, kKBytes = 2 * kHalf;
+    static constexpr int kPiece = 64, kPieceHalf = kPiece * 128, kPieceBytes = 2 * kPieceHalf;   // V: 64 keys, two halves of 64 dimensions
+    static constexpr int kCols = TERMS * ROWS, kOpHalf = kCols * 128, kOpBytes = 2 * kOpHalf;     // queries, and probabilities of a block: [2 halves][terms * rows][128 bytes]
+    static constexpr int kKStages = kCols > 64 ? 2 : 3, kVStages = kCols > 64 ? 4 : 5;
+    static constexpr int kP0 = kOpBytes, kK0 = 3 * kOpBytes, kV0 = kK0 + kKStages * kKBytes, kBars = kV0 + kVStages * kPieceBytes;
+    static constexpr int kMax = kBars + 256, kPart = kMax + ROWS * 4, kSmem = kPart + 4 * ROWS * 4 + 1024;   // the rows' m; [quadrant][row] floats
+    static constexpr int kSoftWarps = 8, kKWarp = 8, kVWarp = 9, kMmaWarp = 10, kThreads = 11 * 32;
+    static constexpr uint32_t kColO = kCols <= 32 ? 32 : kCols <= 64 ? 64 : 128, kTmem = 4 * kColO;  // scores, and from kColO on the products of even and of odd blocks
+    static_assert(kSmem + 6 * 1024 <= 232448 && kCols % 16 == 0 && kCols <= 128, "shared memory and operand sizes");
+};
+// v[0] becomes what `join` makes of value lane / (32 / N) of all lanes: half of the values go to the other half of the lanes in every step
+template <int N, class Join>
+__device__ __forceinline__ void over_lanes(float (&v)[N], int lane, Join join) {
+    int o = 16;
+#pragma unroll
+    for (int n = N / 2; n > 0; n >>= 1, o >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const bool upper = lane & o;
+            const float give = upper ? v[i] : v[i + n], keep = upper ? v[i + n] : v[i];
+            v[i] = join(keep, __shfl_xor_sync(0xffffffffu, give, o));
+        }
+#pragma unroll
+    for (; o > 0; o >>= 1) v[0] = join(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+}
+__device__ __forceinline__ bool any_of(int id, int count, bool mine) {  // the block's named barrier, with an answer
+    uint32_t any;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %3, 0;\nbarrier.cta.red.or.pred q, %1, %2, p;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(any) : "r"(id), "r"(count), "r"(static_cast<uint32_t>(mine)) : "memory");
+    return any != 0;
+}
+
+template <int TERMS, int ROWS>
+__global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_turned_kernel(const __grid_constant__ TreeParams p) {
+    using M = Turned<TERMS, ROWS>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ CtaShared sh;
+    const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t *sm = smem_raw + (base - raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int kKFull = 0, kKEmpty = 3, kVFull = 6, kVEmpty = 11, kQFull = 16, kSFull = 17, kSFree = 18;
+    // one for even, one for odd blocks: a warp may be a block ahead of another here, and a barrier's parity tells two neighbouring phases apart, no more
+    constexpr int kPReady = 19, kOFull = 21;
+    auto bar = [&](int i) { return base + M::kBars + i * 8; };
+    volatile int *abort = &sh.abort;
+    if (tid == 0) {
+        for (int s = 0; s < M::kKStages; ++s) {
+            ptx::mbar_init(bar(kKFull + s), 1);
+            ptx::mbar_init(bar(kKEmpty + s), 1);
+        }
+        for (int s = 0; s < M::kVStages; ++s) {
+            ptx::mbar_init(bar(kVFull + s), 1);
+            ptx::mbar_init(bar(kVEmpty + s), 1);
+        }
+        for (int i : {kQFull, kSFree, kPReady, kPReady + 1}) ptx::mbar_init(bar(i), M::kSoftWarps);
+        for (int i : {kSFull, kOFull, kOFull + 1}) ptx::mbar_init(bar(i), 1);
+        sh.abort = sh.odd = 0;
+        ptx::fence_barrier_init();
+    }
+    if (warp == M::kMmaWarp) {
+        tc::tmem_alloc(ptx::smem_u32(&sh.tmem), M::kTmem);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before();
+    ptx::pdl_wait();
+    ptx::pdl_trigger();  // behind the wait: what the merging kernel reads in front of its own is settled then
+    cut_line<ROWS, M::kKeys>(p, sh.line);
+    tc::tc_fence_after();
+    const uint32_t tmem = *static_cast<volatile uint32_t *>(&sh.tmem);
+    const Shares shares(sh.line.first[p.b], p.workers);
+    const int u0 = shares.begin(blockIdx.x), u1 = shares.begin(blockIdx.x + 1);
+    if (u0 == u1) {
+        if (warp == M::kMmaWarp) tc::tmem_dealloc(tmem, M::kTmem);
+        return;
+    }
+    const int group = p.group;
+    bool ok = true;
+    auto wait = [&](int i, int parity) {
+        if (ok) ok = tc::warp_wait(bar(i), parity, abort);
+        return ok;
+    };
+
+    if (warp == M::kKWarp || warp == M::kVWarp) {
+        produce<M>(p, sh.line, u0, u1, ROWS, warp == M::kKWarp, base, bar(warp == M::kKWarp ? kKFull : kVFull), bar(warp == M::kKWarp ? kKEmpty : kVEmpty), abort, ok);
+    } else if (warp == M::kMmaWarp) {
+        // ================= MMA issue: the warp walks, one lane issues =================
+        // D f32, A and B bf16, M = 128, N = terms * rows; for O^T A is MN-major (bit 15)
+        constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(M::kCols >> 3) << 17) | ((128u >> 4) << 24), idesc_o = idesc_s | (1u << 15);
+        const uint64_t q_desc = tc::smem_desc_sw128(base), p_desc = tc::smem_desc_sw128(base + M::kP0);
+        int ks = 0, kphase = 0, vs = 0, vphase = 0, n = 0, seg = 0;  // n: the block, in the whole walk
+        auto scores = [&]() {
+            if (!wait(kKFull + ks, kphase)) return;
+            tc::tc_fence_after();
+            if (tc::elect_one()) {
+                const uint64_t k_desc = tc::smem_desc_sw128(base + M::kK0 + ks * M::kKBytes);
+#pragma unroll
+                for (int st = 0; st < 8; ++st)
+                    tc::umma_f16_ss(tmem, k_desc + static_cast<uint64_t>((st >> 2) * (M::kHalf >> 4) + (st & 3) * 2), q_desc + static_cast<uint64_t>((st >> 2) * (M::kOpHalf >> 4) + (st & 3) * 2),
+                                    idesc_s, st ? 1u : 0u);
+                tc::umma_commit(bar(kSFull));
+                tc::umma_commit(bar(kKEmpty + ks));
+            }
+            __syncwarp();
+            if (++ks == M::kKStages) {
+                ks = 0;
+                kphase ^= 1;
+            }
+        };
+        for (int u = u0; u < u1 && ok; ++seg) {
+            const Segment s = segment_at(p, sh.line, u, u1, ROWS, M::kKeys);
+            const int blocks = s.end - s.begin;
+            if (wait(kQFull, seg & 1)) scores();
+            for (int j = 0; j < blocks && ok; ++j, ++n) {
+                if (j + 1 < blocks && wait(kSFree, n & 1)) scores();
+                if (!wait(kPReady + (n & 1), n >> 1 & 1)) break;
+#pragma unroll 1
+                for (int piece = 0; piece < 2; ++piece) {
+                    if (!wait(kVFull + vs, vphase)) break;
+                    tc::tc_fence_after();
+                    if (tc::elect_one()) {
+                        const uint64_t v_desc = desc_mn_sw128(base + M::kV0 + vs * M::kPieceBytes, M::kPieceHalf);
+#pragma unroll
+                        for (int st = 0; st < 4; ++st)  // 16 keys: two groups of V
+                            tc::umma_f16_ss(tmem + (1 + (n & 1)) * M::kColO, v_desc + static_cast<uint64_t>(st * (2048 >> 4)),
+                                            p_desc + static_cast<uint64_t>((n & 1) * (M::kOpBytes >> 4) + piece * (M::kOpHalf >> 4) + st * 2), idesc_o,
+                                            piece || st ? 1u : 0u);
+                        tc::umma_commit(bar(kVEmpty + vs));
+                        if (piece) tc::umma_commit(bar(kOFull + (n & 1)));
+                    }
+                    __syncwarp();
+                    if (++vs == M::kVStages) {
+                        vs = 0;
+                        vphase ^= 1;
+                    }
+                }
+            }
+            u += blocks;
+        }
+    } else {
+        // ================= softmax =================
+        constexpr int kR = ROWS / 2;  // rows of a thread
+        const int quad = warp & 3, hf = warp >> 2, key = quad * 32 + lane, first = hf * kR;  // the key of a block, and the dimension
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16) + first;
+        float *const s_max = reinterpret_cast<float *>(sm + M::kMax) + first, *const s_part = reinterpret_cast<float *>(sm + M::kPart) + first;  // s_part[quadrant * ROWS + row]
+        auto arrive = [&](int i) {
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar(i));
+        };
+        auto meet = [&]() { ptx::named_barrier(1, M::kSoftWarps * 32); };
+        auto half_meet = [&]() { ptx::named_barrier(2 + hf, 128); };  // the four warps with the same rows
+        // where this thread's probabilities go: column `key` of the operand, row n at n * 128, its 16-byte units XOR-ed with n & 7
+        uint8_t *const p_at = sm + M::kP0 + (key >> 6) * M::kOpHalf + (key & 7) * 2;
+        const int p_unit = (key >> 3) & 7;
+        int n = 0;  // blocks so far, over all segments
+        for (int u = u0; u < u1;) {
+            const Segment s = segment_at(p, sh.line, u, u1, ROWS, M::kKeys);
+            const int pos = sh.line.pos[s.seq], count = sh.line.count[s.seq], rows_all = count * group, row0 = s.tile * ROWS;
+            const bool nodes = s.end * M::kKeys > pos;  // some blocks hold nodes
+            meet();  // nobody reads what the last segment left in the tree's place any more
+            // the tile's queries, a row as one load of a warp, all of them asked for before the first is looked at
+            constexpr int kEach = ROWS / M::kSoftWarps;
+            float4 qv[kEach];
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) qv[i] = query<TERMS>(p, s.seq, s.kh, group, row0 + warp * kEach + i, rows_all, lane);
+            if (nodes) load_parents(p, sh.parent, s.seq, count, M::kSoftWarps * 32);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                uint2 term[TERMS];
+                query_terms<TERMS>(qv[i], term);
+                const int r = warp * kEach + i;
+#pragma unroll
+                for (int x = 0; x < TERMS; ++x)
+                    *reinterpret_cast<uint2 *>(sm + (lane >> 4) * M::kOpHalf + (x * ROWS + r) * 128 + ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8) = term[x];
+            }
+            ptx::fence_proxy_async();  // the tensor core reads them through the asynchronous proxy
+            arrive(kQFull);
+            if (tid < ROWS) reinterpret_cast<float *>(sm + M::kMax)[tid] = kNoMax;
+            meet();
+            if (nodes) {
+                for (int i = tid; i < count; i += M::kSoftWarps * 32) tree_masks(sh.parent, sh.mask, i);
+                meet();
+            }
+            float acc[kR], l[kR];  // of this thread's dimension; of its key of every block
+#pragma unroll
+            for (int i = 0; i < kR; ++i) acc[i] = l[i] = 0.0f;
+            auto for_rows = [&](uint32_t at, auto &&give) {  // give(row, the terms' sum)
+                constexpr int kChunk = kR < 16 ? kR : 16;
+#pragma unroll
+                for (int c = 0; c < kR; c += kChunk) {
+                    uint32_t w[TERMS][kChunk];
+#pragma unroll
+                    for (int x = 0; x < TERMS; ++x) tc::tmem_ld(at + x * ROWS + c, w[x]);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < kChunk; ++i) {
+                        float v = __uint_as_float(w[TERMS - 1][i]);
+#pragma unroll
+                        for (int x = TERMS - 2; x >= 0; --x) v += __uint_as_float(w[x][i]);
+                        give(c + i, v);
+                    }
+                }
+            };
+            auto add_products = [&](int block) {
+                wait(kOFull + (block & 1), block >> 1 & 1);
+                tc::tc_fence_after();
+                for_rows(lanes + (1 + (block & 1)) * M::kColO, [&](int i, float v) { acc[i] += v; });
+            };
+            for (int j = s.begin; j < s.end; ++j, ++n) {
+                float sv[kR];
+                bool added = j == s.begin;
+                wait(kSFull, n & 1);
+                tc::tc_fence_after();
+                for_rows(lanes, [&](int i, float v) { sv[i] = v * p.scale; });
+                tc::tc_fence_before();
+                arrive(kSFree);
+                const int node = j * M::kKeys + key - pos;  // this thread's key
+                if (j * M::kKeys + quad * 32 + 32 > pos && node >= 0) {
+#pragma unroll
+                    for (int i = 0; i < kR; ++i) {
+                        const int row = row0 + first + i;
+                        if (node >= count || row >= rows_all || !sees(sh.mask[p.node_of(row)], node)) sv[i] = -INFINITY;
+                    }
+                }
+                bool over = false;
+#pragma unroll
+                for (int i = 0; i < kR; i += 4) {
+                    const float4 m = *reinterpret_cast<const float4 *>(s_max + i);
+                    over |= sv[i] > m.x + kSlack || sv[i + 1] > m.y + kSlack || sv[i + 2] > m.z + kSlack || sv[i + 3] > m.w + kSlack;
+                }
+                if (any_of(2 + hf, 128, over)) {  // the rows' maxima move to this block's
+                    if (!added) {
+                        add_products(n - 1);
+                        added = true;
+                    }
+                    float most[kR];
+#pragma unroll
+                    for (int i = 0; i < kR; ++i) most[i] = sv[i];
+                    over_lanes<kR>(most, lane, [](float a, float b) { return fmaxf(a, b); });
+                    if (lane % (32 / kR) == 0) s_part[quad * ROWS + lane / (32 / kR)] = most[0];
+                    half_meet();
+                    auto moved = [&](int i) { return fmaxf(fmaxf(fmaxf(s_part[i], s_part[ROWS + i]), fmaxf(s_part[2 * ROWS + i], s_part[3 * ROWS + i])), s_max[i]); };
+#pragma unroll
+                    for (int i = 0; i < kR; ++i) {
+                        const float corr = ex2(s_max[i] - moved(i));
+                        acc[i] *= corr;
+                        l[i] *= corr;
+                    }
+                    half_meet();
+                    if (quad == 0 && lane < kR) s_max[lane] = moved(lane);
+                    half_meet();
+                }
+#pragma unroll
+                for (int i = 0; i < kR; i += 4) {
+                    const float4 m = *reinterpret_cast<const float4 *>(s_max + i);
+                    sv[i] = ex2(sv[i] - m.x);
+                    sv[i + 1] = ex2(sv[i + 1] - m.y);
+                    sv[i + 2] = ex2(sv[i + 2] - m.z);
+                    sv[i + 3] = ex2(sv[i + 3] - m.w);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) l[i + e] += sv[i + e];
+                }
+                // their place is free: the products of the block in front of the last have been added
+#pragma unroll
+                for (int i = 0; i < kR; i += 2) {
+                    uint32_t term[TERMS];
+                    split_pair<TERMS>(sv[i], sv[i + 1], term);
+#pragma unroll
+                    for (int x = 0; x < TERMS; ++x) {
+                        const int r = x * ROWS + first + i;
+                        *reinterpret_cast<uint16_t *>(p_at + (n & 1) * M::kOpBytes + r * 128 + ((p_unit ^ (r & 7)) << 4)) = static_cast<uint16_t>(term[x]);
+                        *reinterpret_cast<uint16_t *>(p_at + (n & 1) * M::kOpBytes + (r + 1) * 128 + ((p_unit ^ ((r + 1) & 7)) << 4)) = static_cast<uint16_t>(term[x] >> 16);
+                    }
+                }
+                if (j * M::kKeys + M::kKeys > pos) {  // values past the last node, and values of nodes that are no numbers: a thread half a row of this warp's piece
+                    const int piece = 2 * n + hf, vs = piece % M::kVStages, at = j * M::kKeys + hf * 64 + (key & 63) - pos;
+                    if (wait(kVFull + vs, (piece / M::kVStages) & 1) && at >= 0 &&
+                        clean_values(reinterpret_cast<uint4 *>(sm + M::kV0 + vs * M::kPieceBytes + (key >> 6) * M::kPieceHalf + (key & 63) * 128), 8, at >= count))
+                        sh.odd = u + 1;  // read behind a meeting below, written again behind the next segment's first
+                }
+                ptx::fence_proxy_async();
+                tc::tc_fence_before();
+                arrive(kPReady + (n & 1));
+                if (!added) add_products(n - 1);  // while the tensor core works on this block's
+            }
+            add_products(n - 1);
+            // the rows' weights: over the lanes, then the quadrants
+            over_lanes<kR>(l, lane, [](float a, float b) { return a + b; });
+            if (lane % (32 / kR) == 0) s_part[quad * ROWS + lane / (32 / kR)] = l[0];
+            meet();
+            if (nodes && sh.odd == u + 1) {  // what a row sees that is no number
+                for (int i = max(0, s.begin * M::kKeys - pos); i < min(count, s.end * M::kKeys - pos); ++i) {
+                    const uint16_t v = p.vcache[(static_cast<size_t>(s.seq * p.kvh + s.kh) * p.cap + pos + i) * kHd + key];
+                    if ((v & 0x7f80u) != 0x7f80u) continue;
+#pragma unroll
+                    for (int r = 0; r < kR; ++r)
+                        if (row0 + first + r < rows_all && sees(sh.mask[p.node_of(row0 + first + r)], i)) acc[r] += dense::bf16_f32(v);
+                }
+            }
+            const bool whole = s.begin == 0 && s.end == s.blocks;
+            const int here = rows_all - row0 - first;  // of this thread's rows
+            if (ok && here > 0) {
+                auto weight = [&](int r) { return (s_part[r] + s_part[ROWS + r]) + (s_part[2 * ROWS + r] + s_part[3 * ROWS + r]); };
+                if (whole) {
+                    int at_node = p.node_of(row0 + first), g = row0 + first - at_node * group;
+                    size_t at = (static_cast<size_t>(s.seq) * p.t + at_node) * p.out_pitch + (s.kh * group + g) * kHd + key;
+#pragma unroll
+                    for (int r = 0; r < kR; ++r) {
+                        const float x = acc[r] * (1.0f / weight(r));
+                        if (r < here) dense::put(static_cast<std::conditional_t<(TERMS > 1), float, uint16_t> *>(p.out) + at, x);
+                        const bool next = ++g == group;  // the next row is the next head, or the first head of the next node
+                        at += next ? p.out_pitch - (group - 1) * kHd : kHd;
+                        g = next ? 0 : g;
+                    }
+                } else {
+                    const size_t part0 = (static_cast<size_t>(blockIdx.x) * 2 + (u == u0 ? 0 : 1)) * ROWS + first;
+                    float *to = p.part + part0 * kHd + key;
+#pragma unroll
+                    for (int r = 0; r < kR; ++r)
+                        if (r < here) to[r * kHd] = acc[r];
+                    if (quad == 0 && lane < min(kR, here)) p.part_ml[part0 + lane] = make_float2(s_max[lane], weight(lane));
+                }
+            }
+            u += s.end - s.begin;
+        }
+    }
     if (!ok && lane == 0) atomicExch(p.err_word, 5);
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == M::kMmaWarp) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, M::kTmem);
+    }
 }
 
 // ---- many rows: tcgen05, tiles of 128 rows ---------------------------------------------------------------
@@ -517,24 +624,11 @@ struct Many {
     // Scores (128 columns) and, when all have been read, the probabilities (64 a term) of even blocks in one place, of odd ones in another
     static constexpr uint32_t kPlace = 192, kColO = 384;
 };
-struct ManyShared {
-    Line line;
-    int parent[kTreeNodes];
-    ulonglong2 mask[kTreeNodes];
-    int abort, odd;
-    uint32_t tmem;
-};
-// MN-major SWIZZLE_128B operand: groups of 8 keys 1024 bytes apart (stride byte offset), the halves of 64 dimensions `apart` bytes (leading byte offset)
-__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t apart) {
-    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | static_cast<uint64_t>(apart >> 4) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 |
-           static_cast<uint64_t>(2) << 61;
-}
-
 template <int TERMS>
 __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kernel(const __grid_constant__ TreeParams p) {
     using M = Many<TERMS>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ ManyShared sh;
+    __shared__ CtaShared sh;
     const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t *sm = smem_raw + (base - raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -571,47 +665,14 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
         if (warp == M::kMmaWarp) tc::tmem_dealloc(tmem, 512);
         return;
     }
-    const int group = p.nh / p.kvh;
+    const int group = p.group;
     bool ok = true;
 
     // The launch has 20 warps x 96 registers; 4 x 64 + 16 x 104 are as many.
     if (warp >= M::kSoftWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == M::kKWarp || warp == M::kVWarp) {
-            // ================= TMA producers =================
-            const bool is_k = warp == M::kKWarp;
-            const int stages = is_k ? M::kKStages : M::kVStages, full = is_k ? kKFull : kVFull, empty = is_k ? kKEmpty : kVEmpty;
-            if (lane == 0) {
-                int stage = 0, round = 0, sent = 0;
-                for (int u = u0; u < u1 && ok;) {
-                    const Segment s = segment_at(p, sh.line, u, u1, M::kRows, M::kKeys);
-                    const int row0 = (s.seq * p.kvh + s.kh) * p.cap;
-                    for (int i = is_k ? s.begin : 2 * s.begin; i < (is_k ? s.end : 2 * s.end); ++i, ++sent) {
-                        if (round > 0 && !tc::wait_bar(bar(empty + stage), (round - 1) & 1, abort)) {
-                            ok = false;
-                            break;
-                        }
-                        if (is_k) {
-                            const uint32_t at = base + M::kK0 + stage * M::kKBytes;
-                            ptx::mbar_arrive_expect_tx(bar(full + stage), M::kKBytes);
-                            ptx::tma_load_2d(at, &p.k, bar(full + stage), 0, row0 + i * M::kKeys);
-                            ptx::tma_load_2d(at + M::kHalf, &p.k, bar(full + stage), 128, row0 + i * M::kKeys);
-                        } else {
-                            const uint32_t at = base + M::kV0 + stage * M::kPieceBytes;
-                            ptx::mbar_arrive_expect_tx(bar(full + stage), M::kPieceBytes);
-                            ptx::tma_load_2d(at, &p.v, bar(full + stage), 0, row0 + i * M::kPiece);
-                            ptx::tma_load_2d(at + M::kPieceHalf, &p.v, bar(full + stage), 128, row0 + i * M::kPiece);
-                        }
-                        if (++stage == stages) {
-                            stage = 0;
-                            ++round;
-                        }
-                    }
-                    u += s.end - s.begin;
-                }
-                // the copies in flight land before the block may go, whoever has given up
-                for (int n = max(0, sent - stages); n < sent; ++n) ptx::mbar_wait(bar(full + n % stages), (n / stages) & 1, tc::kTcWaitLimit);
-            }
+            produce<M>(p, sh.line, u0, u1, M::kRows, warp == M::kKWarp, base, bar(warp == M::kKWarp ? kKFull : kVFull), bar(warp == M::kKWarp ? kKEmpty : kVEmpty), abort, ok);
         } else if (warp == M::kMmaWarp) {
             // ================= MMA issue: the warp walks, one lane issues =================
             // D f32, A and B bf16, M = 128, N = 128; for P V the B operand is MN-major (bit 16)
@@ -787,22 +848,9 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                 }
                 if (j * M::kKeys + M::kKeys > pos) {  // values past the last node, and values of nodes that are no numbers: a thread 32 dimensions of a row of this warp's piece
                     const int piece = 2 * n + (part >> 1), vs = piece % M::kVStages, quarter = (part & 1) * 2 + (r >> 6), key = r & 63, at = j * M::kKeys + (part >> 1) * 64 + key - pos;
-                    if (wait(kVFull + vs, (piece / M::kVStages) & 1) && at >= 0) {
-                        uint4 *v = reinterpret_cast<uint4 *>(sm + M::kV0 + vs * M::kPieceBytes + (quarter >> 1) * M::kPieceHalf + key * 128 + (quarter & 1) * 64);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint4 x = v[i];
-                            if (at >= count) {
-                                v[i] = make_uint4(0u, 0u, 0u, 0u);
-                            } else {
-                                const uint4 y = make_uint4(only_numbers(x.x), only_numbers(x.y), only_numbers(x.z), only_numbers(x.w));
-                                if (((x.x ^ y.x) | (x.y ^ y.y) | (x.z ^ y.z) | (x.w ^ y.w)) != 0u) {
-                                    v[i] = y;
-                                    sh.odd = u + 1;  // read behind a meeting below, written again behind the next segment's first
-                                }
-                            }
-                        }
-                    }
+                    if (wait(kVFull + vs, (piece / M::kVStages) & 1) && at >= 0 &&
+                        clean_values(reinterpret_cast<uint4 *>(sm + M::kV0 + vs * M::kPieceBytes + (quarter >> 1) * M::kPieceHalf + key * 128 + (quarter & 1) * 64), 4, at >= count))
+                        sh.odd = u + 1;  // read behind a meeting below, written again behind the next segment's first
                     ptx::fence_proxy_async();
                 }
                 // the products of the block in front are added, then their place is free
@@ -873,16 +921,19 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
     }
 }
 
-// Joins the parts of the tiles that were cut. A block takes some rows of the tile that begins in its worker's share and ends behind it, if there is one: a
-// warp a row, four dimensions a lane. Which that is is known before the attention kernel is done.
-constexpr int kMergeRows = 16;  // rows a block
-template <int TERMS, int ROWS, int KEYS>
-__global__ void __launch_bounds__(kMergeRows * 32) attn_tree_merge_kernel(const __grid_constant__ TreeParams p) {
+// Joins the parts of the tiles that were cut. A block takes some rows of the tile that begins in its worker's share and ends behind it, if there is one: SPLIT
+// warps a row, which take every SPLIT-th part, four dimensions a lane. A tile of few rows may have 148 parts, one of 128 rows two or three as a rule. Which tile
+// that is is known before the attention kernel is done.
+constexpr int kMergeWarps = 16;
+template <int TERMS, int ROWS, int KEYS, int SPLIT>
+__global__ void __launch_bounds__(kMergeWarps * 32) attn_tree_merge_kernel(const __grid_constant__ TreeParams p) {
     __shared__ Line line;
+    __shared__ float4 s_sum[kMergeWarps][32];
+    __shared__ float2 s_ml[kMergeWarps];
     ptx::pdl_trigger();
     cut_line<ROWS, KEYS>(p, line);
     const Shares shares(line.first[p.b], p.workers);
-    const int lane = threadIdx.x & 31, r = blockIdx.y * kMergeRows + (threadIdx.x >> 5), group = p.nh / p.kvh, c0 = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, split = warp % SPLIT, r = blockIdx.y * (kMergeWarps / SPLIT) + warp / SPLIT, group = p.group, c0 = blockIdx.x;
     const int u0 = shares.begin(c0), u1 = shares.begin(c0 + 1);
     Segment s{};
     int begin = 0, row = 0, parts = 0;
@@ -894,35 +945,67 @@ __global__ void __launch_bounds__(kMergeRows * 32) attn_tree_merge_kernel(const 
         if (begin >= u0 && end > u1 && row < line.count[s.seq] * group) parts = shares.owner(end - 1) - c0 + 1;  // neighbours that all have a share: this tile goes on in it
     }
     ptx::pdl_wait();  // blocks without a tile too: the next kernel of the stream waits for this one only
+    // part i is the first of its worker's two, but the tile's own first part is the second where the worker came from another tile
+    auto place = [&](int i) { return (static_cast<size_t>(c0 + i) * 2 + (i == 0 && u0 < begin ? 1 : 0)) * ROWS + r; };
+    float m = kNoMax, l = 0.0f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kAtOnce = 8;
+    for (int i0 = split; i0 < parts; i0 += SPLIT * kAtOnce) {
+        float2 ml[kAtOnce];
+        float4 x[kAtOnce];
+        float up = m;
+#pragma unroll
+        for (int e = 0; e < kAtOnce; ++e) {
+            const int i = i0 + e * SPLIT;
+            ml[e] = make_float2(kNoMax, 0.0f);
+            x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i < parts) {
+                ml[e] = p.part_ml[place(i)];
+                x[e] = *reinterpret_cast<const float4 *>(p.part + place(i) * kHd + lane * 4);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kAtOnce; ++e) up = fmaxf(up, ml[e].x);
+        const float corr = ex2(m - up);
+        m = up;
+        l *= corr;
+        sum = make_float4(sum.x * corr, sum.y * corr, sum.z * corr, sum.w * corr);
+#pragma unroll
+        for (int e = 0; e < kAtOnce; ++e) {
+            const float w = ex2(ml[e].x - m);
+            l += ml[e].y * w;
+            sum.x += x[e].x * w;
+            sum.y += x[e].y * w;
+            sum.z += x[e].z * w;
+            sum.w += x[e].w * w;
+        }
+    }
+    if (SPLIT > 1) {
+        s_sum[warp][lane] = sum;
+        if (lane == 0) s_ml[warp] = make_float2(m, l);
+        __syncthreads();
+        if (split) return;
+#pragma unroll
+        for (int e = 1; e < SPLIT; ++e) {
+            const float2 ml = s_ml[warp + e];
+            const float4 x = s_sum[warp + e][lane];
+            const float up = fmaxf(m, ml.x), corr = ex2(m - up), w = ex2(ml.x - up);
+            m = up;
+            l = l * corr + ml.y * w;
+            sum = make_float4(sum.x * corr + x.x * w, sum.y * corr + x.y * w, sum.z * corr + x.z * w, sum.w * corr + x.w * w);
+        }
+    }
     if (!parts) return;
     const int node = p.node_of(row);
-    auto place = [&](int i) { return (static_cast<size_t>(c0 + i) * 2 + (i == 0 && u0 < begin ? 1 : 0)) * ROWS + r; };
-    float m = kNoMax;
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.part_ml[place(i)].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-        const float2 ml = p.part_ml[place(i)];
-        const float4 x = *reinterpret_cast<const float4 *>(p.part + place(i) * kHd + lane * 4);
-        const float w = ex2(ml.x - m);
-        l += ml.y * w;
-        sum.x += x.x * w;
-        sum.y += x.y * w;
-        sum.z += x.z * w;
-        sum.w += x.w * w;
-    }
     const float inv = 1.0f / l;
     const size_t at = (static_cast<size_t>(s.seq) * p.t + node) * p.out_pitch + static_cast<size_t>(s.kh * group + row - node * group) * kHd + lane * 4;
-    if (TERMS > 1) dense::put4(static_cast<float *>(p.out) + at, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
-    else dense::put4(static_cast<uint16_t *>(p.out) + at, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+    dense::put4(static_cast<std::conditional_t<(TERMS > 1), float, uint16_t> *>(p.out) + at, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
 }
 
 int attn_tree_init(Ctx *ctx) {
-    struct { void (*k)(TreeParams); int smem; } kernels[] = {{attn_tree_few_kernel<1, 1>, Few<1>::kSmem}, {attn_tree_few_kernel<3, 1>, Few<1>::kSmem},
-                                                         {attn_tree_few_kernel<1, 2>, Few<2>::kSmem}, {attn_tree_few_kernel<3, 2>, Few<2>::kSmem}, {attn_tree_many_kernel<1>, Many<1>::kSmem}, {attn_tree_many_kernel<3>, Many<3>::kSmem}};
+    struct { void (*k)(TreeParams); int smem; } kernels[] = {
+        {attn_tree_turned_kernel<1, 16>, Turned<1, 16>::kSmem}, {attn_tree_turned_kernel<3, 16>, Turned<3, 16>::kSmem}, {attn_tree_turned_kernel<1, 32>, Turned<1, 32>::kSmem},
+        {attn_tree_turned_kernel<3, 32>, Turned<3, 32>::kSmem}, {attn_tree_many_kernel<1>, Many<1>::kSmem},             {attn_tree_many_kernel<3>, Many<3>::kSmem}};
     for (auto &f : kernels) LBK_CUDA(cudaFuncSetAttribute(f.k, cudaFuncAttributeMaxDynamicSharedMemorySize, f.smem));
     return LBK_OK;
 }
@@ -931,14 +1014,22 @@ const InitHook kInitAttnTree(attn_tree_init);
 // Rows of a tile for t nodes of `group` heads.
 int tile_rows(size_t t, size_t group) { return t * group <= 16 ? 16 : t * group <= 32 ? 32 : 128; }
 
-template <int ROWS, int KEYS>
-int launch_tree(Ctx *ctx, int terms, TreeParams &p, void (*one)(TreeParams), void (*three)(TreeParams), int threads, int smem, cudaStream_t st) {
-    LBK_CUDA(launch_chained(terms == 3 ? three : one, dim3(static_cast<unsigned>(p.workers)), dim3(threads), static_cast<size_t>(smem), st, p));
+template <int TERMS, int ROWS>
+int launch_tree(Ctx *ctx, TreeParams &p, cudaStream_t st) {
+    using T = Turned<TERMS, ROWS <= 32 ? ROWS : 16>;
+    using M = Many<TERMS>;
+    if (ROWS <= 32) LBK_CUDA(launch_chained(attn_tree_turned_kernel<TERMS, ROWS <= 32 ? ROWS : 16>, dim3(static_cast<unsigned>(p.workers)), dim3(T::kThreads), static_cast<size_t>(T::kSmem), st, p));
+    else LBK_CUDA(launch_chained(attn_tree_many_kernel<TERMS>, dim3(static_cast<unsigned>(p.workers)), dim3(M::kThreads), static_cast<size_t>(M::kSmem), st, p));
     ctx->launches++;
-    const dim3 grid(static_cast<unsigned>(p.workers), (std::min(ROWS, p.t * (p.nh / p.kvh)) + kMergeRows - 1) / kMergeRows);
-    LBK_CUDA(launch_chained(terms == 3 ? attn_tree_merge_kernel<3, ROWS, KEYS> : attn_tree_merge_kernel<1, ROWS, KEYS>, grid, dim3(kMergeRows * 32), 0, st, p));
+    constexpr int kSplit = ROWS <= 32 ? 4 : 1, kRows = kMergeWarps / kSplit;
+    const dim3 grid(static_cast<unsigned>(p.workers), (std::min(ROWS, p.t * p.group) + kRows - 1) / kRows);
+    LBK_CUDA(launch_chained(attn_tree_merge_kernel<TERMS, ROWS, 128, kSplit>, grid, dim3(kMergeWarps * 32), 0, st, p));
     ctx->launches++;
     return LBK_OK;
+}
+template <int TERMS>
+int launch_tree(Ctx *ctx, int tile, TreeParams &p, cudaStream_t st) {
+    return tile == 16 ? launch_tree<TERMS, 16>(ctx, p, st) : tile == 32 ? launch_tree<TERMS, 32>(ctx, p, st) : launch_tree<TERMS, 128>(ctx, p, st);
 }
 
 }  // namespace
@@ -983,21 +1074,19 @@ int lbk_attn_tree(lbk_ctx *c, int compute, const void *q_dev, size_t q_pitch, co
     p.counts = counts_dev;
     p.b = static_cast<int>(b);
     p.t = static_cast<int>(t);
-    p.nh = static_cast<int>(n_heads);
+    p.group = static_cast<int>(group);
     p.kvh = static_cast<int>(kv_heads);
     p.cap = static_cast<int>(cap);
     p.scale = scale * 1.4426950408889634f;
     p.workers = ctx->sm_count;
     p.per_group = group > 1 ? static_cast<unsigned>((0x100000000ull + group - 1) / group) : 0u;  // exact: rows * heads of a group < 2^32
     p.err_word = ctx->err_word;
-    const int tile = tile_rows(t, group), terms = compute == LBK_COMPUTE_F32 ? 3 : 1;
+    const int tile = tile_rows(t, group);
     p.part = scratch_dev;
     p.part_ml = reinterpret_cast<float2 *>(scratch_dev + static_cast<size_t>(p.workers) * 2 * tile * kHd);
-    LBK_TRY(encode_bytes_map(&p.k, kcache_dev, 256, rows, 256, 128, tile == 128 ? 128 : 64));
+    LBK_TRY(encode_bytes_map(&p.k, kcache_dev, 256, rows, 256, 128, 128));
     LBK_TRY(encode_bytes_map(&p.v, vcache_dev, 256, rows, 256, 128, 64));
-    if (tile == 16) return launch_tree<16, 64>(ctx, terms, p, attn_tree_few_kernel<1, 1>, attn_tree_few_kernel<3, 1>, Few<1>::kThreads, Few<1>::kSmem, st);
-    if (tile == 128) return launch_tree<128, 128>(ctx, terms, p, attn_tree_many_kernel<1>, attn_tree_many_kernel<3>, Many<1>::kThreads, Many<1>::kSmem, st);
-    return launch_tree<32, 64>(ctx, terms, p, attn_tree_few_kernel<1, 2>, attn_tree_few_kernel<3, 2>, Few<2>::kThreads, Few<2>::kSmem, st);
+    return compute == LBK_COMPUTE_F32 ? launch_tree<3>(ctx, tile, p, st) : launch_tree<1>(ctx, tile, p, st);
 }
 
 }  // extern "C"

@@ -223,9 +223,12 @@ __device__ __forceinline__ bool clean_values(uint4 *v, int units, bool all) {
     }
     return odd;
 }
+constexpr int kQueriesAsked = 8;  // named barrier
 // A producer warp of a kernel with layout M: the K blocks, or the V pieces, of a share. full, empty: the first of the stages' barriers.
 template <class M>
 __device__ __forceinline__ void produce(const TreeParams &p, const Line &line, int u0, int u1, int rows, bool is_k, uint32_t base, uint32_t full, uint32_t empty, volatile int *abort, bool &ok) {
+    // The first queries go first: behind 128 KB of keys and values an SM, which all ask for at the same time, they took 3000 to 6000 cycles
+    ptx::named_barrier(kQueriesAsked, M::kSoftWarps * 32 + 64);
     if ((threadIdx.x & 31) != 0) return;
     const int stages = is_k ? M::kKStages : M::kVStages;
     int stage = 0, round = 0, sent = 0;
@@ -415,6 +418,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
             if (lane == 0) ptx::mbar_arrive(bar(i));
         };
         auto meet = [&]() { ptx::named_barrier(1, M::kSoftWarps * 32); };
+        auto queries_asked = [&]() { asm volatile("barrier.cta.arrive %0, %1;" ::"r"(kQueriesAsked), "r"(M::kSoftWarps * 32 + 64) : "memory"); };
         auto half_meet = [&]() { ptx::named_barrier(2 + hf, 128); };  // the four warps with the same rows
         // where this thread's probabilities go: column `key` of the operand, row n at n * 128, its 16-byte units XOR-ed with n & 7
         uint8_t *const p_at = sm + M::kP0 + (key >> 6) * M::kOpHalf + (key & 7) * 2;
@@ -430,6 +434,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
             float4 qv[kEach];
 #pragma unroll
             for (int i = 0; i < kEach; ++i) qv[i] = query<TERMS>(p, s.seq, s.kh, group, row0 + warp * kEach + i, rows_all, lane);
+            if (u == u0) queries_asked();
             if (nodes) load_parents(p, sh.parent, s.seq, count, M::kSoftWarps * 32);
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
@@ -755,6 +760,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
             if (lane == 0) ptx::mbar_arrive(bar(i));
         };
         auto meet = [&]() { ptx::named_barrier(1, M::kSoftWarps * 32); };
+        auto queries_asked = [&]() { asm volatile("barrier.cta.arrive %0, %1;" ::"r"(kQueriesAsked), "r"(M::kSoftWarps * 32 + 64) : "memory"); };
         auto quad_sync = [&]() { ptx::named_barrier(2 + quad, 128); };  // the four warps of a quadrant
         int n = 0;  // blocks so far, over all segments
         for (int u = u0; u < u1;) {
@@ -768,6 +774,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
             float4 qv[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) qv[i] = query<TERMS>(p, s.seq, s.kh, group, row0 + warp * 8 + i, rows_all, lane);
+            if (u == u0) queries_asked();
             if (nodes) load_parents(p, sh.parent, s.seq, count, M::kSoftWarps * 32);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -921,11 +928,12 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
     }
 }
 
-// Joins the parts of the tiles that were cut. A block takes some rows of the tile that begins in its worker's share and ends behind it, if there is one: SPLIT
-// warps a row, which take every SPLIT-th part, four dimensions a lane. A tile of few rows may have 148 parts, one of 128 rows two or three as a rule. Which tile
-// that is is known before the attention kernel is done.
-constexpr int kMergeWarps = 16;
-template <int TERMS, int ROWS, int KEYS, int SPLIT>
+// Joins the parts of the tiles that were cut. kMergeBlocks blocks share the tile that begins in a worker's share and ends behind it, if there is one. Two or three parts, as
+// a rule: a warp a row; more than two batches of them (up to 148 of one sequence's one tile): four warps a row, which take every fourth part. Four dimensions a lane. Small
+// blocks, all of them beside one another: each has to find its tile first, and beside the attention kernel's blocks there are no registers for these. (us for 1 x 5 nodes, 4001
+// keys, 5 tiles of 32 parts, and 1 x 60 nodes, 65000 keys, 16 of 9: one block of 32 warps a tile 24.8 and 162, blocks of 16 warps in four waves 16.5 and 108.)
+constexpr int kMergeWarps = 4, kMergeBlocks = 8, kAtOnce = 8;
+template <int TERMS, int ROWS, int KEYS>
 __global__ void __launch_bounds__(kMergeWarps * 32) attn_tree_merge_kernel(const __grid_constant__ TreeParams p) {
     __shared__ Line line;
     __shared__ float4 s_sum[kMergeWarps][32];
@@ -933,73 +941,80 @@ __global__ void __launch_bounds__(kMergeWarps * 32) attn_tree_merge_kernel(const
     ptx::pdl_trigger();
     cut_line<ROWS, KEYS>(p, line);
     const Shares shares(line.first[p.b], p.workers);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, split = warp % SPLIT, r = blockIdx.y * (kMergeWarps / SPLIT) + warp / SPLIT, group = p.group, c0 = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = p.group, c0 = blockIdx.x;
     const int u0 = shares.begin(c0), u1 = shares.begin(c0 + 1);
     Segment s{};
-    int begin = 0, row = 0, parts = 0;
+    int begin = 0, parts = 0, rows = 0;
     if (u0 < u1) {
         s = segment_at(p, line, u1 - 1, u1, ROWS, KEYS);  // the last block of the share
         begin = u1 - 1 - s.begin;
-        row = s.tile * ROWS + r;
+        rows = min(ROWS, line.count[s.seq] * group - s.tile * ROWS);
         const int end = begin + s.blocks;
-        if (begin >= u0 && end > u1 && row < line.count[s.seq] * group) parts = shares.owner(end - 1) - c0 + 1;  // neighbours that all have a share: this tile goes on in it
+        if (begin >= u0 && end > u1) parts = shares.owner(end - 1) - c0 + 1;  // neighbours that all have a share: this tile goes on in it
     }
     ptx::pdl_wait();  // blocks without a tile too: the next kernel of the stream waits for this one only
-    // part i is the first of its worker's two, but the tile's own first part is the second where the worker came from another tile
-    auto place = [&](int i) { return (static_cast<size_t>(c0 + i) * 2 + (i == 0 && u0 < begin ? 1 : 0)) * ROWS + r; };
-    float m = kNoMax, l = 0.0f;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kAtOnce = 8;
-    for (int i0 = split; i0 < parts; i0 += SPLIT * kAtOnce) {
-        float2 ml[kAtOnce];
-        float4 x[kAtOnce];
-        float up = m;
+    if (!parts) return;
+    const int splits = parts <= 2 * kAtOnce ? 1 : 4, split = warp & (splits - 1);
+    constexpr int kShare = ROWS / kMergeBlocks;
+    const int r1 = min(rows, static_cast<int>(blockIdx.y + 1) * kShare);
+    for (int r0 = blockIdx.y * kShare; r0 < r1; r0 += kMergeWarps / splits) {
+        const int r = r0 + warp / splits;
+        // part i is the first of its worker's two, but the tile's own first part is the second where the worker came from another tile
+        auto place = [&](int i) { return (static_cast<size_t>(c0 + i) * 2 + (i == 0 && u0 < begin ? 1 : 0)) * ROWS + r; };
+        float m = kNoMax, l = 0.0f;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = split; i0 < (r < r1 ? parts : 0); i0 += splits * kAtOnce) {
+            float2 ml[kAtOnce];
+            float4 x[kAtOnce];
+            float up = m;
 #pragma unroll
-        for (int e = 0; e < kAtOnce; ++e) {
-            const int i = i0 + e * SPLIT;
-            ml[e] = make_float2(kNoMax, 0.0f);
-            x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (i < parts) {
-                ml[e] = p.part_ml[place(i)];
-                x[e] = *reinterpret_cast<const float4 *>(p.part + place(i) * kHd + lane * 4);
+            for (int e = 0; e < kAtOnce; ++e) {
+                const int i = i0 + e * splits;
+                ml[e] = make_float2(kNoMax, 0.0f);
+                x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < parts) {
+                    ml[e] = p.part_ml[place(i)];
+                    x[e] = *reinterpret_cast<const float4 *>(p.part + place(i) * kHd + lane * 4);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) up = fmaxf(up, ml[e].x);
+            const float corr = ex2(m - up);
+            m = up;
+            l *= corr;
+            sum = make_float4(sum.x * corr, sum.y * corr, sum.z * corr, sum.w * corr);
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) {
+                const float w = ex2(ml[e].x - m);
+                l += ml[e].y * w;
+                sum.x += x[e].x * w;
+                sum.y += x[e].y * w;
+                sum.z += x[e].z * w;
+                sum.w += x[e].w * w;
             }
         }
+        if (splits > 1) {
+            s_sum[warp][lane] = sum;
+            if (lane == 0) s_ml[warp] = make_float2(m, l);
+            __syncthreads();
+            if (!split)
 #pragma unroll
-        for (int e = 0; e < kAtOnce; ++e) up = fmaxf(up, ml[e].x);
-        const float corr = ex2(m - up);
-        m = up;
-        l *= corr;
-        sum = make_float4(sum.x * corr, sum.y * corr, sum.z * corr, sum.w * corr);
-#pragma unroll
-        for (int e = 0; e < kAtOnce; ++e) {
-            const float w = ex2(ml[e].x - m);
-            l += ml[e].y * w;
-            sum.x += x[e].x * w;
-            sum.y += x[e].y * w;
-            sum.z += x[e].z * w;
-            sum.w += x[e].w * w;
+                for (int e = 1; e < 4; ++e) {
+                    const float2 ml = s_ml[warp + e];
+                    const float4 x = s_sum[warp + e][lane];
+                    const float up = fmaxf(m, ml.x), corr = ex2(m - up), w = ex2(ml.x - up);
+                    m = up;
+                    l = l * corr + ml.y * w;
+                    sum = make_float4(sum.x * corr + x.x * w, sum.y * corr + x.y * w, sum.z * corr + x.z * w, sum.w * corr + x.w * w);
+                }
+            __syncthreads();
         }
+        if (split || r >= r1) continue;
+        const int row = s.tile * ROWS + r, node = p.node_of(row);
+        const float inv = 1.0f / l;
+        const size_t at = (static_cast<size_t>(s.seq) * p.t + node) * p.out_pitch + static_cast<size_t>(s.kh * group + row - node * group) * kHd + lane * 4;
+        dense::put4(static_cast<std::conditional_t<(TERMS > 1), float, uint16_t> *>(p.out) + at, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
     }
-    if (SPLIT > 1) {
-        s_sum[warp][lane] = sum;
-        if (lane == 0) s_ml[warp] = make_float2(m, l);
-        __syncthreads();
-        if (split) return;
-#pragma unroll
-        for (int e = 1; e < SPLIT; ++e) {
-            const float2 ml = s_ml[warp + e];
-            const float4 x = s_sum[warp + e][lane];
-            const float up = fmaxf(m, ml.x), corr = ex2(m - up), w = ex2(ml.x - up);
-            m = up;
-            l = l * corr + ml.y * w;
-            sum = make_float4(sum.x * corr + x.x * w, sum.y * corr + x.y * w, sum.z * corr + x.z * w, sum.w * corr + x.w * w);
-        }
-    }
-    if (!parts) return;
-    const int node = p.node_of(row);
-    const float inv = 1.0f / l;
-    const size_t at = (static_cast<size_t>(s.seq) * p.t + node) * p.out_pitch + static_cast<size_t>(s.kh * group + row - node * group) * kHd + lane * 4;
-    dense::put4(static_cast<std::conditional_t<(TERMS > 1), float, uint16_t> *>(p.out) + at, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
 }
 
 int attn_tree_init(Ctx *ctx) {
@@ -1021,9 +1036,7 @@ int launch_tree(Ctx *ctx, TreeParams &p, cudaStream_t st) {
     if (ROWS <= 32) LBK_CUDA(launch_chained(attn_tree_turned_kernel<TERMS, ROWS <= 32 ? ROWS : 16>, dim3(static_cast<unsigned>(p.workers)), dim3(T::kThreads), static_cast<size_t>(T::kSmem), st, p));
     else LBK_CUDA(launch_chained(attn_tree_many_kernel<TERMS>, dim3(static_cast<unsigned>(p.workers)), dim3(M::kThreads), static_cast<size_t>(M::kSmem), st, p));
     ctx->launches++;
-    constexpr int kSplit = ROWS <= 32 ? 4 : 1, kRows = kMergeWarps / kSplit;
-    const dim3 grid(static_cast<unsigned>(p.workers), (std::min(ROWS, p.t * p.group) + kRows - 1) / kRows);
-    LBK_CUDA(launch_chained(attn_tree_merge_kernel<TERMS, ROWS, 128, kSplit>, grid, dim3(kMergeWarps * 32), 0, st, p));
+    LBK_CUDA(launch_chained(attn_tree_merge_kernel<TERMS, ROWS, 128>, dim3(static_cast<unsigned>(p.workers), kMergeBlocks), dim3(kMergeWarps * 32), 0, st, p));
     ctx->launches++;
     return LBK_OK;
 }

@@ -63,8 +63,9 @@ __device__ __forceinline__ void split_pair(float x0, float x1, uint32_t (&term)[
     for (int i = 0; i < TERMS; ++i) {
         term[i] = bf16_pair(x0, x1);
         if (i + 1 < TERMS) {
-            x0 -= __uint_as_float(term[i] << 16);
-            x1 -= __uint_as_float(term[i] & 0xffff0000u);
+            const float2 rest = ptx::fma2(make_float2(__uint_as_float(term[i] << 16), __uint_as_float(term[i] & 0xffff0000u)), make_float2(-1.0f, -1.0f), make_float2(x0, x1));
+            x0 = rest.x;
+            x1 = rest.y;
         }
     }
 }
@@ -207,6 +208,11 @@ __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t apart)
            static_cast<uint64_t>(2) << 61;
 }
 
+// A warp's wait for what is complete already as a rule.
+__device__ __forceinline__ bool one_waits(uint32_t bar, uint32_t parity, volatile int *abort) {
+    if (__all_sync(0xffffffffu, ptx::mbar_test_wait(bar, parity))) return true;
+    return tc::warp_wait(bar, parity, abort);
+}
 // Zeros for values that are no numbers, or for all of `units` 16-byte units; whether there was one that is no number.
 __device__ __forceinline__ bool clean_values(uint4 *v, int units, bool all) {
     bool odd = false;
@@ -347,7 +353,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
     const int group = p.group;
     bool ok = true;
     auto wait = [&](int i, int parity) {
-        if (ok) ok = tc::warp_wait(bar(i), parity, abort);
+        if (ok) ok = one_waits(bar(i), parity, abort);
         return ok;
     };
 
@@ -685,7 +691,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
             const uint64_t q_desc = tc::smem_desc_sw128(base);
             int ks = 0, kphase = 0, vs = 0, vphase = 0, n = 0, seg = 0;  // n: blocks whose scores have been asked for
             auto wait = [&](int i, int parity) {
-                if (ok) ok = tc::warp_wait(bar(i), parity, abort);
+                if (ok) ok = one_waits(bar(i), parity, abort);
                 return ok;
             };
             auto scores = [&]() {
@@ -752,7 +758,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
         const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
         float *const s_quad = reinterpret_cast<float *>(sm + M::kPair);  // [2][4 parts][128 rows]
         auto wait = [&](int i, int parity) {
-            if (ok) ok = tc::warp_wait(bar(i), parity, abort);
+            if (ok) ok = one_waits(bar(i), parity, abort);
             return ok;
         };
         auto arrive = [&](int i) {
@@ -803,7 +809,11 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                     tc::tmem_ld16(lanes + M::kColO + part * 32 + c * 16, v);
                     tc::tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[c * 16 + i] = acc[c * 16 + i] * corr + __uint_as_float(v[i]);
+                    for (int i = 0; i < 16; i += 2) {
+                        const float2 x = ptx::fma2(make_float2(acc[c * 16 + i], acc[c * 16 + i + 1]), make_float2(corr, corr), make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+                        acc[c * 16 + i] = x.x;
+                        acc[c * 16 + i + 1] = x.y;
+                    }
                 }
             };
             for (int j = s.begin; j < s.end; ++j, ++n) {
@@ -826,7 +836,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                     }
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(sv[i]));
+                    for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = ptx::max3(mx[(i >> 1) & 3], __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
                     float *quarter = s_quad + (n & 1) * 4 * M::kRows + r;
                     quarter[part * M::kRows] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                     quad_sync();  // the row's scores have all been read; the next block but one writes here again, behind the next block's meeting
@@ -834,24 +844,24 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                     const float nm = fmaxf(m, all * p.scale);
                     step = ex2(m - nm);
                     m = nm;
-                    float sum0 = 0.0f, sum1 = 0.0f;
+                    float2 sum = make_float2(0.0f, 0.0f);
+                    const float2 scale2 = make_float2(p.scale, p.scale), less = make_float2(-nm, -nm);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         uint32_t w[TERMS][8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const float e0 = ex2(__fmaf_rn(__uint_as_float(sv[c * 16 + 2 * i]), p.scale, -nm)), e1 = ex2(__fmaf_rn(__uint_as_float(sv[c * 16 + 2 * i + 1]), p.scale, -nm));
-                            sum0 += e0;
-                            sum1 += e1;
+                            const float2 d = ptx::fma2(make_float2(__uint_as_float(sv[c * 16 + 2 * i]), __uint_as_float(sv[c * 16 + 2 * i + 1])), scale2, less), e = make_float2(ex2(d.x), ex2(d.y));
+                            sum = ptx::add2(sum, e);
                             uint32_t term[TERMS];
-                            split_pair<TERMS>(e0, e1, term);
+                            split_pair<TERMS>(e.x, e.y, term);
 #pragma unroll
                             for (int x = 0; x < TERMS; ++x) w[x][i] = term[x];
                         }
 #pragma unroll
                         for (int x = 0; x < TERMS; ++x) tc::tmem_st8(place + x * 64 + part * 16 + c * 8, w[x]);
                     }
-                    l = l * step + (sum0 + sum1);
+                    l = l * step + (sum.x + sum.y);
                 }
                 if (j * M::kKeys + M::kKeys > pos) {  // values past the last node, and values of nodes that are no numbers: a thread 32 dimensions of a row of this warp's piece
                     const int piece = 2 * n + (part >> 1), vs = piece % M::kVStages, quarter = (part & 1) * 2 + (r >> 6), key = r & 63, at = j * M::kKeys + (part >> 1) * 64 + key - pos;

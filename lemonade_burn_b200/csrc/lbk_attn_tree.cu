@@ -209,7 +209,7 @@ __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t apart)
 }
 
 // A warp's wait for what is complete already as a rule.
-__device__ __forceinline__ bool one_waits(uint32_t bar, uint32_t parity, volatile int *abort) {
+__device__ __forceinline__ bool look_and_wait(uint32_t bar, uint32_t parity, volatile int *abort) {
     if (__all_sync(0xffffffffu, ptx::mbar_test_wait(bar, parity))) return true;
     return tc::warp_wait(bar, parity, abort);
 }
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
     const int group = p.group;
     bool ok = true;
     auto wait = [&](int i, int parity) {
-        if (ok) ok = one_waits(bar(i), parity, abort);
+        if (ok) ok = look_and_wait(bar(i), parity, abort);
         return ok;
     };
 
@@ -691,7 +691,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
             const uint64_t q_desc = tc::smem_desc_sw128(base);
             int ks = 0, kphase = 0, vs = 0, vphase = 0, n = 0, seg = 0;  // n: blocks whose scores have been asked for
             auto wait = [&](int i, int parity) {
-                if (ok) ok = one_waits(bar(i), parity, abort);
+                if (ok) ok = look_and_wait(bar(i), parity, abort);
                 return ok;
             };
             auto scores = [&]() {
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
         const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
         float *const s_quad = reinterpret_cast<float *>(sm + M::kPair);  // [2][4 parts][128 rows]
         auto wait = [&](int i, int parity) {
-            if (ok) ok = one_waits(bar(i), parity, abort);
+            if (ok) ok = look_and_wait(bar(i), parity, abort);
             return ok;
         };
         auto arrive = [&](int i) {

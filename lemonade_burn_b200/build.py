@@ -1,4 +1,4 @@
-"""Builds liblbk.so (the CUDA C-ABI library) in-tree with nvcc for sm_100a."""
+"""Builds liblbk.so (the CUDA C-ABI library) in-tree with nvcc for sm_100a, and _torch_ops.so (the torch side of some of its calls) with g++."""
 from __future__ import annotations
 
 import os
@@ -10,6 +10,7 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "liblbk.so"
+TORCH_SOURCE, TORCH_OPS = CSRC / "lbk_torch.cpp", PKG / "_torch_ops.so"
 OBJ = PKG / "_build"  # object files (git-ignored)
 
 # The runtime every model family needs, and what each family adds. liblbk.so holds all of it; a process that only
@@ -45,9 +46,10 @@ def is_stale(lib: Path = None) -> bool:
 
 
 def _run(cmd, env):
+    """stdout of a compiler."""
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, env=env)
     if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout)
+        raise RuntimeError(f"{Path(cmd[0]).name} failed:\n" + " ".join(cmd) + "\n" + res.stdout)
     return res.stdout
 
 
@@ -61,10 +63,35 @@ def library_for(architecture: str) -> Path:
     return build(lib=PKG / f"liblbk-{architecture}.so", sources=RUNTIME + FAMILIES[architecture])
 
 
+def torch_ops_stale() -> bool:
+    deps = (TORCH_SOURCE, ROOT / "include" / "lbk.h")
+    return not TORCH_OPS.exists() or any(d.stat().st_mtime > TORCH_OPS.stat().st_mtime for d in deps)
+
+
+def build_torch_ops(force: bool = False) -> Path:
+    """Compile the extension module of ops.py. It links torch's libraries and no other: liblbk.so's functions are handed to it."""
+    if not force and not torch_ops_stale():
+        return TORCH_OPS
+    import sysconfig
+
+    import torch
+    home = Path(torch.__file__).resolve().parent
+    include = [home / "include", home / "include" / "torch" / "csrc" / "api" / "include", Path(nvcc_path()).resolve().parent.parent / "include",
+               sysconfig.get_path("include"), ROOT / "include"]
+    part = TORCH_OPS.with_name(f".{TORCH_OPS.name}.{os.getpid()}")
+    _run([shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *[x for i in include for x in ("-isystem", str(i))], "-o", str(part), str(TORCH_SOURCE), f"-L{home / 'lib'}", f"-Wl,-rpath,{home / 'lib'}",
+          "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"], dict(os.environ))
+    os.replace(part, TORCH_OPS)
+    return TORCH_OPS
+
+
 def build(force: bool = False, verbose: bool = False, lib: Path = None, sources=None) -> Path:
     """Compile every .cu (one object each, side by side, only the ones whose source or any header
     changed) and link lemonade_burn_b200/liblbk.so (or `lib` from `sources`). Returns the library path."""
     lib, sources = lib or LIB, sources or SOURCES
+    if lib == LIB:
+        build_torch_ops(force)
     if not force and not is_stale(lib):
         return lib
     from concurrent.futures import ThreadPoolExecutor

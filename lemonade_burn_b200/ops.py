@@ -168,44 +168,26 @@ def bf16_linear(x: torch.Tensor, w: torch.Tensor, ctx: Optional[Context] = None)
 
 TREE_NODES = 128     # node places of a sequence (LBK_TREE_NODES)
 LOGPROBS_TOP = 32    # alternatives of a row (LBK_LOGPROBS_TOP)
+_native = None
 
 
-# The host side of these calls is most of a small one's time (16 us of attn_tree were 11 us of Python): checks are plain comparisons, every result
-# has an allocation of its own (a view of one costs as much as two), pointers go to the library as integers.
-
-def _on(ctx: Context, *tensors: torch.Tensor) -> int:
-    """Checks that the tensors lie on the context's GPU without gaps; the raw current stream of that GPU."""
-    device = ctx.device
-    for t in tensors:
-        if t.get_device() != device:
-            raise ValueError(f"every tensor must live on cuda:{device}")
-        if not t.is_contiguous():
-            raise ValueError("tensors must be contiguous")
-    return torch._C._cuda_getCurrentRawStream(device)
-
-
-def _tree(parents: torch.Tensor, counts: Optional[torch.Tensor], pos: Optional[torch.Tensor] = None) -> Tuple[int, int]:
-    """(sequences, node places) of a batch of trees, or of paths through them."""
-    shape = parents.shape
-    if len(shape) != 2:
-        raise ValueError("the trees are [sequences, nodes]")
-    b, t = shape
-    if not 1 <= t <= TREE_NODES:
-        raise ValueError(f"a tree has 1 to {TREE_NODES} nodes (got {t})")
-    if parents.dtype is not torch.int32:
-        raise TypeError("the trees are int32")
-    if pos is not None and (pos.dtype is not torch.int32 or pos.shape != (b,)) or counts is not None and (counts.dtype is not torch.int32 or counts.shape != (b,)):
-        raise ValueError(f"positions and counts are int32, one for each of the {b} sequences")
-    return b, t
-
-
-def _caches(k: torch.Tensor, v: torch.Tensor, b: int, dims: int) -> torch.Size:
-    if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16:
-        raise TypeError("caches are bf16")
-    shape = k.shape
-    if len(shape) != dims or shape != v.shape or shape[dims - 4] != b:
-        raise ValueError(f"caches are [{'layers, ' if dims == 5 else ''}{b}, kv_heads, capacity, head_dim], keys like values")
-    return shape
+def _torch_ops():
+    """The extension module with the calls below: checks of arguments, results and the library's call (csrc/lbk_torch.cpp). There is no other path."""
+    global _native
+    if _native is None:
+        from importlib.machinery import ExtensionFileLoader
+        from importlib.util import module_from_spec, spec_from_file_location
+        path = _lib.LIB_PATH.with_name("_torch_ops.so")
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build it with `python -m lemonade_burn_b200.build`")
+        loader = ExtensionFileLoader("_torch_ops", str(path))
+        module = module_from_spec(spec_from_file_location("_torch_ops", str(path), loader=loader))
+        loader.exec_module(module)
+        lib = _lib.load()
+        module.bind(*[C.cast(f, C.c_void_p).value for f in (lib.lbk_rope_kv_append_tree, lib.lbk_attn_tree_scratch, lib.lbk_attn_tree, lib.lbk_tree_accept, lib.lbk_kv_keep_path,
+                                                            lib.lbk_advance_pos_by, lib.lbk_token_logprobs)], _lib.check, default_context)
+        _native = module
+    return _native
 
 
 def rope_kv_append_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, parents: torch.Tensor,
@@ -213,35 +195,7 @@ def rope_kv_append_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: 
     """Drafted tokens into the cache (lbk_rope_kv_append_tree): q [b, t, heads * head_dim] f32 is turned in place by pos + depth of its
     node, k and v [b, t, kv_heads * head_dim] f32 go to row pos + i of kcache and vcache [b, kv_heads, cap, head_dim]. parents int32 [b, t]: the
     node a node follows, -1 the committed row pos - 1; counts int32 [b]: how many nodes a sequence has (all t)."""
-    b, t = _tree(parents, counts, pos)
-    _, kvh, cap, hd = _caches(kcache, vcache, b, 4)
-    f32 = torch.float32
-    if q.dtype is not f32 or k.dtype is not f32 or v.dtype is not f32 or cos.dtype is not f32 or sin.dtype is not f32:
-        raise TypeError("queries, keys, values and rotation tables are f32")
-    values, new = q.numel(), k.numel()
-    nh = values // max(1, b * t * hd)
-    if values != b * t * nh * hd or new != b * t * kvh * hd or v.numel() != new:
-        raise ValueError(f"q, k and v are rows of heads of {hd} for {b} x {t} nodes")
-    table = cos.shape
-    if len(table) != 2 or table[0] < cap or table[1] != hd or sin.shape != table:
-        raise ValueError("the rotation tables have a row for every place of the cache")
-    ctx = ctx or default_context()
-    st = _on(ctx, q, k, v, cos, sin, pos, parents, kcache, vcache) if counts is None else _on(ctx, q, k, v, cos, sin, pos, parents, kcache, vcache, counts)
-    status = ctx._lib.lbk_rope_kv_append_tree(ctx.handle, q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), parents.data_ptr(),
-                                              None if counts is None else counts.data_ptr(), b, t, nh, kvh, hd, cap, kcache.data_ptr(), vcache.data_ptr(), st)
-    if status:
-        _lib.check(status)
-
-
-def _node_pitch(x: torch.Tensor, b: int, t: int, nh: int, hd: int) -> int:
-    """Values from one node's row to the next in [b, t, heads, head_dim]."""
-    if x.is_contiguous():
-        return nh * hd
-    seq, row, head, one = x.stride()
-    pitch = row if t > 1 else seq if b > 1 else nh * hd
-    if one != 1 or (nh > 1 and head != hd) or (b > 1 and seq != t * pitch) or pitch < nh * hd:
-        raise ValueError("the heads of a node lie side by side, nodes and sequences at one distance")
-    return pitch
+    (_native or _torch_ops()).rope_kv_append_tree(q, k, v, cos, sin, pos, parents, kcache, vcache, counts, ctx)
 
 
 def attn_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, pos: torch.Tensor, parents: torch.Tensor, counts: Optional[torch.Tensor] = None,
@@ -249,75 +203,25 @@ def attn_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, pos: 
     """Attention of drafted tokens (lbk_attn_tree): q [b, t, heads, 128] f32 or bf16 (nodes any distance apart) over rows 0 .. pos - 1 of kcache
     and vcache [b, kv_heads, cap, 128] and over the node itself and its ancestors, whose rows are pos + node. scale: 128 ** -0.5. Returns
     `out` (made like q without one: rows of places not in use are then whatever was there)."""
-    b, t = _tree(parents, counts, pos)
-    _, kvh, cap, hd = _caches(kcache, vcache, b, 4)
-    dtype, shape = q.dtype, q.shape
-    if dtype is not torch.float32 and dtype is not torch.bfloat16:
-        raise TypeError("queries are f32 or bf16")
-    if len(shape) != 4 or shape[0] != b or shape[1] != t or shape[3] != hd:
-        raise ValueError(f"queries are [{b}, {t}, heads, {hd}]")
-    nh = shape[2]
-    if hd != 128 or not nh or not kvh or nh % kvh:
-        raise ValueError(f"heads of 128, a multiple of the KV heads (got {nh} and {kvh} heads of {hd})")
-    if out is None:
-        out = q.new_empty(shape)
-    elif out.dtype is not dtype or out.shape != shape:
-        raise ValueError("out is like q")
-    q_pitch, out_pitch = _node_pitch(q, b, t, nh, hd), _node_pitch(out, b, t, nh, hd)
-    ctx = ctx or default_context()
-    st = _on(ctx, kcache, vcache, pos, parents) if counts is None else _on(ctx, kcache, vcache, pos, parents, counts)
-    if q.get_device() != ctx.device or out.get_device() != ctx.device:
-        raise ValueError(f"queries and out must live on cuda:{ctx.device}")
-    lib, f32 = ctx._lib, dtype is torch.float32
-    scratch = q.new_empty(lib.lbk_attn_tree_scratch(ctx.handle, t, nh, kvh) * (1 if f32 else 2))
-    status = lib.lbk_attn_tree(ctx.handle, 1 if f32 else 0, q.data_ptr(), q_pitch, kcache.data_ptr(), vcache.data_ptr(), pos.data_ptr(), parents.data_ptr(),
-                               None if counts is None else counts.data_ptr(), b, t, nh, kvh, hd, cap, hd ** -0.5 if scale is None else scale, scratch.data_ptr(), out.data_ptr(),
-                               out_pitch, st)
-    if status:
-        _lib.check(status)
-    return out
+    return (_native or _torch_ops()).attn_tree(q, kcache, vcache, pos, parents, counts, scale, out, ctx)
 
 
 def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, best: torch.Tensor, counts: Optional[torch.Tensor] = None,
                 ctx: Optional[Context] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The greedy walk through drafted tokens (lbk_tree_accept): tokens, parents, best (the argmax of every node's logits) int32 [b, t].
     Returns (path [b, t]: the accepted nodes, then -1; how many of them [b]; the token that follows the last one [b])."""
-    b, t = _tree(parents, counts)
-    if tokens.dtype is not torch.int32 or best.dtype is not torch.int32:
-        raise TypeError("tokens and best are int32")
-    if tokens.shape != parents.shape or best.shape != parents.shape:
-        raise ValueError(f"tokens and best are [{b}, {t}], as parents")
-    ctx = ctx or default_context()
-    st = _on(ctx, tokens, parents, best) if counts is None else _on(ctx, tokens, parents, best, counts)
-    path, count, after = parents.new_empty((b, t)), parents.new_empty(b), parents.new_empty(b)
-    status = ctx._lib.lbk_tree_accept(ctx.handle, tokens.data_ptr(), parents.data_ptr(), best.data_ptr(), None if counts is None else counts.data_ptr(), b, t, path.data_ptr(),
-                                      count.data_ptr(), after.data_ptr(), st)
-    if status:
-        _lib.check(status)
-    return path, count, after
+    return (_native or _torch_ops()).tree_accept(tokens, parents, best, counts, ctx)
 
 
 def kv_keep_path(k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, path: torch.Tensor, count: torch.Tensor, ctx: Optional[Context] = None) -> None:
     """Closes the gaps that refused drafts leave (lbk_kv_keep_path): of caches [layers, b, kv_heads, cap, head_dim] the rows pos + path[j] move
     to pos + j for j < count. path int32 [b, t] ascending. Positions are not changed (advance_pos_by)."""
-    b, t = _tree(path, count, pos)
-    layers, _, kvh, cap, hd = _caches(k, v, b, 5)
-    ctx = ctx or default_context()
-    st = _on(ctx, k, v, pos, path, count)
-    status = ctx._lib.lbk_kv_keep_path(ctx.handle, k.data_ptr(), v.data_ptr(), layers, b * kvh * cap * hd, b, kvh, hd, cap, pos.data_ptr(), path.data_ptr(), count.data_ptr(), t, st)
-    if status:
-        _lib.check(status)
+    (_native or _torch_ops()).kv_keep_path(k, v, pos, path, count, ctx)
 
 
 def advance_pos_by(pos: torch.Tensor, count: torch.Tensor, ctx: Optional[Context] = None) -> None:
     """pos += count, int32 [b] (lbk_advance_pos_by): the accepted nodes are committed."""
-    if pos.dtype is not torch.int32 or count.dtype is not torch.int32 or pos.dim() != 1 or pos.shape != count.shape:
-        raise ValueError("pos and count are int32, one number for each sequence")
-    ctx = ctx or default_context()
-    st = _on(ctx, pos, count)
-    status = ctx._lib.lbk_advance_pos_by(ctx.handle, pos.data_ptr(), count.data_ptr(), pos.shape[0], st)
-    if status:
-        _lib.check(status)
+    (_native or _torch_ops()).advance_pos_by(pos, count, ctx)
 
 
 class TokenLogprobs(NamedTuple):
@@ -330,37 +234,7 @@ class TokenLogprobs(NamedTuple):
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0, scale: float = 1.0, ctx: Optional[Context] = None) -> TokenLogprobs:
     """Log softmax(scale * logits) at the given tokens, entropy and the `top` largest logits with their log probabilities
     (lbk_token_logprobs). logits f32 or bf16 [rows, vocab], rows any distance apart; tokens int32 [rows] or [rows, given]."""
-    dtype, shape = logits.dtype, logits.shape
-    if dtype is not torch.float32 and dtype is not torch.bfloat16:
-        raise TypeError("logits are f32 or bf16")
-    if len(shape) != 2 or shape[1] < 1:
-        raise ValueError("logits are [rows, vocab]")
-    rows, vocab = shape
-    pitch, one = logits.stride()
-    if vocab > 1 and one != 1 or rows > 1 and pitch < vocab:
-        raise ValueError("the values of a row lie side by side, rows do not overlap")
-    if not 0 <= top <= min(vocab, LOGPROBS_TOP):
-        raise ValueError(f"{top} alternatives of {vocab}: at most {LOGPROBS_TOP}")
-    given = 0
-    if tokens is not None:
-        if tokens.dtype is not torch.int32:
-            raise TypeError("tokens are int32")
-        if tokens.dim() not in (1, 2) or tokens.shape[0] != rows:
-            raise ValueError("tokens are [rows] or [rows, given]")
-        given = 1 if tokens.dim() == 1 else tokens.shape[1]
-    ctx = ctx or default_context()
-    st = _on(ctx) if tokens is None else _on(ctx, tokens)
-    device = logits.device
-    if logits.get_device() != ctx.device:
-        raise ValueError(f"logits must live on cuda:{ctx.device}")
-    logprobs, entropy, top_logprobs = (torch.empty((rows, given), dtype=torch.float32, device=device), torch.empty(rows, dtype=torch.float32, device=device),
-                                       torch.empty((rows, top), dtype=torch.float32, device=device))
-    ids = torch.empty((rows, top), dtype=torch.int32, device=device)
-    status = ctx._lib.lbk_token_logprobs(ctx.handle, 0 if dtype is torch.float32 else 1, logits.data_ptr(), pitch if rows > 1 else vocab, rows, vocab,
-                                         tokens.data_ptr() if given else None, given, scale, top, logprobs.data_ptr(), entropy.data_ptr(), ids.data_ptr(), top_logprobs.data_ptr(), st)
-    if status:
-        _lib.check(status)
-    return TokenLogprobs(logprobs, entropy, ids, top_logprobs)
+    return TokenLogprobs(*(_native or _torch_ops()).token_logprobs(logits, tokens, top, scale, ctx))
 
 
 class DecodeStep:

@@ -656,6 +656,12 @@ int lbk_model_forward(lbk_model *model, lbk_kv_cache *cache, const uint32_t *tok
  * them only: logits_out f32 [n_want][vocab] on the host. A portion may be cut anywhere. */
 int lbk_model_forward_rows(lbk_model *model, lbk_kv_cache *cache, size_t seq, const uint32_t *tokens, size_t n, const uint32_t *want,
                            size_t n_want, float *logits_out);
+/* The next n tokens of sequence `seq`, scored instead of handed out as logits: place i gets the log probability of targets[i] after
+ * tokens[0 .. i] (targets null: of tokens[i + 1], NaN at the last place), the entropy and the `top` largest logits, as
+ * lbk_token_logprobs; host memory [n], [n], [n][top] x 2, each of which may be null. What leaves the device is a few words a token in the place of a
+ * row of the vocabulary. */
+int lbk_model_score(lbk_model *model, lbk_kv_cache *cache, size_t seq, const uint32_t *tokens, size_t n, const uint32_t *targets, float scale,
+                    size_t top, float *logprobs_out, float *entropy_out, int32_t *top_ids_out, float *top_logprobs_out);
 int lbk_model_decode(lbk_model *model, lbk_kv_cache *cache, const int32_t *tokens_dev, float *logits_dev,
                      int32_t *next_dev, void *stream);
 /* Rows a prompt pass takes at once (1..8192; default 4096). More rows fill the GEMM's tile rounds

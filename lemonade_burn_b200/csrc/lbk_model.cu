@@ -7,7 +7,9 @@
 // A call with several tokens of one sequence (a prompt, or a portion of one) sends up to 4096 rows at a time
 // through the projections. One decode step is recorded into a CUDA graph the first time a cache is used and
 // replayed afterwards (the positions live in device memory).
+#include <cfloat>
 #include <deque>
+#include <new>
 
 #include "lbk_ptx.cuh"
 #include "lbk_runtime.cuh"
@@ -360,26 +362,40 @@ struct Want {
     bool all = false;
 };
 
-// `n` (at most the model's prefill_rows) consecutive tokens of sequence `seq` in one pass. `rows[i]` (places
-// in this pass) get their logits written to host memory at logits_out[i * vocab]; `next_out` (host) receives
-// the greedy token after the last row (sample.rs:17-25). Synchronous.
+// `n` (at most the model's prefill_rows) consecutive tokens of sequence `seq`: the launches that leave the final norm of rows first .. n - 1 in c->pf_n.
+int enqueue_pass(Model *m, Cache *c, size_t seq, const uint32_t *tokens, size_t n, size_t first) {
+    cudaStream_t st = m->ctx->own_stream;
+    LBK_TRY(ensure_prefill_buffers(m, c, n));
+    std::vector<int32_t> toks(n);
+    for (size_t i = 0; i < n; ++i) toks[i] = static_cast<int32_t>(tokens[i]);
+    LBK_CUDA(cudaMemcpyAsync(c->pf_tokens, toks.data(), n * 4, cudaMemcpyHostToDevice, st));
+    LBK_CUDA(cudaStreamSynchronize(st));  // `toks` is pageable host memory that goes away
+    return m->enqueue_rows(c, seq, n, first, st);
+}
+
+// Waits for the pass and moves the sequence's position by its n tokens.
+int finish_pass(Model *m, Cache *c, size_t seq, size_t n) {
+    const int32_t new_len = static_cast<int32_t>(c->lens[seq] + n);
+    LBK_CUDA(cudaStreamSynchronize(m->ctx->own_stream));
+    LBK_CUDA(cudaMemcpy(c->pos + seq, &new_len, 4, cudaMemcpyHostToDevice));
+    c->lens[seq] += n;
+    return LBK_OK;
+}
+
+// One such pass. `rows[i]` (places in this pass) get their logits written to host memory at logits_out[i * vocab]; `next_out` (host)
+// receives the greedy token after the last row (sample.rs:17-25). Synchronous.
 int run_rows(Model *m, Cache *c, size_t seq, const uint32_t *tokens, size_t n, const std::vector<uint32_t> &rows, float *logits_out,
              int32_t *next_out = nullptr) {
     Ctx *ctx = m->ctx;
     lbk_ctx *h = reinterpret_cast<lbk_ctx *>(ctx);
     cudaStream_t st = ctx->own_stream;
     const size_t H = m->cfg.hidden_size, V = m->cfg.vocab_size;
-    LBK_TRY(ensure_prefill_buffers(m, c, n));
-    std::vector<int32_t> toks(n);
-    for (size_t i = 0; i < n; ++i) toks[i] = static_cast<int32_t>(tokens[i]);
-    LBK_CUDA(cudaMemcpyAsync(c->pf_tokens, toks.data(), n * 4, cudaMemcpyHostToDevice, st));
-    LBK_CUDA(cudaStreamSynchronize(st));  // `toks` is pageable host memory that goes away
     // A prompt is read for the logits of a few places, mostly its last: what the rows in front of them are in the last layer only enters its
     // keys, values or states. That is 1/layers of most of a prompt: eight ternary layers of 2560, 2011 rows, the
     // last 8 wanted 2290 -> 2150 us; two layers, the second with 64 experts, 200 rows, the last wanted 465 -> 300.
     size_t kept = next_out ? n - 1 : n;
     for (uint32_t r : rows) kept = std::min<size_t>(kept, r);
-    LBK_TRY(m->enqueue_rows(c, seq, n, kept, st));
+    LBK_TRY(enqueue_pass(m, c, seq, tokens, n, kept));
     // runs of neighbouring rows go through the head together
     for (size_t i = 0; i < rows.size();) {
         size_t len = 1;
@@ -394,11 +410,38 @@ int run_rows(Model *m, Cache *c, size_t seq, const uint32_t *tokens, size_t n, c
         LBK_TRY(lbk_argmax(h, c->pf_logits, 1, V, c->pf_tokens, st));  // the token buffer is free again
         LBK_CUDA(cudaMemcpyAsync(next_out, c->pf_tokens, 4, cudaMemcpyDeviceToHost, st));
     }
-    const int32_t new_len = static_cast<int32_t>(c->lens[seq] + n);
-    LBK_CUDA(cudaStreamSynchronize(st));
-    LBK_CUDA(cudaMemcpy(c->pos + seq, &new_len, 4, cudaMemcpyHostToDevice));
-    c->lens[seq] += n;
-    return LBK_OK;
+    return finish_pass(m, c, seq, n);
+}
+
+// Host memory that lbk_model_score fills, a row for each token.
+struct Scores {
+    float *logprobs, *entropy;
+    int32_t *top_ids;
+    float *top_logprobs;
+};
+
+// One pass whose rows are scored instead of handed out: the logits of kLogitRows rows at a time stay on the device. targets: one token a row, -1 none.
+int score_rows(Model *m, Cache *c, size_t seq, const uint32_t *tokens, size_t n, const int32_t *targets, float scale, size_t top, const Scores &out) {
+    cudaStream_t st = m->ctx->own_stream;
+    const size_t H = m->cfg.hidden_size, V = m->cfg.vocab_size, words = n * (3 + 2 * top);
+    if (c->score_words < words) {
+        LBK_TRY(dev_alloc(c->device_allocs, words * 4, reinterpret_cast<void **>(&c->score)));  // the smaller ones stay until the cache goes
+        c->score_words = words;
+    }
+    int32_t *at = c->score, *ids = at + 3 * n;
+    float *lp = reinterpret_cast<float *>(at + n), *entropy = lp + n, *best = reinterpret_cast<float *>(ids + n * top);
+    LBK_CUDA(cudaMemcpyAsync(at, targets, n * 4, cudaMemcpyHostToDevice, st));
+    LBK_TRY(enqueue_pass(m, c, seq, tokens, n, 0));
+    for (size_t i = 0; i < n; i += kLogitRows) {
+        const size_t len = std::min(kLogitRows, n - i);
+        LBK_TRY(m->enqueue_head(c->pf_n + i * H, len, c->pf_logits, st));
+        LBK_TRY(lbk_token_logprobs(reinterpret_cast<lbk_ctx *>(m->ctx), LBK_DTYPE_F32, c->pf_logits, V, len, V, at + i, 1, scale, top, lp + i, entropy + i, ids + i * top, best + i * top, st));
+    }
+    struct { void *to; const void *from; size_t bytes; } copies[] = {
+        {out.logprobs, lp, n * 4}, {out.entropy, entropy, n * 4}, {out.top_ids, ids, n * top * 4}, {out.top_logprobs, best, n * top * 4}};
+    for (auto &k : copies)
+        if (k.to && k.bytes) LBK_CUDA(cudaMemcpyAsync(k.to, k.from, k.bytes, cudaMemcpyDeviceToHost, st));
+    return finish_pass(m, c, seq, n);
 }
 
 // One decode step of every slot: the family's launches, the greedy token, the positions.
@@ -675,6 +718,36 @@ int lbk_model_forward_rows(lbk_model *mp, lbk_kv_cache *cp, size_t seq, const ui
     w.places = want;
     w.n = n_want;
     return forward_impl(reinterpret_cast<Model *>(mp), reinterpret_cast<Cache *>(cp), seq, tokens, n, w, logits_out);
+}
+
+int lbk_model_score(lbk_model *mp, lbk_kv_cache *cp, size_t seq, const uint32_t *tokens, size_t n, const uint32_t *targets, float scale, size_t top, float *logprobs_out,
+                    float *entropy_out, int32_t *top_ids_out, float *top_logprobs_out) {
+    if (!mp || !cp || (n && !tokens)) return fail(LBK_ERR_INVALID, "lbk_model_score: null argument");
+    Model *m = reinterpret_cast<Model *>(mp);
+    Cache *c = reinterpret_cast<Cache *>(cp);
+    const size_t V = m->cfg.vocab_size;
+    if (c->model != m) return fail(LBK_ERR_INVALID, "the cache belongs to another model");
+    if (seq >= c->b) return fail(LBK_ERR_INVALID, "sequence %zu of a cache of %zu", seq, c->b);
+    if (top > LBK_LOGPROBS_TOP || top > V) return fail(LBK_ERR_UNSUPPORTED, "lbk_model_score: at most %d alternatives (got %zu)", LBK_LOGPROBS_TOP, top);
+    if (!(scale > 0.0f) || scale > FLT_MAX) return fail(LBK_ERR_INVALID, "lbk_model_score: the scale is a positive number");
+    if (n > c->cap - c->lens[seq]) return fail(LBK_ERR_INVALID, "%zu tokens do not fit: %zu of %zu positions are used", n, c->lens[seq], c->cap);
+    for (size_t i = 0; i < n; ++i)
+        for (uint32_t t : {tokens[i], targets ? targets[i] : 0u})
+            if (t >= V) return fail(LBK_ERR_INVALID, "token %u is outside the vocabulary of %zu", t, V);
+    LBK_CUDA(cudaSetDevice(m->ctx->device));
+    try {
+        std::vector<int32_t> wanted(std::min(n, m->prefill_rows));
+        for (size_t i0 = 0; i0 < n;) {
+            const size_t take = std::min(m->prefill_rows, n - i0);
+            for (size_t i = 0; i < take; ++i) wanted[i] = targets ? static_cast<int32_t>(targets[i0 + i]) : i0 + i + 1 < n ? static_cast<int32_t>(tokens[i0 + i + 1]) : -1;
+            auto part = [&](auto *to, size_t each) { return to ? to + i0 * each : nullptr; };
+            LBK_TRY(score_rows(m, c, seq, tokens + i0, take, wanted.data(), scale, top, Scores{part(logprobs_out, 1), part(entropy_out, 1), part(top_ids_out, top), part(top_logprobs_out, top)}));
+            i0 += take;
+        }
+    } catch (const std::bad_alloc &) {
+        return fail(LBK_ERR_NOMEM, "lbk_model_score: out of host memory");
+    }
+    return LBK_OK;
 }
 
 int lbk_kv_cache_reset_seq(lbk_kv_cache *cp, size_t seq) {

@@ -2,7 +2,8 @@
 
     python -m lemonade_burn_b200.generate --model DIR --prompt 5,17,3 [--prompt 9,2] --max-new 32
 
-prints one line of generated ids per prompt. There is no tokenizer here (the reference's lb-run has one,
+prints one line of generated ids per prompt; with --score, in its place, one line per prompt with the log probability of each of its tokens
+behind the first. There is no tokenizer here (the reference's lb-run has one,
 crates/lb-model/src/bin/lb-run.rs).
 """
 from __future__ import annotations
@@ -30,11 +31,18 @@ def main(argv=None) -> int:
     ap.add_argument("--max-new", type=int, default=32)
     ap.add_argument("--slots", type=int, default=4)
     ap.add_argument("--eos", type=int, default=-1)
+    ap.add_argument("--score", action="store_true", help="print log probabilities of the prompts' tokens, generate nothing")
     a = ap.parse_args(argv)
     from . import _lib, build, runtime
     _lib.use(build.library_for(runtime.architecture_of(a.model)))
     net = runtime.load_model(a.model, dtype=a.dtype)
     prompts = [[int(t) for t in p.split(",")] for p in a.prompt]
+    if a.score:
+        for p in prompts:
+            cache = net.new_cache(1, len(p))
+            print(",".join(f"{x:.6f}" for x in net.score(p, cache).logprobs[:-1]))
+        net.close()
+        return 0
     for toks in generate(net, prompts, a.max_new, a.slots, eos=a.eos):
         print(",".join(str(t) for t in toks))
     net.close()

@@ -3,7 +3,8 @@
 `BitNet.new_cache`, `BitNet.forward`, checkpoint format "lemonade-burn-ternary" v1
 (crates/lb-convert/src/lib.rs:1-16). Differences, all stated: the KV cache is bf16 (the
 reference keeps f32, model.rs:245), `forward` takes one new token per sequence (decode; `b`
-independent sequences advance together), and every op runs in liblbk.so.
+independent sequences advance together), `forward_tree` and `decode_tree` check several drafted
+tokens of each, and every op runs in liblbk.so.
 
 Per layer (model.rs:331-366):
     n1 = rms(x); q,k,v = ternary3(n1); rope(q), rope(k); cache k,v; a = gqa(q, K, V)
@@ -71,9 +72,10 @@ def rope_tables(cfg: Config):
 
 
 class KvCache:
-    """model.rs:136-141, here fixed capacity, bf16, [layers][b][kv_heads][cap][head_dim]."""
+    """model.rs:136-141, here fixed capacity, bf16, [layers][b][kv_heads][cap][head_dim]. own_positions: every sequence has a length of its own,
+    as drafted tokens need them, of which more or fewer are accepted."""
 
-    def __init__(self, cfg: Config, b: int, cap: int, device):
+    def __init__(self, cfg: Config, b: int, cap: int, device, own_positions: bool = False):
         if cap < 1 or cap > cfg.max_position_embeddings:  # the RoPE tables end there (model.rs:213-230, 309)
             raise ValueError(f"capacity {cap} is outside 1..max_position_embeddings ({cfg.max_position_embeddings})")
         if b < 1:
@@ -81,18 +83,26 @@ class KvCache:
         shape = (cfg.num_hidden_layers, b, cfg.num_key_value_heads, cap, cfg.head_dim())
         self.k = torch.zeros(shape, dtype=torch.bfloat16, device=device)
         self.v = torch.zeros(shape, dtype=torch.bfloat16, device=device)
-        self.pos = torch.zeros(1, dtype=torch.int32, device=device)  # cache.len, on the device
+        self.own_positions = own_positions or b == 1
+        self.pos = torch.zeros(b if self.own_positions else 1, dtype=torch.int32, device=device)  # cache.len, on the device
         self.b, self.cap = b, cap
-        self.host_len = 0  # the same length on the host: `forward` refuses a step that would not fit
+        self.host_len = 0  # the same length on the host: `forward` refuses a step that would not fit. After accepted drafts: no less than the longest
+        self.at_most = False  # whether host_len is only a bound
         self.step_work = None  # what the one-launch steps on this cache work in
 
     @property
     def len(self) -> int:
-        return int(self.pos.item())
+        return int(self.pos.max().item())
+
+    def lens(self) -> list:
+        """The length of every sequence."""
+        return self.pos.expand(self.b).tolist()
 
     def reserve(self, n: int = 1) -> None:
         """Raises unless `n` more positions fit (model.rs:309 asserts pos0 + m <= rope_len). Called by
         `BitNet.forward` before anything is launched; the kernels check the device-side position too."""
+        if self.at_most and self.host_len + n > self.cap and not torch.cuda.is_current_stream_capturing():
+            self.host_len, self.at_most = self.len, False  # how many drafts were accepted is on the device
         if self.host_len + n > self.cap:
             raise ValueError(f"the cache is full: {self.host_len} of {self.cap} positions are used, {n} more do not fit")
 
@@ -171,9 +181,9 @@ class BitNet:
                 tensors[k] = f.get_tensor(k)
         return cls(cfg, tensors, ctx, device)
 
-    def new_cache(self, b: int = 1, cap: Optional[int] = None) -> KvCache:
+    def new_cache(self, b: int = 1, cap: Optional[int] = None, own_positions: bool = False) -> KvCache:
         """model.rs:234-236. The capacity cannot exceed the RoPE tables (max_position_embeddings)."""
-        cache = KvCache(self.cfg, b, cap or self.cfg.max_position_embeddings, self.device)
+        cache = KvCache(self.cfg, b, cap or self.cfg.max_position_embeddings, self.device, own_positions)
         self._work_of(cache)
         return cache
 
@@ -206,6 +216,7 @@ class BitNet:
         if splits is None:
             splits = attention_splits(cache.cap)
         H, I, nh, kvh, hd = cfg.hidden_size, cfg.intermediate_size, cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim()
+        own = cache.own_positions and b > 1  # the calls that read a position for every sequence
         st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
         P = lambda t: C.c_void_p(t.data_ptr())
         eps = C.c_float(cfg.rms_norm_eps)
@@ -214,9 +225,9 @@ class BitNet:
         n = self._buf("n", (b, H))
         if one_launch:
             _lib.check(lib.lbk_embed_bf16(h, P(self.lm_head), P(tokens), b, H, P(x), st))
-            self._step.run(x, cache.k, cache.v, self.cos, self.sin, cache.pos, 0, n, self._work_of(cache))
+            self._step.run(x, cache.k, cache.v, self.cos, self.sin, cache.pos, int(own), n, self._work_of(cache))
             logits = ops.bf16_linear(n, self.lm_head, self.ctx)
-            _lib.check(lib.lbk_advance_pos(h, P(cache.pos), st))
+            _lib.check(lib.lbk_advance_pos_seq(h, P(cache.pos), None, b, st) if own else lib.lbk_advance_pos(h, P(cache.pos), st))
             cache.host_len += 1
             return logits
         attn = self._buf("attn", (b, nh * hd))
@@ -275,12 +286,12 @@ class BitNet:
             else:
                 q, k, v = ops.ternary_linear3(add_norm(x, d, l["input_norm"], x), qkv_l)
             if attn_fused:  # RoPE, KV append, attention slices and their merge in one launch
-                chk(lib.lbk_attn_decode_fused(h, P(q), P(k), P(v), P(self.cos), P(self.sin), P(cache.pos), b, nh, kvh, hd, cache.cap,
+                chk((lib.lbk_attn_decode_fused_seq if own else lib.lbk_attn_decode_fused)(h, P(q), P(k), P(v), P(self.cos), P(self.sin), P(cache.pos), b, nh, kvh, hd, cache.cap,
                                               splits, P(cache.k[li]), P(cache.v[li]), P(scratch), P(counters), P(attn), st))
             else:
-                chk(lib.lbk_rope_kv_append(h, P(q), P(k), P(v), P(self.cos), P(self.sin), P(cache.pos), b, nh, kvh, hd, cache.cap,
+                chk((lib.lbk_rope_kv_append_seq if own else lib.lbk_rope_kv_append)(h, P(q), P(k), P(v), P(self.cos), P(self.sin), P(cache.pos), b, nh, kvh, hd, cache.cap,
                                            P(cache.k[li]), P(cache.v[li]), st))
-                chk(lib.lbk_attn_decode(h, P(q), P(cache.k[li]), P(cache.v[li]), P(cache.pos), b, nh, kvh, hd, cache.cap, splits,
+                chk((lib.lbk_attn_decode_seq if own else lib.lbk_attn_decode)(h, P(q), P(cache.k[li]), P(cache.v[li]), P(cache.pos), b, nh, kvh, hd, cache.cap, splits,
                                         P(scratch), P(attn), st))
             if nq:
                 normq(ops.PRE_RMS, attn, None, l["attn_sub_norm"])
@@ -314,9 +325,79 @@ class BitNet:
         else:
             add_norm(x, d, self.final_norm, x)
         logits = ops.bf16_linear(n, self.lm_head, self.ctx)
-        chk(lib.lbk_advance_pos(h, P(cache.pos), st))
+        chk(lib.lbk_advance_pos_seq(h, P(cache.pos), None, b, st) if own else lib.lbk_advance_pos(h, P(cache.pos), st))
         cache.host_len += 1
         return logits
+
+    # ---- drafted tokens --------------------------------------------------------------------------
+    def forward_tree(self, tokens: torch.Tensor, parents: torch.Tensor, cache: KvCache, counts: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Several drafted tokens of every sequence in one pass: tokens, parents int32 CUDA [b, t] (parents[i] < i: the node that node i
+        follows, -1: the last committed token), counts int32 [b] how many of them a sequence has. Returns the logits f32 [b, t, vocab] after each. Their keys
+        and values are in the cache behind the committed ones, which stay as many: `accept_tree` commits a path."""
+        cfg, lib, h = self.cfg, self.ctx._lib, self.ctx.handle
+        if tokens.dtype != torch.int32 or tokens.shape != parents.shape or tokens.dim() != 2 or tokens.shape[0] != cache.b:
+            raise ValueError("tokens and parents are int32 [sequences of the cache, nodes]")
+        if not cache.own_positions:
+            raise ValueError("drafted tokens need a cache whose sequences have positions of their own (new_cache(own_positions=True))")
+        if cfg.head_dim() != 128:
+            raise ValueError("drafted tokens need heads of 128")
+        b, t = tokens.shape
+        cache.reserve(t)
+        m, H, I, nh, hd, eps = b * t, cfg.hidden_size, cfg.intermediate_size, cfg.num_attention_heads, cfg.head_dim(), cfg.rms_norm_eps
+        st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        P = lambda v: C.c_void_p(v.data_ptr())
+        chk, new = _lib.check, lambda *shape: torch.empty(shape, dtype=torch.float32, device=self.device)
+        x, attn = new(m, H), new(b, t, nh, hd)
+        if counts is not None:
+            attn.zero_()  # rows of places not in use are numbers
+        quantised = all(ops.norm_quant_supported(w) for w in (H, I, nh * hd))
+        if quantised:
+            q8 = torch.empty((m, row_bytes(max(H, I, nh * hd)) * 4), dtype=torch.int8, device=self.device)
+            scale, total = new(m), torch.empty(m, dtype=torch.int32, device=self.device)
+
+        def project(pre, a, y, w, width, linears):  # the norm in front of a projection, and the projection
+            if quantised:
+                ops.norm_quant(pre, a, y, w, eps, q8, scale, total, self.ctx)
+                return ops.ternary_gemm_q(q8, scale, total, m, linears)
+            if pre == ops.PRE_ADD_RMS:
+                chk(lib.lbk_add_inplace(h, P(a), P(y), m * width, st))
+            elif pre == ops.PRE_RELU2_MUL_RMS:
+                chk(lib.lbk_relu2_mul(h, P(a), P(y), m * width, P(a), st))
+            n = new(m, width)
+            chk(lib.lbk_rms_norm(h, P(a), P(w), m, width, C.c_float(eps), P(n), st))
+            return ops.ternary_linear_multi(n, linears)
+
+        chk(lib.lbk_embed_bf16(h, P(self.lm_head), P(tokens.contiguous()), m, H, P(x), st))
+        d = None  # output of the previous layer's down projection, not yet added to the residual x
+        for li, l in enumerate(self.layers):
+            q, k, v = project(ops.PRE_RMS if d is None else ops.PRE_ADD_RMS, x, d, l["input_norm"], H, [l["q"], l["k"], l["v"]])
+            ops.rope_kv_append_tree(q, k, v, self.cos, self.sin, cache.pos, parents, cache.k[li], cache.v[li], counts, self.ctx)
+            ops.attn_tree(q.view(b, t, nh, hd), cache.k[li], cache.v[li], cache.pos, parents, counts, out=attn, ctx=self.ctx)
+            o, = project(ops.PRE_RMS, attn.view(m, nh * hd), None, l["attn_sub_norm"], nh * hd, [l["o"]])
+            g, u = project(ops.PRE_ADD_RMS, x, o, l["post_attn_norm"], H, [l["gate"], l["up"]])
+            d, = project(ops.PRE_RELU2_MUL_RMS, g, u, l["ffn_sub_norm"], I, [l["down"]])
+        if d is not None:
+            chk(lib.lbk_add_inplace(h, P(x), P(d), m * H, st))
+        n = new(m, H)
+        chk(lib.lbk_rms_norm(h, P(x), P(self.final_norm), m, H, C.c_float(eps), P(n), st))
+        return ops.bf16_linear(n, self.lm_head, self.ctx).view(b, t, cfg.vocab_size)
+
+    def accept_tree(self, cache: KvCache, path: torch.Tensor, count: torch.Tensor) -> None:
+        """Commits count[s] nodes of every sequence's tree, path int32 [b, t] ascending (ops.tree_accept, or a sampler's choice): their rows of
+        the cache move together behind the committed ones, the others' places are free again."""
+        ops.kv_keep_path(cache.k, cache.v, cache.pos, path, count, self.ctx)
+        ops.advance_pos_by(cache.pos, count, self.ctx)
+        cache.host_len, cache.at_most = min(cache.cap, cache.host_len + path.shape[1]), True
+
+    def decode_tree(self, tokens: torch.Tensor, parents: torch.Tensor, cache: KvCache, counts: Optional[torch.Tensor] = None):
+        """A greedy step with drafts: node 0 is the token the last step gave, the others are guesses of what follows. As many guesses as the
+        model itself would have given are committed. Returns (path, count, next) of ops.tree_accept: with the tokens on the path, and `next`, the same
+        tokens as `forward` one by one."""
+        logits = self.forward_tree(tokens, parents, cache, counts)
+        best = self.argmax(logits.view(-1, logits.shape[2])).view(tokens.shape)
+        path, count, after = ops.tree_accept(tokens, parents, best, counts, self.ctx)
+        self.accept_tree(cache, path, count)
+        return path, count, after
 
     def argmax(self, logits: torch.Tensor) -> torch.Tensor:
         """sample.rs:17-25 on the device."""

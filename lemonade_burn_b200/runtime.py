@@ -7,7 +7,7 @@ from __future__ import annotations
 import ctypes as C
 import json
 from pathlib import Path
-from typing import Callable, Dict, Optional
+from typing import Callable, Dict, NamedTuple, Optional
 
 import numpy as np
 
@@ -53,6 +53,14 @@ class _ModelConfig(C.Structure):
 
 class _LoadStats(C.Structure):
     _fields_ = [("seconds", C.c_double), ("bytes_read", C.c_size_t), ("bytes_to_device", C.c_size_t), ("staging_bytes", C.c_size_t)]
+
+
+class Scores(NamedTuple):
+    """What `NativeModel.score` says of every place of a prompt."""
+    logprobs: np.ndarray      # f32 [n]
+    entropy: np.ndarray       # f32 [n]
+    top_ids: np.ndarray       # int32 [n, top]
+    top_logprobs: np.ndarray  # f32 [n, top]
 
 
 class NativeModel:
@@ -118,6 +126,21 @@ class NativeModel:
         out = np.empty((len(places), self.cfg.vocab_size), dtype=np.float32)
         _lib.check(self._lib.lbk_model_forward_rows(self.handle, cache, seq, toks.ctypes.data_as(C.c_void_p), len(toks),
                                                     places.ctypes.data_as(C.c_void_p), len(places), out.ctypes.data_as(C.c_void_p)))
+        return out
+
+    def score(self, tokens, cache, targets=None, top: int = 0, scale: float = 1.0, seq: int = 0) -> Scores:
+        """The next tokens of sequence `seq`: the log probability of targets[i] after place i (without targets: of the token that follows in
+        `tokens`, NaN at the last place), the entropy and the `top` likeliest tokens there, of softmax(scale * logits)."""
+        toks = np.ascontiguousarray(tokens, dtype=np.uint32)
+        want = None if targets is None else np.ascontiguousarray(targets, dtype=np.uint32)
+        n = len(toks)
+        if want is not None and want.shape != (n,):
+            raise ValueError(f"targets are one token for each of the {n} places")
+        if not 0 <= top <= self.cfg.vocab_size:
+            raise ValueError(f"{top} alternatives of {self.cfg.vocab_size}")
+        out = Scores(np.empty(n, np.float32), np.empty(n, np.float32), np.empty((n, top), np.int32), np.empty((n, top), np.float32))
+        at = lambda a: a.ctypes.data_as(C.c_void_p)  # noqa: E731
+        _lib.check(self._lib.lbk_model_score(self.handle, cache, seq, at(toks), n, None if want is None else at(want), scale, top, *[at(a) for a in out]))
         return out
 
     def decode(self, tokens_dev, cache):

@@ -63,3 +63,14 @@ def test_calls_without_a_context_return_a_status():
     assert lib.lbk_advance_pos_by(None, None, None, 1, None) == 1
     assert lib.lbk_token_logprobs(None, 0, None, 5, 1, 5, None, 0, 1.0, 0, None, None, None, None, None) == 1
     assert b"context" in lib.lbk_last_error()
+    assert lib.lbk_attn_tree(None, 1, None, 0, *[None] * 5, 1, 1, 1, 1, 128, 8, 1.0, None, None, 0, None) == 1
+    assert lib.lbk_attn_tree_scratch(None, 1, 1, 1) == 0
+    assert lib.lbk_model_score(None, None, 0, None, 0, None, 1.0, 0, None, None, None, None) == 1
+
+
+def test_a_missing_extension_module_is_an_error(monkeypatch, tmp_path):
+    from lemonade_burn_b200 import _lib, ops
+    monkeypatch.setattr(ops, "_native", None)
+    monkeypatch.setattr(_lib, "LIB_PATH", tmp_path / "liblbk.so")
+    with pytest.raises(RuntimeError, match="missing"):
+        ops.advance_pos_by(_i(1), _i(1))

@@ -247,6 +247,22 @@ def test_bits_do_not_change_from_run_to_run(ctx):
         assert torch.equal(ops.attn_tree(*args[:3], *dev(*args[3:])), first)
 
 
+@pytest.mark.parametrize("b,t,nh,kvh,length", [(16, 4, 20, 5, 4000), (16, 8, 20, 5, 3000), (16, 16, 32, 8, 1500), (9, 128, 8, 2, 2000), (1, 6, 4, 1, 60000)])
+def test_long_walks_over_and_over(ctx, b, t, nh, kvh, length):
+    """Every worker has tens of blocks of several tiles: its roles run far apart, and each wait has to end."""
+    import torch
+    from lemonade_burn_b200 import ops
+    for dtype in (torch.float32, torch.bfloat16):
+        args = make(b, t, nh, kvh, [length - (7 * i) % 300 for i in range(b)], dtype)
+        on = dev(*args[3:])
+        first = ops.attn_tree(*args[:3], *on)
+        for _ in range(60):
+            got = ops.attn_tree(*args[:3], *on)
+        assert torch.equal(got, first)
+        ctx.check_device_error()
+    check(ctx, args)
+
+
 def test_bad_positions_and_parents(ctx):
     import torch
     from lemonade_burn_b200 import _lib, ops

@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
 
 // ---- many rows: tcgen05, tiles of 128 rows ---------------------------------------------------------------
 // Blocks of 128 keys. S = Q K^T: the queries' terms and the K block from shared memory, scores in tensor memory. P V: the probabilities' terms from tensor
-// memory, the V block as it lies in the cache (its contraction index, the key, is the strided one: the MN-major operand form), every
+// memory, the V block as it lies in the cache (its contraction index, the key, is the strided one: the MN-major operand form), with f32 queries every
 // block into zeroed sums, which the softmax warps add to the rows in their registers.
 //
 //   16 softmax warps four to a quadrant of 32 lanes = rows: warps w, w + 4, .. share rows and take 32 of a block's keys, and of the dimensions, each (eight
@@ -632,6 +632,9 @@ struct Many {
     static constexpr int kK0 = TERMS * 2 * kHalf, kV0 = kK0 + kKStages * kKBytes, kBars = kV0 + kVStages * kPieceBytes;
     static constexpr int kPair = kBars + 256, kSmem = kPair + 2 * 4 * kRows * 4 + 1024;
     static constexpr int kSoftWarps = 16, kKWarp = 16, kVWarp = 17, kMmaWarp = 18, kThreads = 20 * 32;
+    // bf16: the products are summed up in tensor memory, over all blocks, and m is moved as for few rows, with the sums, when a score is over it by kSlack. What the tensor
+    // core cuts off of a long sum (1e-5 at 8000 keys) does not show in a bf16 result, and a block needs no look at the products of the one in front.
+    static constexpr bool kStays = TERMS == 1;
     // Scores (128 columns) and, when all have been read, the probabilities (64 a term) of even blocks in one place, of odd ones in another
     static constexpr uint32_t kPlace = 192, kColO = 384;
 };
@@ -643,7 +646,8 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
     const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t *sm = smem_raw + (base - raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int kKFull = 0, kKEmpty = 3, kVFull = 6, kVEmpty = 11, kQFull = 16, kPReady = 17, kOFull = 18, kSFull = 19;  // scores: one for even, one for odd blocks
+    constexpr int kKFull = 0, kKEmpty = 3, kVFull = 6, kVEmpty = 11, kQFull = 16;
+    constexpr int kPReady = 17, kOFull = 19, kSFull = 21;  // one for even, one for odd blocks: warps may be a block apart
     auto bar = [&](int i) { return base + M::kBars + i * 8; };
     volatile int *abort = &sh.abort;
     if (tid == 0) {
@@ -655,8 +659,8 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
             ptx::mbar_init(bar(kVFull + s), 1);
             ptx::mbar_init(bar(kVEmpty + s), 1);
         }
-        for (int i : {kQFull, kPReady}) ptx::mbar_init(bar(i), M::kSoftWarps);
-        for (int i : {kSFull, kSFull + 1, kOFull}) ptx::mbar_init(bar(i), 1);
+        for (int i : {kQFull, kPReady, kPReady + 1}) ptx::mbar_init(bar(i), M::kSoftWarps);
+        for (int i : {kSFull, kSFull + 1, kOFull, kOFull + 1}) ptx::mbar_init(bar(i), 1);
         sh.abort = sh.odd = 0;
         ptx::fence_barrier_init();
     }
@@ -724,7 +728,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                 if (ok && blocks > 1) scores();
                 for (int j = 0; j < blocks && ok; ++j) {
                     const int done = n - (j + 1 < blocks ? 2 : 1);  // the number, in the whole walk, of block j
-                    if (!wait(kPReady, done & 1)) break;
+                    if (!wait(kPReady + (done & 1), done >> 1 & 1)) break;
 #pragma unroll 1
                     for (int piece = 0; piece < 2; ++piece) {
                         if (!wait(kVFull + vs, vphase)) break;
@@ -736,9 +740,9 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
 #pragma unroll
                                 for (int x = TERMS - 1; x >= 0; --x)
                                     tc::umma_f16_ts(tmem + M::kColO, tmem + (done & 1) * M::kPlace + x * 64 + (piece * 4 + st) * 8, v_desc + static_cast<uint64_t>(st * (2048 >> 4)), idesc_o,
-                                                    piece || st || x < TERMS - 1 ? 1u : 0u);
+                                                    piece || st || x < TERMS - 1 || (M::kStays && j) ? 1u : 0u);
                             tc::umma_commit(bar(kVEmpty + vs));
-                            if (piece) tc::umma_commit(bar(kOFull));
+                            if (piece) tc::umma_commit(bar(kOFull + (done & 1)));
                         }
                         __syncwarp();
                         if (++vs == M::kVStages) {
@@ -841,8 +845,21 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                     quarter[part * M::kRows] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                     quad_sync();  // the row's scores have all been read; the next block but one writes here again, behind the next block's meeting
                     const float all = fmaxf(fmaxf(quarter[0], quarter[M::kRows]), fmaxf(quarter[2 * M::kRows], quarter[3 * M::kRows]));
-                    const float nm = fmaxf(m, all * p.scale);
+                    const float top = all * p.scale, nm = M::kStays ? (top > m + kSlack ? top : m) : fmaxf(m, top);
                     step = ex2(m - nm);
+                    if (M::kStays && j > s.begin && __any_sync(0xffffffffu, nm != m)) {  // the same in the quadrant's four warps
+                        wait(kOFull + ((n - 1) & 1), (n - 1) >> 1 & 1);  // the sums are complete and nothing is added before this block's probabilities are there
+                        tc::tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t v[16];
+                            tc::tmem_ld16(lanes + M::kColO + part * 32 + c * 16, v);
+                            tc::tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * step);
+                            tc::tmem_st16(lanes + M::kColO + part * 32 + c * 16, v);
+                        }
+                    }
                     m = nm;
                     float2 sum = make_float2(0.0f, 0.0f);
                     const float2 scale2 = make_float2(p.scale, p.scale), less = make_float2(-nm, -nm);
@@ -871,16 +888,18 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                     ptx::fence_proxy_async();
                 }
                 // the products of the block in front are added, then their place is free
-                if (j > s.begin) {
-                    wait(kOFull, (n - 1) & 1);
-                    if (live) add_products();
+                if (!M::kStays) {
+                    if (j > s.begin) {
+                        wait(kOFull + ((n - 1) & 1), (n - 1) >> 1 & 1);
+                        if (live) add_products();
+                    }
+                    corr = step;
                 }
-                corr = step;
                 if (live) tc::tmem_st_wait();
                 tc::tc_fence_before();
-                arrive(kPReady);
+                arrive(kPReady + (n & 1));
             }
-            wait(kOFull, (n - 1) & 1);
+            wait(kOFull + ((n - 1) & 1), (n - 1) >> 1 & 1);
             if (live) add_products();
             // the row's weight: the four parts of the keys meet
             float *quarter = s_quad + (n & 1) * 4 * M::kRows + r;

@@ -6,6 +6,7 @@
 // loaded. No exception leaves an entry point: torch's become RuntimeError, a status that is not 0 becomes LbkError.
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/ScalarTypeToTypeMeta.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -116,6 +117,23 @@ Cache caches(const at::Tensor &k, const at::Tensor &v, int64_t b, int64_t dims) 
 }
 at::Tensor like(const at::Tensor &t, at::IntArrayRef shape, at::ScalarType type) { return at::empty(shape, t.options().dtype(type)); }
 
+// Results of one call that share an allocation: four of their own are 4 us. Of 32-bit values, each from a 16-byte boundary on.
+class Results {
+    c10::Storage storage_;
+    int64_t at_ = 0;
+
+public:
+    static int64_t room(int64_t values) { return (values + 3) / 4 * 4; }
+    Results(const at::Tensor &beside, int64_t values) : storage_(like(beside, {values}, at::kFloat).storage()) {}
+    at::Tensor take(at::IntArrayRef shape, at::ScalarType type) {
+        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(storage_), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(type));
+        t.unsafeGetTensorImpl()->set_storage_offset(at_);
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+        at_ += room(t.numel());
+        return t;
+    }
+};
+
 // The body of an entry point: `n` arguments, no exception to Python's side.
 template <class Body>
 PyObject *entry(Py_ssize_t given, Py_ssize_t wanted, Body &&body) {
@@ -221,7 +239,8 @@ PyObject *tree_accept(PyObject *, PyObject *const *a, Py_ssize_t n) {
             refuse(PyExc_ValueError, "tokens and best are [%lld, %lld], as parents", static_cast<long long>(s.b), static_cast<long long>(s.t));
         const Context ctx(a[4]);
         void *st = ctx.stream(tokens, parents, best, counts);
-        const at::Tensor path = like(parents, {s.b, s.t}, at::kInt), count = like(parents, {s.b}, at::kInt), after = like(parents, {s.b}, at::kInt);
+        Results r(parents, Results::room(s.b * s.t) + 2 * Results::room(s.b));
+        const at::Tensor path = r.take({s.b, s.t}, at::kInt), count = r.take({s.b}, at::kInt), after = r.take({s.b}, at::kInt);
         done(lib.accept(ctx.handle, ints(tokens), ints(parents), ints(best), ints(counts), s.b, s.t, data<int32_t>(path), data<int32_t>(count), data<int32_t>(after), st));
         return wrap({path, count, after});
     });
@@ -276,8 +295,9 @@ PyObject *token_logprobs(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const Context ctx(a[4]);
         void *st = ctx.stream(tokens);
         ctx.lives_here(logits);
-        const at::Tensor lp = like(logits, {rows, given}, at::kFloat), entropy = like(logits, {rows}, at::kFloat), ids = like(logits, {rows, static_cast<int64_t>(top)}, at::kInt),
-                         best = like(logits, {rows, static_cast<int64_t>(top)}, at::kFloat);
+        Results r(logits, Results::room(rows * given) + Results::room(rows) + 2 * Results::room(rows * top));
+        const at::Tensor lp = r.take({rows, given}, at::kFloat), entropy = r.take({rows}, at::kFloat), ids = r.take({rows, static_cast<int64_t>(top)}, at::kInt),
+                         best = r.take({rows, static_cast<int64_t>(top)}, at::kFloat);
         done(lib.logprobs(ctx.handle, f32 ? LBK_DTYPE_F32 : LBK_DTYPE_BF16, data(logits), pitch, rows, vocab, given ? ints(tokens) : nullptr, given, static_cast<float>(scale), top,
                           data<float>(lp), data<float>(entropy), data<int32_t>(ids), data<float>(best), st));
         return wrap({lp, entropy, ids, best});

@@ -4,6 +4,7 @@
 //   alternatives: the `top` largest logits, the lower id first among equal ones, with their log probabilities
 //
 // The reference has the greedy token only (crates/lb-model/src/sample.rs:17-25).
+#include <algorithm>
 #include <cfloat>
 
 #include "lbk_dense_dev.cuh"
@@ -105,6 +106,203 @@ __device__ __forceinline__ void unpack(const uint4 &v, float (&x)[8]) {
     }
 }
 
+// What a thread has seen: its maximum, and the sums brought to it, of every other value each.
+struct Seen {
+    float m = -FLT_MAX;
+    float2 s{0.0f, 0.0f}, t{0.0f, 0.0f};
+    __device__ __forceinline__ void reach(float high, float c) {
+        if (!(high > m)) return;
+        const float d = m - high, r = ex2(d * c);
+        t = r == 0.0f ? make_float2(0.0f, 0.0f) : mul2(make_float2(r, r), fma2(s, make_float2(d, d), t));  // s * d may be -inf for the nothing in front
+        s = mul2(s, make_float2(r, r));
+        m = high;
+    }
+    __device__ __forceinline__ void add(float2 v, float c) {  // v.x, v.y <= m, or NaN
+        const float2 d = add2(v, make_float2(-m, -m)), f = mul2(d, make_float2(c, c)), e = make_float2(ex2(f.x), ex2(f.y));
+        s = add2(s, e);
+        t = fma2(e, make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), t);  // 0 * -inf is nothing here
+    }
+    __device__ __forceinline__ Stats stats() const { return {m, s.x + s.y, t.x + t.y}; }
+};
+// A row as it lies: `lead` values up to the first 16-byte boundary, `vectors` of 16 bytes, the rest.
+template <typename T>
+struct Row {
+    static constexpr int kVec = 16 / sizeof(T);
+    const T *x;
+    int lead, vectors, odd;  // odd: values that are in no vector
+    __device__ __forceinline__ Row(const ScoreParams &p, size_t row) : x(static_cast<const T *>(p.logits) + row * p.pitch) {
+        lead = min(p.vocab, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)));
+        vectors = (p.vocab - lead) / kVec;
+        odd = p.vocab - vectors * kVec;
+    }
+    __device__ __forceinline__ const uint4 *units() const { return reinterpret_cast<const uint4 *>(x + lead); }
+    __device__ __forceinline__ int odd_id(int i) const { return i < lead ? i : i + vectors * kVec; }
+    __device__ __forceinline__ int id(int vector, int e) const { return lead + vector * kVec + e; }
+};
+// The results of a row whose statistics are known
+struct Results {
+    float m, log_s, scale;
+    __device__ __forceinline__ Results(const Stats &a, float scale) : m(a.m), log_s(logf(a.s)), scale(scale) {}
+    __device__ __forceinline__ float logprob(float v) const { return (v - m) * scale - log_s; }
+    __device__ __forceinline__ float entropy(const Stats &a) const { return log_s - a.t / a.s * scale; }
+};
+__device__ __forceinline__ float key_value(Key key) { return value_of(static_cast<unsigned>(key >> 32)); }
+__device__ __forceinline__ Key warp_max(Key key) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+    return key;
+}
+// how many of n keys are larger
+__device__ __forceinline__ int rank_of(const Key *keys, int n, Key mine) {
+    int rank = 0, i = 0;
+    for (; i + 8 <= n; i += 8) {
+        ulonglong2 two[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) two[e] = *reinterpret_cast<const ulonglong2 *>(keys + i + 2 * e);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rank += (two[e].x > mine) + (two[e].y > mine);
+    }
+    for (; i < n; ++i) rank += keys[i] > mine;
+    return rank;
+}
+// Of 32 maxima that are shown, the one of rank top - 1, by a warp: a lane finds the rank of one of them; true for the lane that has it
+__device__ __forceinline__ bool has_rank(const unsigned *shown, int lane, int top, unsigned &mine) {
+    mine = shown[lane];
+    int rank = 0;
+#pragma unroll
+    for (int i = 0; i < kTop; i += 4) {
+        const uint4 other = *reinterpret_cast<const uint4 *>(shown + i);
+        rank += (other.x > mine || (other.x == mine && i < lane)) + (other.y > mine || (other.y == mine && i + 1 < lane)) + (other.z > mine || (other.z == mine && i + 2 < lane)) +
+                (other.w > mine || (other.w == mine && i + 3 < lane));
+    }
+    return rank == top - 1;
+}
+
+// ---- short rows: a warp a row ---------------------------------------------------------------------------
+// One walk for the sums and the lanes' maxima, one, from L1 and L2, for the values that reach the `top`-th largest of those. No barrier: a block's meetings are some 5 us a
+// row, and a warp has nothing of them, but takes longer for what is long. us, a block a row / a warp a row: 883 rows of 182 bf16 15.1 / 4.0, 2000 rows of 2000 f32 20.7 / 11.8, 1356 rows
+// of 4721 bf16 19.7 / 16.5, 2000 rows of 5000 f32 26.7 / 22.2, of 8192 33.7 / 36.8; 100 rows of 5000 f32 5.9 / 13.5. So: where there are more rows than the SMs hold
+// blocks, up to kShortBytes a row; in any case up to kTinyBytes.
+constexpr int kShortWarps = 8, kShortList = 256, kShortBytes = 20480, kTinyBytes = 2048;
+template <typename T>
+__global__ void __launch_bounds__(kShortWarps * 32) logprobs_short_kernel(const ScoreParams p, int rows) {
+    constexpr int kVec = 16 / sizeof(T);
+    __shared__ alignas(16) Key s_list[kShortWarps][kShortList];
+    __shared__ alignas(16) unsigned s_shown[kShortWarps][kTop];
+    __shared__ int s_count[kShortWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const size_t row = static_cast<size_t>(blockIdx.x) * (blockDim.x >> 5) + warp;
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    if (row >= static_cast<size_t>(rows)) return;
+    const Row<T> r(p, row);
+    const uint4 *units = r.units();
+    const float c = p.scale * 1.4426950408889634f, odd_value = lane < r.odd ? get(r.x + r.odd_id(lane)) : -INFINITY;
+    const bool one_given = lane < p.given;
+    const int token0 = one_given ? p.tokens[row * p.given + lane] : -1;
+    const float given0 = token0 >= 0 && token0 < p.vocab ? get(r.x + token0) : 0.0f;
+    if (lane == 0) s_count[warp] = 0;
+    Seen seen;
+    uint4 raw[kLoads], next[kLoads];
+    auto ask = [&](uint4 (&into)[kLoads], int base) {
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+            const int i = base + u * 32 + lane;
+            into[u] = i < r.vectors ? __ldg(units + i) : Empty<T>::vector();
+        }
+    };
+    ask(next, 0);
+    seen.reach(odd_value, c);
+    seen.add(make_float2(odd_value, -INFINITY), c);
+    for (int base = 0; base < r.vectors; base += 32 * kLoads) {
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) raw[u] = next[u];
+        ask(next, base + 32 * kLoads);  // on their way while these are looked at
+        float high = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+            float v[kVec];
+            unpack(raw[u], v);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) high = fmaxf(high, v[e]);
+        }
+        seen.reach(high, c);
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+            float v[kVec];
+            unpack(raw[u], v);
+#pragma unroll
+            for (int e = 0; e < kVec; e += 2) seen.add(make_float2(v[e], v[e + 1]), c);
+        }
+    }
+    const Stats a = join_warp(seen.stats(), c);
+    const Results result(a, p.scale);
+    const float none = __uint_as_float(0x7fc00000u);
+    if (lane == 0 && p.entropy) p.entropy[row] = result.entropy(a);
+    if (one_given) p.logprobs[row * p.given + lane] = token0 >= 0 && token0 < p.vocab ? result.logprob(given0) : none;
+    for (int g = lane + 32; g < p.given; g += 32) {
+        const int token = p.tokens[row * p.given + g];
+        p.logprobs[row * p.given + g] = token >= 0 && token < p.vocab ? result.logprob(get(r.x + token)) : none;
+    }
+    if (!p.top) return;
+    auto put = [&](int place, Key key) {
+        p.top_ids[row * p.top + place] = key_id(key);
+        p.top_logprobs[row * p.top + place] = result.logprob(key_value(key));
+    };
+    s_shown[warp][lane] = order_value(seen.m);
+    __syncwarp();
+    unsigned mine;
+    const unsigned who = __ballot_sync(0xffffffffu, has_rank(s_shown[warp], lane, p.top, mine));
+    const float floor = fmaxf(-FLT_MAX, value_of(__shfl_sync(0xffffffffu, mine, __ffs(who) - 1)));  // what a value has to reach; -inf never does
+    auto list = [&](float v, int id) {
+        if (v >= floor) {
+            const int at = atomicAdd(&s_count[warp], 1);
+            if (at < kShortList) s_list[warp][at] = order_key(v, id);
+        }
+    };
+    list(odd_value, r.odd_id(lane));
+#pragma unroll 4
+    for (int i = lane; i < r.vectors; i += 32) {
+        float v[kVec], high;
+        unpack(__ldg(units + i), v);
+        high = v[0];
+#pragma unroll
+        for (int e = 1; e < kVec; ++e) high = fmaxf(high, v[e]);
+        if (!(high < floor)) {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) list(v[e], r.id(i, e));
+        }
+    }
+    __syncwarp();
+    const int n = s_count[warp];
+    if (n <= kShortList && n >= p.top && a.s == a.s && a.s <= FLT_MAX) {
+        for (int k = lane; k < n; k += 32) {
+            const Key key = s_list[warp][k];
+            const int rank = rank_of(s_list[warp], n, key);
+            if (rank < p.top) put(rank, key);
+        }
+        return;
+    }
+    Key last = ~0ull;  // the largest value behind the last one found, `top` times over
+    for (int k = 0; k < p.top; ++k) {
+        Key best = 0;
+        auto look = [&](float v, int id) {
+            const Key key = order_key(v, id);
+            if (key < last && key > best) best = key;
+        };
+        for (int i = lane; i < r.vectors; i += 32) {
+            float v[kVec];
+            unpack(__ldg(units + i), v);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) look(v[e], r.id(i, e));
+        }
+        if (lane < r.odd) look(odd_value, r.odd_id(lane));
+        last = warp_max(best);
+        if (lane == 0) put(k, last);
+    }
+}
+
+// ---- long rows: a block a row, or a cluster -----------------------------------------------------------------
 struct alignas(16) RowShared {
     Key list[kList];
     Key best[kOrder];          // the keys that are put in order
@@ -125,15 +323,7 @@ __device__ void put_in_order(const Key *keys, int n, int top, Key *out, Key *war
     if (n <= kOrder) {
         for (int k = tid; k < n; k += kThreads) {
             const Key mine = keys[k];
-            int rank = 0, i = 0;
-            for (; i + 8 <= n; i += 8) {
-                ulonglong2 four[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) four[e] = *reinterpret_cast<const ulonglong2 *>(keys + i + 2 * e);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) rank += (four[e].x > mine) + (four[e].y > mine);
-            }
-            for (; i < n; ++i) rank += keys[i] > mine;
+            const int rank = rank_of(keys, n, mine);
             if (rank < top && mine) out[rank] = mine;
         }
         __syncthreads();
@@ -144,7 +334,7 @@ __device__ void put_in_order(const Key *keys, int n, int top, Key *out, Key *war
         Key best = 0;
         for (int i = tid; i < n; i += kThreads)
             if (keys[i] < last && keys[i] > best) best = keys[i];
-        for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+        best = warp_max(best);
         if ((tid & 31) == 0) warp_key[tid >> 5] = best;
         __syncthreads();
         for (int w = 0; w < kWarps; ++w) best = max(best, warp_key[w]);
@@ -175,13 +365,13 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const ScoreParams
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = ctas > 1 ? cluster_rank() : 0;
     const size_t row = blockIdx.x / ctas;
-    const T *x = static_cast<const T *>(p.logits) + row * p.pitch;
+    const Row<T> r(p, row);
+    const T *x = r.x;
+    const uint4 *units = r.units();
     const float c = p.scale * 1.4426950408889634f;
-    // the row: `lead` values up to the first 16-byte boundary, vectors, the rest; this CTA's vectors v0 .. v1 - 1. The odd values are the first CTA's.
-    const int lead = min(p.vocab, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)));
-    const int vectors = (p.vocab - lead) / kVec, odd = rank == 0 ? p.vocab - vectors * kVec : 0;
-    const int v0 = static_cast<int>(static_cast<long long>(vectors) * rank / ctas), v1 = static_cast<int>(static_cast<long long>(vectors) * (rank + 1) / ctas);
-    const uint4 *units = reinterpret_cast<const uint4 *>(x + lead);
+    // this CTA's vectors v0 .. v1 - 1; the odd values are the first CTA's
+    const int vectors = r.vectors, odd = rank == 0 ? r.odd : 0, lead = r.lead, each = vectors / ctas, more = vectors - each * ctas;
+    const int v0 = each * rank + min(static_cast<int>(rank), more), v1 = v0 + each + (static_cast<int>(rank) < more ? 1 : 0);
     if (tid == 0) {
         sh.count = sh.kept = 0;
         sh.bound = -FLT_MAX;  // what a value has to reach to go on the list; -inf never does
@@ -190,23 +380,16 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const ScoreParams
     ptx::pdl_trigger();
     ptx::pdl_wait();
 
-    Stats a{-FLT_MAX, 0.0f, 0.0f};
+    Seen seen;
     auto show = [&]() {
-        float most = a.m;
+        float most = seen.m;
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
         if ((tid & 7) == 0) sh.shown[tid >> 3] = order_value(most);
     };
-    auto look_up = [&]() {  // one warp; a lane finds the rank of one of the maxima
-        const unsigned mine = sh.shown[lane];
-        int rank = 0;
-#pragma unroll
-        for (int i = 0; i < kTop; i += 4) {
-            const uint4 other = *reinterpret_cast<const uint4 *>(sh.shown + i);
-            rank += (other.x > mine || (other.x == mine && i < lane)) + (other.y > mine || (other.y == mine && i + 1 < lane)) + (other.z > mine || (other.z == mine && i + 2 < lane)) +
-                    (other.w > mine || (other.w == mine && i + 3 < lane));
-        }
-        if (rank == p.top - 1) sh.bound = fmaxf(sh.bound, value_of(mine));
+    auto look_up = [&]() {  // one warp
+        unsigned mine;
+        if (has_rank(sh.shown, lane, p.top, mine)) sh.bound = fmaxf(sh.bound, value_of(mine));
     };
     float floor = -FLT_MAX;
     auto list = [&](float v, int id) {
@@ -215,15 +398,8 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const ScoreParams
             if (at < kList) sh.list[at] = order_key(v, id);
         }
     };
-    float2 s2 = make_float2(0.0f, 0.0f), t2 = s2;  // the thread's sums, every other value each
-    const float2 c2 = make_float2(c, c);
-    auto see = [&](float2 v, float2 less) {
-        const float2 d = add2(v, less), f = mul2(d, c2), e = make_float2(ex2(f.x), ex2(f.y));
-        s2 = add2(s2, e);
-        t2 = fma2(e, make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), t2);  // 0 * -inf is nothing here
-    };
-    const float odd_value = tid < odd ? get(x + (tid < lead ? tid : tid + vectors * kVec)) : -INFINITY;
-    const int odd_id = tid < lead ? tid : tid + vectors * kVec;
+    const float odd_value = tid < odd ? get(x + r.odd_id(tid)) : -INFINITY;
+    const int odd_id = r.odd_id(tid);
     // the first tokens' values are asked for now
     const bool one_given = rank == 0 && tid < p.given;
     const int token0 = one_given ? p.tokens[row * p.given + tid] : -1;
@@ -252,20 +428,14 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const ScoreParams
             for (int e = 1; e < kVec; ++e) vector_high[u] = fmaxf(vector_high[u], v[e]);
             high = fmaxf(high, vector_high[u]);
         }
-        if (high > a.m) {
-            const float d = a.m - high, r = ex2(d * c);
-            t2 = r == 0.0f ? make_float2(0.0f, 0.0f) : mul2(make_float2(r, r), fma2(s2, make_float2(d, d), t2));  // s * d may be -inf for the nothing in front
-            s2 = mul2(s2, make_float2(r, r));
-            a.m = high;
-        }
-        const float2 less = make_float2(-a.m, -a.m);
-        if (trip == 0) see(make_float2(odd_value, -INFINITY), less);
+        seen.reach(high, c);
+        if (trip == 0) seen.add(make_float2(odd_value, -INFINITY), c);
 #pragma unroll
         for (int u = 0; u < kLoads; ++u) {
             float v[kVec];
             unpack(raw[u], v);
 #pragma unroll
-            for (int e = 0; e < kVec; e += 2) see(make_float2(v[e], v[e + 1]), less);
+            for (int e = 0; e < kVec; e += 2) seen.add(make_float2(v[e], v[e + 1]), c);
         }
         if (p.top) {
             if ((trip & (trip + 1)) == 0) {  // after 1, 2, 4, .. trips
@@ -288,10 +458,8 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const ScoreParams
             }
         }
     }
-    a.s = s2.x + s2.y;
-    a.t = t2.x + t2.y;
     if (p.top) show();
-    a = join_warp(a, c);
+    Stats a = join_warp(seen.stats(), c);
     if (lane == 0) sh.warp_stats[warp] = a;
     __syncthreads();
     if (p.top && warp == 1) look_up();
@@ -332,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const ScoreParams
                     for (int e = 0; e < kVec; ++e) look(v[e], lead + i * kVec + e);
                 }
                 if (tid < odd) look(odd_value, odd_id);
-                for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+                best = warp_max(best);
                 if (lane == 0) sh.warp_key[warp] = best;
                 __syncthreads();
                 for (int w = 0; w < kWarps; ++w) best = max(best, sh.warp_key[w]);
@@ -357,9 +525,7 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const ScoreParams
         a = join_warp(lane < ctas ? sh.cta_stats[lane] : Stats{-FLT_MAX, 0.0f, 0.0f}, c);  // every warp the same
         if (p.top) {
             // a CTA whose last alternative is the largest has `top` that reach it: the others' behind that are none
-            Key least = lane < ctas ? sh.gathered[lane * p.top + p.top - 1] : 0;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) least = max(least, __shfl_xor_sync(0xffffffffu, least, o));
+            const Key least = warp_max(lane < ctas ? sh.gathered[lane * p.top + p.top - 1] : 0);
             if (tid == 0) sh.kept = 0;
             __syncthreads();
             for (int i = tid; i < ctas * p.top; i += kThreads)
@@ -371,19 +537,17 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const ScoreParams
         __syncthreads();
         a = sh.stats;
     }
-    const float log_s = logf(a.s);
-    auto logprob = [&](float v) { return (v - a.m) * p.scale - log_s; };
-    if (tid == 0 && p.entropy) p.entropy[row] = log_s - a.t / a.s * p.scale;
+    const Results result(a, p.scale);
+    if (tid == 0 && p.entropy) p.entropy[row] = result.entropy(a);
     const float none = __uint_as_float(0x7fc00000u);
-    if (one_given) p.logprobs[row * p.given + tid] = token0 >= 0 && token0 < p.vocab ? logprob(given0) : none;
+    if (one_given) p.logprobs[row * p.given + tid] = token0 >= 0 && token0 < p.vocab ? result.logprob(given0) : none;
     for (int g = tid + kThreads; g < p.given; g += kThreads) {
         const int token = p.tokens[row * p.given + g];
-        p.logprobs[row * p.given + g] = token >= 0 && token < p.vocab ? logprob(get(x + token)) : none;
+        p.logprobs[row * p.given + g] = token >= 0 && token < p.vocab ? result.logprob(get(x + token)) : none;
     }
     if (tid < p.top) {
-        const Key key = sh.top[tid];
-        p.top_ids[row * p.top + tid] = key_id(key);
-        p.top_logprobs[row * p.top + tid] = logprob(value_of(static_cast<unsigned>(key >> 32)));
+        p.top_ids[row * p.top + tid] = key_id(sh.top[tid]);
+        p.top_logprobs[row * p.top + tid] = result.logprob(key_value(sh.top[tid]));
     }
 }
 
@@ -413,9 +577,18 @@ int lbk_token_logprobs(lbk_ctx *c, int dtype, const void *logits_dev, size_t pit
         return fail(LBK_ERR_UNSUPPORTED, "lbk_token_logprobs: at most %d alternatives, 2^30 values and 2^20 tokens a row, 2^26 rows", LBK_LOGPROBS_TOP);
     const ScoreParams p{logits_dev, pitch, static_cast<int>(vocab), tokens_dev, static_cast<int>(given), scale, static_cast<int>(top), logprobs_dev, entropy_dev, top_ids_dev,
                         top_logprobs_dev};
+    const size_t size = dtype == LBK_DTYPE_F32 ? 4 : 2;
+    if (vocab * size <= (rows > 3 * static_cast<size_t>(ctx->sm_count) ? kShortBytes : kTinyBytes)) {
+        const size_t warps = std::min<size_t>(kShortWarps, (rows + ctx->sm_count - 1) / ctx->sm_count);  // few rows: an SM each
+        LBK_CUDA(launch_chained(dtype == LBK_DTYPE_F32 ? logprobs_short_kernel<float> : logprobs_short_kernel<uint16_t>, dim3(static_cast<unsigned>((rows + warps - 1) / warps)),
+                                dim3(static_cast<unsigned>(warps * 32)), 0, st, p, static_cast<int>(rows)));
+        ctx->launches++;
+        return LBK_OK;
+    }
     // CTAs a row: as many as the SMs hold beside one another, three each, as long as each has 3.5 trips of loads; of up to 64 CTAs half a trip is
-    // enough. us at 128256 f32 with 1 / 2 / 4 / 8 / 16: 1 row 24 / 19 / 14 / 12 / 10, 30 rows 40 / 28 / 21 / 18 / 26, 100 rows 39 / 30 / 23 / 29 / 42, 300 rows 52 / 59 / 63 / 79 / 132.
-    const size_t trip = static_cast<size_t>(kThreads) * kLoads * 16 / (dtype == LBK_DTYPE_F32 ? 4 : 2);
+    // enough. us at 128256 f32 with 1 / 2 / 4 / 8 / 16: 1 row 16.6 / 12.2 / 9.4 / 7.5 / 6.5, 16 rows 27 / 19 / 14 / 11 / 12, 64 rows 24 / 19 / 14 / 18 / 24, 150 rows 29 / 21 / 26 / 32 / 48,
+    // 300 rows 38 / 44 / 49 / 70 / 116.
+    const size_t trip = static_cast<size_t>(kThreads) * kLoads * 16 / size;
     unsigned ctas = 1;
     while (ctas < kClusterMost && rows * ctas * 2 <= 3 * static_cast<size_t>(ctx->sm_count) && (vocab >= 7 * trip * ctas || (rows * ctas <= 64 && vocab >= trip * ctas))) ctas *= 2;
     cudaLaunchConfig_t cfg{};

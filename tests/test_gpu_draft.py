@@ -238,6 +238,16 @@ def test_logprobs(ctx, dtype, rows, vocab, pad, top):
 @pytest.mark.parametrize("vocab", [40, 5000, 130001])
 def test_logprobs_of_unusual_rows(ctx, dtype, vocab):
     """Ties, rows in order, masks of -inf and of the type's lowest value, rows with a NaN or an infinity, rows with nothing."""
+    _unusual_rows(dtype, vocab, 1)
+
+
+@pytest.mark.parametrize("dtype,vocab", [("float32", 700), ("float32", 5003), ("bfloat16", 1100), ("bfloat16", 10001)])
+def test_logprobs_of_many_unusual_rows(ctx, dtype, vocab):
+    """The same where there are more rows than the SMs hold blocks: rows of a warp each."""
+    _unusual_rows(dtype, vocab, 30)
+
+
+def _unusual_rows(dtype, vocab, times):
     import torch
     dt = getattr(torch, dtype)
     g = torch.Generator(device="cuda").manual_seed(vocab)
@@ -263,8 +273,8 @@ def test_logprobs_of_unusual_rows(ctx, dtype, vocab):
     x[13, vocab - 1] = -50.0
     x[14] = torch.randn(vocab, generator=g, device="cuda") * 1e-30
     x[15, ::2] = -math.inf
-    x = x.to(dt)
-    tokens = torch.tensor([[0, vocab - 1, 7]], dtype=torch.int32, device="cuda").expand(16, 3).contiguous()
+    x = x.to(dt).repeat(times, 1)
+    tokens = torch.tensor([[0, vocab - 1, 7]], dtype=torch.int32, device="cuda").expand(16 * times, 3).contiguous()
     for top in (1, 20, 32):
         _check_logprobs(x, tokens, top)
 

@@ -332,17 +332,26 @@ class BitNet:
     # ---- drafted tokens --------------------------------------------------------------------------
     def forward_tree(self, tokens: torch.Tensor, parents: torch.Tensor, cache: KvCache, counts: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Several drafted tokens of every sequence in one pass: tokens, parents int32 CUDA [b, t] (parents[i] < i: the node that node i
-        follows, -1: the last committed token), counts int32 [b] how many of them a sequence has. Returns the logits f32 [b, t, vocab] after each. Their keys
+        follows, -1: the last committed token), counts int32 [b] how many of them a sequence has; all t places have to fit in the cache. Returns the logits f32 [b, t, vocab] after each. Their keys
         and values are in the cache behind the committed ones, which stay as many: `accept_tree` commits a path."""
-        cfg, lib, h = self.cfg, self.ctx._lib, self.ctx.handle
+        cfg = self.cfg
         if tokens.dtype != torch.int32 or tokens.shape != parents.shape or tokens.dim() != 2 or tokens.shape[0] != cache.b:
             raise ValueError("tokens and parents are int32 [sequences of the cache, nodes]")
+        if not 1 <= tokens.shape[1] <= ops.TREE_NODES:
+            raise ValueError(f"a tree has 1 to {ops.TREE_NODES} nodes (got {tokens.shape[1]})")
+        if any(t is not None and t.device != self.final_norm.device for t in (tokens, parents, counts, cache.pos)):
+            raise ValueError(f"tokens, trees and the cache must live on {self.final_norm.device}")
         if not cache.own_positions:
             raise ValueError("drafted tokens need a cache whose sequences have positions of their own (new_cache(own_positions=True))")
         if cfg.head_dim() != 128:
             raise ValueError("drafted tokens need heads of 128")
+        cache.reserve(tokens.shape[1])
+        with torch.cuda.device(self.final_norm.device):  # the stream of the model's device, whichever is current
+            return self._forward_tree(tokens, parents, cache, counts)
+
+    def _forward_tree(self, tokens: torch.Tensor, parents: torch.Tensor, cache: KvCache, counts: Optional[torch.Tensor]) -> torch.Tensor:
+        cfg, lib, h = self.cfg, self.ctx._lib, self.ctx.handle
         b, t = tokens.shape
-        cache.reserve(t)
         m, H, I, nh, hd, eps = b * t, cfg.hidden_size, cfg.intermediate_size, cfg.num_attention_heads, cfg.head_dim(), cfg.rms_norm_eps
         st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
         P = lambda v: C.c_void_p(v.data_ptr())
@@ -394,7 +403,8 @@ class BitNet:
         model itself would have given are committed. Returns (path, count, next) of ops.tree_accept: with the tokens on the path, and `next`, the same
         tokens as `forward` one by one."""
         logits = self.forward_tree(tokens, parents, cache, counts)
-        best = self.argmax(logits.view(-1, logits.shape[2])).view(tokens.shape)
+        with torch.cuda.device(self.final_norm.device):
+            best = self.argmax(logits.view(-1, logits.shape[2])).view(tokens.shape)
         path, count, after = ops.tree_accept(tokens, parents, best, counts, self.ctx)
         self.accept_tree(cache, path, count)
         return path, count, after

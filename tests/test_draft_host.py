@@ -74,3 +74,19 @@ def test_a_missing_extension_module_is_an_error(monkeypatch, tmp_path):
     monkeypatch.setattr(_lib, "LIB_PATH", tmp_path / "liblbk.so")
     with pytest.raises(RuntimeError, match="missing"):
         ops.advance_pos_by(_i(1), _i(1))
+
+
+def test_a_model_refuses_drafts_before_anything_is_launched():
+    from types import SimpleNamespace
+
+    from lemonade_burn_b200.model import BitNet
+    net = SimpleNamespace(cfg=SimpleNamespace(head_dim=lambda: 128), final_norm=SimpleNamespace(device=torch.device("cuda:0")))
+    there = lambda *shape: SimpleNamespace(dtype=torch.int32, shape=torch.Size(shape), dim=lambda: len(shape), device=torch.device("cuda:0"))  # noqa: E731
+    cache = SimpleNamespace(b=2, own_positions=True, pos=there(2))
+    refused = [(_i(2, 3), _i(2, 3), None), (there(2, 3), _i(2, 3), None), (_i(2, 3), there(2, 3), None), (there(2, 3), there(2, 3), _i(2)), (there(2, 0), there(2, 0), None),
+               (there(2, 129), there(2, 129), None), (there(3, 3), there(3, 3), None), (there(2, 3), there(2, 4), None), (_i(2, 3).long(), _i(2, 3), None)]
+    for tokens, parents, counts in refused:
+        with pytest.raises(ValueError):
+            BitNet.forward_tree(net, tokens, parents, cache, counts)
+    with pytest.raises(ValueError, match="live on"):
+        BitNet.forward_tree(net, there(2, 3), there(2, 3), SimpleNamespace(b=2, own_positions=True, pos=_i(2)))

@@ -567,7 +567,7 @@ int lbk_kv_keep_path(lbk_ctx *ctx, uint16_t *kcache_dev, uint16_t *vcache_dev, s
                      size_t head_dim, size_t cap, const int32_t *pos_dev, const int32_t *path_dev, const int32_t *count_dev, size_t t, void *stream);
 int lbk_advance_pos_by(lbk_ctx *ctx, int32_t *pos_dev, const int32_t *count_dev, size_t b, void *stream);
 
-/* Rows of logits (LBK_DTYPE_*, `pitch` values apart, 0 < scale): logprobs_dev [rows][given] = log softmax(scale * logits) at
+/* Rows of logits (LBK_DTYPE_*, `pitch` values apart, scale from 1e-20 to 1e20): logprobs_dev [rows][given] = log softmax(scale * logits) at
  * tokens_dev [rows][given] (NaN for a token outside the vocabulary), entropy_dev [rows] (may be null) in nats, and the `top` (at most
  * LBK_LOGPROBS_TOP) largest logits: ids top_ids_dev [rows][top], the lower one first among equals, NaN in front, and their log
  * probabilities. Values of -inf have probability 0; a row with a NaN or +inf, or with nothing above -inf, has NaN log probabilities and entropy. */

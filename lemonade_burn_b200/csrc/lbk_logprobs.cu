@@ -143,7 +143,7 @@ struct Row {
 struct Results {
     float m, log_s, scale;
     __device__ __forceinline__ Results(const Stats &a, float scale) : m(a.m), log_s(logf(a.s)), scale(scale) {}
-    __device__ __forceinline__ float logprob(float v) const { return (v - m) * scale - log_s; }
+    __device__ __forceinline__ float logprob(float v) const { return (0.5f * v - 0.5f * m) * scale * 2.0f - log_s; }  // halves: v - m may be more than f32 has
     __device__ __forceinline__ float entropy(const Stats &a) const { return log_s - a.t / a.s * scale; }
 };
 __device__ __forceinline__ float key_value(Key key) { return value_of(static_cast<unsigned>(key >> 32)); }
@@ -572,7 +572,8 @@ int lbk_token_logprobs(lbk_ctx *c, int dtype, const void *logits_dev, size_t pit
         return fail(LBK_ERR_INVALID, "lbk_token_logprobs: null buffer");
     if (dtype != LBK_DTYPE_F32 && dtype != LBK_DTYPE_BF16) return fail(LBK_ERR_INVALID, "lbk_token_logprobs: unknown type %d", dtype);
     if (vocab == 0 || pitch < vocab || top > vocab) return fail(LBK_ERR_SHAPE, "lbk_token_logprobs: rows of %zu values, %zu apart, %zu alternatives", vocab, pitch, top);
-    if (!(scale > 0.0f) || scale > FLT_MAX) return fail(LBK_ERR_INVALID, "lbk_token_logprobs: the scale is a positive number");
+    // inside these, scale * log2(e) is finite, and what lies 1e30 below the largest value has no weight (Seen::add)
+    if (!(scale >= 1e-20f && scale <= 1e20f)) return fail(LBK_ERR_INVALID, "lbk_token_logprobs: the scale is a number from 1e-20 to 1e20");
     if (top > LBK_LOGPROBS_TOP || vocab > (1u << 30) || given > (1u << 20) || rows > (1u << 26))
         return fail(LBK_ERR_UNSUPPORTED, "lbk_token_logprobs: at most %d alternatives, 2^30 values and 2^20 tokens a row, 2^26 rows", LBK_LOGPROBS_TOP);
     const ScoreParams p{logits_dev, pitch, static_cast<int>(vocab), tokens_dev, static_cast<int>(given), scale, static_cast<int>(top), logprobs_dev, entropy_dev, top_ids_dev,

@@ -7,7 +7,6 @@
 // A call with several tokens of one sequence (a prompt, or a portion of one) sends up to 4096 rows at a time
 // through the projections. One decode step is recorded into a CUDA graph the first time a cache is used and
 // replayed afterwards (the positions live in device memory).
-#include <cfloat>
 #include <deque>
 #include <new>
 
@@ -729,7 +728,7 @@ int lbk_model_score(lbk_model *mp, lbk_kv_cache *cp, size_t seq, const uint32_t 
     if (c->model != m) return fail(LBK_ERR_INVALID, "the cache belongs to another model");
     if (seq >= c->b) return fail(LBK_ERR_INVALID, "sequence %zu of a cache of %zu", seq, c->b);
     if (top > LBK_LOGPROBS_TOP || top > V) return fail(LBK_ERR_UNSUPPORTED, "lbk_model_score: at most %d alternatives (got %zu)", LBK_LOGPROBS_TOP, top);
-    if (!(scale > 0.0f) || scale > FLT_MAX) return fail(LBK_ERR_INVALID, "lbk_model_score: the scale is a positive number");
+    if (!(scale >= 1e-20f && scale <= 1e20f)) return fail(LBK_ERR_INVALID, "lbk_model_score: the scale is a number from 1e-20 to 1e20");
     if (n > c->cap - c->lens[seq]) return fail(LBK_ERR_INVALID, "%zu tokens do not fit: %zu of %zu positions are used", n, c->lens[seq], c->cap);
     for (size_t i = 0; i < n; ++i)
         for (uint32_t t : {tokens[i], targets ? targets[i] : 0u})

@@ -232,7 +232,7 @@ class TokenLogprobs(NamedTuple):
 
 
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0, scale: float = 1.0, ctx: Optional[Context] = None) -> TokenLogprobs:
-    """Log softmax(scale * logits) at the given tokens, entropy and the `top` largest logits with their log probabilities
+    """Log softmax(scale * logits), scale from 1e-20 to 1e20, at the given tokens, entropy and the `top` largest logits with their log probabilities
     (lbk_token_logprobs). logits f32 or bf16 [rows, vocab], rows any distance apart; tokens int32 [rows] or [rows, given]."""
     return TokenLogprobs(*(_native or _torch_ops()).token_logprobs(logits, tokens, top, scale, ctx))
 

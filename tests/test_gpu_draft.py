@@ -294,3 +294,34 @@ def test_logprobs_without_tokens_or_alternatives(ctx):
     assert call() == 0
     assert call(dtype=2) == 1 and call(pitch=99) == 2 and call(vocab=0) == 2 and call(scale=0.0) == 1 and call(scale=math.nan) == 1 and call(scale=math.inf) == 1
     assert call(top=3) == 1 and call(top=33, ids=out.data_ptr()) == 4 and call(pitch=200, vocab=101, top=102, ids=out.data_ptr()) == 2
+
+
+@pytest.mark.parametrize("vocab", [50, 9000])
+@pytest.mark.parametrize("scale", [1e-20, 1e-3, 7.0, 1e20])
+def test_logprobs_at_any_scale(ctx, vocab, scale):
+    """What the scale is for: temperatures. At the ends every value has the same weight, or one value all of it."""
+    import torch
+    from lemonade_burn_b200 import ops
+    x = torch.randn(3, vocab, generator=torch.Generator().manual_seed(1)).cuda()
+    x[1, 3], x[1, 7] = 3e38, -3e38
+    tokens = torch.tensor([[0, 3], [7, 3], [1, 3]], dtype=torch.int32).cuda()
+    got = ops.token_logprobs(x, tokens, top=2, scale=scale)
+    factor = torch.tensor(scale, dtype=torch.float32).double().item()  # as the call has it
+    want = torch.log_softmax(x.double() * factor, -1)
+    entropy = -torch.where(want.exp() > 0, want.exp() * want, torch.zeros_like(want)).sum(-1)
+    at = want.gather(1, tokens.long())
+    # In steps of 2^-23. A log probability is (x - m) scale - log s: the product is off by 2 of itself; s, a thread's sum of 18 exponentials at most and eight
+    # joins, by 13 + 2 for the exponentials; its logarithm, at most 10, by 10, and by the exponents' own error, |f| e^f < 1. Entropy is log s - scale t / s: t as s,
+    # times 10, and twice sum p f^2 < 60 for the exponents.
+    finite = at.abs() < 3e38  # f32 ends there
+    assert bool(((got.logprobs.double() - at).abs() <= 2.0 ** -23 * (4 * at.abs() + 40))[finite].all()) and bool((got.logprobs[~finite] < -3e38).all())
+    assert bool(((got.entropy.double() - entropy).abs() <= 2.0 ** -23 * 400).all())
+    assert got.top_ids[1, 0] == 3 and torch.equal(got.top_ids.cpu().long(), x.cpu().topk(2).indices)
+
+
+def test_logprobs_of_scales_that_are_none(ctx):
+    import torch
+    from lemonade_burn_b200 import _lib, ops
+    for scale in (0.0, -1.0, 9e-21, 2e20, 3e38, 1e300, math.inf, math.nan):
+        with pytest.raises(_lib.LbkError):
+            ops.token_logprobs(torch.zeros(2, 9, device="cuda"), scale=scale)

@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) logprobs_short_kernel(const 
 #pragma unroll
         for (int u = 0; u < kLoads; ++u) {
             const int i = base + u * 32 + lane;
-            into[u] = i < r.vectors ? __ldg(units + i) : Empty<T>::vector();
+            into[u] = i < r.vectors ? units[i] : Empty<T>::vector();
         }
     };
     ask(next, 0);
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) logprobs_short_kernel(const 
 #pragma unroll 4
     for (int i = lane; i < r.vectors; i += 32) {
         float v[kVec], high;
-        unpack(__ldg(units + i), v);
+        unpack(units[i], v);
         high = v[0];
 #pragma unroll
         for (int e = 1; e < kVec; ++e) high = fmaxf(high, v[e]);
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) logprobs_short_kernel(const 
         };
         for (int i = lane; i < r.vectors; i += 32) {
             float v[kVec];
-            unpack(__ldg(units + i), v);
+            unpack(units[i], v);
 #pragma unroll
             for (int e = 0; e < kVec; ++e) look(v[e], r.id(i, e));
         }

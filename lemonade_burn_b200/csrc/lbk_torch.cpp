@@ -1,6 +1,6 @@
 // The calls around drafted tokens (lemonade_burn_b200/ops.py) on torch tensors: checks of arguments, results, the current stream, the call into the library.
-// In Python these were most of a small call's time: us a call on the host, before / so: attn_tree 13.0 / 5.9, rope_kv_append_tree 7.8 / 2.9, tree_accept 10.7 /
-// 5.9, kv_keep_path 6.3 / 2.8, token_logprobs 15.8 / 6.9.
+// In Python these were most of a small call's time: us a call on the host, before / so: attn_tree 13.0 / 5.2, rope_kv_append_tree 7.8 / 2.5, tree_accept 10.7 /
+// 4.1, kv_keep_path 6.3 / 2.3, token_logprobs 15.8 / 4.5.
 //
 // The library itself knows nothing of torch: its functions are handed over by address (bind), so that this file works with whatever library the process has
 // loaded. No exception leaves an entry point: torch's become RuntimeError, a status that is not 0 becomes LbkError.
@@ -40,6 +40,13 @@ struct Refused {};
     PyErr_FormatV(kind, format, args);
     va_end(args);
     throw Refused();
+}
+
+// A function that the loaded library has (one family's part of it: _lib.use).
+template <class F>
+F have(F f, const char *name) {
+    if (!f) refuse(PyExc_RuntimeError, "the library that is loaded has no %s", name);
+    return f;
 }
 
 const at::Tensor &tensor(PyObject *o, const char *name) {
@@ -153,6 +160,7 @@ PyObject *entry(Py_ssize_t given, Py_ssize_t wanted, Body &&body) {
 // q, k, v, cos, sin, pos, parents, kcache, vcache, counts, ctx
 PyObject *rope_kv_append_tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return entry(n, 11, [&] {
+        const auto call = have(lib.append, "lbk_rope_kv_append_tree");
         const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v"), &cos = tensor(a[3], "cos"), &sin = tensor(a[4], "sin"), &pos = tensor(a[5], "pos"),
                          &parents = tensor(a[6], "parents"), &kc = tensor(a[7], "kcache"), &vc = tensor(a[8], "vcache");
         const at::Tensor counts = maybe(a[9], "counts");
@@ -166,7 +174,7 @@ PyObject *rope_kv_append_tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
         if (cos.dim() != 2 || cos.size(0) < c.cap || cos.size(1) != c.hd || !sin.sizes().equals(cos.sizes())) refuse(PyExc_ValueError, "the rotation tables have a row for every place of the cache");
         const Context ctx(a[10]);
         void *st = ctx.stream(q, k, v, cos, sin, pos, parents, kc, vc, counts);
-        done(lib.append(ctx.handle, data<float>(q), data<float>(k), data<float>(v), data<float>(cos), data<float>(sin), ints(pos), ints(parents), ints(counts), s.b, s.t, heads, c.kv_heads, c.hd,
+        done(call(ctx.handle, data<float>(q), data<float>(k), data<float>(v), data<float>(cos), data<float>(sin), ints(pos), ints(parents), ints(counts), s.b, s.t, heads, c.kv_heads, c.hd,
                         c.cap, data<uint16_t>(kc), data<uint16_t>(vc), st));
         Py_RETURN_NONE;
     });
@@ -184,6 +192,7 @@ int64_t node_pitch(const at::Tensor &x, const Tree &s, int64_t heads, int64_t hd
 // q, kcache, vcache, pos, parents, counts, scale, out, ctx
 PyObject *attn_tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return entry(n, 9, [&] {
+        const auto call = have(lib.attn, "lbk_attn_tree");
         const at::Tensor &q = tensor(a[0], "q"), &kc = tensor(a[1], "kcache"), &vc = tensor(a[2], "vcache"), &pos = tensor(a[3], "pos"), &parents = tensor(a[4], "parents");
         const at::Tensor counts = maybe(a[5], "counts");
         at::Tensor out = maybe(a[7], "out");
@@ -207,7 +216,7 @@ PyObject *attn_tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
         ctx.lives_here(out);
         if (!out.defined()) out = like(q, q.sizes(), q.scalar_type());
         const at::Tensor scratch = like(q, {static_cast<int64_t>(lib.scratch(ctx.handle, s.t, heads, c.kv_heads))}, at::kFloat);
-        done(lib.attn(ctx.handle, f32 ? LBK_COMPUTE_F32 : LBK_COMPUTE_BF16, data(q), q_pitch, data<uint16_t>(kc), data<uint16_t>(vc), ints(pos), ints(parents), ints(counts), s.b, s.t, heads,
+        done(call(ctx.handle, f32 ? LBK_COMPUTE_F32 : LBK_COMPUTE_BF16, data(q), q_pitch, data<uint16_t>(kc), data<uint16_t>(vc), ints(pos), ints(parents), ints(counts), s.b, s.t, heads,
                       c.kv_heads, c.hd, c.cap, static_cast<float>(scale), data<float>(scratch), data<void>(out), out_pitch, st));
         return a[7] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(a[7]);
     });
@@ -231,6 +240,7 @@ PyObject *wrap(std::initializer_list<at::Tensor> tensors) {
 // tokens, parents, best, counts, ctx
 PyObject *tree_accept(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return entry(n, 5, [&] {
+        const auto call = have(lib.accept, "lbk_tree_accept");
         const at::Tensor &tokens = tensor(a[0], "tokens"), &parents = tensor(a[1], "parents"), &best = tensor(a[2], "best");
         const at::Tensor counts = maybe(a[3], "counts");
         const Tree s = tree(parents, counts, at::Tensor());
@@ -241,7 +251,7 @@ PyObject *tree_accept(PyObject *, PyObject *const *a, Py_ssize_t n) {
         void *st = ctx.stream(tokens, parents, best, counts);
         Results r(parents, Results::room(s.b * s.t) + 2 * Results::room(s.b));
         const at::Tensor path = r.take({s.b, s.t}, at::kInt), count = r.take({s.b}, at::kInt), after = r.take({s.b}, at::kInt);
-        done(lib.accept(ctx.handle, ints(tokens), ints(parents), ints(best), ints(counts), s.b, s.t, data<int32_t>(path), data<int32_t>(count), data<int32_t>(after), st));
+        done(call(ctx.handle, ints(tokens), ints(parents), ints(best), ints(counts), s.b, s.t, data<int32_t>(path), data<int32_t>(count), data<int32_t>(after), st));
         return wrap({path, count, after});
     });
 }
@@ -249,12 +259,13 @@ PyObject *tree_accept(PyObject *, PyObject *const *a, Py_ssize_t n) {
 // k, v, pos, path, count, ctx
 PyObject *kv_keep_path(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return entry(n, 6, [&] {
+        const auto call = have(lib.keep, "lbk_kv_keep_path");
         const at::Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v"), &pos = tensor(a[2], "pos"), &path = tensor(a[3], "path"), &count = tensor(a[4], "count");
         const Tree s = tree(path, count, pos);
         const Cache c = caches(k, v, s.b, 5);
         const Context ctx(a[5]);
         void *st = ctx.stream(k, v, pos, path, count);
-        done(lib.keep(ctx.handle, data<uint16_t>(k), data<uint16_t>(v), c.layers, s.b * c.kv_heads * c.cap * c.hd, s.b, c.kv_heads, c.hd, c.cap, ints(pos), ints(path), ints(count), s.t, st));
+        done(call(ctx.handle, data<uint16_t>(k), data<uint16_t>(v), c.layers, s.b * c.kv_heads * c.cap * c.hd, s.b, c.kv_heads, c.hd, c.cap, ints(pos), ints(path), ints(count), s.t, st));
         Py_RETURN_NONE;
     });
 }
@@ -262,12 +273,13 @@ PyObject *kv_keep_path(PyObject *, PyObject *const *a, Py_ssize_t n) {
 // pos, count, ctx
 PyObject *advance_pos_by(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return entry(n, 3, [&] {
+        const auto call = have(lib.advance, "lbk_advance_pos_by");
         const at::Tensor &pos = tensor(a[0], "pos"), &count = tensor(a[1], "count");
         if (!is(pos, at::kInt) || !is(count, at::kInt) || pos.dim() != 1 || !pos.sizes().equals(count.sizes()))
             refuse(PyExc_ValueError, "pos and count are int32, one number for each sequence");
         const Context ctx(a[2]);
         void *st = ctx.stream(pos, count);
-        done(lib.advance(ctx.handle, data<int32_t>(pos), ints(count), pos.size(0), st));
+        done(call(ctx.handle, data<int32_t>(pos), ints(count), pos.size(0), st));
         Py_RETURN_NONE;
     });
 }
@@ -275,6 +287,7 @@ PyObject *advance_pos_by(PyObject *, PyObject *const *a, Py_ssize_t n) {
 // logits, tokens, top, scale, ctx
 PyObject *token_logprobs(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return entry(n, 5, [&] {
+        const auto call = have(lib.logprobs, "lbk_token_logprobs");
         const at::Tensor &logits = tensor(a[0], "logits");
         const at::Tensor tokens = maybe(a[1], "tokens");
         const long long top = PyLong_AsLongLong(a[2]);
@@ -298,7 +311,7 @@ PyObject *token_logprobs(PyObject *, PyObject *const *a, Py_ssize_t n) {
         Results r(logits, Results::room(rows * given) + Results::room(rows) + 2 * Results::room(rows * top));
         const at::Tensor lp = r.take({rows, given}, at::kFloat), entropy = r.take({rows}, at::kFloat), ids = r.take({rows, static_cast<int64_t>(top)}, at::kInt),
                          best = r.take({rows, static_cast<int64_t>(top)}, at::kFloat);
-        done(lib.logprobs(ctx.handle, f32 ? LBK_DTYPE_F32 : LBK_DTYPE_BF16, data(logits), pitch, rows, vocab, given ? ints(tokens) : nullptr, given, static_cast<float>(scale), top,
+        done(call(ctx.handle, f32 ? LBK_DTYPE_F32 : LBK_DTYPE_BF16, data(logits), pitch, rows, vocab, given ? ints(tokens) : nullptr, given, static_cast<float>(scale), top,
                           data<float>(lp), data<float>(entropy), data<int32_t>(ids), data<float>(best), st));
         return wrap({lp, entropy, ids, best});
     });

@@ -184,8 +184,8 @@ def _torch_ops():
         module = module_from_spec(spec_from_file_location("_torch_ops", str(path), loader=loader))
         loader.exec_module(module)
         lib = _lib.load()
-        module.bind(*[C.cast(f, C.c_void_p).value for f in (lib.lbk_rope_kv_append_tree, lib.lbk_attn_tree_scratch, lib.lbk_attn_tree, lib.lbk_tree_accept, lib.lbk_kv_keep_path,
-                                                            lib.lbk_advance_pos_by, lib.lbk_token_logprobs)], _lib.check, default_context)
+        calls = [getattr(lib, "lbk_" + n, None) for n in ("rope_kv_append_tree", "attn_tree_scratch", "attn_tree", "tree_accept", "kv_keep_path", "advance_pos_by", "token_logprobs")]
+        module.bind(*[C.cast(f, C.c_void_p).value if f else 0 for f in calls], _lib.check, default_context)  # one family's part of the library has some of them only
         _native = module
     return _native
 

@@ -90,3 +90,26 @@ def test_a_model_refuses_drafts_before_anything_is_launched():
             BitNet.forward_tree(net, tokens, parents, cache, counts)
     with pytest.raises(ValueError, match="live on"):
         BitNet.forward_tree(net, there(2, 3), there(2, 3), SimpleNamespace(b=2, own_positions=True, pos=_i(2)))
+
+
+def test_a_part_of_the_library_has_some_of_the_calls():
+    """A process that serves one family may load that family's part: it has log probabilities, but no trees."""
+    import subprocess
+    import sys
+    code = """
+import types, torch
+from lemonade_burn_b200 import _lib, build, ops
+build.build()
+whole = _lib.load()
+_lib._lib = types.SimpleNamespace(lbk_token_logprobs=whole.lbk_token_logprobs)
+ints = lambda *shape: torch.zeros(shape, dtype=torch.int32)
+for call in (lambda: ops.advance_pos_by(ints(1), ints(1)), lambda: ops.tree_accept(ints(1, 1), ints(1, 1), ints(1, 1)), lambda: ops.token_logprobs(torch.zeros(2))):
+    try:
+        call()
+    except Exception as e:
+        print(type(e).__name__, e)
+"""
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert out.returncode == 0, out.stderr
+    assert out.stdout.splitlines() == ["RuntimeError the library that is loaded has no lbk_advance_pos_by", "RuntimeError the library that is loaded has no lbk_tree_accept",
+                                       "ValueError logits are [rows, vocab]"]

@@ -544,14 +544,16 @@ int lbk_moe_route(lbk_ctx *ctx, const float *z_dev, size_t z_pitch, size_t n, si
  *                          [b][t][kv_heads][head_dim] by position pos + depth, k and v appended at row pos + i. The tables have cap rows or more.
  * lbk_attn_tree            softmax(scale * q . k) v over the rows 0 .. pos - 1 and those of the node itself and its ancestors, head_dim
  *                          128. q_dev and out_dev rows [b * t] of n_heads * 128 values, q_pitch and out_pitch values apart: f32 with
- *                          LBK_COMPUTE_F32 (q and the probabilities as two bf16 terms each), bf16 with LBK_COMPUTE_BF16; pitches and buffers are
- *                          multiples of 16 bytes. scratch_dev: lbk_attn_tree_scratch floats, 16-byte aligned, what is in them
- *                          does not matter; calls that may overlap need their own.
+ *                          LBK_COMPUTE_F32 (q and the probabilities as three bf16 terms each), bf16 with LBK_COMPUTE_BF16 (one); pitches and buffers are
+ *                          multiples of 16 bytes; out_dev may be q_dev. 0 < scale <= 1e30; at most 256 sequences, 4096 heads, 2^30 places of a
+ *                          cache, 2^31 rows of all caches of the call. scratch_dev: lbk_attn_tree_scratch floats, 16-byte aligned, what is in
+ *                          them does not matter; calls that may overlap need their own.
  * lbk_tree_accept          the greedy walk: node 0, then as long as there is one the lowest child whose token (tokens_dev) is best_dev of its
  *                          parent (the argmax of the parent's logits). path_dev [b][t]: the nodes, then -1; count_out_dev how many, next_dev
  *                          best_dev of the last one (-1 for a sequence without nodes).
  * lbk_kv_keep_path         rows pos + path[j] move to pos + j, j < count_dev[seq], of keys and values of `layers` layers that lie
- *                          layer_elems elements apart. path_dev [b][t] ascending, any accepted nodes. Positions are not changed.
+ *                          layer_elems elements apart. path_dev [b][t] ascending, any accepted nodes. Positions are not changed. head_dim and
+ *                          layer_elems are multiples of 8, the caches lie on 16 bytes; at most 65535 sequences.
  * lbk_advance_pos_by       pos_dev[seq] += count_dev[seq]. */
 #define LBK_TREE_NODES 128
 int lbk_rope_kv_append_tree(lbk_ctx *ctx, float *q_dev, const float *k_dev, const float *v_dev, const float *cos_dev, const float *sin_dev,

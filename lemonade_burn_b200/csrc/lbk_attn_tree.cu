@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
 // block into zeroed sums, which the softmax warps add to the rows in their registers.
 //
 //   16 softmax warps four to a quadrant of 32 lanes = rows: warps w, w + 4, .. share rows and take 32 of a block's keys, and of the dimensions, each (eight
-//                    warps with 64 took 5900 cycles a block in three terms where the products take 3072: two warps a scheduler do not hide their latencies)
+//                    warps with 64 took 5900 cycles a block in three terms where the products take some 3100: two warps a scheduler do not hide their latencies)
 //   K, V producers   a warp each: K blocks of 128 keys are free again after the scores, V in pieces of 64 keys after their product, and one order for
 //                    both would have the next K block wait for a piece of V
 //   MMA warp         P V of block j - 1, then Q K^T of block j + 1, while the softmax warps work on block j

@@ -201,8 +201,8 @@ def rope_kv_append_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: 
 def attn_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, pos: torch.Tensor, parents: torch.Tensor, counts: Optional[torch.Tensor] = None,
               scale: Optional[float] = None, out: Optional[torch.Tensor] = None, ctx: Optional[Context] = None) -> torch.Tensor:
     """Attention of drafted tokens (lbk_attn_tree): q [b, t, heads, 128] f32 or bf16 (nodes any distance apart) over rows 0 .. pos - 1 of kcache
-    and vcache [b, kv_heads, cap, 128] and over the node itself and its ancestors, whose rows are pos + node. scale: 128 ** -0.5. Returns
-    `out` (made like q without one: rows of places not in use are then whatever was there)."""
+    and vcache [b, kv_heads, cap, 128] and over the node itself and its ancestors, whose rows are pos + node. At most 256 sequences. scale: 128 ** -0.5. Returns
+    `out`, which may be q (made like q without one: rows of places not in use are then whatever was there)."""
     return (_native or _torch_ops()).attn_tree(q, kcache, vcache, pos, parents, counts, scale, out, ctx)
 
 

@@ -321,3 +321,31 @@ def test_refusals(ctx):
                            (dict(out=out.data_ptr() + 8), 2), (dict(compute=0, pitch=516), 2)):
         assert call(**change) == status, change
     ctx.check_device_error()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("b,t,nh,kvh,lengths", [(256, 1, 2, 1, [i % 3 for i in range(256)]), (1, 2, 4096, 1, [70]), (1, 1, 4096, 4096, [3]), (2, 128, 32, 1, [5, 130])])
+def test_the_largest_batches_and_heads(ctx, dtype, b, t, nh, kvh, lengths):
+    import torch
+    check(ctx, make(b, t, nh, kvh, lengths, getattr(torch, dtype)))
+
+
+@pytest.mark.parametrize("t,nh", [(1, 4), (5, 16), (40, 8)])
+def test_a_cache_without_room_to_spare(ctx, t, nh):
+    """The last node's row is the cache's last one, and the sequence the buffer's last."""
+    import torch
+    for pos in (0, 1, 60, 130):
+        q, k, v, lengths, parents, counts = make(2, t, nh, 2, [pos, pos], torch.float32)
+        check(ctx, (q, k[:, :, :pos + t].contiguous(), v[:, :, :pos + t].contiguous(), lengths, parents, counts))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("b,t,nh,kvh,length", [(1, 1, 20, 5, 900), (2, 6, 20, 5, 5000), (1, 60, 8, 2, 9000), (3, 128, 8, 2, 100)])
+def test_results_in_the_place_of_the_queries(ctx, dtype, b, t, nh, kvh, length):
+    import torch
+    from lemonade_burn_b200 import ops
+    q, k, v, pos, parents, counts = make(b, t, nh, kvh, [length] * b, getattr(torch, dtype))
+    on = dev(pos, parents, counts)
+    want = ops.attn_tree(q, k, v, *on, out=q.clone())  # rows of places not in use stay
+    assert ops.attn_tree(q, k, v, *on, out=q) is q and torch.equal(q, want)
+    ctx.check_device_error()

@@ -46,6 +46,7 @@ struct TreeParams {
     float *part;        // [CTA][2][tile rows][128]
     float2 *part_ml;    // [CTA][2][tile rows]: maximum, weight
     int workers;        // CTAs of the attention kernel
+    unsigned per_worker; // 2^32 / workers
     unsigned per_group; // 2^32 / heads of a group, rounded up; 0 for one head
     int *err_word;
     __device__ __forceinline__ int node_of(int row) const { return per_group ? static_cast<int>(__umulhi(static_cast<unsigned>(row), per_group)) : row; }
@@ -82,12 +83,29 @@ struct Line {
     int first[kMaxSeqs + 1];   // units in front of a sequence; [b] is all of them
     int pos[kMaxSeqs], count[kMaxSeqs];
 };
-// A sequence: kv_heads * tiles problems of `blocks` units each.
-__device__ __forceinline__ int line_blocks(const Line &l, int seq, int block_keys) { return (l.pos[seq] + l.count[seq] + block_keys - 1) / block_keys; }
-__device__ __forceinline__ int line_tiles(const Line &l, int seq, int group, int rows) { return (l.count[seq] * group + rows - 1) / rows; }
-
-// Fills the line; a sequence outside its cache has no units. All threads of the block; a warp does it. (Loads from L2: the merging kernel comes here in front of
-// its wait.)
+// A sequence has kv_heads * tiles problems of `blocks` units each.
+// A sequence's rows and its units: none if it lies outside its cache. (Loads from L2: the merging kernel comes here in front of its wait.)
+template <int ROWS, int KEYS>
+__device__ __forceinline__ int line_units(const TreeParams &p, int seq, int &pos, int &count) {
+    pos = count = 0;
+    if (seq >= p.b) return 0;
+    pos = __ldcg(p.pos + seq);
+    count = p.counts ? min(max(__ldcg(p.counts + seq), 0), p.t) : p.t;
+    if (pos < 0 || pos > p.cap - count) {
+        if (blockIdx.x == 0) atomicExch(p.err_word, kErrPos);
+        count = 0;
+    }
+    return count ? (pos + count + KEYS - 1) / KEYS * ((count * p.group + ROWS - 1) / ROWS) * p.kvh : 0;
+}
+__device__ __forceinline__ int sum_up_to(int mine, int lane) {  // over the lanes
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, mine, o);
+        if (lane >= o) mine += up;
+    }
+    return mine;
+}
+// Fills the line. All threads of the block; a warp does it.
 template <int ROWS, int KEYS>
 __device__ __forceinline__ void cut_line(const TreeParams &p, Line &l) {
     if (threadIdx.x < 32) {
@@ -95,22 +113,8 @@ __device__ __forceinline__ void cut_line(const TreeParams &p, Line &l) {
         int before = 0;
         for (int i0 = 0; i0 < p.b; i0 += 32) {
             const int i = i0 + lane;
-            int pos = 0, count = 0;
-            if (i < p.b) {
-                pos = __ldcg(p.pos + i);
-                count = p.counts ? min(max(__ldcg(p.counts + i), 0), p.t) : p.t;
-            }
-            if (pos < 0 || pos > p.cap - count) {
-                if (blockIdx.x == 0) atomicExch(p.err_word, kErrPos);
-                count = 0;
-            }
-            const int mine = count ? (pos + count + KEYS - 1) / KEYS * ((count * p.group + ROWS - 1) / ROWS) * p.kvh : 0;
-            int sum = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += up;
-            }
+            int pos, count;
+            const int mine = line_units<ROWS, KEYS>(p, i, pos, count), sum = sum_up_to(mine, lane);
             if (i < p.b) {
                 l.pos[i] = pos;
                 l.count[i] = count;
@@ -122,10 +126,19 @@ __device__ __forceinline__ void cut_line(const TreeParams &p, Line &l) {
     }
     __syncthreads();
 }
+// a / b for 0 <= a and 0 < b, whose quotient is below 2^20: the approximate one is off by one at most
+__device__ __forceinline__ int quotient(int a, int b) {
+    const int q = static_cast<int>(__fdividef(static_cast<float>(a), static_cast<float>(b))), r = a - q * b;
+    return q + (r >= b) - (r < 0);
+}
 // Worker w takes the units share_begin(w) .. share_begin(w + 1) - 1: `each` of them, one more the first `more` workers.
 struct Shares {
     int each, more;
-    __device__ __forceinline__ Shares(int units, int workers) : each(units / workers), more(units - units / workers * workers) {}
+    __device__ __forceinline__ Shares(int units, const TreeParams &p) {
+        each = static_cast<int>(__umulhi(static_cast<unsigned>(units), p.per_worker));  // or one less
+        each += units - each * p.workers >= p.workers;
+        more = units - each * p.workers;
+    }
     __device__ __forceinline__ int begin(int w) const { return w * each + min(w, more); }
     __device__ __forceinline__ int owner(int u) const { return u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each; }
 };
@@ -134,22 +147,67 @@ struct Segment {
     int seq, kh, tile;     // the problem
     int begin, end;        // its blocks
     int blocks;            // of all there are
+    int pos, count;        // of the sequence
 };
-__device__ __forceinline__ Segment segment_at(const TreeParams &p, const Line &l, int unit, int last, int rows, int keys) {
+// The blocks of a problem from `unit` on, which lies `at` units into the sequence; a share ends in front of `last`
+__device__ __forceinline__ Segment segment_in(const TreeParams &p, int seq, int pos, int count, int unit, int at, int last, int rows, int keys) {
     Segment s;
+    s.seq = seq;
+    s.pos = pos;
+    s.count = count;
+    s.blocks = (pos + count + keys - 1) / keys;
+    const int tiles = (count * p.group + rows - 1) / rows, problem = quotient(at, s.blocks);
+    s.begin = at - problem * s.blocks;
+    s.end = min(s.blocks, s.begin + last - unit);
+    s.kh = quotient(problem, tiles);
+    s.tile = problem - s.kh * tiles;
+    return s;
+}
+__device__ __forceinline__ Segment segment_at(const TreeParams &p, const Line &l, int unit, int last, int rows, int keys) {
     int lo = 0, hi = p.b - 1;   // the last sequence whose units begin at or before this one and that has any
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (l.first[mid] <= unit) lo = mid;
         else hi = mid - 1;
     }
-    s.seq = lo;
-    s.blocks = line_blocks(l, lo, keys);
-    const int tiles = line_tiles(l, lo, p.group, rows), at = unit - l.first[lo], problem = at / s.blocks;
-    s.begin = at - problem * s.blocks;
-    s.end = min(s.blocks, s.begin + last - unit);
-    s.kh = problem / tiles;
-    s.tile = problem - s.kh * tiles;
+    return segment_in(p, lo, l.pos[lo], l.count[lo], unit, unit - l.first[lo], last, rows, keys);
+}
+// A block's units u0 .. u1 - 1, and the first segment of them. Up to 32 sequences every warp finds it by itself, without a meeting, from one load: in front of the first
+// query everything waits for this. Warp 0 leaves the line for the other segments; who looks for those has met it or waited for its queries since.
+struct Share {
+    int u0, u1;
+    Segment first;
+};
+template <int ROWS, int KEYS>
+__device__ __forceinline__ Share own_share(const TreeParams &p, Line &l) {
+    Share s{};
+    if (p.b > 32) {
+        cut_line<ROWS, KEYS>(p, l);
+        const Shares shares(l.first[p.b], p);
+        s.u0 = shares.begin(blockIdx.x);
+        s.u1 = shares.begin(blockIdx.x + 1);
+        if (s.u0 < s.u1) s.first = segment_at(p, l, s.u0, s.u1, ROWS, KEYS);
+        return s;
+    }
+    const int lane = threadIdx.x & 31;
+    int pos, count;
+    const int mine = line_units<ROWS, KEYS>(p, lane, pos, count), sum = sum_up_to(mine, lane), first = sum - mine, all = __shfl_sync(0xffffffffu, sum, 31);
+    const Shares shares(all, p);
+    s.u0 = shares.begin(blockIdx.x);
+    s.u1 = shares.begin(blockIdx.x + 1);
+    const unsigned has = __ballot_sync(0xffffffffu, mine && first <= s.u0);  // the last one of these
+    if (s.u0 < s.u1) {
+        const int seq = 31 - __clz(has);
+        s.first = segment_in(p, seq, __shfl_sync(0xffffffffu, pos, seq), __shfl_sync(0xffffffffu, count, seq), s.u0, s.u0 - __shfl_sync(0xffffffffu, first, seq), s.u1, ROWS, KEYS);
+    }
+    if (threadIdx.x < 32) {
+        if (lane < p.b) {
+            l.pos[lane] = pos;
+            l.count[lane] = count;
+            l.first[lane] = first;
+        }
+        if (lane == 0) l.first[p.b] = all;
+    }
     return s;
 }
 
@@ -197,6 +255,7 @@ __device__ __forceinline__ bool sees(const ulonglong2 &m, int n) { return ((n < 
 
 struct CtaShared {
     Line line;
+    Segment seg[20];   // a warp's present one: eight registers that the loop over its blocks has no room for
     int parent[kTreeNodes];
     ulonglong2 mask[kTreeNodes];
     int abort, odd;
@@ -232,14 +291,14 @@ __device__ __forceinline__ bool clean_values(uint4 *v, int units, bool all) {
 constexpr int kQueriesAsked = 8;  // named barrier
 // A producer warp of a kernel with layout M: the K blocks, or the V pieces, of a share. full, empty: the first of the stages' barriers.
 template <class M>
-__device__ __forceinline__ void produce(const TreeParams &p, const Line &line, int u0, int u1, int rows, bool is_k, uint32_t base, uint32_t full, uint32_t empty, volatile int *abort, bool &ok) {
+__device__ __forceinline__ void produce(const TreeParams &p, const Line &line, const Share &share, int rows, bool is_k, uint32_t base, uint32_t full, uint32_t empty, volatile int *abort, bool &ok) {
     // The first queries go first: behind 128 KB of keys and values an SM, which all ask for at the same time, they took 3000 to 6000 cycles
     ptx::named_barrier(kQueriesAsked, M::kSoftWarps * 32 + 64);
     if ((threadIdx.x & 31) != 0) return;
     const int stages = is_k ? M::kKStages : M::kVStages;
     int stage = 0, round = 0, sent = 0;
-    for (int u = u0; u < u1 && ok;) {
-        const Segment s = segment_at(p, line, u, u1, rows, M::kKeys);
+    Segment s = share.first;
+    for (int u = share.u0; u < share.u1 && ok;) {
         const int row0 = (s.seq * p.kvh + s.kh) * p.cap;
         for (int i = is_k ? s.begin : 2 * s.begin; i < (is_k ? s.end : 2 * s.end); ++i, ++sent) {
             if (round > 0 && !tc::wait_bar(empty + stage * 8, (round - 1) & 1, abort)) {
@@ -256,6 +315,7 @@ __device__ __forceinline__ void produce(const TreeParams &p, const Line &line, i
             }
         }
         u += s.end - s.begin;
+        if (u < share.u1) s = segment_at(p, line, u, share.u1, rows, M::kKeys);
     }
     // the copies in flight land before the block may go, whoever has given up
     for (int n = max(0, sent - stages); n < sent; ++n) ptx::mbar_wait(full + n % stages * 8, (n / stages) & 1, tc::kTcWaitLimit);
@@ -339,13 +399,13 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
         tc::tmem_relinquish();
     }
     tc::tc_fence_before();
-    ptx::pdl_wait();
-    ptx::pdl_trigger();  // behind the wait: what the merging kernel reads in front of its own is settled then
-    cut_line<ROWS, M::kKeys>(p, sh.line);
+    __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = *static_cast<volatile uint32_t *>(&sh.tmem);
-    const Shares shares(sh.line.first[p.b], p.workers);
-    const int u0 = shares.begin(blockIdx.x), u1 = shares.begin(blockIdx.x + 1);
+    ptx::pdl_wait();
+    ptx::pdl_trigger();  // behind the wait: what the merging kernel reads in front of its own is settled then
+    const Share share = own_share<ROWS, M::kKeys>(p, sh.line);
+    const int u0 = share.u0, u1 = share.u1;
     if (u0 == u1) {
         if (warp == M::kMmaWarp) tc::tmem_dealloc(tmem, M::kTmem);
         return;
@@ -358,7 +418,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
     };
 
     if (warp == M::kKWarp || warp == M::kVWarp) {
-        produce<M>(p, sh.line, u0, u1, ROWS, warp == M::kKWarp, base, bar(warp == M::kKWarp ? kKFull : kVFull), bar(warp == M::kKWarp ? kKEmpty : kVEmpty), abort, ok);
+        produce<M>(p, sh.line, share, ROWS, warp == M::kKWarp, base, bar(warp == M::kKWarp ? kKFull : kVFull), bar(warp == M::kKWarp ? kKEmpty : kVEmpty), abort, ok);
     } else if (warp == M::kMmaWarp) {
         // ================= MMA issue: the warp walks, one lane issues =================
         // D f32, A and B bf16, M = 128, N = terms * rows; for O^T A is MN-major (bit 15)
@@ -383,8 +443,8 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
                 kphase ^= 1;
             }
         };
+        Segment s = share.first;
         for (int u = u0; u < u1 && ok; ++seg) {
-            const Segment s = segment_at(p, sh.line, u, u1, ROWS, M::kKeys);
             const int blocks = s.end - s.begin;
             if (wait(kQFull, seg & 1)) scores();
             for (int j = 0; j < blocks && ok; ++j, ++n) {
@@ -412,6 +472,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
                 }
             }
             u += blocks;
+            if (u < u1) s = segment_at(p, sh.line, u, u1, ROWS, M::kKeys);
         }
     } else {
         // ================= softmax =================
@@ -430,9 +491,9 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
         uint8_t *const p_at = sm + M::kP0 + (key >> 6) * M::kOpHalf + (key & 7) * 2;
         const int p_unit = (key >> 3) & 7;
         int n = 0;  // blocks so far, over all segments
+        Segment s = share.first;
         for (int u = u0; u < u1;) {
-            const Segment s = segment_at(p, sh.line, u, u1, ROWS, M::kKeys);
-            const int pos = sh.line.pos[s.seq], count = sh.line.count[s.seq], rows_all = count * group, row0 = s.tile * ROWS;
+            const int pos = s.pos, count = s.count, rows_all = count * group, row0 = s.tile * ROWS;
             const bool nodes = s.end * M::kKeys > pos;  // some blocks hold nodes
             meet();  // nobody reads what the last segment left in the tree's place any more
             // the tile's queries, a row as one load of a warp, all of them asked for before the first is looked at
@@ -600,6 +661,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
                 }
             }
             u += s.end - s.begin;
+            if (u < u1) s = segment_at(p, sh.line, u, u1, ROWS, M::kKeys);
         }
     }
     if (!ok && lane == 0) atomicExch(p.err_word, 5);
@@ -669,13 +731,13 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
         tc::tmem_relinquish();
     }
     tc::tc_fence_before();
-    ptx::pdl_wait();
-    ptx::pdl_trigger();  // behind the wait: what the merging kernel reads in front of its own is settled then
-    cut_line<M::kRows, M::kKeys>(p, sh.line);
+    __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = *static_cast<volatile uint32_t *>(&sh.tmem);
-    const Shares shares(sh.line.first[p.b], p.workers);
-    const int u0 = shares.begin(blockIdx.x), u1 = shares.begin(blockIdx.x + 1);
+    ptx::pdl_wait();
+    ptx::pdl_trigger();  // behind the wait: what the merging kernel reads in front of its own is settled then
+    const Share share = own_share<M::kRows, M::kKeys>(p, sh.line);
+    const int u0 = share.u0, u1 = share.u1;
     if (u0 == u1) {
         if (warp == M::kMmaWarp) tc::tmem_dealloc(tmem, 512);
         return;
@@ -687,7 +749,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
     if (warp >= M::kSoftWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == M::kKWarp || warp == M::kVWarp) {
-            produce<M>(p, sh.line, u0, u1, M::kRows, warp == M::kKWarp, base, bar(warp == M::kKWarp ? kKFull : kVFull), bar(warp == M::kKWarp ? kKEmpty : kVEmpty), abort, ok);
+            produce<M>(p, sh.line, share, M::kRows, warp == M::kKWarp, base, bar(warp == M::kKWarp ? kKFull : kVFull), bar(warp == M::kKWarp ? kKEmpty : kVEmpty), abort, ok);
         } else if (warp == M::kMmaWarp) {
             // ================= MMA issue: the warp walks, one lane issues =================
             // D f32, A and B bf16, M = 128, N = 128; for P V the B operand is MN-major (bit 16)
@@ -720,8 +782,8 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                     kphase ^= 1;
                 }
             };
+            Segment s = share.first;
             for (int u = u0; u < u1 && ok; ++seg) {
-                const Segment s = segment_at(p, sh.line, u, u1, M::kRows, M::kKeys);
                 const int blocks = s.end - s.begin;
                 if (wait(kQFull, seg & 1)) scores();
                 // Products are carried out in the order they are asked for: the scores of block j + 1 go where the probabilities of block j - 1 were read from
@@ -753,6 +815,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                     if (ok && j + 2 < blocks) scores();
                 }
                 u += blocks;
+                if (u < u1) s = segment_at(p, sh.line, u, u1, M::kRows, M::kKeys);
             }
         }
     } else {
@@ -773,9 +836,11 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
         auto queries_asked = [&]() { asm volatile("barrier.cta.arrive %0, %1;" ::"r"(kQueriesAsked), "r"(M::kSoftWarps * 32 + 64) : "memory"); };
         auto quad_sync = [&]() { ptx::named_barrier(2 + quad, 128); };  // the four warps of a quadrant
         int n = 0;  // blocks so far, over all segments
+        if (lane == 0) sh.seg[warp] = share.first;
+        __syncwarp();
         for (int u = u0; u < u1;) {
-            const Segment s = segment_at(p, sh.line, u, u1, M::kRows, M::kKeys);
-            const int pos = sh.line.pos[s.seq], count = sh.line.count[s.seq];
+            const Segment s = sh.seg[warp];
+            const int pos = s.pos, count = s.count;
             const int rows_all = count * group, row0 = s.tile * M::kRows, row = row0 + r, node = p.node_of(row);
             const bool nodes = s.end * M::kKeys > pos, live = row0 + quad * 32 < rows_all;  // some blocks hold nodes; some row of the warp exists
             meet();  // nobody reads what the last segment left in the queries' place and in the tree's any more
@@ -946,6 +1011,11 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                 }
             }
             u += s.end - s.begin;
+            if (u < u1) {
+                const Segment next = segment_at(p, sh.line, u, u1, M::kRows, M::kKeys);
+                if (lane == 0) sh.seg[warp] = next;
+                __syncwarp();
+            }
         }
     }
     if (!ok && lane == 0) atomicExch(p.err_word, 5);
@@ -969,7 +1039,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) attn_tree_merge_kernel(const
     __shared__ float2 s_ml[kMergeWarps];
     ptx::pdl_trigger();
     cut_line<ROWS, KEYS>(p, line);
-    const Shares shares(line.first[p.b], p.workers);
+    const Shares shares(line.first[p.b], p);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = p.group, c0 = blockIdx.x;
     const int u0 = shares.begin(c0), u1 = shares.begin(c0 + 1);
     Segment s{};
@@ -977,7 +1047,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) attn_tree_merge_kernel(const
     if (u0 < u1) {
         s = segment_at(p, line, u1 - 1, u1, ROWS, KEYS);  // the last block of the share
         begin = u1 - 1 - s.begin;
-        rows = min(ROWS, line.count[s.seq] * group - s.tile * ROWS);
+        rows = min(ROWS, s.count * group - s.tile * ROWS);
         const int end = begin + s.blocks;
         if (begin >= u0 && end > u1) parts = shares.owner(end - 1) - c0 + 1;  // neighbours that all have a share: this tile goes on in it
     }
@@ -1121,6 +1191,7 @@ int lbk_attn_tree(lbk_ctx *c, int compute, const void *q_dev, size_t q_pitch, co
     p.cap = static_cast<int>(cap);
     p.scale = scale * 1.4426950408889634f;
     p.workers = ctx->sm_count;
+    p.per_worker = static_cast<unsigned>(std::min<unsigned long long>((1ull << 32) / static_cast<unsigned>(p.workers), 0xffffffffu));
     p.per_group = group > 1 ? static_cast<unsigned>((0x100000000ull + group - 1) / group) : 0u;  // exact: rows * heads of a group < 2^32
     p.err_word = ctx->err_word;
     const int tile = tile_rows(t, group);

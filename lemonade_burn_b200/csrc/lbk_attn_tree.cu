@@ -1027,47 +1027,79 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
     }
 }
 
-// Joins the parts of the tiles that were cut. kMergeBlocks blocks share the tile that begins in a worker's share and ends behind it, if there is one. Two or three parts, as
-// a rule: a warp a row; more than two batches of them (up to 148 of one sequence's one tile): four warps a row, which take every fourth part. Four dimensions a lane. Small
-// blocks, all of them beside one another: each has to find its tile first, and beside the attention kernel's blocks there are no registers for these. (us for 1 x 5 nodes, 4001
-// keys, 5 tiles of 32 parts, and 1 x 60 nodes, 65000 keys, 16 of 9: one block of 32 warps a tile 24.8 and 162, blocks of 16 warps in four waves 16.5 and 108.)
-constexpr int kMergeWarps = 4, kMergeBlocks = 8, kAtOnce = 8;
+// Joins the parts of the tiles that were cut. Every block lists them, a thread a worker: the tile that begins in its share and ends behind it, if there is one. Their rows are
+// cut evenly among the warps, a warp a row, or, of few rows, 2, 4 or 8 warps, which take every 2nd, 4th or 8th part of it; four dimensions a lane. (us in f32 against
+// eight blocks for each worker, most of which had no tile: 1 x 5 nodes of 4001 keys 16.8 -> 12.8, 1 x 60 of 2000 keys, 16 tiles in 10 parts, 40.7 -> 25.4, 16 x 64 of 300 keys 34.4 -> 29.9.)
+constexpr int kMergeWarps = 8, kMergeAtOnce = 4, kMergeBlocks = 4;  // parts on their way; blocks an SM
+constexpr int kMaxWorkers = kMergeWarps * 32;
 template <int TERMS, int ROWS, int KEYS>
-__global__ void __launch_bounds__(kMergeWarps * 32) attn_tree_merge_kernel(const __grid_constant__ TreeParams p) {
+__global__ void __launch_bounds__(kMergeWarps * 32, kMergeBlocks) attn_tree_merge_kernel(const __grid_constant__ TreeParams p) {
     __shared__ Line line;
+    __shared__ int s_first[kMaxWorkers];   // rows in front of a worker's tile
+    __shared__ int4 s_tile[kMaxWorkers];   // sequence, KV head, tile, parts; negative: the first part is its worker's second
+    __shared__ int s_warp[kMergeWarps], s_most[kMergeWarps];
     __shared__ float4 s_sum[kMergeWarps][32];
     __shared__ float2 s_ml[kMergeWarps];
     ptx::pdl_trigger();
     cut_line<ROWS, KEYS>(p, line);
-    const Shares shares(line.first[p.b], p);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = p.group, c0 = blockIdx.x;
-    const int u0 = shares.begin(c0), u1 = shares.begin(c0 + 1);
-    Segment s{};
-    int begin = 0, parts = 0, rows = 0;
-    if (u0 < u1) {
-        s = segment_at(p, line, u1 - 1, u1, ROWS, KEYS);  // the last block of the share
-        begin = u1 - 1 - s.begin;
-        rows = min(ROWS, s.count * group - s.tile * ROWS);
-        const int end = begin + s.blocks;
-        if (begin >= u0 && end > u1) parts = shares.owner(end - 1) - c0 + 1;  // neighbours that all have a share: this tile goes on in it
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = p.group;
+    {
+        const Shares shares(line.first[p.b], p);
+        const int u0 = shares.begin(tid), u1 = tid < p.workers ? shares.begin(tid + 1) : u0;
+        int rows = 0, parts = 0;
+        if (u0 < u1) {
+            const Segment s = segment_at(p, line, u1 - 1, u1, ROWS, KEYS);  // the last block of the share
+            const int begin = u1 - 1 - s.begin, end = begin + s.blocks;
+            if (begin >= u0 && end > u1) {
+                parts = shares.owner(end - 1) - tid + 1;  // neighbours that all have a share: this tile goes on in it
+                rows = min(ROWS, s.count * group - s.tile * ROWS);
+                s_tile[tid] = make_int4(s.seq, s.kh, s.tile, u0 < begin ? -parts : parts);
+            }
+        }
+        const int sum = sum_up_to(rows, lane);
+        const int most = __reduce_max_sync(0xffffffffu, parts);
+        if (lane == 31) {
+            s_warp[warp] = sum;
+            s_most[warp] = most;
+        }
+        __syncthreads();
+        int before = 0;
+        for (int w = 0; w < warp; ++w) before += s_warp[w];
+        s_first[tid] = before + sum - rows;
     }
-    ptx::pdl_wait();  // blocks without a tile too: the next kernel of the stream waits for this one only
-    if (!parts) return;
-    const int splits = parts <= 2 * kAtOnce ? 1 : 4, split = warp & (splits - 1);
-    constexpr int kShare = ROWS / kMergeBlocks;
-    const int r1 = min(rows, static_cast<int>(blockIdx.y + 1) * kShare);
-    for (int r0 = blockIdx.y * kShare; r0 < r1; r0 += kMergeWarps / splits) {
-        const int r = r0 + warp / splits;
+    int all = 0, most = 0;
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; ++w) {
+        all += s_warp[w];
+        most = max(most, s_most[w]);
+    }
+    __syncthreads();
+    int splits = kMergeWarps;
+    while (splits > 1 && (all * splits > static_cast<int>(gridDim.x) * kMergeWarps || splits * kMergeAtOnce >= 2 * most)) splits >>= 1;
+    const int split = warp & (splits - 1), each = kMergeWarps / splits;
+    auto worker_of = [&](int index) {  // the last one with `index` rows or fewer in front of its tile
+        int c = 0;
+#pragma unroll
+        for (int step = kMaxWorkers / 2; step > 0; step >>= 1)
+            if (s_first[c + step] <= index) c += step;
+        return c;
+    };
+    int index = blockIdx.x * each + warp / splits, c0 = worker_of(index);
+    ptx::pdl_wait();  // blocks without a row too: the next kernel of the stream waits for this one only
+    for (int r0 = blockIdx.x * each; r0 < all; r0 += gridDim.x * each, index += gridDim.x * each, c0 = worker_of(index)) {
+        const int r = index - s_first[c0];
+        const int4 tile = s_tile[c0];
+        const int parts = index < all ? abs(tile.w) : 0;
         // part i is the first of its worker's two, but the tile's own first part is the second where the worker came from another tile
-        auto place = [&](int i) { return (static_cast<size_t>(c0 + i) * 2 + (i == 0 && u0 < begin ? 1 : 0)) * ROWS + r; };
+        auto place = [&](int i) { return (static_cast<size_t>(c0 + i) * 2 + (i == 0 && tile.w < 0 ? 1 : 0)) * ROWS + r; };
         float m = kNoMax, l = 0.0f;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = split; i0 < (r < r1 ? parts : 0); i0 += splits * kAtOnce) {
-            float2 ml[kAtOnce];
-            float4 x[kAtOnce];
+        for (int i0 = split; i0 < parts; i0 += splits * kMergeAtOnce) {
+            float2 ml[kMergeAtOnce];
+            float4 x[kMergeAtOnce];
             float up = m;
 #pragma unroll
-            for (int e = 0; e < kAtOnce; ++e) {
+            for (int e = 0; e < kMergeAtOnce; ++e) {
                 const int i = i0 + e * splits;
                 ml[e] = make_float2(kNoMax, 0.0f);
                 x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1077,13 +1109,13 @@ __global__ void __launch_bounds__(kMergeWarps * 32) attn_tree_merge_kernel(const
                 }
             }
 #pragma unroll
-            for (int e = 0; e < kAtOnce; ++e) up = fmaxf(up, ml[e].x);
+            for (int e = 0; e < kMergeAtOnce; ++e) up = fmaxf(up, ml[e].x);
             const float corr = ex2(m - up);
             m = up;
             l *= corr;
             sum = make_float4(sum.x * corr, sum.y * corr, sum.z * corr, sum.w * corr);
 #pragma unroll
-            for (int e = 0; e < kAtOnce; ++e) {
+            for (int e = 0; e < kMergeAtOnce; ++e) {
                 const float w = ex2(ml[e].x - m);
                 l += ml[e].y * w;
                 sum.x += x[e].x * w;
@@ -1097,8 +1129,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) attn_tree_merge_kernel(const
             if (lane == 0) s_ml[warp] = make_float2(m, l);
             __syncthreads();
             if (!split)
-#pragma unroll
-                for (int e = 1; e < 4; ++e) {
+                for (int e = 1; e < splits; ++e) {
                     const float2 ml = s_ml[warp + e];
                     const float4 x = s_sum[warp + e][lane];
                     const float up = fmaxf(m, ml.x), corr = ex2(m - up), w = ex2(ml.x - up);
@@ -1108,10 +1139,10 @@ __global__ void __launch_bounds__(kMergeWarps * 32) attn_tree_merge_kernel(const
                 }
             __syncthreads();
         }
-        if (split || r >= r1) continue;
-        const int row = s.tile * ROWS + r, node = p.node_of(row);
+        if (split || !parts) continue;
+        const int row = tile.z * ROWS + r, node = p.node_of(row);
         const float inv = 1.0f / l;
-        const size_t at = (static_cast<size_t>(s.seq) * p.t + node) * p.out_pitch + static_cast<size_t>(s.kh * group + row - node * group) * kHd + lane * 4;
+        const size_t at = (static_cast<size_t>(tile.x) * p.t + node) * p.out_pitch + static_cast<size_t>(tile.y * group + row - node * group) * kHd + lane * 4;
         dense::put4(static_cast<std::conditional_t<(TERMS > 1), float, uint16_t> *>(p.out) + at, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
     }
 }
@@ -1135,7 +1166,7 @@ int launch_tree(Ctx *ctx, TreeParams &p, cudaStream_t st) {
     if (ROWS <= 32) LBK_CUDA(launch_chained(attn_tree_turned_kernel<TERMS, ROWS <= 32 ? ROWS : 16>, dim3(static_cast<unsigned>(p.workers)), dim3(T::kThreads), static_cast<size_t>(T::kSmem), st, p));
     else LBK_CUDA(launch_chained(attn_tree_many_kernel<TERMS>, dim3(static_cast<unsigned>(p.workers)), dim3(M::kThreads), static_cast<size_t>(M::kSmem), st, p));
     ctx->launches++;
-    LBK_CUDA(launch_chained(attn_tree_merge_kernel<TERMS, ROWS, 128>, dim3(static_cast<unsigned>(p.workers), kMergeBlocks), dim3(kMergeWarps * 32), 0, st, p));
+    LBK_CUDA(launch_chained(attn_tree_merge_kernel<TERMS, ROWS, 128>, dim3(static_cast<unsigned>(std::min<size_t>(static_cast<size_t>(kMergeBlocks) * ctx->sm_count, static_cast<size_t>(p.b) * p.t * p.kvh * p.group))), dim3(kMergeWarps * 32), 0, st, p));
     ctx->launches++;
     return LBK_OK;
 }
@@ -1190,7 +1221,7 @@ int lbk_attn_tree(lbk_ctx *c, int compute, const void *q_dev, size_t q_pitch, co
     p.kvh = static_cast<int>(kv_heads);
     p.cap = static_cast<int>(cap);
     p.scale = scale * 1.4426950408889634f;
-    p.workers = ctx->sm_count;
+    p.workers = std::min(ctx->sm_count, kMaxWorkers);
     p.per_worker = static_cast<unsigned>(std::min<unsigned long long>((1ull << 32) / static_cast<unsigned>(p.workers), 0xffffffffu));
     p.per_group = group > 1 ? static_cast<unsigned>((0x100000000ull + group - 1) / group) : 0u;  // exact: rows * heads of a group < 2^32
     p.err_word = ctx->err_word;

@@ -332,7 +332,8 @@ __device__ __forceinline__ void produce(const TreeParams &p, const Line &line, c
 // (and the sums with it) when some score is over it by more than kSlack.
 //
 //   8 softmax warps  warp w and w + 4: the quadrant of 32 lanes w % 4, the first and the second half of the rows
-//   K, V producers, MMA warp  as below: Q K^T of block j + 1 as soon as the scores of block j have been read, then P V of block j
+//   K, V producers, MMA warp  as below, but one MMA warp: Q K^T of block j + 1 as soon as the scores of block j have been read, then P V of block j (two warps: 40.1 -> 43.7
+//                             us for 6 nodes of 65000 keys)
 constexpr float kSlack = 8.0f;  // in units of log 2: probabilities stay below 2^8
 template <int TERMS, int ROWS>
 struct Turned {
@@ -682,7 +683,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
 //                    warps with 64 took 5900 cycles a block in three terms where the products take some 3100: two warps a scheduler do not hide their latencies)
 //   K, V producers   a warp each: K blocks of 128 keys are free again after the scores, V in pieces of 64 keys after their product, and one order for
 //                    both would have the next K block wait for a piece of V
-//   MMA warp         P V of block j - 1, then Q K^T of block j + 1, while the softmax warps work on block j
+//   MMA warps        one for P V of block j - 1, one for Q K^T of block j + 1, while the softmax warps work on block j
 //
 // 512 bytes a key from HBM are 22 cycles of an SM, its products for 128 rows 24 in three terms and 8 in one: f32 is bound by the tensor core, bf16 by
 // the stream and by the softmax warps (an exponential per row and key). Padding rows cost nothing but the products: their warps only keep step.
@@ -693,7 +694,7 @@ struct Many {
     static constexpr int kKStages = TERMS == 3 ? 2 : 3, kVStages = TERMS == 3 ? 3 : 5;
     static constexpr int kK0 = TERMS * 2 * kHalf, kV0 = kK0 + kKStages * kKBytes, kBars = kV0 + kVStages * kPieceBytes;
     static constexpr int kPair = kBars + 256, kSmem = kPair + 2 * 4 * kRows * 4 + 1024;
-    static constexpr int kSoftWarps = 16, kKWarp = 16, kVWarp = 17, kMmaWarp = 18, kThreads = 20 * 32;
+    static constexpr int kSoftWarps = 16, kKWarp = 16, kVWarp = 17, kScoreWarp = 18, kThreads = 20 * 32;  // the last one: products
     // bf16: the products are summed up in tensor memory, over all blocks, and m is moved as for few rows, with the sums, when a score is over it by kSlack. What the tensor
     // core cuts off of a long sum (1e-5 at 8000 keys) does not show in a bf16 result, and a block needs no look at the products of the one in front.
     static constexpr bool kStays = TERMS == 1;
@@ -726,7 +727,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
         sh.abort = sh.odd = 0;
         ptx::fence_barrier_init();
     }
-    if (warp == M::kMmaWarp) {
+    if (warp == M::kScoreWarp) {
         tc::tmem_alloc(ptx::smem_u32(&sh.tmem), 512);
         tc::tmem_relinquish();
     }
@@ -739,7 +740,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
     const Share share = own_share<M::kRows, M::kKeys>(p, sh.line);
     const int u0 = share.u0, u1 = share.u1;
     if (u0 == u1) {
-        if (warp == M::kMmaWarp) tc::tmem_dealloc(tmem, 512);
+        if (warp == M::kScoreWarp) tc::tmem_dealloc(tmem, 512);
         return;
     }
     const int group = p.group;
@@ -750,69 +751,68 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == M::kKWarp || warp == M::kVWarp) {
             produce<M>(p, sh.line, share, M::kRows, warp == M::kKWarp, base, bar(warp == M::kKWarp ? kKFull : kVFull), bar(warp == M::kKWarp ? kKEmpty : kVEmpty), abort, ok);
-        } else if (warp == M::kMmaWarp) {
-            // ================= MMA issue: the warp walks, one lane issues =================
+        } else {
+            // ================= MMA issue, scores by one warp, products by another: the warps walk, one lane of each issues =================
+            // A turn of a wait, products and a commit costs a warp some 400 cycles beside its products, in which those of the other go on: one warp for both took 214 us for
+            // 16 x 64 nodes of 8100 keys in f32 where these take 207, and 100 where these take 97 for 60 nodes of 65000 in bf16
             // D f32, A and B bf16, M = 128, N = 128; for P V the B operand is MN-major (bit 16)
             constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24), idesc_o = idesc_s | (1u << 16);
-            const uint64_t q_desc = tc::smem_desc_sw128(base);
-            int ks = 0, kphase = 0, vs = 0, vphase = 0, n = 0, seg = 0;  // n: blocks whose scores have been asked for
             auto wait = [&](int i, int parity) {
                 if (ok) ok = look_and_wait(bar(i), parity, abort);
                 return ok;
             };
-            auto scores = [&]() {
-                if (!wait(kKFull + ks, kphase)) return;
-                tc::tc_fence_after();
-                if (tc::elect_one()) {
-                    const uint64_t k_desc = tc::smem_desc_sw128(base + M::kK0 + ks * M::kKBytes);
-#pragma unroll 1
-                    for (int x = TERMS - 1; x >= 0; --x)  // the small ones first
-#pragma unroll
-                        for (int st = 0; st < 8; ++st) {
-                            const uint64_t off = static_cast<uint64_t>((st >> 2) * (M::kHalf >> 4) + (st & 3) * 2);
-                            tc::umma_f16_ss(tmem + (n & 1) * M::kPlace, q_desc + static_cast<uint64_t>(x * 2 * (M::kHalf >> 4)) + off, k_desc + off, idesc_s, x < TERMS - 1 || st ? 1u : 0u);
-                        }
-                    tc::umma_commit(bar(kSFull + (n & 1)));
-                    tc::umma_commit(bar(kKEmpty + ks));
-                }
-                __syncwarp();
-                ++n;
-                if (++ks == M::kKStages) {
-                    ks = 0;
-                    kphase ^= 1;
-                }
-            };
+            const uint64_t q_desc = tc::smem_desc_sw128(base);
+            const bool scores = warp == M::kScoreWarp;
+            int stage = 0, phase = 0, n = 0, seg = 0;  // of K or of V; n: the block, in the whole walk
             Segment s = share.first;
             for (int u = u0; u < u1 && ok; ++seg) {
                 const int blocks = s.end - s.begin;
-                if (wait(kQFull, seg & 1)) scores();
-                // Products are carried out in the order they are asked for: the scores of block j + 1 go where the probabilities of block j - 1 were read from
-                if (ok && blocks > 1) scores();
-                for (int j = 0; j < blocks && ok; ++j) {
-                    const int done = n - (j + 1 < blocks ? 2 : 1);  // the number, in the whole walk, of block j
-                    if (!wait(kPReady + (done & 1), done >> 1 & 1)) break;
-#pragma unroll 1
-                    for (int piece = 0; piece < 2; ++piece) {
-                        if (!wait(kVFull + vs, vphase)) break;
+                if (scores) wait(kQFull, seg & 1);
+                for (int j = 0; j < blocks && ok; ++j, ++n) {
+                    if (scores) {
+                        // the place of this block's scores: the probabilities of the block but one in front of it have been read (the last segment's all)
+                        if (!wait(kKFull + stage, phase) || (j >= 2 && !wait(kOFull + (n & 1), (n - 2) >> 1 & 1))) break;
                         tc::tc_fence_after();
                         if (tc::elect_one()) {
-                            const uint64_t v_desc = desc_mn_sw128(base + M::kV0 + vs * M::kPieceBytes, M::kPieceHalf);
+                            const uint64_t k_desc = tc::smem_desc_sw128(base + M::kK0 + stage * M::kKBytes);
+#pragma unroll 1
+                            for (int x = TERMS - 1; x >= 0; --x)  // the small ones first
+#pragma unroll
+                                for (int st = 0; st < 8; ++st) {
+                                    const uint64_t off = static_cast<uint64_t>((st >> 2) * (M::kHalf >> 4) + (st & 3) * 2);
+                                    tc::umma_f16_ss(tmem + (n & 1) * M::kPlace, q_desc + static_cast<uint64_t>(x * 2 * (M::kHalf >> 4)) + off, k_desc + off, idesc_s, x < TERMS - 1 || st ? 1u : 0u);
+                                }
+                            tc::umma_commit(bar(kSFull + (n & 1)));
+                            tc::umma_commit(bar(kKEmpty + stage));
+                        }
+                        __syncwarp();
+                        if (++stage == M::kKStages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                        continue;
+                    }
+                    if (!wait(kPReady + (n & 1), n >> 1 & 1)) break;
+#pragma unroll 1
+                    for (int piece = 0; piece < 2; ++piece) {
+                        if (!wait(kVFull + stage, phase)) break;
+                        tc::tc_fence_after();
+                        if (tc::elect_one()) {
+                            const uint64_t v_desc = desc_mn_sw128(base + M::kV0 + stage * M::kPieceBytes, M::kPieceHalf);
 #pragma unroll
                             for (int st = 0; st < 4; ++st)  // 16 keys: 8 columns of P, two groups of V
 #pragma unroll
                                 for (int x = TERMS - 1; x >= 0; --x)
-                                    tc::umma_f16_ts(tmem + M::kColO, tmem + (done & 1) * M::kPlace + x * 64 + (piece * 4 + st) * 8, v_desc + static_cast<uint64_t>(st * (2048 >> 4)), idesc_o,
-                                                    piece || st || x < TERMS - 1 || (M::kStays && j) ? 1u : 0u);
-                            tc::umma_commit(bar(kVEmpty + vs));
-                            if (piece) tc::umma_commit(bar(kOFull + (done & 1)));
+                                    tc::umma_f16_ts(tmem + M::kColO, tmem + (n & 1) * M::kPlace + x * 64 + (piece * 4 + st) * 8, v_desc + static_cast<uint64_t>(st * (2048 >> 4)), idesc_o, piece || st || x < TERMS - 1 || (M::kStays && j) ? 1u : 0u);
+                            tc::umma_commit(bar(kVEmpty + stage));
+                            if (piece) tc::umma_commit(bar(kOFull + (n & 1)));
                         }
                         __syncwarp();
-                        if (++vs == M::kVStages) {
-                            vs = 0;
-                            vphase ^= 1;
+                        if (++stage == M::kVStages) {
+                            stage = 0;
+                            phase ^= 1;
                         }
                     }
-                    if (ok && j + 2 < blocks) scores();
                 }
                 u += blocks;
                 if (u < u1) s = segment_at(p, sh.line, u, u1, M::kRows, M::kKeys);
@@ -1021,7 +1021,7 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
     if (!ok && lane == 0) atomicExch(p.err_word, 5);
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == M::kMmaWarp) {
+    if (warp == M::kScoreWarp) {
         tc::tc_fence_after();
         tc::tmem_dealloc(tmem, 512);
     }

@@ -349,3 +349,16 @@ def test_results_in_the_place_of_the_queries(ctx, dtype, b, t, nh, kvh, length):
     want = ops.attn_tree(q, k, v, *on, out=q.clone())  # rows of places not in use stay
     assert ops.attn_tree(q, k, v, *on, out=q) is q and torch.equal(q, want)
     ctx.check_device_error()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_values_that_are_no_numbers_where_the_walk_goes_round(ctx, dtype):
+    """Two tiles a head and many blocks a worker: the nodes' block comes up in the middle of a walk."""
+    test_values_that_are_no_numbers(ctx, dtype, 60, 8, 2, 40000)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_walks_that_go_round(ctx, dtype):
+    import torch
+    for b, t, nh, kvh, lengths in ((1, 70, 8, 2, [30011]), (3, 100, 4, 1, [9000, 0, 20500]), (40, 65, 4, 2, [700 + 37 * i for i in range(40)])):
+        check(ctx, make(b, t, nh, kvh, lengths, getattr(torch, dtype), counts=[t - i % 3 for i in range(b)]))

@@ -84,17 +84,19 @@ struct Line {
     int pos[kMaxSeqs], count[kMaxSeqs];
 };
 // A sequence has kv_heads * tiles problems of `blocks` units each.
-// A sequence's rows and its units: none if it lies outside its cache. (Loads from L2: the merging kernel comes here in front of its wait.)
-template <int ROWS, int KEYS>
-__device__ __forceinline__ int line_units(const TreeParams &p, int seq, int &pos, int &count) {
+// A sequence's rows: no nodes if it lies outside its cache. (Loads from L2: the merging kernel comes here in front of its wait.)
+__device__ __forceinline__ void line_rows(const TreeParams &p, int seq, int &pos, int &count) {
     pos = count = 0;
-    if (seq >= p.b) return 0;
+    if (seq >= p.b) return;
     pos = __ldcg(p.pos + seq);
     count = p.counts ? min(max(__ldcg(p.counts + seq), 0), p.t) : p.t;
     if (pos < 0 || pos > p.cap - count) {
         if (blockIdx.x == 0) atomicExch(p.err_word, kErrPos);
         count = 0;
     }
+}
+template <int ROWS, int KEYS>
+__device__ __forceinline__ int line_units(const TreeParams &p, int pos, int count) {
     return count ? (pos + count + KEYS - 1) / KEYS * ((count * p.group + ROWS - 1) / ROWS) * p.kvh : 0;
 }
 __device__ __forceinline__ int sum_up_to(int mine, int lane) {  // over the lanes
@@ -114,7 +116,8 @@ __device__ __forceinline__ void cut_line(const TreeParams &p, Line &l) {
         for (int i0 = 0; i0 < p.b; i0 += 32) {
             const int i = i0 + lane;
             int pos, count;
-            const int mine = line_units<ROWS, KEYS>(p, i, pos, count), sum = sum_up_to(mine, lane);
+            line_rows(p, i, pos, count);
+            const int mine = line_units<ROWS, KEYS>(p, pos, count), sum = sum_up_to(mine, lane);
             if (i < p.b) {
                 l.pos[i] = pos;
                 l.count[i] = count;
@@ -172,7 +175,7 @@ __device__ __forceinline__ Segment segment_at(const TreeParams &p, const Line &l
     }
     return segment_in(p, lo, l.pos[lo], l.count[lo], unit, unit - l.first[lo], last, rows, keys);
 }
-// A block's units u0 .. u1 - 1, and the first segment of them. Up to 32 sequences every warp finds it by itself, without a meeting, from one load: in front of the first
+// A block's units u0 .. u1 - 1, and the first segment of them. Up to 32 sequences every warp finds it by itself from the sequences' rows: in front of the first
 // query everything waits for this. Warp 0 leaves the line for the other segments; who looks for those has met it or waited for its queries since.
 struct Share {
     int u0, u1, most;   // most: the largest share of all
@@ -200,7 +203,15 @@ __device__ __forceinline__ Share own_share(const TreeParams &p, Line &l) {
     }
     const int lane = threadIdx.x & 31;
     int pos, count;
-    const int mine = line_units<ROWS, KEYS>(p, lane, pos, count), sum = sum_up_to(mine, lane), first = sum - mine, all = __shfl_sync(0xffffffffu, sum, 31);
+    if (threadIdx.x < 32) {  // one warp reads, so that all see the same, whatever happens to the positions meanwhile
+        line_rows(p, lane, pos, count);
+        l.pos[lane] = pos;
+        l.count[lane] = count;
+    }
+    __syncthreads();
+    pos = l.pos[lane];
+    count = l.count[lane];
+    const int mine = line_units<ROWS, KEYS>(p, pos, count), sum = sum_up_to(mine, lane), first = sum - mine, all = __shfl_sync(0xffffffffu, sum, 31);
     const Shares shares(all, p);
     s.most = shares.each + (shares.more > 0);
     s.u0 = shares.begin(blockIdx.x);
@@ -211,11 +222,7 @@ __device__ __forceinline__ Share own_share(const TreeParams &p, Line &l) {
         s.first = segment_in(p, seq, __shfl_sync(0xffffffffu, pos, seq), __shfl_sync(0xffffffffu, count, seq), s.u0, s.u0 - __shfl_sync(0xffffffffu, first, seq), s.u1, ROWS, KEYS);
     }
     if (threadIdx.x < 32) {
-        if (lane < p.b) {
-            l.pos[lane] = pos;
-            l.count[lane] = count;
-            l.first[lane] = first;
-        }
+        if (lane < p.b) l.first[lane] = first;
         if (lane == 0) l.first[p.b] = all;
     }
     return s;

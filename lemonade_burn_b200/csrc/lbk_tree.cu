@@ -153,7 +153,14 @@ __global__ void __launch_bounds__(128) kv_keep_path_kernel(uint4 *kcache, uint4 
     ptx::pdl_wait();
     __shared__ int s_path[kTreeNodes];
     __shared__ uint4 *s_rows[kPlanes];
-    const int seq = blockIdx.y, tid = threadIdx.x, count = tree_count(counts, seq, t), pos = pos_dev[seq], plane0 = blockIdx.x * kPlanes;
+    __shared__ int s_count, s_pos;
+    const int seq = blockIdx.y, tid = threadIdx.x, plane0 = blockIdx.x * kPlanes;
+    if (tid == 0) {  // one thread reads, so that all take the same way, whatever happens to the positions meanwhile
+        s_count = tree_count(counts, seq, t);
+        s_pos = pos_dev[seq];
+    }
+    __syncthreads();
+    const int count = s_count, pos = s_pos;
     if (tid < kPlanes) {
         const int layer = (plane0 + tid) / (2 * heads), rest = plane0 + tid - layer * 2 * heads;
         s_rows[tid] = (rest & 1 ? vcache : kcache) + static_cast<size_t>(layer) * layer_units + ((static_cast<size_t>(seq) * heads + (rest >> 1)) * cap + pos) * units;

@@ -253,3 +253,21 @@ def test_scores_from_the_command_line(families, ctx, tmp_path, capsys):
     net = model.NativeBitNet(tmp_path, ctx)
     want = net.score([5, 17, 3], net.new_cache(1, 8)).logprobs
     assert [float(x) for x in lines[0].split(",")] == pytest.approx(want[:2].tolist(), abs=1e-5) and lines[1] == ""
+
+
+def test_the_largest_pass(ctx):
+    """256 sequences of 128 nodes, 32768 rows: each sequence as it is in a pass by itself."""
+    import torch
+    net = small(ctx, layers=1, max_pos=140)
+    b, t, V = 256, 128, net.cfg.vocab_size
+    tokens, parents = dev(torch.randint(0, V, (b, t), generator=torch.Generator().manual_seed(5), dtype=torch.int32), trees(b, t, 5, "random"))
+    cache = net.new_cache(b, 140, own_positions=True)
+    logits = net.forward_tree(tokens, parents, cache)
+    for s in (0, 130, 255):
+        alone = net.forward_tree(tokens[s:s + 1].contiguous(), parents[s:s + 1].contiguous(), net.new_cache(1, 140))
+        assert near(logits[s], alone[0])
+    path, count, after = net.decode_tree(tokens, parents, cache)
+    best = net.argmax(logits[255])
+    want, last = walk(tokens[255].tolist(), parents[255].tolist(), best.tolist(), t)
+    assert count[255].item() == len(want) and path[255, :len(want)].tolist() == want and after[255].item() == last
+    ctx.check_device_error()

@@ -551,8 +551,13 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const ScoreParams
     }
 }
 
+constexpr int kAlone = 100 << 10, kInPairs = 60 << 10;  // with RowShared more than a half, and a third, of an SM's 228 KB
+static_assert(sizeof(RowShared) + kAlone > (114 << 10) && sizeof(RowShared) + kInPairs > (76 << 10) && sizeof(RowShared) + kInPairs < (112 << 10), "shared memory");
 int logprobs_init(Ctx *) {
-    for (void (*k)(ScoreParams, int) : {logprobs_kernel<float>, logprobs_kernel<uint16_t>}) LBK_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    for (void (*k)(ScoreParams, int) : {logprobs_kernel<float>, logprobs_kernel<uint16_t>}) {
+        LBK_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        LBK_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kAlone));
+    }
     return LBK_OK;
 }
 const InitHook kInitLogprobs(logprobs_init);
@@ -596,6 +601,11 @@ int lbk_token_logprobs(lbk_ctx *c, int dtype, const void *logits_dev, size_t pit
     cfg.gridDim = dim3(static_cast<unsigned>(rows * ctas));
     cfg.blockDim = dim3(kThreads);
     cfg.stream = st;
+    // No more CTAs to an SM than it takes: a launch that begins beside the last CTAs of the one in front puts as many as fit on the SMs that are free, and the others
+    // stay empty. Shared memory that nobody uses keeps them apart: us of 50021 bf16, one alternative, one call behind the other, 120 rows 12.4 -> 8.9, 203 12.6 -> 10.9. (Clusters
+    // are placed by the GPC, and find less room so: 16 rows of 128256 f32 9.0 -> 14.4.)
+    const size_t each_sm = (rows + ctx->sm_count - 1) / ctx->sm_count;
+    cfg.dynamicSmemBytes = ctas > 1 ? 0 : each_sm == 1 ? kAlone : each_sm == 2 ? kInPairs : 0;
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;

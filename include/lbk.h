@@ -544,7 +544,8 @@ int lbk_moe_route(lbk_ctx *ctx, const float *z_dev, size_t z_pitch, size_t n, si
  *                          [b][t][kv_heads][head_dim] by position pos + depth, k and v appended at row pos + i. The tables have cap rows or more.
  * lbk_attn_tree            softmax(scale * q . k) v over the rows 0 .. pos - 1 and those of the node itself and its ancestors, head_dim
  *                          128. q_dev and out_dev rows [b * t] of n_heads * 128 values, q_pitch and out_pitch values apart: f32 with
- *                          LBK_COMPUTE_F32 (q and the probabilities as three bf16 terms each), bf16 with LBK_COMPUTE_BF16 (one); pitches and buffers are
+ *                          LBK_COMPUTE_F32 (q and the probabilities as three bf16 terms each), bf16 with LBK_COMPUTE_BF16 (q as it is, the
+ *                          probabilities as two terms: what is rounded to bf16 is the result); pitches and buffers are
  *                          multiples of 16 bytes; out_dev may be q_dev. 0 < scale <= 1e30; at most 256 sequences, 4096 heads, 2^30 places of a
  *                          cache, 2^31 rows of all caches of the call. scratch_dev: lbk_attn_tree_scratch floats, 16-byte aligned, what is in
  *                          them does not matter; calls that may overlap need their own.

@@ -11,8 +11,10 @@
 // f32 queries and probabilities are three bf16 terms each (8 bits a term: an f32 has 24), keys and values are bf16 as they are: every product is exact, and
 // what is left are f32 sums. Two terms, as in the decode and prompt kernels, are off by 2^-17 of a query or probability, which was 3 to 6 times
 // the error of plain f32 arithmetic. A tensor core cuts its sums off instead of rounding them (2e-8 of a sum for 16 keys), so the products of a block of keys start from
-// zero and are added to the row in registers, one rounded addition a block. bf16 queries are exact in one term; their results are rounded to bf16,
-// 2^-8 of themselves at most, and so is a probability, whose roundings are of either sign and average out over the keys.
+// zero and are added to the row in registers, one rounded addition a block. bf16 queries are exact in one term, and their probabilities are two terms, as in
+// the decode and prompt kernels: off by 2^-16 of themselves at most, where the result is rounded by 2^-8 of itself. In one term a weight is off by as much as the result's
+// rounding, and what that adds to a result does not average out: over many keys of like weights a sum of values of either sign shrinks as its error does (60 nodes of 65000
+// keys: 0.0023 of the result against 0.0017 by its rounding alone), and of a few heavy keys whose values cancel the error is any multiple of the result.
 //
 // Rows of V that nobody has written may hold anything, and 0 * NaN is NaN: values past the sequence's last node are taken as zeros. Values of OTHER
 // branches may be infinite or NaN too; a row that does not see them must not notice. So in the blocks of the nodes values that are no numbers are
@@ -57,6 +59,8 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, the hardware's approxim
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// bf16 terms of a probability for queries of TERMS
+constexpr int weight_terms(int terms) { return terms == 1 ? 2 : terms; }
 // Two values at once as bf16 terms: term[i] = bf16(x - the terms in front of it), and with three of them their sum is x
 template <int TERMS>
 __device__ __forceinline__ void split_pair(float x0, float x1, uint32_t (&term)[TERMS]) {
@@ -358,13 +362,14 @@ struct Turned {
     static constexpr bool kGoesRound = false;  // one tile a problem
     static constexpr int kKeys = 128, kHalf = kKeys * 128, kKBytes = 2 * kHalf;
     static constexpr int kPiece = 64, kPieceHalf = kPiece * 128, kPieceBytes = 2 * kPieceHalf;   // V: 64 keys, two halves of 64 dimensions
-    static constexpr int kCols = TERMS * ROWS, kOpHalf = kCols * 128, kOpBytes = 2 * kOpHalf;     // queries, and probabilities of a block: [2 halves][terms * rows][128 bytes]
-    static constexpr int kKStages = kCols > 64 ? 2 : 3, kVStages = kCols > 64 ? 4 : 5;
-    static constexpr int kP0 = kOpBytes, kK0 = 3 * kOpBytes, kV0 = kK0 + kKStages * kKBytes, kBars = kV0 + kVStages * kPieceBytes;
+    // queries, and probabilities of a block (a place for even, one for odd ones): [2 halves][terms * rows][128 bytes]
+    static constexpr int kPTerms = weight_terms(TERMS), kQCols = TERMS * ROWS, kQHalf = kQCols * 128, kQBytes = 2 * kQHalf, kPCols = kPTerms * ROWS, kPHalf = kPCols * 128, kPBytes = 2 * kPHalf;
+    static constexpr int kKStages = kPCols > 64 ? 2 : 3, kVStages = kPCols > 64 ? 4 : 5;
+    static constexpr int kP0 = kQBytes, kK0 = kP0 + 2 * kPBytes, kV0 = kK0 + kKStages * kKBytes, kBars = kV0 + kVStages * kPieceBytes;
     static constexpr int kMax = kBars + 256, kPart = kMax + ROWS * 4, kSmem = kPart + 4 * ROWS * 4 + 1024;   // the rows' m; [quadrant][row] floats
     static constexpr int kSoftWarps = 8, kKWarp = 8, kVWarp = 9, kMmaWarp = 10, kThreads = 11 * 32;
-    static constexpr uint32_t kColO = kCols <= 32 ? 32 : kCols <= 64 ? 64 : 128, kTmem = 4 * kColO;  // scores, and from kColO on the products of even and of odd blocks
-    static_assert(kSmem + 6 * 1024 <= 232448 && kCols % 16 == 0 && kCols <= 128, "shared memory and operand sizes");
+    static constexpr uint32_t kColO = kPCols <= 32 ? 32 : kPCols <= 64 ? 64 : 128, kTmem = 4 * kColO;  // scores, and from kColO on the products of even and of odd blocks
+    static_assert(kSmem + 6 * 1024 <= 232448 && kQCols % 16 == 0 && kPCols % 16 == 0 && kQCols <= kPCols && kPCols <= 128, "shared memory and operand sizes");
 };
 // v[0] becomes what `join` makes of value lane / (32 / N) of all lanes: half of the values go to the other half of the lanes in every step
 template <int N, class Join>
@@ -442,7 +447,8 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
     } else if (warp == M::kMmaWarp) {
         // ================= MMA issue: the warp walks, one lane issues =================
         // D f32, A and B bf16, M = 128, N = terms * rows; for O^T A is MN-major (bit 15)
-        constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(M::kCols >> 3) << 17) | ((128u >> 4) << 24), idesc_o = idesc_s | (1u << 15);
+        constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24), idesc_s = idesc | (static_cast<uint32_t>(M::kQCols >> 3) << 17),
+                           idesc_o = idesc | (static_cast<uint32_t>(M::kPCols >> 3) << 17) | (1u << 15);
         const uint64_t q_desc = tc::smem_desc_sw128(base), p_desc = tc::smem_desc_sw128(base + M::kP0);
         int ks = 0, kphase = 0, vs = 0, vphase = 0, n = 0, seg = 0;  // n: the block, in the whole walk
         auto scores = [&]() {
@@ -452,7 +458,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
                 const uint64_t k_desc = tc::smem_desc_sw128(base + M::kK0 + ks * M::kKBytes);
 #pragma unroll
                 for (int st = 0; st < 8; ++st)
-                    tc::umma_f16_ss(tmem, k_desc + static_cast<uint64_t>((st >> 2) * (M::kHalf >> 4) + (st & 3) * 2), q_desc + static_cast<uint64_t>((st >> 2) * (M::kOpHalf >> 4) + (st & 3) * 2),
+                    tc::umma_f16_ss(tmem, k_desc + static_cast<uint64_t>((st >> 2) * (M::kHalf >> 4) + (st & 3) * 2), q_desc + static_cast<uint64_t>((st >> 2) * (M::kQHalf >> 4) + (st & 3) * 2),
                                     idesc_s, st ? 1u : 0u);
                 tc::umma_commit(bar(kSFull));
                 tc::umma_commit(bar(kKEmpty + ks));
@@ -479,7 +485,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
 #pragma unroll
                         for (int st = 0; st < 4; ++st)  // 16 keys: two groups of V
                             tc::umma_f16_ss(tmem + (1 + (n & 1)) * M::kColO, v_desc + static_cast<uint64_t>(st * (2048 >> 4)),
-                                            p_desc + static_cast<uint64_t>((n & 1) * (M::kOpBytes >> 4) + piece * (M::kOpHalf >> 4) + st * 2), idesc_o,
+                                            p_desc + static_cast<uint64_t>((n & 1) * (M::kPBytes >> 4) + piece * (M::kPHalf >> 4) + st * 2), idesc_o,
                                             piece || st ? 1u : 0u);
                         tc::umma_commit(bar(kVEmpty + vs));
                         if (piece) tc::umma_commit(bar(kOFull + (n & 1)));
@@ -508,7 +514,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
         auto queries_asked = [&]() { asm volatile("barrier.cta.arrive %0, %1;" ::"r"(kQueriesAsked), "r"(M::kSoftWarps * 32 + 64) : "memory"); };
         auto half_meet = [&]() { ptx::named_barrier(2 + hf, 128); };  // the four warps with the same rows
         // where this thread's probabilities go: column `key` of the operand, row n at n * 128, its 16-byte units XOR-ed with n & 7
-        uint8_t *const p_at = sm + M::kP0 + (key >> 6) * M::kOpHalf + (key & 7) * 2;
+        uint8_t *const p_at = sm + M::kP0 + (key >> 6) * M::kPHalf + (key & 7) * 2;
         const int p_unit = (key >> 3) & 7;
         int n = 0;  // blocks so far, over all segments
         Segment s = share.first;
@@ -530,7 +536,7 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
                 const int r = warp * kEach + i;
 #pragma unroll
                 for (int x = 0; x < TERMS; ++x)
-                    *reinterpret_cast<uint2 *>(sm + (lane >> 4) * M::kOpHalf + (x * ROWS + r) * 128 + ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8) = term[x];
+                    *reinterpret_cast<uint2 *>(sm + (lane >> 4) * M::kQHalf + (x * ROWS + r) * 128 + ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8) = term[x];
             }
             ptx::fence_proxy_async();  // the tensor core reads them through the asynchronous proxy
             arrive(kQFull);
@@ -543,19 +549,19 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
             float acc[kR], l[kR];  // of this thread's dimension; of its key of every block
 #pragma unroll
             for (int i = 0; i < kR; ++i) acc[i] = l[i] = 0.0f;
-            auto for_rows = [&](uint32_t at, auto &&give) {  // give(row, the terms' sum)
-                constexpr int kChunk = kR < 16 ? kR : 16;
+            auto for_rows = [&](auto n_terms, uint32_t at, auto &&give) {  // give(row, the terms' sum)
+                constexpr int kChunk = kR < 16 ? kR : 16, kN = decltype(n_terms)::value;
 #pragma unroll
                 for (int c = 0; c < kR; c += kChunk) {
-                    uint32_t w[TERMS][kChunk];
+                    uint32_t w[kN][kChunk];
 #pragma unroll
-                    for (int x = 0; x < TERMS; ++x) tc::tmem_ld(at + x * ROWS + c, w[x]);
+                    for (int x = 0; x < kN; ++x) tc::tmem_ld(at + x * ROWS + c, w[x]);
                     tc::tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < kChunk; ++i) {
-                        float v = __uint_as_float(w[TERMS - 1][i]);
+                        float v = __uint_as_float(w[kN - 1][i]);
 #pragma unroll
-                        for (int x = TERMS - 2; x >= 0; --x) v += __uint_as_float(w[x][i]);
+                        for (int x = kN - 2; x >= 0; --x) v += __uint_as_float(w[x][i]);
                         give(c + i, v);
                     }
                 }
@@ -563,14 +569,14 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
             auto add_products = [&](int block) {
                 wait(kOFull + (block & 1), block >> 1 & 1);
                 tc::tc_fence_after();
-                for_rows(lanes + (1 + (block & 1)) * M::kColO, [&](int i, float v) { acc[i] += v; });
+                for_rows(std::integral_constant<int, M::kPTerms>(), lanes + (1 + (block & 1)) * M::kColO, [&](int i, float v) { acc[i] += v; });
             };
             for (int j = s.begin; j < s.end; ++j, ++n) {
                 float sv[kR];
                 bool added = j == s.begin;
                 wait(kSFull, n & 1);
                 tc::tc_fence_after();
-                for_rows(lanes, [&](int i, float v) { sv[i] = v * p.scale; });
+                for_rows(std::integral_constant<int, TERMS>(), lanes, [&](int i, float v) { sv[i] = v * p.scale; });
                 tc::tc_fence_before();
                 arrive(kSFree);
                 const int node = j * M::kKeys + key - pos;  // this thread's key
@@ -622,13 +628,13 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
                 // their place is free: the products of the block in front of the last have been added
 #pragma unroll
                 for (int i = 0; i < kR; i += 2) {
-                    uint32_t term[TERMS];
-                    split_pair<TERMS>(sv[i], sv[i + 1], term);
+                    uint32_t term[M::kPTerms];
+                    split_pair<M::kPTerms>(sv[i], sv[i + 1], term);
 #pragma unroll
-                    for (int x = 0; x < TERMS; ++x) {
+                    for (int x = 0; x < M::kPTerms; ++x) {
                         const int r = x * ROWS + first + i;
-                        *reinterpret_cast<uint16_t *>(p_at + (n & 1) * M::kOpBytes + r * 128 + ((p_unit ^ (r & 7)) << 4)) = static_cast<uint16_t>(term[x]);
-                        *reinterpret_cast<uint16_t *>(p_at + (n & 1) * M::kOpBytes + (r + 1) * 128 + ((p_unit ^ ((r + 1) & 7)) << 4)) = static_cast<uint16_t>(term[x] >> 16);
+                        *reinterpret_cast<uint16_t *>(p_at + (n & 1) * M::kPBytes + r * 128 + ((p_unit ^ (r & 7)) << 4)) = static_cast<uint16_t>(term[x]);
+                        *reinterpret_cast<uint16_t *>(p_at + (n & 1) * M::kPBytes + (r + 1) * 128 + ((p_unit ^ ((r + 1) & 7)) << 4)) = static_cast<uint16_t>(term[x] >> 16);
                     }
                 }
                 if (j * M::kKeys + M::kKeys > pos) {  // values past the last node, and values of nodes that are no numbers: a thread half a row of this warp's piece
@@ -718,8 +724,10 @@ struct Many {
     // bf16: the products are summed up in tensor memory, over all blocks, and m is moved as for few rows, with the sums, when a score is over it by kSlack. What the tensor
     // core cuts off of a long sum (1e-5 at 8000 keys) does not show in a bf16 result, and a block needs no look at the products of the one in front.
     static constexpr bool kStays = TERMS == 1;
+    static constexpr int kPTerms = weight_terms(TERMS);
     // Scores (128 columns) and, when all have been read, the probabilities (64 a term) of even blocks in one place, of odd ones in another
     static constexpr uint32_t kPlace = 192, kColO = 384;
+    static_assert(kPTerms * 64 <= kPlace && 2 * kPlace <= kColO, "tensor memory");
 };
 template <int TERMS>
 __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kernel(const __grid_constant__ TreeParams p) {
@@ -822,8 +830,8 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
 #pragma unroll
                             for (int st = 0; st < 4; ++st)  // 16 keys: 8 columns of P, two groups of V
 #pragma unroll
-                                for (int x = TERMS - 1; x >= 0; --x)
-                                    tc::umma_f16_ts(tmem + M::kColO, tmem + (n & 1) * M::kPlace + x * 64 + (piece * 4 + st) * 8, v_desc + static_cast<uint64_t>(st * (2048 >> 4)), idesc_o, piece || st || x < TERMS - 1 || (M::kStays && j) ? 1u : 0u);
+                                for (int x = M::kPTerms - 1; x >= 0; --x)
+                                    tc::umma_f16_ts(tmem + M::kColO, tmem + (n & 1) * M::kPlace + x * 64 + (piece * 4 + st) * 8, v_desc + static_cast<uint64_t>(st * (2048 >> 4)), idesc_o, piece || st || x < M::kPTerms - 1 || (M::kStays && j) ? 1u : 0u);
                             tc::umma_commit(bar(kVEmpty + stage));
                             if (piece) tc::umma_commit(bar(kOFull + (n & 1)));
                         }
@@ -952,18 +960,18 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                     const float2 scale2 = make_float2(p.scale, p.scale), less = make_float2(-nm, -nm);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        uint32_t w[TERMS][8];
+                        uint32_t w[M::kPTerms][8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const float2 d = ptx::fma2(make_float2(__uint_as_float(sv[c * 16 + 2 * i]), __uint_as_float(sv[c * 16 + 2 * i + 1])), scale2, less), e = make_float2(ex2(d.x), ex2(d.y));
                             sum = ptx::add2(sum, e);
-                            uint32_t term[TERMS];
-                            split_pair<TERMS>(e.x, e.y, term);
+                            uint32_t term[M::kPTerms];
+                            split_pair<M::kPTerms>(e.x, e.y, term);
 #pragma unroll
-                            for (int x = 0; x < TERMS; ++x) w[x][i] = term[x];
+                            for (int x = 0; x < M::kPTerms; ++x) w[x][i] = term[x];
                         }
 #pragma unroll
-                        for (int x = 0; x < TERMS; ++x) tc::tmem_st8(place + x * 64 + part * 16 + c * 8, w[x]);
+                        for (int x = 0; x < M::kPTerms; ++x) tc::tmem_st8(place + x * 64 + part * 16 + c * 8, w[x]);
                     }
                     l = l * step + (sum.x + sum.y);
                 }

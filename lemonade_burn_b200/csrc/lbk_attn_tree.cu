@@ -368,6 +368,7 @@ struct Turned {
     static constexpr int kP0 = kQBytes, kK0 = kP0 + 2 * kPBytes, kV0 = kK0 + kKStages * kKBytes, kBars = kV0 + kVStages * kPieceBytes;
     static constexpr int kMax = kBars + 256, kPart = kMax + ROWS * 4, kSmem = kPart + 4 * ROWS * 4 + 1024;   // the rows' m; [quadrant][row] floats
     static constexpr int kSoftWarps = 8, kKWarp = 8, kVWarp = 9, kMmaWarp = 10, kThreads = 11 * 32;
+    static_assert(kVStages >= 2 * 2, "as of Many::kBehind: a warp in block n has added the products of block n - 2");
     static constexpr uint32_t kColO = kPCols <= 32 ? 32 : kPCols <= 64 ? 64 : 128, kTmem = 4 * kColO;  // scores, and from kColO on the products of even and of odd blocks
     static_assert(kSmem + 6 * 1024 <= 232448 && kQCols % 16 == 0 && kPCols % 16 == 0 && kQCols <= kPCols && kPCols <= 128, "shared memory and operand sizes");
 };
@@ -727,6 +728,12 @@ struct Many {
     static constexpr int kPTerms = weight_terms(TERMS);
     // Scores (128 columns) and, when all have been read, the probabilities (64 a term) of even blocks in one place, of odd ones in another
     static constexpr uint32_t kPlace = 192, kColO = 384;
+    // A wait for a parity tells a phase from the one in front of it, no more. All roles but one wait for every phase of their barriers, or for one that shows that the phase in
+    // front is complete. The one: softmax warps wait for a piece of values only where they clean it (clean_values), in block n for 2n and 2n + 1 at most, having
+    // waited for the products of block n - kBehind: in f32 by themselves, in bf16 through the scores of block n, which the score warp asks for behind the products of block
+    // n - 2. So piece 2 (n - kBehind) + 1 has landed, and the one that lay in 2n + 1's stage in front of it, 2n + 1 - kVStages, must be none later.
+    static constexpr int kBehind = kStays ? 2 : 1;
+    static_assert(kVStages >= 2 * kBehind, "the phase in front of the one that is waited for is complete");
     static_assert(kPTerms * 64 <= kPlace && 2 * kPlace <= kColO, "tensor memory");
 };
 template <int TERMS>
@@ -975,20 +982,20 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
                     }
                     l = l * step + (sum.x + sum.y);
                 }
-                if (j * M::kKeys + M::kKeys > pos) {  // values past the last node, and values of nodes that are no numbers: a thread 32 dimensions of a row of this warp's piece
-                    const int piece = 2 * n + (part >> 1), vs = piece % M::kVStages, quarter = (part & 1) * 2 + (r >> 6), key = r & 63, at = j * M::kKeys + (part >> 1) * 64 + key - pos;
-                    if (wait(kVFull + vs, (piece / M::kVStages) & 1) && at >= 0 &&
-                        clean_values(reinterpret_cast<uint4 *>(sm + M::kV0 + vs * M::kPieceBytes + (quarter >> 1) * M::kPieceHalf + key * 128 + (quarter & 1) * 64), 4, at >= count))
-                        sh.odd = u + 1;  // read behind a meeting below, written again behind the next segment's first
-                    ptx::fence_proxy_async();
-                }
-                // the products of the block in front are added, then their place is free
+                // the products of the block in front are added, then their place is free; the values of that block have landed and been read then
                 if (!M::kStays) {
                     if (begun) {
                         wait(kOFull + ((n - 1) & 1), (n - 1) >> 1 & 1);
                         if (live) add_products();
                     }
                     corr = step;
+                }
+                if (j * M::kKeys + M::kKeys > pos) {  // values past the last node, and values of nodes that are no numbers: a thread 32 dimensions of a row of this warp's piece
+                    const int piece = 2 * n + (part >> 1), vs = piece % M::kVStages, quarter = (part & 1) * 2 + (r >> 6), key = r & 63, at = j * M::kKeys + (part >> 1) * 64 + key - pos;
+                    if (wait(kVFull + vs, (piece / M::kVStages) & 1) && at >= 0 &&
+                        clean_values(reinterpret_cast<uint4 *>(sm + M::kV0 + vs * M::kPieceBytes + (quarter >> 1) * M::kPieceHalf + key * 128 + (quarter & 1) * 64), 4, at >= count))
+                        sh.odd = u + 1;  // read behind a meeting below, written again behind the next segment's first
+                    ptx::fence_proxy_async();
                 }
                 if (live) tc::tmem_st_wait();
                 tc::tc_fence_before();

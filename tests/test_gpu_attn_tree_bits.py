@@ -95,3 +95,26 @@ def test_f32_weights_are_whole(ctx, t, nh, kvh):
         # terms 1; sums of three products 6. The weights' sum: its smaller part's 10, and 1; the quotient and the product 3. A weight in two terms is off by up to 256.
         assert bool(((got - want).abs() <= 32 * 2.0 ** -24 * want.abs()).all()), float(((got - want) / want).abs().max() * 2.0 ** 24)
     ctx.check_device_error()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("kvh,length", [(148, 200), (74, 470), (1, 37000)])
+def test_values_that_come_late(ctx, dtype, kvh, length):
+    """Walks whose last block holds the nodes and rows that nobody has written, right behind one that holds none, while something else takes the memory's bandwidth: values are
+    looked at when they have landed, not when the ones in front of them in their place have."""
+    import torch
+    from lemonade_burn_b200 import ops
+    t = 40 if kvh > 1 else 70
+    q, k, v, pos, parents, counts = make(1, t, kvh if kvh > 1 else 4, kvh, [length], getattr(torch, dtype), room=90)
+    on = dev(pos, parents, counts)
+    first = ops.attn_tree(q, k, v, *on)
+    want, wide, _ = in_64_bits(q, k, v, pos, parents, counts)
+    assert bool(((first.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * wide).all())
+    big = [torch.empty(1 << 28, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    side = torch.cuda.Stream()
+    for i in range(40):
+        with torch.cuda.stream(side):
+            big[i & 1].copy_(big[1 - (i & 1)])
+        assert torch.equal(ops.attn_tree(q, k, v, *on), first)
+        torch.cuda.synchronize()
+    ctx.check_device_error()

@@ -36,17 +36,19 @@ struct ScoreParams {
     float *top_logprobs;
 };
 
-// A place in the order of the alternatives: larger values first, then lower ids; every NaN in front of every number, as a sort has it; 0 is
-// behind every place.
+// A place in the order of the alternatives: larger values first, then lower ids; every NaN in front of every number, as a sort has it. 0 is
+// behind every place, kInFront in front of every one: ids are below 2^30, so the lower word has its upper bit clear.
+constexpr unsigned kLastId = 0x7fffffffu;
+constexpr unsigned long long kInFront = ~0ull;
 __device__ __forceinline__ unsigned order_value(float x) {  // the order of numbers as that of whole ones
     const unsigned bits = __float_as_uint(x + 0.0f);         // -0 and 0 are equal
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(unsigned order) { return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order); }
 __device__ __forceinline__ unsigned long long order_key(float x, int id) {
-    return static_cast<unsigned long long>(x != x ? 0xffffffffu : order_value(x)) << 32 | static_cast<unsigned>(~id);
+    return static_cast<unsigned long long>(x != x ? 0xffffffffu : order_value(x)) << 32 | (kLastId - static_cast<unsigned>(id));
 }
-__device__ __forceinline__ int key_id(unsigned long long key) { return static_cast<int>(~static_cast<unsigned>(key)); }
+__device__ __forceinline__ int key_id(unsigned long long key) { return static_cast<int>(kLastId - static_cast<unsigned>(key)); }
 
 // One pass over the row. A thread keeps the maximum m of what it has seen, s = sum e^(c (x - m)) and t = sum e^(c (x - m)) (x - m); entropy = log s - c t / s.
 //
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) logprobs_short_kernel(const 
         }
         return;
     }
-    Key last = ~0ull;  // the largest value behind the last one found, `top` times over
+    Key last = kInFront;  // the largest value behind the last one found, `top` times over
     for (int k = 0; k < p.top; ++k) {
         Key best = 0;
         auto look = [&](float v, int id) {
@@ -329,7 +331,7 @@ __device__ void put_in_order(const Key *keys, int n, int top, Key *out, Key *war
         __syncthreads();
         return;
     }
-    Key last = ~0ull;
+    Key last = kInFront;
     for (int k = 0; k < top && last; ++k) {
         Key best = 0;
         for (int i = tid; i < n; i += kThreads)
@@ -474,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const ScoreParams
         floor = sh.bound;
         if (n <= kList && n >= want && s == s && s <= FLT_MAX) {
             // what reaches the last bounds
-            const Key least = order_key(floor, 0x7fffffff);
+            const Key least = order_key(floor, kLastId);
             for (int i = tid; i < n; i += kThreads)
                 if (sh.list[i] >= least) {
                     const int at = atomicAdd(&sh.kept, 1);
@@ -486,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const ScoreParams
         } else {
             // the largest value behind the last one found, `top` times over
             if (tid < p.top) sh.top[tid] = 0;
-            Key last = ~0ull;
+            Key last = kInFront;
             for (int k = 0; k < want; ++k) {
                 Key best = 0;
                 auto look = [&](float v, int id) {

@@ -554,8 +554,10 @@ int lbk_moe_route(lbk_ctx *ctx, const float *z_dev, size_t z_pitch, size_t n, si
  *                          best_dev of the last one (-1 for a sequence without nodes).
  * lbk_kv_keep_path         rows pos + path[j] move to pos + j, j < count_dev[seq], of keys and values of `layers` layers that lie
  *                          layer_elems elements apart. path_dev [b][t] ascending, any accepted nodes. Positions are not changed. head_dim and
- *                          layer_elems are multiples of 8, the caches lie on 16 bytes; at most 65535 sequences.
- * lbk_advance_pos_by       pos_dev[seq] += count_dev[seq]. */
+ *                          layer_elems are multiples of 8, the caches lie on 16 bytes; at most 65535 sequences. A count outside 0 .. t is the nearest inside.
+ * lbk_advance_pos_by       pos_dev[seq] += count_dev[seq], at most LBK_TREE_NODES.
+ * lbk_advance_pos_path     the same for the sequences whose path lbk_kv_keep_path takes; of the others it leaves position and rows as they were. For
+ *                          paths that the caller has not made by lbk_tree_accept. */
 #define LBK_TREE_NODES 128
 int lbk_rope_kv_append_tree(lbk_ctx *ctx, float *q_dev, const float *k_dev, const float *v_dev, const float *cos_dev, const float *sin_dev,
                             const int32_t *pos_dev, const int32_t *parents_dev, const int32_t *counts_dev, size_t b, size_t t, size_t n_heads,
@@ -569,6 +571,7 @@ int lbk_tree_accept(lbk_ctx *ctx, const int32_t *tokens_dev, const int32_t *pare
 int lbk_kv_keep_path(lbk_ctx *ctx, uint16_t *kcache_dev, uint16_t *vcache_dev, size_t layers, size_t layer_elems, size_t b, size_t kv_heads,
                      size_t head_dim, size_t cap, const int32_t *pos_dev, const int32_t *path_dev, const int32_t *count_dev, size_t t, void *stream);
 int lbk_advance_pos_by(lbk_ctx *ctx, int32_t *pos_dev, const int32_t *count_dev, size_t b, void *stream);
+int lbk_advance_pos_path(lbk_ctx *ctx, int32_t *pos_dev, const int32_t *path_dev, const int32_t *count_dev, size_t b, size_t t, size_t cap, void *stream);
 
 /* Rows of logits (LBK_DTYPE_*, `pitch` values apart, scale from 1e-20 to 1e20): logprobs_dev [rows][given] = log softmax(scale * logits) at
  * tokens_dev [rows][given] (NaN for a token outside the vocabulary), entropy_dev [rows] (may be null) in nats, and the `top` (at most

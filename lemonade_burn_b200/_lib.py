@@ -128,6 +128,7 @@ SYMBOLS = [
     ("lbk_tree_accept", _i, [_vp] * 5 + [_sz, _sz] + [_vp] * 4),
     ("lbk_kv_keep_path", _i, [_vp, _vp, _vp] + [_sz] * 6 + [_vp] * 3 + [_sz, _vp]),
     ("lbk_advance_pos_by", _i, [_vp, _vp, _vp, _sz, _vp]),
+    ("lbk_advance_pos_path", _i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp]),
     ("lbk_token_logprobs", _i, [_vp, _i, _vp, _sz, _sz, _sz, _vp, _sz, _f, _sz, _vp, _vp, _vp, _vp, _vp]),
     ("lbk_model_load", _i, [_vp, C.c_char_p, _pp]),
     ("lbk_model_load_compute", _i, [_vp, C.c_char_p, _i, _pp]),

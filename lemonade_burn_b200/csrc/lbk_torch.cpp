@@ -28,6 +28,7 @@ struct Library {
     decltype(&lbk_kv_keep_path) keep = nullptr;
     decltype(&lbk_advance_pos_by) advance = nullptr;
     decltype(&lbk_token_logprobs) logprobs = nullptr;
+    decltype(&lbk_advance_pos_path) advance_path = nullptr;
 } lib;
 PyObject *g_check = nullptr, *g_context = nullptr;  // raises for a status; the default context
 PyObject *g_handle = nullptr, *g_value = nullptr, *g_device = nullptr;  // attribute names
@@ -256,16 +257,20 @@ PyObject *tree_accept(PyObject *, PyObject *const *a, Py_ssize_t n) {
     });
 }
 
-// k, v, pos, path, count, ctx
+// k, v, pos, path, count, ctx, advance
 PyObject *kv_keep_path(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    return entry(n, 6, [&] {
+    return entry(n, 7, [&] {
         const auto call = have(lib.keep, "lbk_kv_keep_path");
+        const auto move = have(lib.advance_path, "lbk_advance_pos_path");
+        const int advance = PyObject_IsTrue(a[6]);
+        if (advance < 0) throw Refused();
         const at::Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v"), &pos = tensor(a[2], "pos"), &path = tensor(a[3], "path"), &count = tensor(a[4], "count");
         const Tree s = tree(path, count, pos);
         const Cache c = caches(k, v, s.b, 5);
         const Context ctx(a[5]);
         void *st = ctx.stream(k, v, pos, path, count);
         done(call(ctx.handle, data<uint16_t>(k), data<uint16_t>(v), c.layers, s.b * c.kv_heads * c.cap * c.hd, s.b, c.kv_heads, c.hd, c.cap, ints(pos), ints(path), ints(count), s.t, st));
+        if (advance) done(move(ctx.handle, data<int32_t>(pos), ints(path), ints(count), s.b, s.t, c.cap, st));
         Py_RETURN_NONE;
     });
 }
@@ -319,15 +324,15 @@ PyObject *token_logprobs(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 // the library's functions by address, what raises for a status, what gives the default context
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    return entry(n, 9, [&] {
-        void *at[7];
-        for (int i = 0; i < 7; ++i) at[i] = PyLong_AsVoidPtr(a[i]);
+    return entry(n, 10, [&] {
+        void *at[8];
+        for (int i = 0; i < 8; ++i) at[i] = PyLong_AsVoidPtr(a[i]);
         if (PyErr_Occurred()) throw Refused();
         lib = {reinterpret_cast<decltype(lib.append)>(at[0]), reinterpret_cast<decltype(lib.scratch)>(at[1]), reinterpret_cast<decltype(lib.attn)>(at[2]),
                reinterpret_cast<decltype(lib.accept)>(at[3]), reinterpret_cast<decltype(lib.keep)>(at[4]), reinterpret_cast<decltype(lib.advance)>(at[5]),
-               reinterpret_cast<decltype(lib.logprobs)>(at[6])};
-        Py_XSETREF(g_check, Py_NewRef(a[7]));
-        Py_XSETREF(g_context, Py_NewRef(a[8]));
+               reinterpret_cast<decltype(lib.logprobs)>(at[6]), reinterpret_cast<decltype(lib.advance_path)>(at[7])};
+        Py_XSETREF(g_check, Py_NewRef(a[8]));
+        Py_XSETREF(g_context, Py_NewRef(a[9]));
         Py_RETURN_NONE;
     });
 }

@@ -5,6 +5,7 @@
 //   tree_accept        the greedy walk: node 0, then the child whose token is the best one of its parent's row
 //   kv_keep_path       the rows of the accepted nodes moved together behind the committed ones, in all layers
 //   advance_by         positions moved by the accepted nodes
+//   advance_path       the same for the sequences whose path kv_keep_path takes
 //
 // A decode step of one token is the tree with one node: the same rows of the cache, the same rotation
 // (crates/lb-model/src/model.rs:295-303, 334-347). Everything is read from device memory, so a step can be recorded once.
@@ -143,6 +144,12 @@ __global__ void __launch_bounds__(kTreeNodes) tree_accept_kernel(const int *__re
     }
 }
 
+// Whether a path is wrong at place j: it ascends, inside the tree
+__device__ __forceinline__ bool path_wrong(const int *__restrict__ path, int j, int t) {
+    const int from = path[j];
+    return from < j || from >= t || (j > 0 && from <= path[j - 1]);
+}
+
 // One block per sequence and kPlanes of its (layer, KV head, keys or values), 16 bytes a thread and row: the accepted nodes of a step are a few rows of 256 bytes
 // each, and a block for each plane was launch and waiting (16 sequences, 30 layers of 5 heads, 8 rows, 20 MB: 8.4 -> 5.8 us). Rows move down only (path[j] >= j,
 // ascending), so portions in ascending order, each read before it is written, never overwrite a row that is still wanted.
@@ -167,9 +174,8 @@ __global__ void __launch_bounds__(128) kv_keep_path_kernel(uint4 *kcache, uint4 
     }
     bool wrong = false;
     for (int j = tid; j < count; j += blockDim.x) {
-        const int from = path[static_cast<size_t>(seq) * t + j];
-        s_path[j] = from;
-        wrong |= from < j || from >= t || (j > 0 && from <= path[static_cast<size_t>(seq) * t + j - 1]);
+        s_path[j] = path[static_cast<size_t>(seq) * t + j];
+        wrong |= path_wrong(path + static_cast<size_t>(seq) * t, j, t);
     }
     if (__syncthreads_or(wrong)) {
         if (tid == 0) atomicExch(err_word, kErrTree);
@@ -207,6 +213,23 @@ __global__ void advance_by_kernel(int *pos, const int *__restrict__ count, int n
     const int i = blockIdx.x * blockDim.x + threadIdx.x;
     // a position that was refused stays refused (advance_pos_kernel)
     if (i < n && count[i] > 0 && pos[i] < (1 << 30)) pos[i] += min(count[i], kTreeNodes);
+}
+
+// A warp a sequence. What kv_keep_path leaves as it was keeps its position too: rows that have not been moved are none of the sequence's.
+constexpr int kAdvanceWarps = 4;
+__global__ void __launch_bounds__(kAdvanceWarps * 32) advance_path_kernel(int *pos, const int *__restrict__ path, const int *__restrict__ counts, int b, int t, int cap, int *err_word) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int seq = blockIdx.x * kAdvanceWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (seq >= b) return;
+    const int count = tree_count(counts, seq, t), *own = path + static_cast<size_t>(seq) * t;
+    bool wrong = false;
+    for (int j = lane; j < count; j += 32) wrong |= path_wrong(own, j, t);
+    wrong = __any_sync(0xffffffffu, wrong);
+    if (lane || !count) return;
+    const int at = pos[seq];
+    if (wrong || at < 0 || at > cap - (own[count - 1] + 1)) atomicExch(err_word, wrong ? kErrTree : kErrPos);
+    else pos[seq] = at + count;
 }
 
 }  // namespace
@@ -279,6 +302,18 @@ int lbk_advance_pos_by(lbk_ctx *c, int32_t *pos_dev, const int32_t *count_dev, s
     if (!pos_dev || !count_dev) return fail(LBK_ERR_INVALID, "lbk_advance_pos_by: null buffer");
     if (b > INT32_MAX) return fail(LBK_ERR_UNSUPPORTED, "lbk_advance_pos_by: more sequences than 2^31");
     LBK_CUDA(launch_chained(advance_by_kernel, dim3(static_cast<unsigned>((b + 127) / 128)), dim3(128), 0, st, pos_dev, count_dev, static_cast<int>(b)));
+    ctx->launches++;
+    return LBK_OK;
+}
+
+int lbk_advance_pos_path(lbk_ctx *c, int32_t *pos_dev, const int32_t *path_dev, const int32_t *count_dev, size_t b, size_t t, size_t cap, void *stream) {
+    LBK_TREE_PRE("lbk_advance_pos_path");
+    if (b == 0) return LBK_OK;
+    if (!pos_dev || !path_dev || !count_dev) return fail(LBK_ERR_INVALID, "lbk_advance_pos_path: null buffer");
+    if (t == 0 || t > LBK_TREE_NODES) return fail(LBK_ERR_UNSUPPORTED, "a tree has 1 to %d nodes (got %zu)", LBK_TREE_NODES, t);
+    if (b > INT32_MAX || cap > INT32_MAX) return fail(LBK_ERR_UNSUPPORTED, "lbk_advance_pos_path: more than 2^31 sequences or rows");
+    LBK_CUDA(launch_chained(advance_path_kernel, dim3(static_cast<unsigned>((b + kAdvanceWarps - 1) / kAdvanceWarps)), dim3(kAdvanceWarps * 32), 0, st, pos_dev, path_dev, count_dev,
+                            static_cast<int>(b), static_cast<int>(t), static_cast<int>(cap), ctx->err_word));
     ctx->launches++;
     return LBK_OK;
 }

@@ -393,9 +393,9 @@ class BitNet:
 
     def accept_tree(self, cache: KvCache, path: torch.Tensor, count: torch.Tensor) -> None:
         """Commits count[s] nodes of every sequence's tree, path int32 [b, t] ascending (ops.tree_accept, or a sampler's choice): their rows of
-        the cache move together behind the committed ones, the others' places are free again."""
-        ops.kv_keep_path(cache.k, cache.v, cache.pos, path, count, self.ctx)
-        ops.advance_pos_by(cache.pos, count, self.ctx)
+        the cache move together behind the committed ones, the others' places are free again. Of a path that is none (not ascending, outside the tree or the
+        cache) nothing is committed: `ctx.check_device_error` tells of it."""
+        ops.kv_keep_path(cache.k, cache.v, cache.pos, path, count, self.ctx, advance=True)
         cache.host_len, cache.at_most = min(cache.cap, cache.host_len + path.shape[1]), True
 
     def decode_tree(self, tokens: torch.Tensor, parents: torch.Tensor, cache: KvCache, counts: Optional[torch.Tensor] = None):

@@ -184,7 +184,7 @@ def _torch_ops():
         module = module_from_spec(spec_from_file_location("_torch_ops", str(path), loader=loader))
         loader.exec_module(module)
         lib = _lib.load()
-        calls = [getattr(lib, "lbk_" + n, None) for n in ("rope_kv_append_tree", "attn_tree_scratch", "attn_tree", "tree_accept", "kv_keep_path", "advance_pos_by", "token_logprobs")]
+        calls = [getattr(lib, "lbk_" + n, None) for n in ("rope_kv_append_tree", "attn_tree_scratch", "attn_tree", "tree_accept", "kv_keep_path", "advance_pos_by", "token_logprobs", "advance_pos_path")]
         module.bind(*[C.cast(f, C.c_void_p).value if f else 0 for f in calls], _lib.check, default_context)  # one family's part of the library has some of them only
         _native = module
     return _native
@@ -213,10 +213,12 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, best: torch.Tensor,
     return (_native or _torch_ops()).tree_accept(tokens, parents, best, counts, ctx)
 
 
-def kv_keep_path(k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, path: torch.Tensor, count: torch.Tensor, ctx: Optional[Context] = None) -> None:
+def kv_keep_path(k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, path: torch.Tensor, count: torch.Tensor, ctx: Optional[Context] = None, advance: bool = False) -> None:
     """Closes the gaps that refused drafts leave (lbk_kv_keep_path): of caches [layers, b, kv_heads, cap, head_dim] the rows pos + path[j] move
-    to pos + j for j < count. path int32 [b, t] ascending. Positions are not changed (advance_pos_by)."""
-    (_native or _torch_ops()).kv_keep_path(k, v, pos, path, count, ctx)
+    to pos + j for j < count. path int32 [b, t] ascending. A path that does not ascend inside the tree, or rows
+    outside the cache, are refused, and `ctx.check_device_error` tells of it. Positions are not changed (advance_pos_by), or, with `advance`, move by the count where the
+    path was taken (lbk_advance_pos_path)."""
+    (_native or _torch_ops()).kv_keep_path(k, v, pos, path, count, ctx, advance)
 
 
 def advance_pos_by(pos: torch.Tensor, count: torch.Tensor, ctx: Optional[Context] = None) -> None:

@@ -113,3 +113,12 @@ for call in (lambda: ops.advance_pos_by(ints(1), ints(1)), lambda: ops.tree_acce
     assert out.returncode == 0, out.stderr
     assert out.stdout.splitlines() == ["RuntimeError the library that is loaded has no lbk_advance_pos_by", "RuntimeError the library that is loaded has no lbk_tree_accept",
                                        "ValueError logits are [rows, vocab]"]
+
+
+def test_keep_that_advances_refuses():
+    from lemonade_burn_b200 import _lib, build, ops
+    build.build()
+    c = torch.zeros(3, 2, 1, 8, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        ops.kv_keep_path(c, c, _i(2), _i(3, 4), _i(2), advance=True)
+    assert _lib.load().lbk_advance_pos_path(None, None, None, None, 1, 1, 8, None) == 1

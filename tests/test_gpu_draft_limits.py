@@ -28,3 +28,54 @@ def test_a_nan_at_the_first_token(ctx, dtype, rows, vocab, shift):
     tokens = torch.tensor([[0, vocab - 1]], dtype=torch.int32, device="cuda").expand(rows, 2).contiguous()
     for top in {1, min(vocab, 5), min(vocab, 32)}:
         _check_logprobs(x, tokens, top)
+
+
+def test_a_path_that_is_none_commits_nothing(ctx):
+    """A sampler's path that does not ascend, leaves the tree or the cache: neither rows nor position of that sequence move; the others' do."""
+    import torch
+    from lemonade_burn_b200 import _lib
+    from test_gpu_draft_models import small
+    net = small(ctx, layers=2, max_pos=40)
+    for path, count, at in (([1, 0, -1, -1], 2, 9), ([0, 0, 1, -1], 3, 9), ([0, 4, -1, -1], 2, 9), ([-1, 1, -1, -1], 2, 9), ([0, 1, 3, -1], 3, 37), ([0, 1, 3, -1], 3, -1), ([0, 2, 3, -1], 4, 9)):
+        cache = net.new_cache(3, 40, own_positions=True)
+        cache.k.normal_()
+        cache.v.normal_()
+        cache.pos.copy_(ints([5, at, 7]))
+        old = cache.k.clone(), cache.v.clone()
+        net.accept_tree(cache, *dev(ints([[0, 3, -1, -1], path, [2, -1, -1, -1]]), ints([2, count, 1])))
+        with pytest.raises(_lib.LbkError) as e:
+            ctx.check_device_error()
+        assert e.value.status == 1
+        assert cache.pos.tolist() == [7, at, 8]
+        for now, was in zip((cache.k, cache.v), old):
+            assert torch.equal(now[:, 1], was[:, 1])
+            assert torch.equal(now[:, 0, :, 6], was[:, 0, :, 8]) and torch.equal(now[:, 2, :, 7], was[:, 2, :, 9])
+
+
+def test_counts_outside_the_tree_are_the_nearest_inside(ctx):
+    """What keeps the rows and what moves the position take a count alike."""
+    from test_gpu_draft_models import small
+    net = small(ctx, layers=1, max_pos=40)
+    cache = net.new_cache(4, 40, own_positions=True)
+    cache.pos.fill_(5)
+    net.accept_tree(cache, *dev(ints([[0, 1, 2]] * 4), ints([100, -3, 2 ** 31 - 1, 3])))
+    ctx.check_device_error()
+    assert cache.lens() == [8, 5, 8, 8] and cache.host_len >= 3
+
+
+@pytest.mark.parametrize("b,t", [(1, 1), (5, 128), (9, 70), (300, 33)])
+def test_keep_and_advance_in_one_call(ctx, b, t):
+    import torch
+    from lemonade_burn_b200 import ops
+    g = torch.Generator().manual_seed(b)
+    cap, count = t + 4, [(i * 7) % (t + 1) for i in range(b)]
+    path = torch.full((b, t), -1, dtype=torch.int32)
+    for i, n in enumerate(count):
+        path[i, :n] = torch.randperm(t, generator=g)[:n].sort().values.int()
+    k = torch.randn(2, b, 1, cap, 8, device="cuda").to(torch.bfloat16)
+    v, pos, moved = k + 1, *dev(ints([i % 5 for i in range(b)]), ints([i % 5 for i in range(b)]))
+    k2, v2 = k.clone(), v.clone()
+    ops.kv_keep_path(k, v, pos, *dev(path, ints(count)))
+    ops.kv_keep_path(k2, v2, moved, *dev(path, ints(count)), advance=True)
+    assert torch.equal(k, k2) and torch.equal(v, v2) and pos.tolist() == [i % 5 for i in range(b)] and moved.tolist() == [i % 5 + n for i, n in enumerate(count)]
+    ctx.check_device_error()

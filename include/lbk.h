@@ -540,6 +540,8 @@ int lbk_moe_route(lbk_ctx *ctx, const float *z_dev, size_t z_pitch, size_t n, si
  * whatever its depth, and pos + count <= cap. A sequence whose positions or parents break these rules is not computed and
  * its buffers are left as they were, except that lbk_attn_tree takes a parent that is none for -1; lbk_check_device_error then returns
  * LBK_ERR_INVALID. Rows of places not in use are left as they were. b sequences, everything read from device memory: a step can be recorded.
+ * lbk_embed_tree_bf16      lbk_embed_bf16 for the nodes, rows [b * t]: places not in use get token 0's row, whatever stands in tokens_dev; so does a node whose token is
+ *                          outside the vocabulary, and lbk_check_device_error returns LBK_ERR_INVALID.
  * lbk_rope_kv_append_tree  lbk_rope_kv_append for the nodes: q_dev [b][t][n_heads][head_dim] turned in place and k_dev
  *                          [b][t][kv_heads][head_dim] by position pos + depth, k and v appended at row pos + i. The tables have cap rows or more.
  * lbk_attn_tree            softmax(scale * q . k) v over the rows 0 .. pos - 1 and those of the node itself and its ancestors, head_dim
@@ -559,6 +561,8 @@ int lbk_moe_route(lbk_ctx *ctx, const float *z_dev, size_t z_pitch, size_t n, si
  * lbk_advance_pos_path     the same for the sequences whose path lbk_kv_keep_path takes; of the others it leaves position and rows as they were. For
  *                          paths that the caller has not made by lbk_tree_accept. */
 #define LBK_TREE_NODES 128
+int lbk_embed_tree_bf16(lbk_ctx *ctx, const uint16_t *table_dev, size_t vocab, const int32_t *tokens_dev, const int32_t *counts_dev, size_t b, size_t t,
+                        size_t hidden, float *out_dev, void *stream);
 int lbk_rope_kv_append_tree(lbk_ctx *ctx, float *q_dev, const float *k_dev, const float *v_dev, const float *cos_dev, const float *sin_dev,
                             const int32_t *pos_dev, const int32_t *parents_dev, const int32_t *counts_dev, size_t b, size_t t, size_t n_heads,
                             size_t kv_heads, size_t head_dim, size_t cap, uint16_t *kcache_dev, uint16_t *vcache_dev, void *stream);

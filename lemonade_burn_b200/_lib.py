@@ -122,6 +122,7 @@ SYMBOLS = [
     ("lbk_attn_window", _i, [_vp, _i, _vp, _vp, _vp, _vp, _sz, _i, _sz, _sz, _sz, _sz, _sz, _sz, _sz, _f, _sz, _sz, _i, _vp, _vp, _sz, _vp]),
     ("lbk_moe_route_ints", _sz, [_sz, _sz, _sz]),
     ("lbk_moe_route", _i, [_vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp]),
+    ("lbk_embed_tree_bf16", _i, [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _vp]),
     ("lbk_rope_kv_append_tree", _i, [_vp] * 9 + [_sz] * 6 + [_vp] * 3),
     ("lbk_attn_tree_scratch", _sz, [_vp, _sz, _sz, _sz]),
     ("lbk_attn_tree", _i, [_vp, _i, _vp, _sz] + [_vp] * 5 + [_sz] * 6 + [_f, _vp, _vp, _sz, _vp]),

@@ -93,8 +93,8 @@ int device_error_status(int word) {
         return fail(LBK_ERR_INVALID, "a decode position was outside its cache (position < 0 or >= capacity); the kernels of that step "
                                      "refused to run and its results are invalid");
     if (word == 8)
-        return fail(LBK_ERR_INVALID, "a tree of drafted tokens had a parent that is not in front of its node, or a path that does not ascend inside it; "
-                                     "the kernels of that step refused the sequence and its results are invalid");
+        return fail(LBK_ERR_INVALID, "a tree of drafted tokens had a parent that is not in front of its node, a token outside the vocabulary, or a path that does not ascend "
+                                     "inside it; the results of that sequence are invalid");
     return fail(LBK_ERR_TIMEOUT, "a bounded device-side wait gave up (code %d); results of that launch are invalid", word);
 }
 

@@ -1,5 +1,6 @@
 // Drafted tokens: the kernels around their attention (lbk_attn_tree.cu).
 //
+//   embed_tree         rows of the embedding table for the nodes
 //   rope_append_tree   queries and keys turned by their node's DEPTH (position pos + number of ancestors), keys and values
 //                      appended as bf16 at the node's PLACE (row pos + i)
 //   tree_accept        the greedy walk: node 0, then the child whose token is the best one of its parent's row
@@ -15,6 +16,35 @@
 namespace lbk {
 
 namespace {
+
+// One block per node place. A place that is not in use may hold anything as its token (a batch is padded with -1, or with what was there): its row is token 0's, a number that
+// the rows of a pass can work with. So is that of a token outside the vocabulary, and the host hears of it. Rows as embed_kernel (lbk_decoder.cu) copies them.
+// UNITS: values by four.
+template <bool UNITS>
+__global__ void embed_tree_kernel(const uint16_t *__restrict__ table, int vocab, const int *__restrict__ tokens, const int *__restrict__ counts, int t, int hidden, float *__restrict__ out,
+                                  int *err_word) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int row = blockIdx.x, seq = row / t;
+    int token = 0;
+    if (row - seq * t < tree_count(counts, seq, t)) {
+        token = tokens[row];
+        if (token < 0 || token >= vocab) {
+            if (threadIdx.x == 0) atomicExch(err_word, kErrTree);
+            token = 0;
+        }
+    }
+    const uint16_t *from = table + static_cast<size_t>(token) * hidden;
+    float *to = out + static_cast<size_t>(row) * hidden;
+    if (UNITS) {
+        for (int i = threadIdx.x; i < hidden >> 2; i += blockDim.x) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(from) + i);
+            reinterpret_cast<float4 *>(to)[i] = make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+        }
+        return;
+    }
+    for (int i = threadIdx.x; i < hidden; i += blockDim.x) to[i] = __uint_as_float(static_cast<uint32_t>(from[i]) << 16);
+}
 
 // x * cos + other * sin with the rounding of the prompt pass (lbk_decoder.cu): the product with sin rounded, the rest in one step
 __device__ __forceinline__ float turned(float x, float c, float other, float s) { return __fmaf_rn(x, c, __fmul_rn(other, s)); }
@@ -238,6 +268,23 @@ __global__ void __launch_bounds__(kAdvanceWarps * 32) advance_path_kernel(int *p
 using namespace lbk;
 
 extern "C" {
+
+int lbk_embed_tree_bf16(lbk_ctx *c, const uint16_t *table_dev, size_t vocab, const int32_t *tokens_dev, const int32_t *counts_dev, size_t b, size_t t, size_t hidden, float *out_dev,
+                        void *stream) {
+    LBK_TREE_PRE("lbk_embed_tree_bf16");
+    if (b == 0 || t == 0) return LBK_OK;
+    if (!table_dev || !tokens_dev || !out_dev) return fail(LBK_ERR_INVALID, "lbk_embed_tree_bf16: null buffer");
+    if (t > LBK_TREE_NODES) return fail(LBK_ERR_UNSUPPORTED, "a tree has at most %d nodes (got %zu)", LBK_TREE_NODES, t);
+    if (!vocab || !hidden || vocab > INT32_MAX || hidden > INT32_MAX) return fail(LBK_ERR_SHAPE, "lbk_embed_tree_bf16: %zu rows of %zu values", vocab, hidden);
+    if (b * t > INT32_MAX) return fail(LBK_ERR_UNSUPPORTED, "lbk_embed_tree_bf16: more rows than 2^31");
+    const bool units = hidden % 4 == 0 && (reinterpret_cast<uintptr_t>(table_dev) & 7) == 0 && (reinterpret_cast<uintptr_t>(out_dev) & 15) == 0;
+    // by 512 threads up to three rows an SM, by 128 more of them (lbk_embed_bf16)
+    const unsigned threads = b * t <= 3 * static_cast<size_t>(ctx->sm_count) ? 512 : 128;
+    LBK_CUDA(launch_chained(units ? embed_tree_kernel<true> : embed_tree_kernel<false>, dim3(static_cast<unsigned>(b * t)), dim3(threads), 0, st, table_dev, static_cast<int>(vocab), tokens_dev,
+                            counts_dev, static_cast<int>(t), static_cast<int>(hidden), out_dev, ctx->err_word));
+    ctx->launches++;
+    return LBK_OK;
+}
 
 int lbk_rope_kv_append_tree(lbk_ctx *c, float *q_dev, const float *k_dev, const float *v_dev, const float *cos_dev, const float *sin_dev, const int32_t *pos_dev,
                             const int32_t *parents_dev, const int32_t *counts_dev, size_t b, size_t t, size_t n_heads, size_t kv_heads, size_t head_dim, size_t cap,

@@ -332,7 +332,7 @@ class BitNet:
     # ---- drafted tokens --------------------------------------------------------------------------
     def forward_tree(self, tokens: torch.Tensor, parents: torch.Tensor, cache: KvCache, counts: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Several drafted tokens of every sequence in one pass: tokens, parents int32 CUDA [b, t] (parents[i] < i: the node that node i
-        follows, -1: the last committed token), counts int32 [b] how many of them a sequence has; all t places have to fit in the cache. Returns the logits f32 [b, t, vocab] after each. Their keys
+        follows, -1: the last committed token), counts int32 [b] how many of them a sequence has (what the other places hold does not matter); all t places have to fit in the cache. Returns the logits f32 [b, t, vocab] after each. Their keys
         and values are in the cache behind the committed ones, which stay as many: `accept_tree` commits a path."""
         cfg = self.cfg
         if tokens.dtype != torch.int32 or tokens.shape != parents.shape or tokens.dim() != 2 or tokens.shape[0] != cache.b:
@@ -345,6 +345,8 @@ class BitNet:
             raise ValueError("drafted tokens need a cache whose sequences have positions of their own (new_cache(own_positions=True))")
         if cfg.head_dim() != 128:
             raise ValueError("drafted tokens need heads of 128")
+        if counts is not None and (counts.dtype != torch.int32 or counts.shape != (cache.b,) or not counts.is_contiguous()):
+            raise ValueError("counts are int32, one for each sequence")
         cache.reserve(tokens.shape[1])
         with torch.cuda.device(self.final_norm.device):  # the stream of the model's device, whichever is current
             return self._forward_tree(tokens, parents, cache, counts)
@@ -376,7 +378,8 @@ class BitNet:
             chk(lib.lbk_rms_norm(h, P(a), P(w), m, width, C.c_float(eps), P(n), st))
             return ops.ternary_linear_multi(n, linears)
 
-        chk(lib.lbk_embed_bf16(h, P(self.lm_head), P(tokens.contiguous()), m, H, P(x), st))
+        tokens = tokens.contiguous()
+        chk(lib.lbk_embed_tree_bf16(h, P(self.lm_head), cfg.vocab_size, P(tokens), None if counts is None else P(counts), b, t, H, P(x), st))
         d = None  # output of the previous layer's down projection, not yet added to the residual x
         for li, l in enumerate(self.layers):
             q, k, v = project(ops.PRE_RMS if d is None else ops.PRE_ADD_RMS, x, d, l["input_norm"], H, [l["q"], l["k"], l["v"]])

@@ -122,3 +122,9 @@ def test_keep_that_advances_refuses():
     with pytest.raises(ValueError):
         ops.kv_keep_path(c, c, _i(2), _i(3, 4), _i(2), advance=True)
     assert _lib.load().lbk_advance_pos_path(None, None, None, None, 1, 1, 8, None) == 1
+
+
+def test_rows_of_nodes_without_a_context():
+    from lemonade_burn_b200 import _lib, build
+    build.build()
+    assert _lib.load().lbk_embed_tree_bf16(None, None, 5, None, None, 1, 1, 8, None, None) == 1

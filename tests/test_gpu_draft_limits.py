@@ -79,3 +79,73 @@ def test_keep_and_advance_in_one_call(ctx, b, t):
     ops.kv_keep_path(k2, v2, moved, *dev(path, ints(count)), advance=True)
     assert torch.equal(k, k2) and torch.equal(v, v2) and pos.tolist() == [i % 5 for i in range(b)] and moved.tolist() == [i % 5 + n for i, n in enumerate(count)]
     ctx.check_device_error()
+
+
+@pytest.mark.parametrize("heads,vocab", [(4, 700), (2, 300)])
+def test_places_that_are_not_in_use_hold_anything(ctx, heads, vocab):
+    """A batch of trees of different sizes is padded with whatever was there: with -1, as paths and `after` of a sequence without nodes are, or with any number."""
+    import torch
+    from test_gpu_draft_models import near, small
+    net = small(ctx, heads=heads, layers=2, vocab=vocab)
+    b, t = 4, 6
+    g = torch.Generator().manual_seed(1)
+    counts = ints([3, 0, 6, 1])
+    tokens, parents = torch.randint(0, vocab, (b, t), generator=g, dtype=torch.int32), trees(b, t, 2)
+    unused = torch.arange(t) >= counts[:, None]
+    results = []
+    for fill in (0, -1, 2 ** 31 - 1, -2 ** 31, vocab):
+        padded = torch.where(unused, torch.tensor(fill, dtype=torch.int32), tokens)
+        at = torch.where(unused, torch.tensor(fill, dtype=torch.int32), parents)
+        cache = net.new_cache(b, 64, own_positions=True)
+        logits = net.forward_tree(*dev(padded, at), cache, counts.cuda())
+        assert bool(logits.isfinite().all())
+        path, count, after = net.decode_tree(*dev(padded, at), cache, counts.cuda())
+        results.append((logits[~unused], path, count, after, cache.k, cache.v))
+        ctx.check_device_error()
+    for r in results[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(r, results[0]))
+    alone = net.forward_tree(tokens[2:3].cuda(), parents[2:3].cuda(), net.new_cache(1, 64))
+    assert near(results[0][0][-7:-1], alone[0])
+
+
+def test_tokens_outside_the_vocabulary_are_reported(ctx):
+    import torch
+    from lemonade_burn_b200 import _lib
+    from test_gpu_draft_models import near, small
+    net = small(ctx, layers=1)
+    for bad in (-1, 700, 2 ** 31 - 1, -2 ** 31):
+        tokens, parents = ints([[5, 6, 7], [5, bad, 7]]), trees(2, 3, 0, "star")
+        cache = net.new_cache(2, 32, own_positions=True)
+        logits = net.forward_tree(*dev(tokens, parents), cache)
+        with pytest.raises(_lib.LbkError) as e:
+            ctx.check_device_error()
+        assert e.value.status == 1 and "vocabulary" in str(e.value)
+        assert near(logits[0], net.forward_tree(tokens[:1].cuda(), parents[:1].cuda(), net.new_cache(1, 32))[0])
+    for counts in (torch.zeros(2, dtype=torch.int64), ints([1]), ints([[1, 1]])):
+        with pytest.raises(ValueError, match="counts"):
+            net.forward_tree(*dev(ints([[1], [2]]), ints([[-1], [-1]])), net.new_cache(2, 32, own_positions=True), counts.cuda())
+    ctx.check_device_error()
+
+
+@pytest.mark.parametrize("hidden,shift", [(64, 0), (512, 0), (2560, 0), (514, 0), (33, 0), (512, 1)])
+@pytest.mark.parametrize("b,t", [(1, 1), (3, 7), (9, 128)])
+def test_rows_of_nodes(ctx, hidden, shift, b, t):
+    """The rows of the call for one token a sequence, bit by bit; the form by four and the form by one."""
+    import torch
+    from lemonade_burn_b200 import _lib
+    lib, st = _lib.load(), torch.cuda.current_stream().cuda_stream
+    g = torch.Generator(device="cuda").manual_seed(hidden)
+    table = torch.randn(301 * hidden + shift, generator=g, device="cuda").to(torch.bfloat16)[shift:].view(301, hidden)
+    tokens = torch.randint(0, 301, (b, t), generator=g, device="cuda", dtype=torch.int32)
+    counts = [(3 * i + 1) % (t + 1) for i in range(b)]
+    out = torch.empty(b, t, hidden, device="cuda")
+    for c in (None, ints(counts).cuda()):
+        _lib.check(lib.lbk_embed_tree_bf16(ctx.handle, table.data_ptr(), 301, tokens.data_ptr(), None if c is None else c.data_ptr(), b, t, hidden, out.data_ptr(), st))
+        want = table[tokens.long()].float()
+        if c is not None:
+            want[torch.arange(t, device="cuda") >= c[:, None]] = table[0].float()
+        assert torch.equal(out, want)
+    assert lib.lbk_embed_tree_bf16(ctx.handle, table.data_ptr(), 0, tokens.data_ptr(), None, b, t, hidden, out.data_ptr(), st) == 2
+    assert lib.lbk_embed_tree_bf16(ctx.handle, table.data_ptr(), 301, tokens.data_ptr(), None, b, 129, hidden, out.data_ptr(), st) == 4
+    assert lib.lbk_embed_tree_bf16(ctx.handle, None, 301, tokens.data_ptr(), None, b, t, hidden, out.data_ptr(), st) == 1
+    ctx.check_device_error()

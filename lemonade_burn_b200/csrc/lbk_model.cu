@@ -336,6 +336,7 @@ struct Batcher {
 namespace {
 
 constexpr size_t kLogitRows = 128;      // rows of logits staged on the device at a time
+constexpr size_t kScoreWords = 3 + 2 * LBK_LOGPROBS_TOP;  // of a row that is scored: target, log probability, entropy, ids and log probabilities of the alternatives
 
 // Work buffers for prompt passes of up to `rows` rows, allocated for the rows a prompt really has (more rows
 // fill the GEMM's tile rounds better: a 4032-token prompt at 2B4T shapes takes 41.3 ms at 1024 rows a pass,
@@ -349,6 +350,7 @@ int ensure_prefill_buffers(Model *m, Cache *c, size_t rows) {
     LBK_TRY(dev_alloc(c->pf_allocs, rows * 4, reinterpret_cast<void **>(&c->pf_tokens)));
     LBK_TRY(dev_alloc(c->pf_allocs, rows * m->cfg.hidden_size * 4, reinterpret_cast<void **>(&c->pf_n)));
     LBK_TRY(dev_alloc(c->pf_allocs, kLogitRows * m->cfg.vocab_size * 4, reinterpret_cast<void **>(&c->pf_logits)));
+    LBK_TRY(dev_alloc(c->pf_allocs, rows * kScoreWords * 4, reinterpret_cast<void **>(&c->score)));
     LBK_TRY(m->make_prefill_buffers(c, rows));
     c->pf_rows = rows;
     return LBK_OK;
@@ -422,11 +424,8 @@ struct Scores {
 // One pass whose rows are scored instead of handed out: the logits of kLogitRows rows at a time stay on the device. targets: one token a row, -1 none.
 int score_rows(Model *m, Cache *c, size_t seq, const uint32_t *tokens, size_t n, const int32_t *targets, float scale, size_t top, const Scores &out) {
     cudaStream_t st = m->ctx->own_stream;
-    const size_t H = m->cfg.hidden_size, V = m->cfg.vocab_size, words = n * (3 + 2 * top);
-    if (c->score_words < words) {
-        LBK_TRY(dev_alloc(c->device_allocs, words * 4, reinterpret_cast<void **>(&c->score)));  // the smaller ones stay until the cache goes
-        c->score_words = words;
-    }
+    const size_t H = m->cfg.hidden_size, V = m->cfg.vocab_size;
+    LBK_TRY(ensure_prefill_buffers(m, c, n));
     int32_t *at = c->score, *ids = at + 3 * n;
     float *lp = reinterpret_cast<float *>(at + n), *entropy = lp + n, *best = reinterpret_cast<float *>(ids + n * top);
     LBK_CUDA(cudaMemcpyAsync(at, targets, n * 4, cudaMemcpyHostToDevice, st));

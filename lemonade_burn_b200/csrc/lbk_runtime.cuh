@@ -374,8 +374,7 @@ struct Cache {
     std::vector<void *> pf_allocs;
     int32_t *pf_tokens = nullptr;
     float *pf_n = nullptr, *pf_logits = nullptr;
-    int32_t *score = nullptr;             // what lbk_model_score brings in and takes out, score_words words
-    size_t score_words = 0;
+    int32_t *score = nullptr;             // what lbk_model_score brings in and takes out
     virtual ~Cache();
 };
 

@@ -149,3 +149,31 @@ def test_rows_of_nodes(ctx, hidden, shift, b, t):
     assert lib.lbk_embed_tree_bf16(ctx.handle, table.data_ptr(), 301, tokens.data_ptr(), None, b, 129, hidden, out.data_ptr(), st) == 4
     assert lib.lbk_embed_tree_bf16(ctx.handle, None, 301, tokens.data_ptr(), None, b, t, hidden, out.data_ptr(), st) == 1
     ctx.check_device_error()
+
+
+def test_scores_of_texts_of_all_lengths_take_no_more_memory_than_the_longest(ctx, tmp_path):
+    """A cache that is reset and scored with longer and longer texts."""
+    import numpy as np
+    import torch
+    from lemonade_burn_b200 import model
+    longest = 1200
+    cfg = model.Config(256, 384, 2, 1, 1, 300, 1e-5, 500000.0, 2048)
+    model.save_checkpoint(tmp_path, cfg, model.random_checkpoint(cfg, 8))
+    net = model.NativeBitNet(tmp_path, ctx)
+    toks = np.random.default_rng(0).integers(0, 300, longest).astype(np.uint32)
+    net.score(toks, net.new_cache(1, longest), top=20)  # what the library itself keeps
+
+    def room(lengths):
+        cache = net.new_cache(1, longest)
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        for n in lengths:
+            net.reset_cache(cache)
+            scores = net.score(toks[:n], cache, top=20)
+        return before - torch.cuda.mem_get_info()[0], scores
+    alone, want = room([longest])
+    grown, got = room(range(1, longest + 1))
+    # 1, 2, .., 1200 rows of 43 words are 124 MB; the allocator's pages are 2 MB
+    assert grown <= alone + (16 << 20)
+    assert all(np.array_equal(a, b, equal_nan=True) for a, b in zip(got, want))
+    net.close()

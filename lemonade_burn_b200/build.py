@@ -1,9 +1,15 @@
-"""Builds liblbk.so (the CUDA C-ABI library) in-tree with nvcc for sm_100a, and _torch_ops.so (the torch side of some of its calls) with g++."""
+"""Builds liblbk.so (the CUDA C-ABI library) in-tree with nvcc for sm_100a and, for whoever has torch, _torch_ops.so (the torch side of some of its
+calls) with g++."""
 from __future__ import annotations
 
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
+import sys
+import sysconfig
+import warnings
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -63,23 +69,37 @@ def library_for(architecture: str) -> Path:
     return build(lib=PKG / f"liblbk-{architecture}.so", sources=RUNTIME + FAMILIES[architecture])
 
 
+def torch_ops_target() -> str:
+    """What _torch_ops.so is compiled against, and holds as a string: torch's C++ interface is another with every version."""
+    return f"lbk torch ops: torch {importlib.metadata.version('torch')}, {sys.implementation.cache_tag}"
+
+
+def torch_ops_unavailable() -> str:
+    """Why the extension module cannot be built here, or "". The library itself needs nvcc alone."""
+    if importlib.util.find_spec("torch") is None:
+        return "torch is not installed"
+    if not (Path(sysconfig.get_path("include")) / "Python.h").exists():
+        return f"Python.h is not in {sysconfig.get_path('include')}"
+    return ""
+
+
 def torch_ops_stale() -> bool:
     deps = (TORCH_SOURCE, ROOT / "include" / "lbk.h")
-    return not TORCH_OPS.exists() or any(d.stat().st_mtime > TORCH_OPS.stat().st_mtime for d in deps)
+    return (not TORCH_OPS.exists() or any(d.stat().st_mtime > TORCH_OPS.stat().st_mtime for d in deps)
+            or torch_ops_target().encode() + b"\0" not in TORCH_OPS.read_bytes())
 
 
 def build_torch_ops(force: bool = False) -> Path:
     """Compile the extension module of ops.py. It links torch's libraries and no other: liblbk.so's functions are handed to it."""
     if not force and not torch_ops_stale():
         return TORCH_OPS
-    import sysconfig
-
     import torch
     home = Path(torch.__file__).resolve().parent
     include = [home / "include", home / "include" / "torch" / "csrc" / "api" / "include", Path(nvcc_path()).resolve().parent.parent / "include",
                sysconfig.get_path("include"), ROOT / "include"]
     part = TORCH_OPS.with_name(f".{TORCH_OPS.name}.{os.getpid()}")
     _run([shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          f'-DLBK_TORCH_TARGET="{torch_ops_target()}"',
           *[x for i in include for x in ("-isystem", str(i))], "-o", str(part), str(TORCH_SOURCE), f"-L{home / 'lib'}", f"-Wl,-rpath,{home / 'lib'}",
           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"], dict(os.environ))
     os.replace(part, TORCH_OPS)
@@ -88,12 +108,20 @@ def build_torch_ops(force: bool = False) -> Path:
 
 def build(force: bool = False, verbose: bool = False, lib: Path = None, sources=None) -> Path:
     """Compile every .cu (one object each, side by side, only the ones whose source or any header
-    changed) and link lemonade_burn_b200/liblbk.so (or `lib` from `sources`). Returns the library path."""
+    changed) and link lemonade_burn_b200/liblbk.so (or `lib` from `sources`); then the extension module, whose calls every part of the
+    library has some of. Returns the library path."""
     lib, sources = lib or LIB, sources or SOURCES
-    if lib == LIB:
+    if force or is_stale(lib):
+        _build_library(force, verbose, lib, sources)
+    missing = torch_ops_unavailable()
+    if not missing:
         build_torch_ops(force)
-    if not force and not is_stale(lib):
-        return lib
+    elif missing != "torch is not installed":  # who has no torch has no use for it
+        warnings.warn(f"_torch_ops.so, which ops.py needs, is not built: {missing}")
+    return lib
+
+
+def _build_library(force: bool, verbose: bool, lib: Path, sources) -> None:
     from concurrent.futures import ThreadPoolExecutor
     OBJ.mkdir(exist_ok=True)
     env = dict(os.environ)
@@ -117,10 +145,7 @@ def build(force: bool = False, verbose: bool = False, lib: Path = None, sources=
     part = lib.with_name(f".{lib.name}.{os.getpid()}")  # a half-written library is never loaded
     _run([nvcc, "-shared", "-o", str(part)] + [str(OBJ / (Path(s).stem + ".o")) for s in sources], env)
     os.replace(part, lib)
-    return lib
 
 
 if __name__ == "__main__":
-    import sys
-
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))

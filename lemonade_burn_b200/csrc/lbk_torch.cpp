@@ -351,11 +351,20 @@ PyMethodDef methods[] = {{"bind", fast(bind), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
+// What this was compiled against (build.torch_ops_target): build.py looks for it in the file, ops.py in the module.
+#ifndef LBK_TORCH_TARGET
+#error "LBK_TORCH_TARGET says what this is compiled against"
+#endif
+const char target[] = LBK_TORCH_TARGET;
+
 }  // namespace
 
 PyMODINIT_FUNC PyInit__torch_ops() {
     g_handle = PyUnicode_InternFromString("handle");
     g_value = PyUnicode_InternFromString("value");
     g_device = PyUnicode_InternFromString("device");
-    return g_handle && g_value && g_device ? PyModule_Create(&module) : nullptr;
+    if (!g_handle || !g_value || !g_device) return nullptr;
+    PyObject *m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "target", target) < 0) Py_CLEAR(m);
+    return m;
 }

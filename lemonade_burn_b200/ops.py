@@ -177,12 +177,20 @@ def _torch_ops():
     if _native is None:
         from importlib.machinery import ExtensionFileLoader
         from importlib.util import module_from_spec, spec_from_file_location
+
+        from . import build
         path = _lib.LIB_PATH.with_name("_torch_ops.so")
         if not path.exists():
             raise RuntimeError(f"{path} is missing: build it with `python -m lemonade_burn_b200.build`")
         loader = ExtensionFileLoader("_torch_ops", str(path))
-        module = module_from_spec(spec_from_file_location("_torch_ops", str(path), loader=loader))
-        loader.exec_module(module)
+        try:
+            module = module_from_spec(spec_from_file_location("_torch_ops", str(path), loader=loader))
+            loader.exec_module(module)
+            target = module.target
+        except (ImportError, AttributeError) as e:  # symbols that this torch does not have
+            target = str(e)
+        if target != build.torch_ops_target():
+            raise RuntimeError(f"{path} is of another torch than this one ({target}): build it with `python -m lemonade_burn_b200.build`")
         lib = _lib.load()
         calls = [getattr(lib, "lbk_" + n, None) for n in ("rope_kv_append_tree", "attn_tree_scratch", "attn_tree", "tree_accept", "kv_keep_path", "advance_pos_by", "token_logprobs", "advance_pos_path")]
         module.bind(*[C.cast(f, C.c_void_p).value if f else 0 for f in calls], _lib.check, default_context)  # one family's part of the library has some of them only

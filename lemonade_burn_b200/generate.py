@@ -38,8 +38,9 @@ def main(argv=None) -> int:
     net = runtime.load_model(a.model, dtype=a.dtype)
     prompts = [[int(t) for t in p.split(",")] for p in a.prompt]
     if a.score:
+        cache = net.new_cache(1, max(map(len, prompts)))
         for p in prompts:
-            cache = net.new_cache(1, len(p))
+            net.reset_cache(cache)
             print(",".join(f"{x:.6f}" for x in net.score(p, cache).logprobs[:-1]))
         net.close()
         return 0

@@ -128,3 +128,36 @@ def test_rows_of_nodes_without_a_context():
     from lemonade_burn_b200 import _lib, build
     build.build()
     assert _lib.load().lbk_embed_tree_bf16(None, None, 5, None, None, 1, 1, 8, None, None) == 1
+
+
+def test_scores_of_many_prompts_take_one_cache(monkeypatch, capsys):
+    """The command's prompts come one behind the other: one cache, as long as the longest, serves them."""
+    from types import SimpleNamespace
+
+    import numpy as np
+
+    from lemonade_burn_b200 import _lib, build, generate, runtime
+    made, used = [], []
+
+    class Net:
+        def new_cache(self, b, cap):
+            made.append((b, cap))
+            return SimpleNamespace(free=cap)
+
+        def reset_cache(self, cache):
+            cache.free = made[0][1]
+
+        def score(self, prompt, cache):
+            cache.free -= len(prompt)
+            used.append(cache.free)
+            return SimpleNamespace(logprobs=np.arange(len(prompt), dtype=np.float32))
+
+        def close(self):
+            pass
+    monkeypatch.setattr(_lib, "use", lambda path: None)
+    monkeypatch.setattr(build, "library_for", lambda architecture: None)
+    monkeypatch.setattr(runtime, "architecture_of", lambda directory: "")
+    monkeypatch.setattr(runtime, "load_model", lambda directory, dtype: Net())
+    assert generate.main(["--model", "x", "--score", "--prompt", "1,2", "--prompt", "3,4,5,6", "--prompt", "7"]) == 0
+    assert made == [(1, 4)] and used == [2, 0, 3]
+    assert capsys.readouterr().out.splitlines() == ["0.000000", "0.000000,1.000000,2.000000", ""]

@@ -59,8 +59,10 @@ def test_f32_queries_are_whole(ctx, t, nh, kvh, length):
     q[..., 0] = 1 + rand(1, t, nh)
     q[..., 1] = q[..., 0] + rand(1, t, nh) / 32
     k = torch.zeros(1, kvh, length + t, HD, device="cuda", dtype=torch.bfloat16)
-    k[..., 0] = 256 * (1 + rand(1, kvh, length + t)).to(torch.bfloat16)
-    v = torch.randn(k.shape, generator=g, device="cuda").to(torch.bfloat16)
+    sign = torch.where(rand(1, kvh, length + t) < 0.5, -1.0, 1.0)
+    k[..., 0] = (256 * sign * (1 + rand(1, kvh, length + t))).to(torch.bfloat16)
+    # values of the key's sign: what a query's missing bits do to the scores is of that sign, too, and does not average out
+    v = ((1 + rand(*k.shape)) * sign[..., None]).to(torch.bfloat16)
     # the second product takes most of the first one away
     k[..., 1] = (-k[..., 0].float() + 40 * (rand(1, kvh, length + t) - 0.5)).to(torch.bfloat16)
     args = q, k, v, ints([length]), trees(1, t, t), ints([t])

@@ -534,12 +534,14 @@ int lbk_moe_route(lbk_ctx *ctx, const float *z_dev, size_t z_pitch, size_t n, si
                   int32_t *place_out_dev, int32_t *offs_out_dev, void *stream);
 
 /* ---- drafted tokens: several tokens of a sequence checked in one pass (no counterpart in the reference) ----------------
- * A sequence has t node places (1..LBK_TREE_NODES), the first counts_dev[seq] of them in use (counts_dev may be null: all).
+ * A sequence has t node places (1..LBK_TREE_NODES), the first counts_dev[seq] of them in use (counts_dev may be null: all; a number
+ * outside 0 .. t is the nearest inside).
  * parents_dev[seq][i] is the node that node i follows, -1 <= parent < i; -1: it follows the committed position pos_dev[seq] - 1. A
  * node's depth is the number of its ancestors. Caches as everywhere: bf16 [seq][kv_heads][cap][head_dim]; node i's row is pos + i
  * whatever its depth, and pos + count <= cap. A sequence whose positions or parents break these rules is not computed and
  * its buffers are left as they were, except that lbk_attn_tree takes a parent that is none for -1; lbk_check_device_error then returns
- * LBK_ERR_INVALID. Rows of places not in use are left as they were. b sequences, everything read from device memory: a step can be recorded.
+ * LBK_ERR_INVALID. lbk_tree_accept gives such a sequence a path of -1, a count of 0 and a next token of -1. Rows of places not in
+ * use are left as they were. b sequences, everything read from device memory: a step can be recorded.
  * lbk_embed_tree_bf16      lbk_embed_bf16 for the nodes, rows [b * t]: places not in use get token 0's row, whatever stands in tokens_dev; so does a node whose token is
  *                          outside the vocabulary, and lbk_check_device_error returns LBK_ERR_INVALID.
  * lbk_rope_kv_append_tree  lbk_rope_kv_append for the nodes: q_dev [b][t][n_heads][head_dim] turned in place and k_dev
@@ -556,7 +558,7 @@ int lbk_moe_route(lbk_ctx *ctx, const float *z_dev, size_t z_pitch, size_t n, si
  *                          best_dev of the last one (-1 for a sequence without nodes).
  * lbk_kv_keep_path         rows pos + path[j] move to pos + j, j < count_dev[seq], of keys and values of `layers` layers that lie
  *                          layer_elems elements apart. path_dev [b][t] ascending, any accepted nodes. Positions are not changed. head_dim and
- *                          layer_elems are multiples of 8, the caches lie on 16 bytes; at most 65535 sequences. A count outside 0 .. t is the nearest inside.
+ *                          layer_elems are multiples of 8, the caches lie on 16 bytes; at most 65535 sequences.
  * lbk_advance_pos_by       pos_dev[seq] += count_dev[seq], at most LBK_TREE_NODES.
  * lbk_advance_pos_path     the same for the sequences whose path lbk_kv_keep_path takes; of the others it leaves position and rows as they were. For
  *                          paths that the caller has not made by lbk_tree_accept. */

@@ -187,7 +187,8 @@ struct Share {
 };
 // Where the walk over a segment's blocks begins, and goes round: block x comes up when x mod `most` units of the share are done, as far as that can be. The tiles of a KV
 // head are walked by different CTAs, each from somewhere else; so they come to a block at about the same time, and HBM is asked for it once: 60 nodes of 65000 keys with 8 heads
-// of 4, two tiles, read 518 MB where the cache has 266; us without / with it 97.6 / 87.2 in bf16, 166 / 158 in f32. Of one tile the walk is straight.
+// of 4, two tiles, read 518 MB where the cache has 266, and 282 so; us of 36 calls behind one another, without / with it 104.9 / 98.7 in bf16, 159.7 / 153.5 in f32. Of one tile the walk is
+// straight.
 __device__ __forceinline__ int first_block(const Share &share, const Segment &s, int unit, int group, int rows) {
     if (s.count * group <= rows) return s.begin;
     const int ahead = (unit - share.u0 - s.begin) % share.most, at = s.begin + (ahead < 0 ? ahead + share.most : ahead);
@@ -347,7 +348,8 @@ __device__ __forceinline__ void produce(const TreeParams &p, const Line &line, c
 // Tiles of 16 and 32 rows. The 128 lanes of an accumulator are a block's keys, S^T = K Q^T, and then the dimensions, O^T = V^T P^T; rows and terms are its columns, so
 // that a product costs what the rows need: 512 and 768 cycles of the tensor core for a block of 128 keys and 16 and 32 rows in three terms, where the block's 64 KB are
 // 2800 cycles of an SM's share of HBM. The stream is the bound. (mma.sync has 16 x 16 x 8 products at a sixteenth of this rate: 16 rows in three terms took 4600 cycles for
-// 128 keys, 32 rows 6400. Tiles of 64 rows, us at 16 sequences of 8100 keys: so 136, bf16 102; tiles of 128 half empty 124 and 81.)
+// 128 keys, 32 rows 6400. Tiles of 64 rows, us at 16 sequences of 8100 keys: so 136, bf16 102; tiles of 128 half empty 124 and 81,
+// bf16 with weights in one term. Few sequences of 33 to 64 rows were not measured by themselves.)
 //
 // All terms of the queries are rows of one operand, and so are those of the probabilities, which go through shared memory. A thread has one key and half of the rows:
 // a row's maximum is not at hand, and not needed: probabilities are 2^(s - m) with any m that keeps them in range. m is the maximum of the tile's first block, and is moved
@@ -711,8 +713,10 @@ __global__ void __launch_bounds__(Turned<TERMS, ROWS>::kThreads, 1) attn_tree_tu
 //                    both would have the next K block wait for a piece of V
 //   MMA warps        one for P V of block j - 1, one for Q K^T of block j + 1, while the softmax warps work on block j
 //
-// 512 bytes a key from HBM are 22 cycles of an SM, its products for 128 rows 24 in three terms and 8 in one: f32 is bound by the tensor core, bf16 by
-// the stream and by the softmax warps (an exponential per row and key). Padding rows cost nothing but the products: their warps only keep step.
+// 512 bytes a key from HBM are 22 cycles of an SM, its products for 128 rows 24 in f32 and 12 in bf16: f32 is bound by the tensor core, bf16 by
+// the way of a block's scores through the softmax warps and back: 2700 cycles a block of 128 keys, with 1560 of products and 1150 of exponentials; the block's 64 KB are 2600 of
+// an SM's share of HBM, half of that where two tiles share them. us of 36 calls behind one another, weights in one term / in two: 60 nodes of 65000 keys 83 / 99, 16 x 64 of 8100
+// keys 112 / 131. Padding rows cost nothing but the products: their warps only keep step.
 template <int TERMS>
 struct Many {
     static constexpr bool kGoesRound = true;
@@ -723,7 +727,7 @@ struct Many {
     static constexpr int kPair = kBars + 256, kSmem = kPair + 2 * 4 * kRows * 4 + 1024;
     static constexpr int kSoftWarps = 16, kKWarp = 16, kVWarp = 17, kScoreWarp = 18, kThreads = 20 * 32;  // the last one: products
     // bf16: the products are summed up in tensor memory, over all blocks, and m is moved as for few rows, with the sums, when a score is over it by kSlack. What the tensor
-    // core cuts off of a long sum (1e-5 at 8000 keys) does not show in a bf16 result, and a block needs no look at the products of the one in front.
+    // core cuts off of a long sum (some 2e-5 at 8000 keys) does not show in a bf16 result, and a block needs no look at the products of the one in front.
     static constexpr bool kStays = TERMS == 1;
     static constexpr int kPTerms = weight_terms(TERMS);
     // Scores (128 columns) and, when all have been read, the probabilities (64 a term) of even blocks in one place, of odd ones in another
@@ -789,7 +793,8 @@ __global__ void __launch_bounds__(Many<TERMS>::kThreads, 1) attn_tree_many_kerne
         } else {
             // ================= MMA issue, scores by one warp, products by another: the warps walk, one lane of each issues =================
             // A turn of a wait, products and a commit costs a warp some 400 cycles beside its products, in which those of the other go on: one warp for both took 214 us for
-            // 16 x 64 nodes of 8100 keys in f32 where these take 207, and 100 where these take 97 for 60 nodes of 65000 in bf16
+            // 16 x 64 nodes of 8100 keys in f32 where these took 207, and 100 where these took 97 for 60 nodes of 65000 in bf16 (36 calls behind one another; weights in one term
+            // then, and walks that did not go round)
             // D f32, A and B bf16, M = 128, N = 128; for P V the B operand is MN-major (bit 16)
             constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24), idesc_o = idesc_s | (1u << 16);
             auto wait = [&](int i, int parity) {

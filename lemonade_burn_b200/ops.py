@@ -209,7 +209,8 @@ def rope_kv_append_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: 
 def attn_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, pos: torch.Tensor, parents: torch.Tensor, counts: Optional[torch.Tensor] = None,
               scale: Optional[float] = None, out: Optional[torch.Tensor] = None, ctx: Optional[Context] = None) -> torch.Tensor:
     """Attention of drafted tokens (lbk_attn_tree): q [b, t, heads, 128] f32 or bf16 (nodes any distance apart) over rows 0 .. pos - 1 of kcache
-    and vcache [b, kv_heads, cap, 128] and over the node itself and its ancestors, whose rows are pos + node. At most 256 sequences. scale: 128 ** -0.5. Returns
+    and vcache [b, kv_heads, cap, 128] and over the node itself and its ancestors, whose rows are pos + node. At most 256 sequences. What is rounded to bf16 is a bf16 result, queries and
+    weights are not. scale: 128 ** -0.5. Returns
     `out`, which may be q (made like q without one: rows of places not in use are then whatever was there)."""
     return (_native or _torch_ops()).attn_tree(q, kcache, vcache, pos, parents, counts, scale, out, ctx)
 
@@ -217,7 +218,8 @@ def attn_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, pos: 
 def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, best: torch.Tensor, counts: Optional[torch.Tensor] = None,
                 ctx: Optional[Context] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The greedy walk through drafted tokens (lbk_tree_accept): tokens, parents, best (the argmax of every node's logits) int32 [b, t].
-    Returns (path [b, t]: the accepted nodes, then -1; how many of them [b]; the token that follows the last one [b])."""
+    Returns (path [b, t]: the accepted nodes, then -1; how many of them [b]; the token that follows the last one [b]; -1 for a sequence without nodes, or whose
+    tree is none). The three share one storage: clone what is kept for long, or saved."""
     return (_native or _torch_ops()).tree_accept(tokens, parents, best, counts, ctx)
 
 
@@ -243,7 +245,8 @@ class TokenLogprobs(NamedTuple):
 
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0, scale: float = 1.0, ctx: Optional[Context] = None) -> TokenLogprobs:
     """Log softmax(scale * logits), scale from 1e-20 to 1e20, at the given tokens, entropy and the `top` largest logits with their log probabilities
-    (lbk_token_logprobs). logits f32 or bf16 [rows, vocab], rows any distance apart; tokens int32 [rows] or [rows, given]."""
+    (lbk_token_logprobs). logits f32 or bf16 [rows, vocab], rows any distance apart; tokens int32 [rows] or [rows, given]. The results share one storage: clone what is kept for
+    long, or saved."""
     return TokenLogprobs(*(_native or _torch_ops()).token_logprobs(logits, tokens, top, scale, ctx))
 
 

@@ -25,14 +25,12 @@ __global__ void embed_tree_kernel(const uint16_t *__restrict__ table, int vocab,
                                   int *err_word) {
     ptx::pdl_trigger();
     ptx::pdl_wait();
-    const int row = blockIdx.x, seq = row / t;
-    int token = 0;
-    if (row - seq * t < tree_count(counts, seq, t)) {
-        token = tokens[row];
-        if (token < 0 || token >= vocab) {
-            if (threadIdx.x == 0) atomicExch(err_word, kErrTree);
-            token = 0;
-        }
+    const int row = blockIdx.x;
+    int token = tokens[row];
+    if (counts && row % t >= tree_count(counts, row / t, t)) token = 0;
+    if (static_cast<unsigned>(token) >= static_cast<unsigned>(vocab)) {
+        if (threadIdx.x == 0) atomicExch(err_word, kErrTree);
+        token = 0;
     }
     const uint16_t *from = table + static_cast<size_t>(token) * hidden;
     float *to = out + static_cast<size_t>(row) * hidden;
@@ -277,9 +275,9 @@ int lbk_embed_tree_bf16(lbk_ctx *c, const uint16_t *table_dev, size_t vocab, con
     if (t > LBK_TREE_NODES) return fail(LBK_ERR_UNSUPPORTED, "a tree has at most %d nodes (got %zu)", LBK_TREE_NODES, t);
     if (!vocab || !hidden || vocab > INT32_MAX || hidden > INT32_MAX) return fail(LBK_ERR_SHAPE, "lbk_embed_tree_bf16: %zu rows of %zu values", vocab, hidden);
     if (b * t > INT32_MAX) return fail(LBK_ERR_UNSUPPORTED, "lbk_embed_tree_bf16: more rows than 2^31");
-    const bool units = hidden % 4 == 0 && (reinterpret_cast<uintptr_t>(table_dev) & 7) == 0 && (reinterpret_cast<uintptr_t>(out_dev) & 15) == 0;
-    // by 512 threads up to three rows an SM, by 128 more of them (lbk_embed_bf16)
-    const unsigned threads = b * t <= 3 * static_cast<size_t>(ctx->sm_count) ? 512 : 128;
+    // units and threads as lbk_embed_bf16 has them
+    const bool units = hidden >= 512 && hidden % 4 == 0 && (reinterpret_cast<uintptr_t>(table_dev) & 7) == 0 && (reinterpret_cast<uintptr_t>(out_dev) & 15) == 0;
+    const unsigned threads = !units ? 256 : b * t <= 3 * static_cast<size_t>(ctx->sm_count) ? 512 : 128;
     LBK_CUDA(launch_chained(units ? embed_tree_kernel<true> : embed_tree_kernel<false>, dim3(static_cast<unsigned>(b * t)), dim3(threads), 0, st, table_dev, static_cast<int>(vocab), tokens_dev,
                             counts_dev, static_cast<int>(t), static_cast<int>(hidden), out_dev, ctx->err_word));
     ctx->launches++;

@@ -202,7 +202,8 @@ class BitNet:
 
     def forward(self, tokens: torch.Tensor, cache: KvCache, splits: Optional[int] = None) -> torch.Tensor:
         """One new token per sequence at position cache.len (model.rs:305-374 with m = 1).
-        tokens: int32 CUDA [b]. Returns logits f32 [b, vocab] and advances the cache."""
+        tokens: int32 CUDA [b]. Returns logits f32 [b, vocab] and advances the cache. A token outside the vocabulary (the -1 that `decode_tree` gives for a
+        sequence without nodes) is taken for token 0, and `ctx.check_device_error` tells of it."""
         cfg, lib, h = self.cfg, self.ctx._lib, self.ctx.handle
         b = tokens.shape[0]
         if b != cache.b:
@@ -224,7 +225,7 @@ class BitNet:
         x2 = self._buf("x2", (b, H))
         n = self._buf("n", (b, H))
         if one_launch:
-            _lib.check(lib.lbk_embed_bf16(h, P(self.lm_head), P(tokens), b, H, P(x), st))
+            _lib.check(lib.lbk_embed_tree_bf16(h, P(self.lm_head), cfg.vocab_size, P(tokens), None, b, 1, H, P(x), st))
             self._step.run(x, cache.k, cache.v, self.cos, self.sin, cache.pos, int(own), n, self._work_of(cache))
             logits = ops.bf16_linear(n, self.lm_head, self.ctx)
             _lib.check(lib.lbk_advance_pos_seq(h, P(cache.pos), None, b, st) if own else lib.lbk_advance_pos(h, P(cache.pos), st))
@@ -264,7 +265,7 @@ class BitNet:
             normq = lambda pre, xx, yy, w: ops.norm_quant(pre, xx, yy, w, e, q8, qs, qsum, self.ctx)
             projq = lambda lins: ops.ternary_gemm_q(q8, qs, qsum, b, lins)
 
-        chk(lib.lbk_embed_bf16(h, P(self.lm_head), P(tokens), b, H, P(x), st))
+        chk(lib.lbk_embed_tree_bf16(h, P(self.lm_head), cfg.vocab_size, P(tokens), None, b, 1, H, P(x), st))
         d = None  # output of the previous layer's down projection, not yet added to the residual x
         for li, l in enumerate(self.layers):
             qkv_l = [l["q"], l["k"], l["v"]]
@@ -403,7 +404,7 @@ class BitNet:
 
     def decode_tree(self, tokens: torch.Tensor, parents: torch.Tensor, cache: KvCache, counts: Optional[torch.Tensor] = None):
         """A greedy step with drafts: node 0 is the token the last step gave, the others are guesses of what follows. As many guesses as the
-        model itself would have given are committed. Returns (path, count, next) of ops.tree_accept: with the tokens on the path, and `next`, the same
+        model itself would have given are committed. Returns (path, count, next) of ops.tree_accept (next is -1 for a sequence without nodes): with the tokens on the path, and `next`, the same
         tokens as `forward` one by one."""
         logits = self.forward_tree(tokens, parents, cache, counts)
         with torch.cuda.device(self.final_norm.device):

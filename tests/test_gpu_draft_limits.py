@@ -177,3 +177,29 @@ def test_scores_of_texts_of_all_lengths_take_no_more_memory_than_the_longest(ctx
     assert grown <= alone + (16 << 20)
     assert all(np.array_equal(a, b, equal_nan=True) for a, b in zip(got, want))
     net.close()
+
+
+@pytest.mark.parametrize("layers,one_launch", [(1, True), (2, False)])
+def test_a_step_with_a_token_outside_the_vocabulary(ctx, layers, one_launch):
+    """decode_tree gives -1 for a sequence without nodes; a step that is handed it reads no row in front of the table, and the other sequences do not notice."""
+    import torch
+    from lemonade_burn_b200 import _lib
+    from test_gpu_draft_models import small
+    net = small(ctx, layers=layers)
+    how = {} if one_launch else {"splits": 2}
+    cache = net.new_cache(2, 32, own_positions=True)
+    _, count, after = net.decode_tree(*dev(ints([[5, 6], [7, 8]]), ints([[-1, 0], [-1, 0]])), cache, ints([2, 0]).cuda())
+    assert int(after[1]) == -1 and int(count[1]) == 0
+    ctx.check_device_error()
+    got = net.forward(after, cache, **how)
+    with pytest.raises(_lib.LbkError) as e:
+        ctx.check_device_error()
+    assert "vocabulary" in str(e.value) and bool(got.isfinite().all())
+    for token in (0, 700, 2 ** 31 - 1, -2 ** 31):
+        other = net.new_cache(2, 32, own_positions=True)
+        net.decode_tree(*dev(ints([[5, 6], [7, 8]]), ints([[-1, 0], [-1, 0]])), other, ints([2, 0]).cuda())
+        assert torch.equal(net.forward(torch.stack([after[0], torch.tensor(token, dtype=torch.int32, device="cuda")]), other, **how), got)
+        if token:
+            with pytest.raises(_lib.LbkError):
+                ctx.check_device_error()
+    ctx.check_device_error()
